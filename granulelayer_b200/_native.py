@@ -16,11 +16,12 @@ from pathlib import Path
 
 import torch
 
-ABI_VERSION = 17
+ABI_VERSION = 18
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libgranule_b200.so"
 
 POOL_MEAN, POOL_SUM, POOL_MAX, POOL_LME, POOL_POWER, POOL_SOFTMAX, POOL_TOPK = 0, 1, 2, 3, 4, 5, 6
 ACT_IDS = {"identity": 0, "relu": 1, "gelu": 2}
+DENSE_ACT_IDS = {**ACT_IDS, "silu": 3}   # the dense operators' (linear_act, group_norm_act)
 DTYPE_F32, DTYPE_BF16 = 0, 1
 
 
@@ -44,7 +45,9 @@ EXPORTS = ("gl_abi_version", "gl_status_string", "gl_last_cuda_error", "gl_fwd_f
            "gl_k16_bwd_f32", "gl_k16_auto_tokens", "gl_k16_fwd_tc", "gl_k16_bwd_tc", "gl_k16_fwd_tc_f32",
            "gl_k16_bwd_tc_f32", "gl_struct_layout", "gl_struct_fields", "gl_group_octets", "gl_fwd_octet_f32",
            "gl_bwd_octet_f32", "gl_k16_fwd_t5", "gl_k16_fwd_t5_f32", "gl_k16_bwd_t5", "gl_k16_bwd_t5_f32",
-           "gl_bwd_octet_prefix_f32", "gl_group_feature_prefix")
+           "gl_bwd_octet_prefix_f32", "gl_group_feature_prefix", "gl_linear_fwd", "gl_linear_bwd",
+           "gl_linear_work_bytes", "gl_norm_fwd", "gl_norm_bwd", "gl_norm_work_bytes", "gl_act8_encode",
+           "gl_act8_decode")
 
 
 class GlSetArgs(ctypes.Structure):
@@ -117,8 +120,42 @@ class GlK16Args(ctypes.Structure):
                [("act", ctypes.c_int32), ("tokens", ctypes.c_int32)]
 
 
+class GlLinearArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "w", "bias", "residual", "y", "z", "slope", "work")] + \
+               [(n, ctypes.c_int64) for n in ("M", "N", "K", "ldx", "ldw", "ldr", "ldy", "ldz", "lds", "work_bytes")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "act")]
+
+
+class GlLinearBwdArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dy", "z", "slope", "x", "codes", "exps", "w", "dx", "dw", "db",
+                                                "work")] + \
+               [(n, ctypes.c_int64) for n in ("M", "N", "K", "lddy", "ldz", "lds", "ldx", "ldc", "ldw", "lddx",
+                                              "work_bytes")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "act", "accumulate", "reserved")]
+
+
+class GlNormArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "w", "b", "y", "mean", "rstd", "work")] + \
+               [(n, ctypes.c_int64) for n in ("S", "P", "C", "G", "sx", "px", "work_bytes")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "pdtype", "act")] + [("eps", ctypes.c_float)]
+
+
+class GlNormBwdArgs(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dy", "x", "codes", "exps", "w", "b", "mean", "rstd", "dx", "dw", "db",
+                                                "work")] + \
+               [(n, ctypes.c_int64) for n in ("S", "P", "C", "G", "sx", "px", "sdy", "pdy", "ldc", "work_bytes")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "pdtype", "act", "accumulate")]
+
+
+class GlAct8Args(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "out", "codes", "exps")] + \
+               [(n, ctypes.c_int64) for n in ("rows", "C", "ldx", "ldc")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "reserved")]
+
+
 # gl_struct_layout ids 0 .. GL_STRUCT_COUNT-1, in header order.
-STRUCTS = (GlFwdArgs, GlBwdArgs, GlAdamArgs, GlSharedArgs, GlSetArgs, GlEventArgs, GlK16Args)
+STRUCTS = (GlFwdArgs, GlBwdArgs, GlAdamArgs, GlSharedArgs, GlSetArgs, GlEventArgs, GlK16Args, GlLinearArgs,
+           GlLinearBwdArgs, GlNormArgs, GlNormBwdArgs, GlAct8Args)
 
 
 def check_struct_layouts(lib, path="library"):
@@ -170,7 +207,10 @@ def load(path=None) -> ctypes.CDLL:
                          ("gl_k16_fwd_f32", GlK16Args), ("gl_k16_bwd_f32", GlK16Args),
                          ("gl_k16_fwd_tc", GlK16Args), ("gl_k16_fwd_tc_f32", GlK16Args),
                          ("gl_fwd_shared_f32", GlSharedArgs), ("gl_bwd_shared_f32", GlSharedArgs),
-                         ("gl_bwd_events_f32", GlEventArgs)):
+                         ("gl_bwd_events_f32", GlEventArgs), ("gl_linear_fwd", GlLinearArgs),
+                         ("gl_linear_bwd", GlLinearBwdArgs), ("gl_norm_fwd", GlNormArgs),
+                         ("gl_norm_bwd", GlNormBwdArgs), ("gl_act8_encode", GlAct8Args),
+                         ("gl_act8_decode", GlAct8Args)):
             fn = getattr(lib, name)
             fn.restype = ctypes.c_int
             fn.argtypes = [ctypes.POINTER(st), ctypes.c_void_p]
@@ -225,6 +265,10 @@ def load(path=None) -> ctypes.CDLL:
         for name in ("gl_k16_fwd_t5", "gl_k16_fwd_t5_f32", "gl_k16_bwd_t5", "gl_k16_bwd_t5_f32"):
             getattr(lib, name).argtypes = [ctypes.POINTER(GlK16Args), ctypes.c_void_p, ctypes.c_void_p]
             getattr(lib, name).restype = ctypes.c_int
+        lib.gl_linear_work_bytes.restype = ctypes.c_int64
+        lib.gl_linear_work_bytes.argtypes = [ctypes.c_int64] * 3 + [ctypes.c_int32] * 2
+        lib.gl_norm_work_bytes.restype = ctypes.c_int64
+        lib.gl_norm_work_bytes.argtypes = [ctypes.c_int64] * 4 + [ctypes.c_int32] * 2
         lib.gl_k16_auto_tokens.restype = ctypes.c_int
         lib.gl_k16_auto_tokens.argtypes = [ctypes.c_int64, ctypes.c_int64, ctypes.c_int32]
         if path is None:
@@ -668,3 +712,120 @@ def k16_bwd_t5(x, sched: dict, w, b, counts, c1t, dx, dw, db, NB16: int, act: in
 
 def k16_auto_tokens(B: int, S: int, backward: bool) -> int:
     return int(load().gl_k16_auto_tokens(B, S, int(bool(backward))))
+
+
+# ---- dense operators (dense.py) ----
+# The launches are short, so these helpers keep the host's share small: no device switch when the tensors'
+# device is current, and one call for the workspace size of each new set of sizes.
+
+_work_sizes = {}
+
+
+def _work(name: str, dev: torch.device, *sizes):
+    """Scratch of gl_<name>_work_bytes(*sizes) bytes on ``dev`` (None where the call needs none)."""
+    key = (name, dev.index, sizes)
+    n = _work_sizes.get(key)
+    if n is None:
+        lib = load()
+        with torch.cuda.device(dev):
+            n = int(getattr(lib, name)(*sizes))
+        if n < 0:
+            _check(lib, n, name)
+        if len(_work_sizes) > 4096:
+            _work_sizes.clear()
+        _work_sizes[key] = n
+    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+
+
+def _launch(name: str, a, dev: torch.device):
+    lib = _lib or load()
+    if dev.index == torch.cuda.current_device():
+        rc = getattr(lib, name)(ctypes.byref(a), torch._C._cuda_getCurrentRawStream(dev.index))
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(lib, name)(ctypes.byref(a), _stream(dev))
+    if rc:
+        _check(lib, rc, name)
+
+
+def _unaligned(*rows) -> int:
+    """GL_LINEAR_UNALIGNED where a matrix's base or row stride is no multiple of 16 bytes."""
+    for t in rows:
+        if t is not None and ((t.data_ptr() | t.stride(0) * t.element_size()) & 15):
+            return 4
+    return 0
+
+
+def linear_fwd(x, w, bias, residual, y, z, slope, act: int):
+    """y = act(x w^T + bias) + residual (GlLinearArgs); 2-d tensors with unit column stride."""
+    _require_cuda(x, w, bias, residual, y, z, slope)
+    M, K = x.shape
+    N, dt = w.shape[0], _wdtype(w)
+    work = _work("gl_linear_work_bytes", x.device, M, N, K, dt, _unaligned(x, w))
+    _launch("gl_linear_fwd", GlLinearArgs(
+        x.data_ptr(), w.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(z), _ptr(slope), _ptr(work),
+        M, N, K, x.stride(0), w.stride(0), residual.stride(0) if residual is not None else 0, y.stride(0),
+        z.stride(0) if z is not None else 0, slope.stride(0) if slope is not None else 0,
+        work.numel() if work is not None else 0, dt, act), x.device)
+
+
+def linear_bwd(dy, z, slope, x, codes, exps, w, dx, dw, db, K: int, act: int, accumulate: bool):
+    """dx, dw, db (each may be None) of linear_fwd for the output gradient dy (GlLinearBwdArgs)."""
+    _require_cuda(dy, z, slope, x, codes, exps, w, dx, dw, db)
+    M, N = dy.shape
+    dt = _wdtype(dy)
+    work = _work("gl_linear_work_bytes", dy.device, M, N, K, dt, 1 | (2 if codes is not None else 0) |
+                 _unaligned(w if dx is not None else None, x if dw is not None else None))
+
+    def ld(t):
+        return t.stride(0) if t is not None else 0
+
+    _launch("gl_linear_bwd", GlLinearBwdArgs(
+        dy.data_ptr(), _ptr(z), _ptr(slope), _ptr(x), _ptr(codes), _ptr(exps), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db),
+        _ptr(work), M, N, K, dy.stride(0), ld(z), ld(slope), ld(x), ld(codes), ld(w), ld(dx),
+        work.numel() if work is not None else 0, dt, act, int(accumulate), 0), dy.device)
+
+
+def _pdtype(*params) -> int:
+    """GL_DTYPE_* of the parameters that are given (fp32 when none is)."""
+    return next((_wdtype(p) for p in params if p is not None), DTYPE_F32)
+
+
+def norm_fwd(x, w, b, y, mean, rstd, G: int, act: int, eps: float):
+    """y = act(group_norm(x) w + b) of x [S, P, C] (GlNormArgs); mean / rstd [S, G] fp32 are written."""
+    _require_cuda(x, w, b, y, mean, rstd)
+    S, P, C = x.shape
+    dt = _wdtype(x)
+    work = _work("gl_norm_work_bytes", x.device, S, P, C, G, dt, 0)
+    _launch("gl_norm_fwd", GlNormArgs(
+        x.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(work), S, P, C, G,
+        x.stride(0), x.stride(1), work.numel() if work is not None else 0, dt,
+        _pdtype(w, b), act, eps), x.device)
+
+
+def norm_bwd(dy, x, codes, exps, w, b, mean, rstd, dx, dw, db, G: int, act: int, accumulate: bool):
+    """dx, dw, db (the last two may be None) of norm_fwd (GlNormBwdArgs)."""
+    _require_cuda(dy, x, codes, exps, w, b, mean, rstd, dx, dw, db)
+    S, P, C = dy.shape
+    dt = _wdtype(dy)
+    work = _work("gl_norm_work_bytes", dy.device, S, P, C, G, dt, 1)
+    _launch("gl_norm_bwd", GlNormBwdArgs(
+        dy.data_ptr(), _ptr(x), _ptr(codes), _ptr(exps), _ptr(w), _ptr(b), mean.data_ptr(), rstd.data_ptr(),
+        dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(work), S, P, C, G, x.stride(0) if x is not None else 0,
+        x.stride(1) if x is not None else 0, dy.stride(0), dy.stride(1),
+        codes.stride(0) if codes is not None else 0, work.numel() if work is not None else 0, dt,
+        _pdtype(w, b), act, int(accumulate)), dy.device)
+
+
+def act8_encode(x, codes, exps):
+    """int8 codes and exponent bytes of x [rows, C] (GlAct8Args)."""
+    _require_cuda(x, codes, exps)
+    _launch("gl_act8_encode", GlAct8Args(x.data_ptr(), 0, codes.data_ptr(), exps.data_ptr(), x.shape[0], x.shape[1],
+                                         x.stride(0), codes.stride(0), _wdtype(x), 0), x.device)
+
+
+def act8_decode(codes, exps, out):
+    """out [rows, C] = the values of an 8-bit checkpoint (GlAct8Args)."""
+    _require_cuda(codes, exps, out)
+    _launch("gl_act8_decode", GlAct8Args(0, out.data_ptr(), codes.data_ptr(), exps.data_ptr(), out.shape[0],
+                                         out.shape[1], out.stride(0), codes.stride(0), _wdtype(out), 0), out.device)

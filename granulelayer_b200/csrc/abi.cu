@@ -117,6 +117,7 @@ extern "C" const char* gl_status_string(int status) {
     case GL_ERR_LAUNCH: return "CUDA launch failed";
     case GL_ERR_DEVICE: return "no usable CUDA device";
     case GL_ERR_CAPACITY: return "the problem exceeds the fixed scratch of the allocation-free entry point";
+    case GL_ERR_WORKSPACE: return "the workspace is smaller than the entry point's *_work_bytes";
     default: return "unknown status";
   }
 }
@@ -148,6 +149,20 @@ extern "C" const char* gl_status_string(int status) {
   F(x) F(env) F(feat) F(buckets) F(q_off) F(rec_off) F(w) F(b) F(counts) F(pre) F(c1t) F(dx) F(dw) F(db) F(B)    \
   F(D) F(G) F(NB16) F(Q) F(S) F(nbuckets) F(ldx) F(ldp) F(ldc) F(lddx) F(act) F(tokens)
 
+#define GL_LINEAR_FIELDS(F)                                                                                      \
+  F(x) F(w) F(bias) F(residual) F(y) F(z) F(slope) F(work) F(M) F(N) F(K) F(ldx) F(ldw) F(ldr) F(ldy) F(ldz)     \
+  F(lds) F(work_bytes) F(dtype) F(act)
+#define GL_LINEAR_BWD_FIELDS(F)                                                                                  \
+  F(dy) F(z) F(slope) F(x) F(codes) F(exps) F(w) F(dx) F(dw) F(db) F(work) F(M) F(N) F(K) F(lddy) F(ldz) F(lds)  \
+  F(ldx) F(ldc) F(ldw) F(lddx) F(work_bytes) F(dtype) F(act) F(accumulate) F(reserved)
+#define GL_NORM_FIELDS(F)                                                                                        \
+  F(x) F(w) F(b) F(y) F(mean) F(rstd) F(work) F(S) F(P) F(C) F(G) F(sx) F(px) F(work_bytes) F(dtype) F(pdtype)   \
+  F(act) F(eps)
+#define GL_NORM_BWD_FIELDS(F)                                                                                    \
+  F(dy) F(x) F(codes) F(exps) F(w) F(b) F(mean) F(rstd) F(dx) F(dw) F(db) F(work) F(S) F(P) F(C) F(G) F(sx)      \
+  F(px) F(sdy) F(pdy) F(ldc) F(work_bytes) F(dtype) F(pdtype) F(act) F(accumulate)
+#define GL_ACT8_FIELDS(F) F(x) F(out) F(codes) F(exps) F(rows) F(C) F(ldx) F(ldc) F(dtype) F(reserved)
+
 #define GL_NAME(f) #f ","
 
 namespace {
@@ -172,6 +187,11 @@ int write_layout(const int64_t* off, int nf, int64_t* out, int n) {
 #define GL_OFF_GlSetArgs(f) (int64_t) offsetof(GlSetArgs, f),
 #define GL_OFF_GlEventArgs(f) (int64_t) offsetof(GlEventArgs, f),
 #define GL_OFF_GlK16Args(f) (int64_t) offsetof(GlK16Args, f),
+#define GL_OFF_GlLinearArgs(f) (int64_t) offsetof(GlLinearArgs, f),
+#define GL_OFF_GlLinearBwdArgs(f) (int64_t) offsetof(GlLinearBwdArgs, f),
+#define GL_OFF_GlNormArgs(f) (int64_t) offsetof(GlNormArgs, f),
+#define GL_OFF_GlNormBwdArgs(f) (int64_t) offsetof(GlNormBwdArgs, f),
+#define GL_OFF_GlAct8Args(f) (int64_t) offsetof(GlAct8Args, f),
 
 }  // namespace
 
@@ -184,6 +204,11 @@ extern "C" int gl_struct_layout(int which, int64_t* out, int n) {
     GL_LAYOUT_CASE(4, GlSetArgs, GL_SET_FIELDS)
     GL_LAYOUT_CASE(5, GlEventArgs, GL_EVENT_FIELDS)
     GL_LAYOUT_CASE(6, GlK16Args, GL_K16_FIELDS)
+    GL_LAYOUT_CASE(7, GlLinearArgs, GL_LINEAR_FIELDS)
+    GL_LAYOUT_CASE(8, GlLinearBwdArgs, GL_LINEAR_BWD_FIELDS)
+    GL_LAYOUT_CASE(9, GlNormArgs, GL_NORM_FIELDS)
+    GL_LAYOUT_CASE(10, GlNormBwdArgs, GL_NORM_BWD_FIELDS)
+    GL_LAYOUT_CASE(11, GlAct8Args, GL_ACT8_FIELDS)
     default: return GL_ERR_UNSUPPORTED;
   }
 }
@@ -197,6 +222,11 @@ extern "C" const char* gl_struct_fields(int which) {
     case 4: return GL_SET_FIELDS(GL_NAME);
     case 5: return GL_EVENT_FIELDS(GL_NAME);
     case 6: return GL_K16_FIELDS(GL_NAME);
+    case 7: return GL_LINEAR_FIELDS(GL_NAME);
+    case 8: return GL_LINEAR_BWD_FIELDS(GL_NAME);
+    case 9: return GL_NORM_FIELDS(GL_NAME);
+    case 10: return GL_NORM_BWD_FIELDS(GL_NAME);
+    case 11: return GL_ACT8_FIELDS(GL_NAME);
     default: return nullptr;
   }
 }

@@ -1,0 +1,445 @@
+// Matrix product with bias, activation and residual, forward and backward (no counterpart in the reference).
+//   z = x w^T + bias, y = act(z) + residual
+//   dz = dy act'(z), dx = dz w, dw = dz^T x, db = sum over rows of dz
+//
+// The products run on the tensor cores (mma.cu).  bf16 operands whose rows are 16-byte aligned are read where they
+// lie; others are first copied to aligned rows, and fp32 operands are split into three bf16 planes
+// (v = v1 + v2 + v3, 24 significand bits for 2^-110 <= |v| below bf16's largest value; an infinity gives NaN).
+// An 8-bit checkpoint of x is one plane even for fp32 layers: its values are bf16 numbers.  A few rows (serving
+// single tokens) run row kernels instead, which read w once and are bound by HBM.
+//
+// dz is written once, rounded to bf16 in bf16 layers and split in fp32 ones, with the column sums of its fp32
+// values; where dy itself is dz (identity, bf16, aligned) only the sums are taken.
+#include "mma.cuh"
+
+namespace gl {
+
+// ---- operands for the tensor cores ----
+
+// v as NP bf16 terms.  A NaN or an infinity stays in the first term (and its remainder is NaN).
+template <int NP>
+__device__ __forceinline__ void bf16_terms(const float (&v)[8], uint4 (&out)[NP]) {
+  float r[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r[i] = v[i];
+#pragma unroll
+  for (int j = 0; j < NP; ++j) {
+    uint32_t u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      u[i] = pack_bf16(r[2 * i], r[2 * i + 1]);
+      r[2 * i] -= __uint_as_float(u[i] << 16);
+      r[2 * i + 1] -= __uint_as_float(u[i] & 0xFFFF0000u);
+    }
+    out[j] = make_uint4(u[0], u[1], u[2], u[3]);
+  }
+}
+
+// 8 elements from p on, `left` of them inside the row (others 0).
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int64_t left, bool aligned, float (&v)[8]) {
+  if (aligned && left >= 8) {
+    if constexpr (sizeof(T) == 2) {
+      load_vec<T, 8>(p, v);
+    } else {
+      float a[4], b[4];
+      load_vec<T, 4>(p, a);
+      load_vec<T, 4>(p + 4, b);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        v[i] = a[i];
+        v[4 + i] = b[i];
+      }
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = i < left ? to_f32<T>(p[i]) : 0.f;
+  }
+}
+
+// rows x K (row stride ld) -> planes [NP][rows][Kp], Kp = K rounded up to 8.
+template <typename T, int NP>
+__global__ void __launch_bounds__(256) lin_pack_kernel(const T* src, uint16_t* dst, int64_t rows, int64_t K,
+                                                       int64_t ld, int aligned) {
+  const int64_t nk = (K + 7) / 8, total = rows * nk, plane = total * 8;
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
+    const int64_t r = i / nk, k = (i - r * nk) * 8;
+    float v[8];
+    load8<T>(src + r * ld + k, K - k, aligned, v);
+    uint4 u[NP];
+    bf16_terms<NP>(v, u);
+#pragma unroll
+    for (int j = 0; j < NP; ++j) *reinterpret_cast<uint4*>(dst + j * plane + i * 8) = u[j];
+  }
+}
+
+constexpr int kDzRows = 64;   // rows of one block of the dz kernel, and of one partial column sum
+
+// dz planes [NP][M][Np] (where `dz` is given) and the column sums of each block of kDzRows rows.  A warp spans 256
+// columns, eight per lane; the block's eight warps take every eighth row.
+template <typename T, int NP>
+__global__ void __launch_bounds__(256) lin_dz_kernel(const T* dy, const T* z, const uint8_t* slope, uint16_t* dz,
+                                                     float* part, int64_t M, int64_t N, int64_t lddy, int64_t ldz,
+                                                     int64_t lds, int act, int aligned) {
+  __shared__ float red[8][256 + 8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t segs = (N + 255) / 256, Np = (N + 7) / 8 * 8, plane = M * Np;
+  const int64_t rc = blockIdx.x / segs, n = (blockIdx.x - rc * segs) * 256 + lane * 8, left = N - n;
+  float sum[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+  if (left > 0) {
+    const int64_t m1 = min(M, (rc + 1) * kDzRows);
+#pragma unroll 2
+    for (int64_t m = rc * kDzRows + warp; m < m1; m += 8) {
+      float d[8];
+      load8<T>(dy + m * lddy + n, left, aligned, d);
+      if (slope) {
+        const uint8_t* q = slope + m * lds + n;
+        if (aligned && left >= 8) {
+          const uint2 u = *reinterpret_cast<const uint2*>(q);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) d[i] *= slope_value(((i < 4 ? u.x : u.y) >> (8 * (i % 4))) & 0xFF);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i < left) d[i] *= slope_value(q[i]);
+        }
+      } else if (z) {
+        float zz[8];
+        load8<T>(z + m * ldz + n, left, aligned, zz);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] *= dense_slope(act, zz[i]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += d[i];
+      if (dz) {
+        uint4 u[NP];
+        bf16_terms<NP>(d, u);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) *reinterpret_cast<uint4*>(dz + j * plane + m * Np + n) = u[j];
+      }
+    }
+  }
+  if (part == nullptr) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) red[warp][lane + 33 * i] = sum[i];
+  __syncthreads();
+  const int c = threadIdx.x, src = c / 8 + 33 * (c % 8);   // column c of the block's 256
+  const int64_t col = n - lane * 8 + c;
+  if (col < N) {
+    float s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s += red[r][src];
+    part[rc * N + col] = s;
+  }
+}
+
+// db = the partial column sums in block order; 32 columns per block, 8 row lanes.
+__global__ void __launch_bounds__(256) lin_db_kernel(const float* part, int64_t rows, int64_t N, void* db, int dtype,
+                                                     int accumulate) {
+  __shared__ float red[8][33];
+  const int lane = threadIdx.x & 31, r0 = threadIdx.x >> 5;
+  const int64_t n = (int64_t)blockIdx.x * 32 + lane;
+  float s = 0.f;
+  if (n < N) {
+#pragma unroll 4
+    for (int64_t r = r0; r < rows; r += 8) s += part[r * N + n];
+  }
+  red[r0][lane] = s;
+  __syncthreads();
+  if (r0 == 0 && n < N) {
+    s = 0.f;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) s += red[r][lane];
+    if (accumulate) reinterpret_cast<float*>(db)[n] += s;
+    else st_dense(db, n, dtype, s);
+  }
+}
+
+// ---- a few rows ----
+
+// One warp per output column n: the warp streams w's row n, four 16-byte loads in flight, against MT rows of x (from
+// L1), fp32 sums, one shuffle reduction.  Bound by reading w.
+template <typename T, int MT, bool ALIGNED>
+__global__ void __launch_bounds__(128) lin_rows_kernel(const T* x, const T* w, int M, int64_t N, int64_t K,
+                                                       int64_t ldx, int64_t ldw, LinEpilogue e) {
+  constexpr int V = ALIGNED ? kVec16<T> : 1, U = 4;
+  const int lane = threadIdx.x & 31;
+  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
+  if (n >= N) return;
+  const T* row = w + n * ldw;
+  float acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = 0.f;
+  int64_t k = lane * V;
+  for (; k + (U - 1) * 32 * V + V <= K; k += U * 32 * V) {
+    float wv[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u) load_vec<T, V>(row + k + u * 32 * V, wv[u]);
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) {
+        if (t < M) {
+          float xv[V];
+          load_vec<T, V>(x + t * ldx + k + u * 32 * V, xv);
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[t] = fmaf(xv[i], wv[u][i], acc[t]);
+        }
+      }
+  }
+  for (; k < K; k += 32 * V) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      if (k + i < K) {
+        const float wv = to_f32<T>(row[k + i]);
+#pragma unroll
+        for (int t = 0; t < MT; ++t)
+          if (t < M) acc[t] = fmaf(to_f32<T>(x[t * ldx + k + i]), wv, acc[t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t)
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) acc[t] += __shfl_xor_sync(kFullMask, acc[t], o);
+  float z = acc[0];
+#pragma unroll
+  for (int t = 1; t < MT; ++t)
+    if (lane == t) z = acc[t];
+  if (lane < M) lin_finish(e, lane, n, z);
+}
+
+// Rows up to which the row kernels run: beyond, w's fp32 splitting or the tensor cores' fixed cost is paid back.
+constexpr int kRowsBf16 = 4, kRowsF32 = 8;
+
+template <typename T, int MT>
+static void launch_rows(const GlLinearArgs& a, const LinEpilogue& e, bool aligned, cudaStream_t st) {
+  const unsigned blocks = (unsigned)((a.N + 3) / 4);
+  if (aligned)
+    lin_rows_kernel<T, MT, true><<<blocks, 128, 0, st>>>((const T*)a.x, (const T*)a.w, (int)a.M, a.N, a.K, a.ldx,
+                                                         a.ldw, e);
+  else
+    lin_rows_kernel<T, MT, false><<<blocks, 128, 0, st>>>((const T*)a.x, (const T*)a.w, (int)a.M, a.N, a.K, a.ldx,
+                                                          a.ldw, e);
+}
+
+template <typename T>
+static int run_rows(const GlLinearArgs& a, const LinEpilogue& e, bool aligned, cudaStream_t st) {
+  if (a.M == 1) launch_rows<T, 1>(a, e, aligned, st);
+  else if (a.M == 2) launch_rows<T, 2>(a, e, aligned, st);
+  else if (a.M <= 4) launch_rows<T, 4>(a, e, aligned, st);
+  else launch_rows<T, 8>(a, e, aligned, st);
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return set_cuda_error(err);
+  count_launches(1);
+  return GL_OK;
+}
+
+// ---- host ----
+
+static bool rows16(const void* p, int64_t ld, int esize) {
+  return ((uintptr_t)p & 15) == 0 && (ld * esize) % 16 == 0;
+}
+static int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+static int lin_checks(int64_t M, int64_t N, int64_t K, int dtype, int act) {
+  if (M < 0 || N < 1 || K < 1) return GL_ERR_SHAPE;
+  if ((dtype != GL_DTYPE_F32 && dtype != GL_DTYPE_BF16) || act < GL_ACT_IDENTITY || act > GL_ACT_SILU)
+    return GL_ERR_UNSUPPORTED;
+  return GL_OK;
+}
+
+// Byte offsets of the workspace's parts (each 256-byte aligned) and its size.
+struct LinWork {
+  int64_t part = 0, dz = 0, x = 0, w = 0, split = 0, total = 0;
+  int64_t take(int64_t bytes) {
+    const int64_t at = total;
+    total += up(bytes, 256);
+    return at;
+  }
+};
+
+static bool few_rows(int64_t M, int dtype) { return M <= (dtype == GL_DTYPE_F32 ? kRowsF32 : kRowsBf16); }
+
+static LinWork lin_fwd_work(int64_t M, int64_t N, int64_t K, int dtype, bool unaligned, int sms) {
+  LinWork w;
+  if (M == 0 || few_rows(M, dtype)) return w;
+  const int np = dtype == GL_DTYPE_F32 ? 3 : 1;
+  if (np == 3 || unaligned) {
+    w.x = w.take(np * M * up(K, 8) * 2);
+    w.w = w.take(np * N * up(K, 8) * 2);
+  }
+  w.split = w.take(mma_work_bytes(M, N, K, np, np, sms));
+  return w;
+}
+
+static LinWork lin_bwd_work(int64_t M, int64_t N, int64_t K, int dtype, bool codes, bool unaligned, int sms) {
+  LinWork w;
+  if (M == 0) return w;
+  const int np = dtype == GL_DTYPE_F32 ? 3 : 1, npx = codes ? 1 : np;
+  w.part = w.take(up(M, kDzRows) / kDzRows * N * 4);
+  w.dz = w.take(np * M * up(N, 8) * 2);
+  if (np == 3 || unaligned) w.w = w.take(np * N * up(K, 8) * 2);
+  if (np == 3 || unaligned || codes) w.x = w.take(npx * M * up(K, 8) * 2);
+  const int64_t s1 = mma_work_bytes(M, K, N, np, np, sms), s2 = mma_work_bytes(N, K, M, np, npx, sms);
+  w.split = w.take(s1 > s2 ? s1 : s2);
+  return w;
+}
+
+// `src` [rows, K] as an operand of the tensor cores: itself where it is aligned bf16, else packed into `dst`.
+template <typename T>
+static int make_operand(MmaOperand* o, const void* src, int64_t rows, int64_t K, int64_t ld, int mn, void* dst,
+                        int sms, cudaStream_t st) {
+  const bool aligned = rows16(src, ld, sizeof(T));
+  if (sizeof(T) == 2 && aligned) {
+    *o = MmaOperand{src, ld, 0, 1, mn};
+    return GL_OK;
+  }
+  constexpr int NP = sizeof(T) == 4 ? 3 : 1;
+  const int64_t total = rows * ((K + 7) / 8), need = (total + 255) / 256, cap = 16ll * sms;
+  lin_pack_kernel<T, NP><<<(unsigned)(need < cap ? need : cap), 256, 0, st>>>((const T*)src, (uint16_t*)dst, rows, K,
+                                                                           ld, aligned);
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return set_cuda_error(err);
+  count_launches(1);
+  *o = MmaOperand{dst, up(K, 8), rows * up(K, 8), NP, mn};
+  return GL_OK;
+}
+
+template <typename T>
+static int run_linear_fwd(const GlLinearArgs& a, const LinEpilogue& e, const LinWork& w, int sms, cudaStream_t st) {
+  char* work = (char*)a.work;
+  MmaOperand x, wt;
+  if (int rc = make_operand<T>(&x, a.x, a.M, a.K, a.ldx, 0, work + w.x, sms, st)) return rc;
+  if (int rc = make_operand<T>(&wt, a.w, a.N, a.K, a.ldw, 0, work + w.w, sms, st)) return rc;
+  return mma_product(x, wt, a.M, a.N, a.K, e, work + w.split, st);
+}
+
+template <typename T>
+static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, cudaStream_t st) {
+  constexpr int NP = sizeof(T) == 4 ? 3 : 1;
+  char* work = (char*)a.work;
+  const bool aligned = rows16(a.dy, a.lddy, sizeof(T)) && (!a.z || rows16(a.z, a.ldz, sizeof(T))) &&
+                       (!a.slope || (((uintptr_t)a.slope & 7) == 0 && a.lds % 8 == 0));
+  const bool dy_is_dz = NP == 1 && aligned && !a.z && !a.slope;
+  const bool write = !dy_is_dz && (a.dx || a.dw);
+  MmaOperand dz{a.dy, a.lddy, 0, 1, 0};
+  if (!dy_is_dz) dz = MmaOperand{work + w.dz, up(a.N, 8), a.M * up(a.N, 8), NP, 0};
+  int launches = 0;
+  if (write || a.db) {
+    const int64_t rc = up(a.M, kDzRows) / kDzRows, segs = (a.N + 255) / 256;
+    if (rc * segs > 0x7FFFFFFF) return GL_ERR_SHAPE;
+    float* part = a.db ? (float*)(work + w.part) : nullptr;
+    lin_dz_kernel<T, NP><<<(unsigned)(rc * segs), 256, 0, st>>>(
+        (const T*)a.dy, (const T*)a.z, a.slope, write ? (uint16_t*)(work + w.dz) : nullptr, part, a.M, a.N, a.lddy,
+        a.ldz, a.lds, a.act, aligned);
+    ++launches;
+    if (a.db) {
+      lin_db_kernel<<<(unsigned)((a.N + 31) / 32), 256, 0, st>>>(part, rc, a.N, a.db, a.dtype, a.accumulate);
+      ++launches;
+    }
+  }
+  LinEpilogue e{};
+  e.dtype = a.dtype;
+  if (a.dx) {   // [M, K] = dz [M, N] w [N, K]: w with its K columns as rows
+    MmaOperand wt;
+    if (int rc = make_operand<T>(&wt, a.w, a.N, a.K, a.ldw, 1, work + w.w, sms, st)) return rc;
+    e.out = a.dx;
+    e.ldo = a.lddx;
+    if (int rc = mma_product(dz, wt, a.M, a.K, a.N, e, work + w.split, st)) return rc;
+  }
+  if (a.dw) {   // [N, K] = dz^T [N, M] x [M, K]
+    MmaOperand x;
+    if (a.codes) {
+      GlAct8Args d{};
+      d.out = work + w.x;
+      d.codes = const_cast<int8_t*>(a.codes);
+      d.exps = const_cast<uint8_t*>(a.exps);
+      d.rows = a.M; d.C = a.K; d.ldx = up(a.K, 8); d.ldc = a.ldc; d.dtype = GL_DTYPE_BF16;
+      if (int rc = gl_act8_decode(&d, st)) return rc;
+      x = MmaOperand{work + w.x, up(a.K, 8), 0, 1, 1};
+    } else if (int rc = make_operand<T>(&x, a.x, a.M, a.K, a.ldx, 1, work + w.x, sms, st)) {
+      return rc;
+    }
+    dz.mn = 1;
+    e.out = a.dw;
+    e.ldo = a.K;
+    e.accumulate = a.accumulate;
+    if (int rc = mma_product(dz, x, a.N, a.K, a.M, e, work + w.split, st)) return rc;
+  }
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return set_cuda_error(err);
+  count_launches(launches);
+  return GL_OK;
+}
+
+}  // namespace gl
+
+using namespace gl;
+
+extern "C" int64_t gl_linear_work_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t flags) {
+  if (int rc = lin_checks(M, N, K, dtype, 0)) return rc;
+  int sms = 0;
+  if (int rc = device_sm_count(&sms)) return rc;
+  const bool unaligned = (flags & GL_LINEAR_UNALIGNED) != 0;
+  if (flags & GL_LINEAR_BACKWARD) return lin_bwd_work(M, N, K, dtype, (flags & GL_LINEAR_CODES) != 0, unaligned, sms).total;
+  return lin_fwd_work(M, N, K, dtype, unaligned, sms).total;
+}
+
+extern "C" int gl_linear_fwd(const GlLinearArgs* args, void* stream) {
+  if (!args) return GL_ERR_NULL;
+  const GlLinearArgs& a = *args;
+  if (int rc = lin_checks(a.M, a.N, a.K, a.dtype, a.act)) return rc;
+  if (a.ldx < a.K || a.ldw < a.K || a.ldy < a.N || (a.residual && a.ldr < a.N) || (a.z && a.ldz < a.N) ||
+      (a.slope && a.lds < a.N))
+    return GL_ERR_SHAPE;
+  if (a.M == 0) return GL_OK;
+  if (!a.x || !a.w || !a.y) return GL_ERR_NULL;
+  const int es = a.dtype == GL_DTYPE_F32 ? 4 : 2;
+  const LinEpilogue e{a.bias, a.residual, a.y, a.z, a.slope, a.ldr, a.ldy, a.ldz, a.lds, a.dtype, a.act, 0};
+  const bool aligned = rows16(a.x, a.ldx, es) && rows16(a.w, a.ldw, es);
+  cudaStream_t st = (cudaStream_t)stream;
+  if (few_rows(a.M, a.dtype))
+    return a.dtype == GL_DTYPE_F32 ? run_rows<float>(a, e, aligned, st) : run_rows<__nv_bfloat16>(a, e, aligned, st);
+  int sms = 0;
+  if (int rc = device_sm_count(&sms)) return rc;
+  const LinWork w = lin_fwd_work(a.M, a.N, a.K, a.dtype, !aligned, sms);
+  if (w.total > 0 && (!a.work || a.work_bytes < w.total)) return GL_ERR_WORKSPACE;
+  if ((uintptr_t)a.work & 255) return GL_ERR_ALIGN;
+  return a.dtype == GL_DTYPE_F32 ? run_linear_fwd<float>(a, e, w, sms, st)
+                                 : run_linear_fwd<__nv_bfloat16>(a, e, w, sms, st);
+}
+
+extern "C" int gl_linear_bwd(const GlLinearBwdArgs* args, void* stream) {
+  if (!args) return GL_ERR_NULL;
+  const GlLinearBwdArgs& a = *args;
+  if (int rc = lin_checks(a.M, a.N, a.K, a.dtype, a.act)) return rc;
+  const bool codes = a.codes != nullptr;
+  if (a.lddy < a.N || (a.z && a.ldz < a.N) || (a.slope && a.lds < a.N) || (a.dw && !codes && a.ldx < a.K) ||
+      (codes && (a.ldc < up(a.K, kActBlock) || a.ldc % kActBlock)) || (a.dx && (a.ldw < a.K || a.lddx < a.K)))
+    return GL_ERR_SHAPE;
+  cudaStream_t st = (cudaStream_t)stream;
+  if (a.M == 0) {   // an empty batch: zero gradients (nothing is added to accumulated ones)
+    if (a.accumulate) return GL_OK;
+    const size_t es = a.dtype == GL_DTYPE_F32 ? 4 : 2;
+    cudaError_t e = cudaSuccess;
+    if (a.dw) e = cudaMemsetAsync(a.dw, 0, (size_t)(a.N * a.K) * es, st);
+    if (e == cudaSuccess && a.db) e = cudaMemsetAsync(a.db, 0, (size_t)a.N * es, st);
+    return e == cudaSuccess ? GL_OK : set_cuda_error(e);
+  }
+  if (!a.dx && !a.dw && !a.db) return GL_OK;
+  if (!a.dy || (a.act != GL_ACT_IDENTITY && !a.z && !a.slope) || (a.dx && !a.w) ||
+      (a.dw && !codes && !a.x) || (codes && !a.exps))
+    return GL_ERR_NULL;
+  if (codes && ((uintptr_t)a.codes & 15)) return GL_ERR_ALIGN;
+  const int es = a.dtype == GL_DTYPE_F32 ? 4 : 2;
+  const bool aligned = (!a.dx || rows16(a.w, a.ldw, es)) && (!a.dw || codes || rows16(a.x, a.ldx, es));
+  int sms = 0;
+  if (int rc = device_sm_count(&sms)) return rc;
+  const LinWork w = lin_bwd_work(a.M, a.N, a.K, a.dtype, codes, !aligned, sms);
+  if (w.total > 0 && (!a.work || a.work_bytes < w.total)) return GL_ERR_WORKSPACE;
+  if ((uintptr_t)a.work & 255) return GL_ERR_ALIGN;
+  return a.dtype == GL_DTYPE_F32 ? run_linear_bwd<float>(a, w, sms, st) : run_linear_bwd<__nv_bfloat16>(a, w, sms, st);
+}

@@ -1,0 +1,366 @@
+"""Dense operators around sparse-pooling layers (no counterpart in the reference).
+
+``linear_act``          y = act(x W^T + b) + residual, forward and backward;
+``group_norm_act``      channels-last group norm with an affine map and an activation, forward and backward;
+``encode_activation`` / ``decode_activation``   an activation in 8 bits and back;
+``LinearAct`` / ``GroupNormAct``                the first two as modules, with the framework's ``main_grad``.
+
+``checkpoint="int8"`` makes the first two keep what their backward pass reads in 8 bits: the input as int8 codes
+with one power-of-two scale per 32 channels (1.03 bytes per element), and ``linear_act`` the activation's
+derivative as one byte (multiples of 1/192, exact at 0 and 1).  The forward result does not change; the gradients
+are those of the read-back input.
+
+Storage is float32 or bfloat16; sums and statistics are float32.  The kernels run in the in-tree sm_100a library on
+the current CUDA stream; there is no CPU path (``NativeLibraryError``) and nothing falls back to PyTorch math.
+"""
+from __future__ import annotations
+
+from dataclasses import dataclass
+from typing import Optional, Tuple
+
+import torch
+from torch import nn
+from torch.autograd.function import once_differentiable
+
+from . import _native
+
+BLOCK = 32        # channels that share an exponent in an 8-bit checkpoint
+CHECKPOINTS = ("none", "int8")
+_DTYPES = (torch.float32, torch.bfloat16)
+
+
+def _act_id(activation: str) -> int:
+    try:
+        return _native.DENSE_ACT_IDS[activation]
+    except KeyError:
+        raise ValueError(f"activation must be one of {tuple(_native.DENSE_ACT_IDS)}, not {activation!r}") from None
+
+
+def _check_checkpoint(checkpoint: str):
+    if checkpoint not in CHECKPOINTS:
+        raise ValueError(f"checkpoint must be one of {CHECKPOINTS}, not {checkpoint!r}")
+
+
+def _check_tensors(name: str, dtype: torch.dtype, **tensors):
+    """One supported dtype and one device for all tensors that are given."""
+    if dtype not in _DTYPES:
+        raise ValueError(f"{name}: float32 or bfloat16 tensors, not {dtype}")
+    dev = None
+    for k, t in tensors.items():
+        if t is None:
+            continue
+        if t.dtype != dtype:
+            raise ValueError(f"{name}: {k} is {t.dtype}, the input {dtype}")
+        if dev is None:
+            dev = t.device
+        elif t.device != dev:
+            raise ValueError(f"{name}: {k} is on {t.device}, the input on {dev}")
+
+
+def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
+    """``t`` [..., width] as [rows, width] with unit column stride and rows that do not overlap (a copy where the
+    strides allow no such view)."""
+    t2 = t if t.dim() == 2 else t.reshape(-1, width)
+    if (width > 1 and t2.stride(1) != 1) or t2.stride(0) < width:
+        t2 = t2.contiguous()
+        if t2.stride(0) < width or (width > 1 and t2.stride(1) != 1):   # one row or column: any stride is "contiguous"
+            t2 = t2.as_strided(t2.shape, (width, 1))
+    return t2
+
+
+# ---- 8-bit checkpoints ----
+
+@dataclass(frozen=True)
+class Activation8:
+    """An activation [..., C] in 8 bits: ``codes`` [rows, C rounded up to 32] int8, ``exponents`` [rows,
+    ceil(C / 32)] uint8, and the shape and dtype it had.  A value is code * 2^(exponent - 127); a block that held a
+    NaN or an infinity has exponent 255 and reads back as NaN."""
+    codes: torch.Tensor
+    exponents: torch.Tensor
+    shape: Tuple[int, ...]
+    dtype: torch.dtype
+
+    def nbytes(self) -> int:
+        return self.codes.numel() + self.exponents.numel()
+
+
+def _encode(x2: torch.Tensor):
+    rows, C = x2.shape
+    nblk = -(-C // BLOCK)
+    codes = torch.empty((rows, nblk * BLOCK), dtype=torch.int8, device=x2.device)
+    exps = torch.empty((rows, nblk), dtype=torch.uint8, device=x2.device)
+    if rows:
+        _native.act8_encode(x2, codes, exps)
+    return codes, exps
+
+
+def encode_activation(x: torch.Tensor) -> Activation8:
+    """``x`` [..., C] (float32 or bfloat16) in 8 bits."""
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"encode_activation: x needs at least one channel, got shape {tuple(x.shape)}")
+    _check_tensors("encode_activation", x.dtype, x=x)
+    _native._require_cuda(x)
+    codes, exps = _encode(_rows(x.detach(), x.shape[-1]))
+    return Activation8(codes, exps, tuple(x.shape), x.dtype)
+
+
+def decode_activation(a: Activation8, dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """The values of ``a`` in ``dtype`` (default: what it was); exact in both float32 and bfloat16."""
+    dtype = dtype or a.dtype
+    if dtype not in _DTYPES:
+        raise ValueError(f"decode_activation: float32 or bfloat16, not {dtype}")
+    out = torch.empty(a.shape, dtype=dtype, device=a.codes.device)
+    if out.numel():
+        _native.act8_decode(a.codes, a.exponents, out.view(-1, a.shape[-1]))
+    else:
+        _native._require_cuda(a.codes)
+    return out
+
+
+# ---- gradients of parameters ----
+
+def _grad_buffers(*params):
+    """(buffers, accumulate): per (parameter, wanted) the buffer its gradient goes to.  With a ``main_grad`` among
+    them all are fp32 and added to (fresh zeros where a parameter has none), as SparsePoolingLayer's are."""
+    main = any(want and getattr(p, "main_grad", None) is not None for p, want in params if p is not None)
+    out = []
+    for p, want in params:
+        if p is None or not want:
+            out.append(None)
+        elif not main:
+            out.append(torch.empty(p.shape, dtype=p.dtype, device=p.device))
+        else:
+            g = getattr(p, "main_grad", None)
+            if g is not None and (g.dtype != torch.float32 or not g.is_contiguous() or g.shape != p.shape):
+                raise ValueError("main_grad must be a contiguous float32 tensor of the parameter's shape")
+            out.append(g if g is not None else torch.zeros(p.shape, dtype=torch.float32, device=p.device))
+    return out, main
+
+
+def _returned(p, buf):
+    """What autograd gets for a parameter: None for ``main_grad``, else the buffer in the parameter's dtype."""
+    if buf is None or getattr(p, "main_grad", None) is not None:
+        return None
+    return buf if buf.dtype == p.dtype else buf.to(p.dtype)
+
+
+# ---- linear ----
+
+def _linear_forward(x2, weight, bias, r2, act, z, slope):
+    y = torch.empty((x2.shape[0], weight.shape[0]), dtype=x2.dtype, device=x2.device)
+    if x2.shape[0]:
+        _native.linear_fwd(x2, weight, bias, r2, y, z, slope, act)
+    return y
+
+
+class LinearActFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, residual, act, checkpoint):
+        M, K, N = x.numel() // x.shape[-1], x.shape[-1], weight.shape[0]
+        x2, w2 = _rows(x, K), _rows(weight, K)
+        r2 = None if residual is None else _rows(residual, N)
+        z = slope = codes = exps = None
+        if act != 0:
+            if checkpoint == "int8":
+                slope = torch.empty((M, N), dtype=torch.uint8, device=x.device)
+            else:
+                z = torch.empty((M, N), dtype=x.dtype, device=x.device)
+        y = _linear_forward(x2, w2, bias, r2, act, z, slope)
+        if checkpoint == "int8":
+            codes, exps = _encode(x2)
+        ctx.save_for_backward(x2 if codes is None else None, codes, exps, weight, bias, z, slope)
+        ctx.act, ctx.xshape = act, x.shape
+        return y.view(*x.shape[:-1], N)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x2, codes, exps, weight, bias, z, slope = ctx.saved_tensors
+        need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
+        N, K = weight.shape
+        dx = torch.empty(ctx.xshape, dtype=dy.dtype, device=dy.device) if need_x else None
+        (dw, db), main = _grad_buffers((weight, need_w), (bias, need_b))
+        if need_x or need_w or need_b:
+            w2 = _rows(weight, K) if need_x else None
+            _native.linear_bwd(_rows(dy, N), z, slope, x2, codes, exps, w2, dx.view(-1, K) if need_x else None, dw, db,
+                               K, ctx.act, main)
+        return dx, _returned(weight, dw), _returned(bias, db), dy if need_r else None, None, None
+
+
+def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
+               residual: Optional[torch.Tensor] = None, activation: str = "identity",
+               checkpoint: str = "none") -> torch.Tensor:
+    """act(x W^T + bias) + residual for x [..., K], weight [N, K], bias [N], residual [..., N].
+
+    ``activation``: "identity", "relu", "gelu" (erf form) or "silu".  ``checkpoint="int8"`` keeps the input and the
+    activation's derivative in 8 bits for the backward pass.  All tensors share one dtype (float32 or bfloat16;
+    float32 products run as exact three-term bf16 splits on the tensor cores or in fp32).  Parameters with a
+    ``main_grad`` receive their gradients there."""
+    act = _act_id(activation)
+    _check_checkpoint(checkpoint)
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"linear_act: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    N = weight.shape[0]
+    if bias is not None and (bias.shape != (N,) or (N > 1 and bias.stride(0) != 1)):
+        raise ValueError(f"linear_act: bias must be a contiguous [{N}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != x.shape[:-1] + (N,):
+        raise ValueError(f"linear_act: residual {tuple(residual.shape)} must have the output's shape "
+                         f"{tuple(x.shape[:-1]) + (N,)}")
+    _check_tensors("linear_act", x.dtype, x=x, weight=weight, bias=bias, residual=residual)
+    _native._require_cuda(x)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        return LinearActFunction.apply(x, weight, bias, residual, act, checkpoint)
+    K = x.shape[-1]
+    y = _linear_forward(_rows(x, K), _rows(weight, K), bias, None if residual is None else _rows(residual, N), act,
+                        None, None)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+
+
+# ---- group norm ----
+
+def _positions(t: torch.Tensor, S: int, P: int, C: int) -> torch.Tensor:
+    """``t`` [S, ..., C] as [S, P, C] with unit channel stride and positions that do not overlap."""
+    t3 = t.reshape(S, P, C)
+    if (C > 1 and t3.stride(2) != 1) or (P > 1 and t3.stride(1) < C) or (S > 1 and t3.stride(0) < C):
+        t3 = t3.contiguous()
+    if t3.stride(1) < C or t3.stride(0) < C or (C == 1 and t3.stride(2) != 1):   # strides of dimensions of size one
+        t3 = t3.as_strided(t3.shape, (t3.stride(0) if S > 1 else P * C, t3.stride(1) if P > 1 else C, 1))
+    return t3
+
+
+def _norm_forward(x, num_groups, weight, bias, act, eps):
+    S, C = x.shape[0], x.shape[-1]
+    P = x.numel() // (S * C) if S else 0
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean, rstd = torch.empty((2, S, num_groups), dtype=torch.float32, device=x.device).unbind(0)
+    x3 = None
+    if y.numel():
+        x3 = _positions(x, S, P, C)
+        _native.norm_fwd(x3, weight, bias, y, mean, rstd, num_groups, act, eps)
+    return y, x3, mean, rstd
+
+
+class GroupNormActFunction(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, num_groups, act, eps, checkpoint):
+        y, x3, mean, rstd = _norm_forward(x, num_groups, weight, bias, act, eps)
+        codes = exps = None
+        if checkpoint == "int8" and x3 is not None:
+            codes, exps = _encode(_rows(x3, x.shape[-1]))
+            x3 = None
+        ctx.save_for_backward(x3, codes, exps, weight, bias, mean, rstd)
+        ctx.act, ctx.groups = act, num_groups
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x3, codes, exps, weight, bias, mean, rstd = ctx.saved_tensors
+        _, need_w, need_b = ctx.needs_input_grad[:3]
+        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+        (dw, db), main = _grad_buffers((weight, need_w), (bias, need_b))
+        S, C = dy.shape[0], dy.shape[-1]
+        if dy.numel():
+            dy3 = _positions(dy, S, dy.numel() // (S * C), C)
+            _native.norm_bwd(dy3, x3, codes, exps, weight, bias, mean, rstd, dx, dw, db, ctx.groups, ctx.act, main)
+        elif not main:
+            for g in (dw, db):
+                if g is not None:
+                    g.zero_()
+        return dx, _returned(weight, dw), _returned(bias, db), None, None, None, None
+
+
+def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
+                   bias: Optional[torch.Tensor] = None, eps: float = 1e-5, activation: str = "identity",
+                   checkpoint: str = "none") -> torch.Tensor:
+    """act(group_norm(x) * weight + bias) over channels-last x [S, ..., C].
+
+    Statistics (mean, biased variance) run over a sample's positions and each of ``num_groups`` groups of
+    consecutive channels; with x [S, C] that is per token.  ``weight`` and ``bias`` [C] are float32 or bfloat16 (one
+    dtype for both), whatever x's.  ``activation`` and ``checkpoint`` as in ``linear_act``."""
+    act = _act_id(activation)
+    _check_checkpoint(checkpoint)
+    if x.dim() < 2 or x.shape[-1] < 1:
+        raise ValueError(f"group_norm_act: x must be [samples, ..., channels], got {tuple(x.shape)}")
+    C = x.shape[-1]
+    if num_groups < 1 or C % num_groups:
+        raise ValueError(f"group_norm_act: {C} channels do not split into {num_groups} groups")
+    if not eps > 0:
+        raise ValueError("group_norm_act: eps must be positive")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.shape != (C,) or (C > 1 and p.stride(0) != 1)):
+            raise ValueError(f"group_norm_act: {name} must be a contiguous [{C}], got {tuple(p.shape)}")
+        if p is not None and p.device != x.device:
+            raise ValueError(f"group_norm_act: {name} is on {p.device}, the input on {x.device}")
+    _check_tensors("group_norm_act", x.dtype, x=x)
+    ps = [p for p in (weight, bias) if p is not None]
+    if ps:
+        _check_tensors("group_norm_act", ps[0].dtype, weight=weight, bias=bias)
+    _native._require_cuda(x)
+    if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in ps)):
+        return GroupNormActFunction.apply(x, weight, bias, num_groups, act, eps, checkpoint)
+    return _norm_forward(x, num_groups, weight, bias, act, eps)[0]
+
+
+# ---- modules ----
+
+class _MainGradModule(nn.Module):
+    def enable_main_grad(self):
+        """Accumulate parameter gradients into persistent FP32 ``main_grad`` buffers (autograd then returns None
+        for them), as SparsePoolingLayer.enable_main_grad."""
+        for p in self.parameters(recurse=False):
+            if getattr(p, "main_grad", None) is None:
+                p.main_grad = torch.zeros(p.shape, device=p.device, dtype=torch.float32)
+
+    def zero_main_grad(self):
+        for p in self.parameters(recurse=False):
+            if getattr(p, "main_grad", None) is not None:
+                p.main_grad.zero_()
+
+
+class LinearAct(_MainGradModule):
+    """``linear_act`` with its parameters: weight [out, in] drawn from N(0, 1 / in), bias zero."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, activation: str = "identity",
+                 checkpoint: str = "none", dtype: torch.dtype = torch.bfloat16, device=None, seed: int = 0):
+        super().__init__()
+        _act_id(activation)
+        _check_checkpoint(checkpoint)
+        if in_features < 1 or out_features < 1 or dtype not in _DTYPES:
+            raise ValueError("LinearAct: positive sizes and float32 or bfloat16 parameters")
+        self.in_features, self.out_features = in_features, out_features
+        self.activation, self.checkpoint = activation, checkpoint
+        gen = torch.Generator().manual_seed(seed)
+        w = torch.randn(out_features, in_features, generator=gen) * in_features ** -0.5
+        self.weight = nn.Parameter(w.to(device=device or "cpu", dtype=dtype))
+        self.bias = nn.Parameter(torch.zeros(out_features, device=device, dtype=dtype)) if bias else None
+
+    def forward(self, x, residual=None):
+        return linear_act(x, self.weight, self.bias, residual, self.activation, self.checkpoint)
+
+    def extra_repr(self):
+        return (f"in={self.in_features}, out={self.out_features}, bias={self.bias is not None}, "
+                f"activation={self.activation}, checkpoint={self.checkpoint}")
+
+
+class GroupNormAct(_MainGradModule):
+    """``group_norm_act`` with its parameters (ones and zeros)."""
+
+    def __init__(self, channels: int, num_groups: int, eps: float = 1e-5, activation: str = "identity",
+                 checkpoint: str = "none", affine: bool = True, dtype: torch.dtype = torch.bfloat16, device=None):
+        super().__init__()
+        _act_id(activation)
+        _check_checkpoint(checkpoint)
+        if num_groups < 1 or channels < 1 or channels % num_groups or dtype not in _DTYPES or not eps > 0:
+            raise ValueError("GroupNormAct: channels in whole groups, positive eps, float32 or bfloat16 parameters")
+        self.channels, self.num_groups, self.eps = channels, num_groups, eps
+        self.activation, self.checkpoint = activation, checkpoint
+        self.weight = nn.Parameter(torch.ones(channels, device=device, dtype=dtype)) if affine else None
+        self.bias = nn.Parameter(torch.zeros(channels, device=device, dtype=dtype)) if affine else None
+
+    def forward(self, x):
+        return group_norm_act(x, self.num_groups, self.weight, self.bias, self.eps, self.activation, self.checkpoint)
+
+    def extra_repr(self):
+        return (f"channels={self.channels}, groups={self.num_groups}, eps={self.eps}, "
+                f"activation={self.activation}, checkpoint={self.checkpoint}")

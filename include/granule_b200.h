@@ -44,7 +44,7 @@
 extern "C" {
 #endif
 
-#define GL_ABI_VERSION 17
+#define GL_ABI_VERSION 18
 
 typedef enum GlStatus {
   GL_OK = 0,
@@ -55,7 +55,8 @@ typedef enum GlStatus {
   GL_ERR_SMEM = -5,          /* the tile does not fit in shared memory */
   GL_ERR_LAUNCH = -6,        /* the CUDA launch failed (see gl_last_cuda_error) */
   GL_ERR_DEVICE = -7,        /* no usable device / attribute query failed */
-  GL_ERR_CAPACITY = -8       /* the problem is larger than an allocation-free entry point's fixed scratch */
+  GL_ERR_CAPACITY = -8,      /* the problem is larger than an allocation-free entry point's fixed scratch */
+  GL_ERR_WORKSPACE = -9      /* the workspace is smaller than the entry point's *_work_bytes */
 } GlStatus;
 
 /* Pool ids: the reference's operators (sparse_pooling/config.py:22-29) and the "sum"
@@ -82,7 +83,8 @@ typedef enum GlStatus {
                                                       c1 = gpre, c2 = L2, c3 = pre */
 enum { GL_POOL_MEAN = 0, GL_POOL_SUM = 1, GL_POOL_MAX = 2, GL_POOL_LME = 3, GL_POOL_POWER = 4, GL_POOL_SOFTMAX = 5,
        GL_POOL_TOPK = 6 };
-enum { GL_ACT_IDENTITY = 0, GL_ACT_RELU = 1, GL_ACT_GELU = 2 };
+enum { GL_ACT_IDENTITY = 0, GL_ACT_RELU = 1, GL_ACT_GELU = 2,
+       GL_ACT_SILU = 3 /* the dense operators (gl_linear_*, gl_norm_*) only */ };
 /* Storage types of parameters (the reference's default layer dtype is bfloat16); the kernels
    compute in fp32 and write fp32 gradients. */
 enum { GL_DTYPE_F32 = 0, GL_DTYPE_BF16 = 1 };
@@ -490,14 +492,124 @@ int gl_k16_fwd_t5_f32(const GlK16Args* args, int32_t* status, void* stream);
 int gl_k16_bwd_t5(const GlK16Args* args, int32_t* status, void* stream);
 int gl_k16_bwd_t5_f32(const GlK16Args* args, int32_t* status, void* stream);
 
+/* ---- dense operators: the layers between sparse-pooling layers (no counterpart in the reference) ----
+ * Storage is fp32 or bf16 (`dtype`), all arithmetic and every sum fp32.  Rows have unit element stride and
+ * the row strides given (elements).  Activations: GL_ACT_IDENTITY / RELU / GELU (erf form) / SILU.
+ * `work` is caller-owned scratch of at least the *_work_bytes of the call's sizes (negative = GlStatus); it may be
+ * NULL where that is 0.
+ * fp32 products run on the tensor cores as the six products of three-term bf16 splits (as gl_k16_fwd_tc_f32) and
+ * agree with fp32 arithmetic to its rounding; an infinity in such an operand gives NaN.  Every wait in these
+ * kernels has an iteration limit; a tile whose wait ran out is written as NaN. */
+
+/* Forward of a fused matrix product: y = act(z) + residual, z[m, n] = sum_k x[m, k] w[n, k] + bias[n].
+ * `bias` [N], `residual` [M, ldr], `z` and `slope` are optional.  For the backward pass the call also keeps
+ * `z` [M, ldz] (dtype) or `slope` [M, lds] (one byte per element: round(192 act'(z)) + 32), as given. */
+typedef struct GlLinearArgs {
+  const void* x;            /* [M, ldx] */
+  const void* w;            /* [N, ldw] */
+  const void* bias;
+  const void* residual;
+  void* y;                  /* [M, ldy] */
+  void* z;
+  uint8_t* slope;
+  void* work;
+  int64_t M, N, K, ldx, ldw, ldr, ldy, ldz, lds, work_bytes;
+  int32_t dtype, act;
+} GlLinearArgs;
+int gl_linear_fwd(const GlLinearArgs* args, void* stream);
+
+/* Backward: dz = dy act'(z) with act' from `z` or `slope` (neither: act is the identity),
+ *   dx = dz w, dw = dz^T x, db = column sums of dz, each where its output is given.
+ * x comes as it was (`x`) or as an 8-bit checkpoint (`codes` [M, ldc] and `exps` [M, ceil(K / 32)], gl_act8_*).
+ * dx [M, lddx] has the storage type; dw [N, K] and db [N] (contiguous) too, or, with `accumulate`, are fp32 and
+ * added to. */
+typedef struct GlLinearBwdArgs {
+  const void* dy;           /* [M, lddy] */
+  const void* z;
+  const uint8_t* slope;
+  const void* x;
+  const int8_t* codes;
+  const uint8_t* exps;
+  const void* w;
+  void* dx;
+  void* dw;
+  void* db;
+  void* work;
+  int64_t M, N, K, lddy, ldz, lds, ldx, ldc, ldw, lddx, work_bytes;
+  int32_t dtype, act, accumulate, reserved;
+} GlLinearBwdArgs;
+int gl_linear_bwd(const GlLinearBwdArgs* args, void* stream);
+/* `flags`: of GL_LINEAR_*; UNALIGNED where x, or w, has a base or row stride that 16 bytes do not divide (needed for
+ * bf16 only), CODES for a backward call on a checkpoint.  `work` itself is 256-byte aligned. */
+enum { GL_LINEAR_BACKWARD = 1, GL_LINEAR_CODES = 2, GL_LINEAR_UNALIGNED = 4 };
+int64_t gl_linear_work_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t flags);
+
+/* Group norm with an affine map and an activation, channels last: x [S, P, C] (sample stride sx, position
+ * stride px, unit channel stride), G groups of C / G consecutive channels, statistics over a sample's P
+ * positions and a group's channels (biased variance):
+ *   y = act((x - mean) rstd w + b), rstd = 1 / sqrt(var + eps); y [S, P, C] contiguous, w / b [C] of type
+ * `pdtype` (NULL: 1 and 0), mean / rstd [S, G] fp32 are written (the backward reads them). */
+typedef struct GlNormArgs {
+  const void* x;
+  const void* w;
+  const void* b;
+  void* y;
+  float* mean;
+  float* rstd;
+  void* work;
+  int64_t S, P, C, G, sx, px, work_bytes;
+  int32_t dtype, pdtype, act;
+  float eps;
+} GlNormArgs;
+int gl_norm_fwd(const GlNormArgs* args, void* stream);
+
+/* Backward of gl_norm_fwd: dx [S, P, C] contiguous; dw / db [C] (NULL: not wanted) of type pdtype, or, with
+ * `accumulate`, fp32 and added to.  x as it was, or an 8-bit checkpoint of its S P rows (`codes` given). */
+typedef struct GlNormBwdArgs {
+  const void* dy;           /* sample stride sdy, position stride pdy */
+  const void* x;
+  const int8_t* codes;
+  const uint8_t* exps;
+  const void* w;
+  const void* b;
+  const float* mean;
+  const float* rstd;
+  void* dx;
+  void* dw;
+  void* db;
+  void* work;
+  int64_t S, P, C, G, sx, px, sdy, pdy, ldc, work_bytes;
+  int32_t dtype, pdtype, act, accumulate;
+} GlNormBwdArgs;
+int gl_norm_bwd(const GlNormBwdArgs* args, void* stream);
+int64_t gl_norm_work_bytes(int64_t S, int64_t P, int64_t C, int64_t G, int32_t dtype, int32_t backward);
+
+/* Activation checkpoints in 8 bits: per row and 32 consecutive channels one exponent byte, x ~ code 2^(byte - 127)
+ * with the smallest such power of two (from 2^-126 on) that keeps |code| <= 127, codes rounded to nearest even
+ * (and to at most 63 at 2^122, so that a finite value reads back finite).
+ * Byte 255 marks a block that held a NaN or an infinity and reads back as NaN.  codes [rows, ldc], ldc a
+ * multiple of 32 and codes 16-byte aligned (columns past C are written as 0); exps [rows, ceil(C / 32)].
+ * encode reads x [rows, ldx]; decode writes out [rows, ldx]. */
+typedef struct GlAct8Args {
+  const void* x;
+  void* out;
+  int8_t* codes;
+  uint8_t* exps;
+  int64_t rows, C, ldx, ldc;
+  int32_t dtype, reserved;
+} GlAct8Args;
+int gl_act8_encode(const GlAct8Args* args, void* stream);
+int gl_act8_decode(const GlAct8Args* args, void* stream);
+
 /* Layout of the argument structs, for bindings that declare them field by field (replaces the
  * reference's sp_struct_layout, sparse_pooling/kernels/cuda/abi.cu:25, which its ctypes bridge checks
  * at load, backends/cuda/runtime.py:103-121).  which: 0 GlFwdArgs, 1 GlBwdArgs, 2 GlAdamArgs,
- * 3 GlSharedArgs, 4 GlSetArgs, 5 GlEventArgs, 6 GlK16Args.  gl_struct_layout writes sizeof(struct)
+ * 3 GlSharedArgs, 4 GlSetArgs, 5 GlEventArgs, 6 GlK16Args, 7 GlLinearArgs, 8 GlLinearBwdArgs, 9 GlNormArgs,
+ * 10 GlNormBwdArgs, 11 GlAct8Args.  gl_struct_layout writes sizeof(struct)
  * and then every field's offset, in declaration order, into out[0 .. n) and returns the number of
  * values (GL_ERR_SHAPE when n is too small, GL_ERR_UNSUPPORTED for an unknown id); gl_struct_fields
  * returns the field names in declaration order, each followed by a comma (NULL for an unknown id). */
-#define GL_STRUCT_COUNT 7
+#define GL_STRUCT_COUNT 12
 int gl_struct_layout(int which, int64_t* out, int n);
 const char* gl_struct_fields(int which);
 
