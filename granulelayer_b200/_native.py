@@ -121,17 +121,16 @@ class GlK16Args(ctypes.Structure):
 
 
 class GlLinearArgs(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "w", "bias", "residual", "y", "z", "slope", "work")] + \
-               [(n, ctypes.c_int64) for n in ("M", "N", "K", "ldx", "ldw", "ldr", "ldy", "ldz", "lds", "work_bytes")] + \
-               [(n, ctypes.c_int32) for n in ("dtype", "act")]
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "w", "bias", "residual", "y", "slope", "work")] + \
+               [(n, ctypes.c_int64) for n in ("M", "N", "K", "ldx", "ldw", "ldr", "ldy", "lds", "work_bytes")] + \
+               [(n, ctypes.c_int32) for n in ("dtype", "act", "slope_kind", "reserved")]
 
 
 class GlLinearBwdArgs(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("dy", "z", "slope", "x", "codes", "exps", "w", "dx", "dw", "db",
-                                                "work")] + \
-               [(n, ctypes.c_int64) for n in ("M", "N", "K", "lddy", "ldz", "lds", "ldx", "ldc", "ldw", "lddx",
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dy", "slope", "x", "codes", "exps", "w", "dx", "dw", "db", "work")] + \
+               [(n, ctypes.c_int64) for n in ("M", "N", "K", "lddy", "lds", "ldx", "ldc", "ldw", "lddx",
                                               "work_bytes")] + \
-               [(n, ctypes.c_int32) for n in ("dtype", "act", "accumulate", "reserved")]
+               [(n, ctypes.c_int32) for n in ("dtype", "slope_kind", "accumulate", "reserved")]
 
 
 class GlNormArgs(ctypes.Structure):
@@ -756,22 +755,27 @@ def _unaligned(*rows) -> int:
     return 0
 
 
-def linear_fwd(x, w, bias, residual, y, z, slope, act: int):
-    """y = act(x w^T + bias) + residual (GlLinearArgs); 2-d tensors with unit column stride."""
-    _require_cuda(x, w, bias, residual, y, z, slope)
+# GL_SLOPE_*: how linear_fwd keeps act'(z), by the storage type of `slope`
+_SLOPE_KINDS = {torch.float32: 1, torch.int16: 2, torch.uint8: 3}
+
+
+def linear_fwd(x, w, bias, residual, y, slope, act: int):
+    """y = act(x w^T + bias) + residual (GlLinearArgs); 2-d tensors with unit column stride.  ``slope`` (optional,
+    float32, int16 or uint8 [M, N]) receives act'(z)."""
+    _require_cuda(x, w, bias, residual, y, slope)
     M, K = x.shape
     N, dt = w.shape[0], _wdtype(w)
     work = _work("gl_linear_work_bytes", x.device, M, N, K, dt, _unaligned(x, w))
     _launch("gl_linear_fwd", GlLinearArgs(
-        x.data_ptr(), w.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(z), _ptr(slope), _ptr(work),
+        x.data_ptr(), w.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(slope), _ptr(work),
         M, N, K, x.stride(0), w.stride(0), residual.stride(0) if residual is not None else 0, y.stride(0),
-        z.stride(0) if z is not None else 0, slope.stride(0) if slope is not None else 0,
-        work.numel() if work is not None else 0, dt, act), x.device)
+        slope.stride(0) if slope is not None else 0, work.numel() if work is not None else 0, dt, act,
+        _SLOPE_KINDS[slope.dtype] if slope is not None else 0, 0), x.device)
 
 
-def linear_bwd(dy, z, slope, x, codes, exps, w, dx, dw, db, K: int, act: int, accumulate: bool):
+def linear_bwd(dy, slope, x, codes, exps, w, dx, dw, db, K: int, accumulate: bool):
     """dx, dw, db (each may be None) of linear_fwd for the output gradient dy (GlLinearBwdArgs)."""
-    _require_cuda(dy, z, slope, x, codes, exps, w, dx, dw, db)
+    _require_cuda(dy, slope, x, codes, exps, w, dx, dw, db)
     M, N = dy.shape
     dt = _wdtype(dy)
     work = _work("gl_linear_work_bytes", dy.device, M, N, K, dt, 1 | (2 if codes is not None else 0) |
@@ -781,9 +785,10 @@ def linear_bwd(dy, z, slope, x, codes, exps, w, dx, dw, db, K: int, act: int, ac
         return t.stride(0) if t is not None else 0
 
     _launch("gl_linear_bwd", GlLinearBwdArgs(
-        dy.data_ptr(), _ptr(z), _ptr(slope), _ptr(x), _ptr(codes), _ptr(exps), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db),
-        _ptr(work), M, N, K, dy.stride(0), ld(z), ld(slope), ld(x), ld(codes), ld(w), ld(dx),
-        work.numel() if work is not None else 0, dt, act, int(accumulate), 0), dy.device)
+        dy.data_ptr(), _ptr(slope), _ptr(x), _ptr(codes), _ptr(exps), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db),
+        _ptr(work), M, N, K, dy.stride(0), ld(slope), ld(x), ld(codes), ld(w), ld(dx),
+        work.numel() if work is not None else 0, dt, _SLOPE_KINDS[slope.dtype] if slope is not None else 0,
+        int(accumulate), 0), dy.device)
 
 
 def _pdtype(*params) -> int:

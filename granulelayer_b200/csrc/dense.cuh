@@ -64,19 +64,85 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
 
 // act(z) and act'(z) of the dense operators: the framework's identity / ReLU / GELU (erf form) and
 // SiLU z / (1 + e^-z).  Unlike the pooled layers' fmaxf, ReLU hands a NaN on.
-__device__ __forceinline__ float dense_act(int act, float z) {
-  if (act == GL_ACT_IDENTITY) return z;
-  if (act == GL_ACT_RELU) return z < 0.f ? 0.f : z;
-  if (act == GL_ACT_GELU) return act_f<GL_ACT_GELU>(z);
-  return z / (1.f + expf(-z));
+//
+// FAST is for results that are stored in bf16: exponentials and quotients by the hardware's approximations, and
+// the normal distribution's tail by Abramowitz & Stegun 7.1.26, erfc(t) = (a1 s + .. + a5 s^5) e^(-t^2) with
+// s = 1 / (1 + 0.3275911 t), whose error is at most 1.5e-7 (a bf16 step is 4e-3) and whose exponential is also
+// the density that act' needs.  With erff and expf the backward kernels were bound by arithmetic, not memory.
+template <bool FAST>
+__device__ __forceinline__ void normal_cdf_pdf(float z, float& cdf, float& pdf) {
+  if constexpr (FAST) {
+    const float e = __expf(-0.5f * z * z), t = fabsf(z) * 0.7071067811865476f;
+    const float s = __fdividef(1.f, fmaf(0.3275911f, t, 1.f));
+    const float q = s * fmaf(s, fmaf(s, fmaf(s, fmaf(s, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
+                             0.254829592f);
+    const float tail = 0.5f * q * e;
+    cdf = z < 0.f ? tail : 1.f - tail;
+    pdf = 0.3989422804014327f * e;
+  } else {
+    cdf = 0.5f * (1.f + erff(z * 0.7071067811865476f));
+    pdf = 0.3989422804014327f * expf(-0.5f * z * z);
+  }
 }
 
-__device__ __forceinline__ float dense_slope(int act, float z) {
-  if (act == GL_ACT_IDENTITY) return 1.f;
-  if (act == GL_ACT_RELU) return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
-  if (act == GL_ACT_GELU) return dact_f<GL_ACT_GELU>(z);
-  const float s = 1.f / (1.f + expf(-z));
-  return s * (1.f + z * (1.f - s));
+template <bool FAST>
+__device__ __forceinline__ float logistic(float z) {
+  if constexpr (FAST) return __fdividef(1.f, 1.f + __expf(-z));
+  else return 1.f / (1.f + expf(-z));
+}
+
+template <int ACT, bool FAST>
+__device__ __forceinline__ float dense_act(float z) {
+  if constexpr (ACT == GL_ACT_IDENTITY) return z;
+  if constexpr (ACT == GL_ACT_RELU) return z < 0.f ? 0.f : z;
+  if constexpr (ACT == GL_ACT_GELU) {
+    if constexpr (!FAST) return act_f<GL_ACT_GELU>(z);
+    float cdf, pdf;
+    normal_cdf_pdf<FAST>(z, cdf, pdf);
+    return z * cdf;
+  }
+  return z * logistic<FAST>(z);
+}
+
+// act'(z), and act(z) in `a`.
+template <int ACT, bool FAST>
+__device__ __forceinline__ float dense_slope(float z, float& a) {
+  if constexpr (ACT == GL_ACT_IDENTITY) {
+    a = z;
+    return 1.f;
+  } else if constexpr (ACT == GL_ACT_RELU) {
+    a = z < 0.f ? 0.f : z;
+    return z > 0.f ? 1.f : (z <= 0.f ? 0.f : z);
+  } else if constexpr (ACT == GL_ACT_GELU) {
+    float cdf, pdf;
+    normal_cdf_pdf<FAST>(z, cdf, pdf);
+    a = z * cdf;
+    return fmaf(z, pdf, cdf);
+  } else {
+    const float s = logistic<FAST>(z);
+    a = z * s;
+    return s * fmaf(z, 1.f - s, 1.f);
+  }
+}
+
+template <int ACT, bool FAST>
+__device__ __forceinline__ float dense_slope(float z) {
+  float a;
+  return dense_slope<ACT, FAST>(z, a);
+}
+
+// f(constant<activation>) for the activation chosen at run time: the branch stays outside f's loops.
+template <int ACT>
+struct ActTag {
+  static constexpr int value = ACT;
+};
+#pragma nv_exec_check_disable
+template <typename F>
+__host__ __device__ __forceinline__ void with_act(int act, F f) {
+  if (act == GL_ACT_IDENTITY) f(ActTag<GL_ACT_IDENTITY>());
+  else if (act == GL_ACT_RELU) f(ActTag<GL_ACT_RELU>());
+  else if (act == GL_ACT_GELU) f(ActTag<GL_ACT_GELU>());
+  else f(ActTag<GL_ACT_SILU>());
 }
 
 // ---- 8-bit codes ----
@@ -108,5 +174,14 @@ __device__ __forceinline__ uint32_t slope_code(float d) {
 }
 
 __device__ __forceinline__ float slope_value(uint32_t code) { return (float)((int)code - 32) * (1.f / 192.f); }
+
+// act'(z) in 16 bits (bf16 layers): steps of 2^-14, exact at 0 and 1.  A NaN becomes the code that reads as -2, which
+// no act' has; it reads back as NaN.
+__device__ __forceinline__ uint32_t slope_code16(float d) {
+  return d != d ? 0x8000u : (uint32_t)(__float2int_rn(d * 16384.f) & 0xFFFF);
+}
+__device__ __forceinline__ float slope_value16(uint32_t code) {
+  return code == 0x8000u ? __int_as_float(0x7FC00000) : (float)(int16_t)code * (1.f / 16384.f);
+}
 
 }  // namespace gl

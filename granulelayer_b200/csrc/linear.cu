@@ -75,12 +75,40 @@ __global__ void __launch_bounds__(256) lin_pack_kernel(const T* src, uint16_t* d
 
 constexpr int kDzRows = 64;   // rows of one block of the dz kernel, and of one partial column sum
 
+// Eight saved derivatives from element i of `slope` on (`left` of them inside the row).
+template <int KIND>
+__device__ __forceinline__ void load_slope8(const void* slope, int64_t i, int64_t left, bool aligned, float (&d)[8]) {
+  if constexpr (KIND == GL_SLOPE_F32) {
+    load8<float>(reinterpret_cast<const float*>(slope) + i, left, aligned, d);
+  } else if constexpr (KIND == GL_SLOPE_I16) {
+    const uint16_t* q = reinterpret_cast<const uint16_t*>(slope) + i;
+    if (aligned && left >= 8) {
+      const uint4 t = *reinterpret_cast<const uint4*>(q);
+      const uint32_t u[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = slope_value16((u[k / 2] >> (16 * (k & 1))) & 0xFFFF);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = k < left ? slope_value16(q[k]) : 0.f;
+    }
+  } else {
+    const uint8_t* q = reinterpret_cast<const uint8_t*>(slope) + i;
+    if (aligned && left >= 8) {
+      const uint2 u = *reinterpret_cast<const uint2*>(q);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = slope_value(((k < 4 ? u.x : u.y) >> (8 * (k % 4))) & 0xFF);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) d[k] = k < left ? slope_value(q[k]) : 0.f;
+    }
+  }
+}
+
 // dz planes [NP][M][Np] (where `dz` is given) and the column sums of each block of kDzRows rows.  A warp spans 256
 // columns, eight per lane; the block's eight warps take every eighth row.
-template <typename T, int NP>
-__global__ void __launch_bounds__(256) lin_dz_kernel(const T* dy, const T* z, const uint8_t* slope, uint16_t* dz,
-                                                     float* part, int64_t M, int64_t N, int64_t lddy, int64_t ldz,
-                                                     int64_t lds, int act, int aligned) {
+template <typename T, int NP, int KIND>
+__global__ void __launch_bounds__(256) lin_dz_kernel(const T* dy, const void* slope, uint16_t* dz, float* part,
+                                                     int64_t M, int64_t N, int64_t lddy, int64_t lds, int aligned) {
   __shared__ float red[8][256 + 8];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t segs = (N + 255) / 256, Np = (N + 7) / 8 * 8, plane = M * Np;
@@ -90,26 +118,15 @@ __global__ void __launch_bounds__(256) lin_dz_kernel(const T* dy, const T* z, co
   for (int i = 0; i < 8; ++i) sum[i] = 0.f;
   if (left > 0) {
     const int64_t m1 = min(M, (rc + 1) * kDzRows);
-#pragma unroll 2
+#pragma unroll 4
     for (int64_t m = rc * kDzRows + warp; m < m1; m += 8) {
       float d[8];
       load8<T>(dy + m * lddy + n, left, aligned, d);
-      if (slope) {
-        const uint8_t* q = slope + m * lds + n;
-        if (aligned && left >= 8) {
-          const uint2 u = *reinterpret_cast<const uint2*>(q);
+      if constexpr (KIND != GL_SLOPE_NONE) {
+        float s[8];
+        load_slope8<KIND>(slope, m * lds + n, left, aligned, s);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) d[i] *= slope_value(((i < 4 ? u.x : u.y) >> (8 * (i % 4))) & 0xFF);
-        } else {
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
-            if (i < left) d[i] *= slope_value(q[i]);
-        }
-      } else if (z) {
-        float zz[8];
-        load8<T>(z + m * ldz + n, left, aligned, zz);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] *= dense_slope(act, zz[i]);
+        for (int i = 0; i < 8; ++i) d[i] *= s[i];
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) sum[i] += d[i];
@@ -153,7 +170,8 @@ __global__ void __launch_bounds__(256) lin_db_kernel(const float* part, int64_t 
 #pragma unroll
     for (int r = 0; r < 8; ++r) s += red[r][lane];
     if (accumulate) reinterpret_cast<float*>(db)[n] += s;
-    else st_dense(db, n, dtype, s);
+    else if (dtype == GL_DTYPE_F32) reinterpret_cast<float*>(db)[n] = s;
+    else reinterpret_cast<__nv_bfloat16*>(db)[n] = __float2bfloat16_rn(s);
   }
 }
 
@@ -204,11 +222,11 @@ __global__ void __launch_bounds__(128) lin_rows_kernel(const T* x, const T* w, i
   for (int t = 0; t < MT; ++t)
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) acc[t] += __shfl_xor_sync(kFullMask, acc[t], o);
-  float z = acc[0];
+  float z[1] = {acc[0]};
 #pragma unroll
   for (int t = 1; t < MT; ++t)
-    if (lane == t) z = acc[t];
-  if (lane < M) lin_finish(e, lane, n, z);
+    if (lane == t) z[0] = acc[t];
+  if (lane < M) lin_finish<1>(e, lane, n, false, z);
 }
 
 // Rows up to which the row kernels run: beyond, w's fp32 splitting or the tensor cores' fixed cost is paid back.
@@ -321,9 +339,11 @@ template <typename T>
 static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, cudaStream_t st) {
   constexpr int NP = sizeof(T) == 4 ? 3 : 1;
   char* work = (char*)a.work;
-  const bool aligned = rows16(a.dy, a.lddy, sizeof(T)) && (!a.z || rows16(a.z, a.ldz, sizeof(T))) &&
-                       (!a.slope || (((uintptr_t)a.slope & 7) == 0 && a.lds % 8 == 0));
-  const bool dy_is_dz = NP == 1 && aligned && !a.z && !a.slope;
+  const int ss = a.slope_kind == GL_SLOPE_F32 ? 4 : 2;
+  const bool aligned = rows16(a.dy, a.lddy, sizeof(T)) &&
+                       (a.slope_kind == GL_SLOPE_NONE ||
+                        (a.slope_kind == GL_SLOPE_U8 ? (((uintptr_t)a.slope | a.lds) & 7) == 0 : rows16(a.slope, a.lds, ss)));
+  const bool dy_is_dz = NP == 1 && aligned && a.slope_kind == GL_SLOPE_NONE;
   const bool write = !dy_is_dz && (a.dx || a.dw);
   MmaOperand dz{a.dy, a.lddy, 0, 1, 0};
   if (!dy_is_dz) dz = MmaOperand{work + w.dz, up(a.N, 8), a.M * up(a.N, 8), NP, 0};
@@ -332,9 +352,12 @@ static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, c
     const int64_t rc = up(a.M, kDzRows) / kDzRows, segs = (a.N + 255) / 256;
     if (rc * segs > 0x7FFFFFFF) return GL_ERR_SHAPE;
     float* part = a.db ? (float*)(work + w.part) : nullptr;
-    lin_dz_kernel<T, NP><<<(unsigned)(rc * segs), 256, 0, st>>>(
-        (const T*)a.dy, (const T*)a.z, a.slope, write ? (uint16_t*)(work + w.dz) : nullptr, part, a.M, a.N, a.lddy,
-        a.ldz, a.lds, a.act, aligned);
+    const auto kernel = a.slope_kind == GL_SLOPE_NONE  ? lin_dz_kernel<T, NP, GL_SLOPE_NONE>
+                        : a.slope_kind == GL_SLOPE_F32 ? lin_dz_kernel<T, NP, GL_SLOPE_F32>
+                        : a.slope_kind == GL_SLOPE_I16 ? lin_dz_kernel<T, NP, GL_SLOPE_I16>
+                                                       : lin_dz_kernel<T, NP, GL_SLOPE_U8>;
+    kernel<<<(unsigned)(rc * segs), 256, 0, st>>>((const T*)a.dy, a.slope, write ? (uint16_t*)(work + w.dz) : nullptr,
+                                               part, a.M, a.N, a.lddy, a.lds, aligned);
     ++launches;
     if (a.db) {
       lin_db_kernel<<<(unsigned)((a.N + 31) / 32), 256, 0, st>>>(part, rc, a.N, a.db, a.dtype, a.accumulate);
@@ -392,13 +415,13 @@ extern "C" int gl_linear_fwd(const GlLinearArgs* args, void* stream) {
   if (!args) return GL_ERR_NULL;
   const GlLinearArgs& a = *args;
   if (int rc = lin_checks(a.M, a.N, a.K, a.dtype, a.act)) return rc;
-  if (a.ldx < a.K || a.ldw < a.K || a.ldy < a.N || (a.residual && a.ldr < a.N) || (a.z && a.ldz < a.N) ||
-      (a.slope && a.lds < a.N))
+  if (a.slope_kind < GL_SLOPE_NONE || a.slope_kind > GL_SLOPE_U8) return GL_ERR_UNSUPPORTED;
+  if (a.ldx < a.K || a.ldw < a.K || a.ldy < a.N || (a.residual && a.ldr < a.N) || (a.slope_kind && a.lds < a.N))
     return GL_ERR_SHAPE;
   if (a.M == 0) return GL_OK;
-  if (!a.x || !a.w || !a.y) return GL_ERR_NULL;
+  if (!a.x || !a.w || !a.y || (a.slope_kind && !a.slope)) return GL_ERR_NULL;
   const int es = a.dtype == GL_DTYPE_F32 ? 4 : 2;
-  const LinEpilogue e{a.bias, a.residual, a.y, a.z, a.slope, a.ldr, a.ldy, a.ldz, a.lds, a.dtype, a.act, 0};
+  const LinEpilogue e{a.bias, a.residual, a.y, a.slope, a.ldr, a.ldy, a.lds, a.dtype, a.act, 0, a.slope_kind};
   const bool aligned = rows16(a.x, a.ldx, es) && rows16(a.w, a.ldw, es);
   cudaStream_t st = (cudaStream_t)stream;
   if (few_rows(a.M, a.dtype))
@@ -415,9 +438,10 @@ extern "C" int gl_linear_fwd(const GlLinearArgs* args, void* stream) {
 extern "C" int gl_linear_bwd(const GlLinearBwdArgs* args, void* stream) {
   if (!args) return GL_ERR_NULL;
   const GlLinearBwdArgs& a = *args;
-  if (int rc = lin_checks(a.M, a.N, a.K, a.dtype, a.act)) return rc;
+  if (int rc = lin_checks(a.M, a.N, a.K, a.dtype, GL_ACT_IDENTITY)) return rc;
+  if (a.slope_kind < GL_SLOPE_NONE || a.slope_kind > GL_SLOPE_U8) return GL_ERR_UNSUPPORTED;
   const bool codes = a.codes != nullptr;
-  if (a.lddy < a.N || (a.z && a.ldz < a.N) || (a.slope && a.lds < a.N) || (a.dw && !codes && a.ldx < a.K) ||
+  if (a.lddy < a.N || (a.slope_kind && a.lds < a.N) || (a.dw && !codes && a.ldx < a.K) ||
       (codes && (a.ldc < up(a.K, kActBlock) || a.ldc % kActBlock)) || (a.dx && (a.ldw < a.K || a.lddx < a.K)))
     return GL_ERR_SHAPE;
   cudaStream_t st = (cudaStream_t)stream;
@@ -430,7 +454,7 @@ extern "C" int gl_linear_bwd(const GlLinearBwdArgs* args, void* stream) {
     return e == cudaSuccess ? GL_OK : set_cuda_error(e);
   }
   if (!a.dx && !a.dw && !a.db) return GL_OK;
-  if (!a.dy || (a.act != GL_ACT_IDENTITY && !a.z && !a.slope) || (a.dx && !a.w) ||
+  if (!a.dy || (a.slope_kind && !a.slope) || (a.dx && !a.w) ||
       (a.dw && !codes && !a.x) || (codes && !a.exps))
     return GL_ERR_NULL;
   if (codes && ((uintptr_t)a.codes & 15)) return GL_ERR_ALIGN;

@@ -1,19 +1,27 @@
 // The matrix product of the linear operator on the 5th-generation tensor cores (mma.cuh states it).
 //
-// A persistent CTA takes output tiles of 128 x BN (and, with split sums, ranges of k).  Ten warps:
-//   producer (one lane)  TMA loads of 64 k of every plane of A and B into a ring of 128-byte-swizzled stages
-//   issuer (one lane)    tcgen05.mma 128 x BN x 16 per 16 k and term pair, accumulators in TMEM (two buffers)
-//   eight epilogue warps TMEM -> registers -> bias, activation, residual -> memory, while the next tile runs
-// handing over through mbarriers: full / empty per stage, done / free per accumulator.
+// A persistent CTA, or a pair of CTAs, takes output tiles of 128 (256) x BN and, with split sums, ranges of k.  Ten
+// warps per CTA:
+//   producer (one lane)  TMA loads of 64 k of a plane of A and of B into a ring of 128-byte-swizzled slots
+//   issuer (one lane; of a pair, the even CTA's)  tcgen05.mma per 16 k and term pair, two accumulators in TMEM
+//   eight epilogue warps TMEM -> registers -> shared memory -> bias, activation, residual -> memory, row by row in
+//                        whole sectors, while the next tile runs
+// handing over through mbarriers: full / empty per slot, done / free per accumulator.
 //
-// fp32 operands come as three bf16 planes; the six products of term pairs i + j <= 2 run smallest first.  The
-// tensor core's fp32 accumulation does not round to nearest, so with several planes a sum over k is cut into
-// chunks: each chunk's accumulator is added to registers in fp32 while the next one runs.
+// Pairs (cta_group::2, 256 x 256 tiles): each CTA loads its 128 rows of A and half of B, so a CTA moves 32 KB through
+// its shared memory per 64 k instead of 48 KB, both from L2 and to the tensor core; that traffic, not the MMA
+// rate, bounds the 128 x 256 tile of one CTA.
 //
-// K-major tiles are one TMA box (64 k wide, 128 or BN rows).  MN-major tiles are boxes of 64 rows-by-64 k; the
-// matrix descriptor walks them with 2048 bytes per 16 k and 8192 bytes per 64 rows.  Edges in every
-// dimension are the tensor map's zero fill.  Every wait has an iteration limit; a CTA whose wait runs out writes
-// NaN to what it has not computed, waits (again bounded) for its own copies and leaves.
+// fp32 operands come as three bf16 planes; a slot holds plane i of both and the products of term pairs (i, j),
+// i + j <= 2, run as their slots arrive: (0,0), (0,1) (1,0) (1,1), (0,2) (2,0).  The tensor core's fp32 accumulation
+// truncates, so with several planes a sum over k is cut into chunks of 128: each chunk's accumulator is added to
+// registers in fp32 (rounding to nearest) while the next one runs.  At K = 4096 chunks of 512 were 3.9e-6 off in
+// the 2-norm, chunks of 128 0.8e-6 (plain fp32 products: 1.0e-6).
+//
+// K-major tiles are one TMA box (64 k wide, all rows of the tile); MN-major tiles are boxes of 64 rows by 64 k, which
+// the matrix descriptor walks with 2048 bytes per 16 k and 8192 bytes per 64 rows.  Edges in every dimension are
+// the tensor map's zero fill.  Every wait has an iteration limit; a CTA whose wait runs out writes NaN to what it
+// has not computed, waits (again bounded) for its own copies and leaves.
 #include <cuda.h>
 
 #include "mma.cuh"
@@ -21,9 +29,11 @@
 
 namespace gl {
 
-constexpr int kMmBM = 128, kMmBK = 64, kMmThreads = 320, kMmEpiWarps = 8;
+constexpr int kMmBM = 128, kMmBK = 64, kMmThreads = 320, kMmEpiWarps = 8, kMmMaxSlots = 8;
 constexpr uint32_t kMmWaitLimit = 1u << 20;
 constexpr uint32_t kMmPlaneA = kMmBM * kMmBK * 2;
+constexpr int kMmPitch = 36;                                   // floats per row of a warp's 32 x 32 epilogue tile
+constexpr uint32_t kMmEpiBytes = kMmEpiWarps * 32 * kMmPitch * 4;
 
 struct MmaParams {
   int64_t M, N;
@@ -33,16 +43,15 @@ struct MmaParams {
   LinEpilogue e;
 };
 
-__host__ __device__ constexpr uint32_t mm_stage_bytes(int BN, int NPA, int NPB) {
-  return NPA * kMmPlaneA + NPB * (uint32_t)BN * kMmBK * 2;
-}
-__host__ __device__ constexpr int mm_stages(int BN, int NPA, int NPB) {
-  const int n = (int)((227 * 1024 - 2048) / mm_stage_bytes(BN, NPA, NPB));
-  return n > 8 ? 8 : n;
+// A slot: a plane of A (128 rows) and of B (this CTA's share of BN rows), 64 k each.
+__host__ __device__ constexpr uint32_t mm_slot_bytes(int BN, int CTAS) { return kMmPlaneA + (uint32_t)(BN / CTAS) * kMmBK * 2; }
+__host__ __device__ constexpr int mm_slots(int BN, int CTAS) {
+  const int n = (int)((227 * 1024 - 2048 - kMmEpiBytes) / mm_slot_bytes(BN, CTAS));
+  return n > kMmMaxSlots ? kMmMaxSlots : n;
 }
 
 struct MmaShared {
-  uint64_t full[8], empty[8], done[2], free_[2];
+  uint64_t full[kMmMaxSlots], empty[kMmMaxSlots], done[2], free_[2];
   uint32_t tmem;
   int dead;
 };
@@ -50,15 +59,36 @@ struct MmaShared {
 __device__ __forceinline__ void mm_expect(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.arrive.expect_tx.release.cta.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
+
+// Arrive on an mbarrier of the even CTA of the pair (or of this CTA).
+template <int CTAS>
 __device__ __forceinline__ void mm_arrive(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+  if constexpr (CTAS == 1) {
+    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+  } else {
+    uint32_t remote;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(remote) : "r"(bar));
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote) : "memory");
+  }
 }
+
+// TMA load into this CTA's shared memory; its bytes count on `bar` (of a pair: a shared::cluster address in the even
+// CTA).
+template <int CTAS>
 __device__ __forceinline__ void mm_load(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
-          dst),
-      "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
-      : "memory");
+  if constexpr (CTAS == 1) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], "
+        "[%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, "
+        "%3, %4}], [%5];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
+        : "memory");
+  }
 }
 
 // Bounded wait; after the first one that ran out anywhere in the CTA all give up at once.
@@ -80,32 +110,73 @@ struct MmaTile {
 };
 
 // Work item -> tile and k range.  Tiles run in bands of 8 rows of tiles so that concurrent CTAs share operands in L2.
-__device__ __forceinline__ MmaTile mm_tile(const MmaParams& p, int64_t item, int BN) {
+__device__ __forceinline__ MmaTile mm_tile(const MmaParams& p, int64_t item, int BM, int BN) {
   MmaTile t;
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
   t.split = (int)(item / tiles);
   const int64_t i = item - t.split * tiles, band = i / (8ll * p.tiles_n), first = band * 8;
   const int64_t rows = min((int64_t)8, p.tiles_m - first), j = i - band * 8 * p.tiles_n;
-  t.m0 = (first + j % rows) * kMmBM;
+  t.m0 = (first + j % rows) * BM;
   t.n0 = (j / rows) * BN;
   t.k0 = t.split * p.split_blocks;
   t.k1 = min(p.kblocks, t.k0 + p.split_blocks);
   return t;
 }
 
-template <int BN, int NPA, int NPB>
+// The warp's 32 x 32 block at (m0, n0), lane r holding row r: through shared memory, so that four lanes finish 32
+// columns of a row (or, where rows are not 16-byte aligned or the block is cut, a lane each column).
+__device__ __forceinline__ void mm_store_block(const MmaParams& p, float* tile, const float (&v)[32], int64_t m0,
+                                               int64_t n0, int split) {
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int j = 0; j < 32; j += 4)
+    *reinterpret_cast<float4*>(tile + lane * kMmPitch + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+  __syncwarp();
+  const int64_t rows = p.M - m0;
+  if (n0 + 32 <= p.N && p.vec) {
+    const int c = (lane & 3) * 8;
+#pragma unroll 2
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2);
+      if (r >= rows) break;
+      const float4 a = *reinterpret_cast<const float4*>(tile + r * kMmPitch + c);
+      const float4 b = *reinterpret_cast<const float4*>(tile + r * kMmPitch + c + 4);
+      float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+      if (p.part) st_span<float, 8>(p.part + (split * p.M + m0 + r) * p.N + n0 + c, true, z);
+      else lin_finish<8>(p.e, m0 + r, n0 + c, true, z);
+    }
+  } else if (n0 + lane < p.N) {
+    const int n = rows < 32 ? (int)rows : 32;
+#pragma unroll 4
+    for (int r = 0; r < n; ++r) {
+      float z[1] = {tile[r * kMmPitch + lane]};
+      if (p.part) p.part[(split * p.M + m0 + r) * p.N + n0 + lane] = z[0];
+      else lin_finish<1>(p.e, m0 + r, n0 + lane, false, z);
+    }
+  }
+  __syncwarp();
+}
+
+template <int CTAS, int BN, int NPA, int NPB>
 __global__ void __launch_bounds__(kMmThreads, 1)
     mma_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const MmaParams p) {
-  constexpr int ST = mm_stages(BN, NPA, NPB);
-  constexpr uint32_t kStage = mm_stage_bytes(BN, NPA, NPB), kPlaneB = BN * kMmBK * 2;
+  constexpr int ST = mm_slots(BN, CTAS), BNC = BN / CTAS, BM = kMmBM * CTAS;
+  constexpr uint32_t kSlot = mm_slot_bytes(BN, CTAS);
   constexpr uint32_t kCols = 2 * BN;                 // TMEM columns: two accumulators
   constexpr bool MULTI = NPA > 1;
   constexpr int HALF = BN >= 64 ? BN / 2 : BN;        // columns per epilogue warp
+  constexpr int kEpi = BN >= 64 ? kMmEpiWarps : 4;    // epilogue warps at work
   extern __shared__ unsigned char mm_raw[];
   __shared__ MmaShared sh;
-  const uint32_t smem = (t5_smem_u32(mm_raw) + 1023u) & ~1023u;
+  const uint32_t pad = ((t5_smem_u32(mm_raw) + 1023u) & ~1023u) - t5_smem_u32(mm_raw);
+  const uint32_t smem = t5_smem_u32(mm_raw) + pad;
+  float* epi = reinterpret_cast<float*>(mm_raw + pad + ST * kSlot);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (warp == 9) t5_tmem_alloc(t5_smem_u32(&sh.tmem), kCols);
+  const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1);
+  if (warp == 9) {
+    if constexpr (CTAS == 1) t5_tmem_alloc(t5_smem_u32(&sh.tmem), kCols);
+    else t5_tmem_alloc2(t5_smem_u32(&sh.tmem), kCols);
+  }
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) {
       t5_mbar_init(t5_smem_u32(&sh.full[i]), 1);
@@ -113,63 +184,74 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       t5_mbar_init(t5_smem_u32(&sh.done[i]), 1);
-      t5_mbar_init(t5_smem_u32(&sh.free_[i]), BN >= 64 ? kMmEpiWarps : 4);
+      t5_mbar_init(t5_smem_u32(&sh.free_[i]), kEpi * CTAS);
     }
     sh.dead = 0;
   }
+  __syncwarp();
   t5_fence_before_sync();
-  __syncthreads();
+  if constexpr (CTAS == 1) __syncthreads();
+  else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   t5_fence_after_sync();
   const uint32_t tmem = sh.tmem;
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+  const int64_t first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (warp == 8) {
     if (lane == 0) {
       uint32_t it = 0;
       bool live = true;
-      for (int64_t item = blockIdx.x; item < items && live; item += gridDim.x) {
-        const MmaTile t = mm_tile(p, item, BN);
-        for (int kb = t.k0; kb < t.k1; ++kb, ++it) {
-          const int s = it % ST;
-          if (it >= ST && !mm_wait(sh, sh.empty[s], ((it / ST) - 1) & 1)) {
-            live = false;
-            break;
-          }
-          const uint32_t bar = t5_smem_u32(&sh.full[s]), a = smem + s * kStage, b = a + NPA * kMmPlaneA;
-          mm_expect(bar, kStage);
+      for (int64_t item = first; item < items && live; item += step) {
+        const MmaTile t = mm_tile(p, item, BM, BN);
+        const int m0 = (int)t.m0 + kMmBM * rank, n0 = (int)t.n0 + BNC * rank;
+        for (int kb = t.k0; kb < t.k1 && live; ++kb) {
 #pragma unroll
-          for (int i = 0; i < NPA; ++i) {
-            if (p.a_mn) {
-              for (int h = 0; h < 2; ++h)
-                mm_load(a + i * kMmPlaneA + h * 8192, &ta, (int)t.m0 + 64 * h, kb * kMmBK, i, bar);
-            } else {
-              mm_load(a + i * kMmPlaneA, &ta, kb * kMmBK, (int)t.m0, i, bar);
+          for (int i = 0; i < NPA; ++i, ++it) {
+            const int s = it % ST;
+            if (it >= ST && !mm_wait(sh, sh.empty[s], ((it / ST) - 1) & 1)) {
+              live = false;
+              break;
             }
-          }
-#pragma unroll
-          for (int i = 0; i < NPB; ++i) {
-            if (BN >= 64 && p.b_mn) {
-              for (int h = 0; h < BN / 64; ++h)
-                mm_load(b + i * kPlaneB + h * 8192, &tb, (int)t.n0 + 64 * h, kb * kMmBK, i, bar);
+            uint32_t bar = t5_smem_u32(&sh.full[s]);
+            const uint32_t a = smem + s * kSlot, b = a + kMmPlaneA;
+            const uint32_t bytes = i < NPB ? kSlot : kMmPlaneA;
+            if (rank == 0) mm_expect(bar, CTAS * bytes);
+            if constexpr (CTAS == 2) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(bar) : "r"(bar));
+            if (p.a_mn) {
+              mm_load<CTAS>(a, &ta, m0, kb * kMmBK, i, bar);
+              mm_load<CTAS>(a + 8192, &ta, m0 + 64, kb * kMmBK, i, bar);
             } else {
-              mm_load(b + i * kPlaneB, &tb, kb * kMmBK, (int)t.n0, i, bar);
+              mm_load<CTAS>(a, &ta, kb * kMmBK, m0, i, bar);
+            }
+            if (i < NPB) {
+              if (BNC >= 64 && p.b_mn) {
+#pragma unroll
+                for (int h = 0; h < BNC / 64; ++h)
+                  mm_load<CTAS>(b + h * 8192, &tb, n0 + 64 * h, kb * kMmBK, i, bar);
+              } else {
+                mm_load<CTAS>(b, &tb, kb * kMmBK, n0, i, bar);
+              }
             }
           }
         }
       }
-      if (!live) {   // the copies in flight must land before the CTA's shared memory goes away
+      if (!live && rank == 0) {   // the copies in flight must land before the shared memory goes away
         for (uint32_t j = it > ST ? it - ST : 0; j < it; ++j)
           t5_mbar_wait(t5_smem_u32(&sh.full[j % ST]), (j / ST) & 1, kMmWaitLimit);
       }
     }
   } else if (warp == 9) {
-    if (lane == 0) {
-      const uint32_t idesc = t5_idesc_bf16(kMmBM, BN, p.a_mn, p.b_mn);
+    if (lane == 0 && rank == 0) {
+      const uint32_t idesc = t5_idesc_bf16(BM, BN, p.a_mn, p.b_mn);
       const uint32_t ka = p.a_mn ? 2048u : 32u, kb_ = p.b_mn ? 2048u : 32u;   // bytes per 16 k
-      uint32_t it = 0, ch = 0;
+      uint32_t it = 0, ch = 0, acc = 0;
       bool live = true;
-      for (int64_t item = blockIdx.x; item < items && live; item += gridDim.x) {
-        const MmaTile t = mm_tile(p, item, BN);
+      auto commit = [&](uint64_t& bar) {
+        if constexpr (CTAS == 1) t5_commit(t5_smem_u32(&bar));
+        else t5_commit_pair(t5_smem_u32(&bar));
+      };
+      for (int64_t item = first; item < items && live; item += step) {
+        const MmaTile t = mm_tile(p, item, BM, BN);
         for (int c0 = t.k0; c0 < t.k1 && live; c0 += p.chunk, ++ch) {
           const int c1 = min(t.k1, c0 + p.chunk), buf = ch & 1;
           if (ch >= 2 && !mm_wait(sh, sh.free_[buf], ((ch >> 1) - 1) & 1)) {
@@ -178,48 +260,62 @@ __global__ void __launch_bounds__(kMmThreads, 1)
           }
           t5_fence_after_sync();
           const uint32_t d = tmem + buf * BN;
-          uint32_t acc = 0;
-          for (int kb = c0; kb < c1; ++kb, ++it) {
-            const int s = it % ST;
-            if (!mm_wait(sh, sh.full[s], (it / ST) & 1)) {
-              live = false;
-              break;
+          acc = 0;
+          auto product = [&](uint32_t a, uint32_t b) {   // a plane of A (slot address) by one of B
+#pragma unroll
+            for (int k = 0; k < kMmBK / 16; ++k) {
+              const uint64_t ad = t5_desc_sw128(a + k * ka, 8192, 1024);
+              const uint64_t bd = t5_desc_sw128(b + kMmPlaneA + k * kb_, 8192, 1024);
+              if constexpr (CTAS == 1) t5_mma_bf16(d, ad, bd, idesc, acc);
+              else t5_mma_bf16_pair(d, ad, bd, idesc, acc);
+              acc = 1;
             }
-            t5_fence_after_sync();
-            const uint32_t a = smem + s * kStage, b = a + NPA * kMmPlaneA;
+          };
+          for (int kb = c0; kb < c1 && live; ++kb, it += NPA) {
+            uint32_t slot[NPA];
 #pragma unroll
-            for (int sum = (NPA > 1 ? 2 : 0); sum >= 0; --sum) {
-#pragma unroll
-              for (int i = 0; i < NPA; ++i) {
-                const int j = sum - i;
-                if (j < 0 || j >= NPB) continue;
-#pragma unroll
-                for (int k = 0; k < kMmBK / 16; ++k) {
-                  t5_mma_bf16(d, t5_desc_sw128(a + i * kMmPlaneA + k * ka, 8192, 1024),
-                              t5_desc_sw128(b + j * kPlaneB + k * kb_, 8192, 1024), idesc, acc);
-                  acc = 1;
-                }
+            for (int i = 0; i < NPA; ++i) {
+              const int s = (it + i) % ST;
+              slot[i] = smem + s * kSlot;
+              if (!mm_wait(sh, sh.full[s], ((it + i) / ST) & 1)) {
+                live = false;
+                break;
               }
+              t5_fence_after_sync();
+              if (i == 0) product(slot[0], slot[0]);
+              if (NPB == 1) {
+                if (i > 0) product(slot[i], slot[0]);
+                if (i > 0 || NPA == 1) commit(sh.empty[s]);
+              } else if (i == 1) {
+                product(slot[0], slot[1]);
+                product(slot[1], slot[0]);
+                product(slot[1], slot[1]);
+                commit(sh.empty[s]);
+              } else if (i == 2) {
+                product(slot[0], slot[2]);
+                product(slot[2], slot[0]);
+                commit(sh.empty[s]);
+              }
+              if (NPA > 1 && i == NPA - 1) commit(sh.empty[it % ST]);
             }
-            t5_commit(t5_smem_u32(&sh.empty[s]));
           }
-          if (live) t5_commit(t5_smem_u32(&sh.done[buf]));
+          if (live) commit(sh.done[buf]);
         }
       }
     }
-  } else if (BN >= 64 || warp < 4) {
-    const int row = 32 * (warp & 3) + lane, half = BN >= 64 ? warp >> 2 : 0;
+  } else if (warp < kEpi) {
+    const int half = warp >> 2;
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
+    float* tile = epi + warp * 32 * kMmPitch;
     uint32_t ch = 0;
-    for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-      const MmaTile t = mm_tile(p, item, BN);
-      const int64_t m = t.m0 + row, n0 = t.n0 + half * HALF;
+    for (int64_t item = first; item < items; item += step) {
+      const MmaTile t = mm_tile(p, item, BM, BN);
+      const int64_t m0 = t.m0 + kMmBM * rank + 32 * (warp & 3), n0 = t.n0 + half * HALF;
       float sum[MULTI ? HALF : 1];
       for (int c0 = t.k0; c0 < t.k1; c0 += p.chunk, ++ch) {
         const int buf = ch & 1;
         const bool ok = __all_sync(kFullMask, mm_wait(sh, sh.done[buf], (ch >> 1) & 1));
         t5_fence_after_sync();
-        const bool last = c0 + p.chunk >= t.k1;
 #pragma unroll
         for (int q = 0; q < HALF / 32; ++q) {
           float v[32];
@@ -228,132 +324,95 @@ __global__ void __launch_bounds__(kMmThreads, 1)
 #pragma unroll
             for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7FC00000);
           }
+          if (q == HALF / 32 - 1) {                      // the accumulator is read: free it before the stores
+            t5_fence_before_sync();
+            __syncwarp();
+            if (lane == 0) mm_arrive<CTAS>(t5_smem_u32(&sh.free_[buf]));
+          }
           if constexpr (MULTI) {
 #pragma unroll
             for (int i = 0; i < 32; ++i) sum[32 * q + i] = c0 == t.k0 ? v[i] : sum[32 * q + i] + v[i];
-          } else {
-            if (q == HALF / 32 - 1) {                   // the accumulator is read: free it before the stores
-              t5_fence_before_sync();
-              __syncwarp();
-              if (lane == 0) mm_arrive(t5_smem_u32(&sh.free_[buf]));
-            }
-          }
-          if constexpr (!MULTI) {
-            const int64_t n = n0 + 32 * q;
-            if (m < p.M && n < p.N) {
-              if (p.part) {
-                float* out = p.part + (t.split * p.M + m) * p.N;
-                if (n + 32 <= p.N) {
-                  st_span<32>(out, n, GL_DTYPE_F32, (p.N & 3) == 0, v);
-                } else {
-#pragma unroll
-                  for (int i = 0; i < 32; ++i)
-                    if (n + i < p.N) out[n + i] = v[i];
-                }
-              } else if (n + 32 <= p.N) {
-                lin_finish_span<32>(p.e, m, n, p.vec, v);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (n + i < p.N) lin_finish(p.e, m, n + i, v[i]);
-              }
-            }
+          } else if (m0 < p.M && n0 + 32 * q < p.N) {
+            mm_store_block(p, tile, v, m0, n0 + 32 * q, t.split);
           }
         }
-        if constexpr (MULTI) {
-          t5_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mm_arrive(t5_smem_u32(&sh.free_[buf]));
-          if (last) {
+      }
+      if constexpr (MULTI) {
 #pragma unroll
-            for (int q = 0; q < HALF / 32; ++q) {
-              const int64_t n = n0 + 32 * q;
-              float v[32];
+        for (int q = 0; q < HALF / 32; ++q) {
+          float v[32];
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] = sum[32 * q + i];
-              if (m >= p.M || n >= p.N) continue;
-              if (p.part) {
-                float* out = p.part + (t.split * p.M + m) * p.N;
-                if (n + 32 <= p.N) {
-                  st_span<32>(out, n, GL_DTYPE_F32, (p.N & 3) == 0, v);
-                } else {
-#pragma unroll
-                  for (int i = 0; i < 32; ++i)
-                    if (n + i < p.N) out[n + i] = v[i];
-                }
-              } else if (n + 32 <= p.N) {
-                lin_finish_span<32>(p.e, m, n, p.vec, v);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i)
-                  if (n + i < p.N) lin_finish(p.e, m, n + i, v[i]);
-              }
-            }
-          }
+          for (int i = 0; i < 32; ++i) v[i] = sum[32 * q + i];
+          if (m0 < p.M && n0 + 32 * q < p.N) mm_store_block(p, tile, v, m0, n0 + 32 * q, t.split);
         }
       }
     }
   }
-  __syncthreads();
+  __syncwarp();
+  t5_fence_before_sync();
+  if constexpr (CTAS == 1) {
+    __syncthreads();
+  } else {   // no CTA of a pair leaves while the other may still signal it or use its memory
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  }
   t5_fence_after_sync();
-  if (warp == 9) t5_tmem_dealloc(tmem, kCols);
+  if (warp == 9) {
+    if constexpr (CTAS == 1) t5_tmem_dealloc(tmem, kCols);
+    else t5_tmem_dealloc2(tmem, kCols);
+  }
 }
 
-// Sums the splits of a product in split order and finishes the elements, four columns per thread.
+// Sums the splits of a product in split order and finishes the elements, eight columns per thread (one where rows are
+// not aligned).
+template <int W>
 __global__ void __launch_bounds__(256) mma_join_kernel(const float* part, int64_t M, int64_t N, int splits,
-                                                       LinEpilogue e, int vec) {
-  const int64_t nq = (N + 3) / 4, total = M * nq;
+                                                       LinEpilogue e) {
+  const int64_t nq = N / W, total = M * nq;
   for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int64_t m = i / nq, n = (i - m * nq) * 4;
-    const float* src = part + m * N + n;
-    if ((N & 3) == 0) {
-      float4 s = *reinterpret_cast<const float4*>(src);
-      for (int k = 1; k < splits; ++k) {
-        const float4 t = *reinterpret_cast<const float4*>(src + k * M * N);
-        s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
-      }
-      const float z[4] = {s.x, s.y, s.z, s.w};
+    const int64_t m = i / nq, n = (i - m * nq) * W;
+    float z[W], t[W];
+    ld_span<float, W>(part + m * N + n, true, z);
+#pragma unroll 4
+    for (int k = 1; k < splits; ++k) {
+      ld_span<float, W>(part + (k * M + m) * N + n, true, t);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) lin_finish(e, m, n + j, z[j]);
-    } else {
-      for (int j = 0; j < 4 && n + j < N; ++j) {
-        float s = src[j];
-        for (int k = 1; k < splits; ++k) s += src[k * M * N + j];
-        lin_finish(e, m, n + j, s);
-      }
+      for (int j = 0; j < W; ++j) z[j] += t[j];
     }
+    lin_finish<W>(e, m, n, true, z);
   }
 }
 
 // ---- host ----
 struct MmaPlan {
-  int BN, splits, split_blocks, chunk;
+  int ctas, BN, splits, split_blocks, chunk;
   int64_t tiles_m, tiles_n;
 };
 
-// Tile width and number of splits of k: the least estimated time, in clocks of one SM.  A 64-wide k block costs the
-// larger of its MMAs (BN / 2 clocks a term) and its loads (about 56 bytes a clock for one SM of many); split
-// sums add their partial tiles' traffic and a second launch.
+// Tile shape and number of splits of k: the least estimated time, in clocks of one SM.  64 k cost the larger of
+// the MMAs (2 BN / ctas clocks a term of 128 x BN) and the loads (about 44 bytes a clock into one SM of many);
+// split sums add their partial tiles' traffic and a second launch.
 static MmaPlan mma_plan(int64_t M, int64_t N, int64_t K, int npa, int npb, bool b_mn, int sms) {
   MmaPlan best{};
   double best_t = 1e300;
   const int64_t kb = (K + kMmBK - 1) / kMmBK;
   const int terms = npa == 1 ? 1 : (npb == 1 ? 3 : 6);
-  for (int BN : {256, 128, 64, 32}) {
-    if (BN == 256 && npa > 1) continue;
-    if (BN == 32 && (b_mn || npa > 1)) continue;
-    const int64_t tm = (M + kMmBM - 1) / kMmBM, tn = (N + BN - 1) / BN, tiles = tm * tn;
-    const double load = mm_stage_bytes(BN, npa, npb) / 56.0, mma = terms * 2.0 * BN;
+  struct Shape { int ctas, BN; };
+  for (Shape sh : {Shape{2, 256}, Shape{1, 128}, Shape{1, 64}, Shape{1, 32}}) {
+    if (sh.BN == 32 && (b_mn || npa > 1)) continue;
+    const int64_t tm = (M + kMmBM * sh.ctas - 1) / (kMmBM * sh.ctas), tn = (N + sh.BN - 1) / sh.BN, tiles = tm * tn;
+    const double bytes = npa * (double)kMmPlaneA + npb * (double)(sh.BN / sh.ctas) * kMmBK * 2;
+    const double load = bytes / 44.0, mma = terms * 2.0 * sh.BN;
     const double block = (load > mma ? load : mma) + 20;
+    const int64_t wide = sms / sh.ctas;
     for (int s = 1; s <= 32 && s <= kb; ++s) {
       const int64_t sb = (kb + s - 1) / s;
       if ((kb + sb - 1) / sb != s) continue;
-      const int64_t waves = (tiles * s + sms - 1) / sms;
-      double t = (double)waves * sb * block + 2500.0 + (double)BN * 6 * waves;
-      if (s > 1) t += 3000.0 + (double)M * N * (s + 1) * 4 / 2500.0;
+      const int64_t waves = (tiles * s + wide - 1) / wide;
+      double t = (double)waves * sb * block + 3000.0 + (double)sh.BN * 12 + 500.0 * (sh.ctas - 1);
+      if (s > 1) t += 4000.0 + (double)M * N * (s + 1) * 4 / 2500.0;
       if (t < best_t) {
         best_t = t;
-        best = MmaPlan{BN, s, (int)sb, npa > 1 ? 2 : 1 << 30, tm, tn};
+        best = MmaPlan{sh.ctas, sh.BN, s, (int)sb, npa > 1 ? 2 : 1 << 30, tm, tn};
       }
     }
   }
@@ -400,16 +459,37 @@ static int operand_map(CUtensorMap* map, const MmaOperand& o, int64_t rows, int6
   return r == CUDA_SUCCESS ? GL_OK : GL_ERR_SHAPE;
 }
 
-template <int BN, int NPA, int NPB>
+template <int CTAS, int BN, int NPA, int NPB>
 static int launch_mma(const CUtensorMap& ta, const CUtensorMap& tb, const MmaParams& p, int sms, cudaStream_t st) {
-  const size_t smem = mm_stages(BN, NPA, NPB) * mm_stage_bytes(BN, NPA, NPB) + 1024;
-  if (int rc = ensure_dynamic_smem((const void*)mma_kernel<BN, NPA, NPB>, smem)) return rc;
-  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-  mma_kernel<BN, NPA, NPB><<<(unsigned)(items < sms ? items : sms), kMmThreads, smem, st>>>(ta, tb, p);
-  const cudaError_t e = cudaGetLastError();
+  const auto kernel = mma_kernel<CTAS, BN, NPA, NPB>;
+  const size_t smem = mm_slots(BN, CTAS) * mm_slot_bytes(BN, CTAS) + kMmEpiBytes + 1024;
+  if (int rc = ensure_dynamic_smem((const void*)kernel, smem)) return rc;
+  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits, most = sms / CTAS;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((items < most ? items : most) * CTAS));
+  cfg.blockDim = dim3(kMmThreads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = CTAS;
+  at.val.clusterDim.y = at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = CTAS > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
   if (e != cudaSuccess) return set_cuda_error(e);
   count_launches(1);
   return GL_OK;
+}
+
+template <int NPA, int NPB>
+static int launch_shape(const MmaPlan& pl, const CUtensorMap& ta, const CUtensorMap& tb, const MmaParams& p, int sms,
+                        cudaStream_t st) {
+  if (pl.ctas == 2) return launch_mma<2, 256, NPA, NPB>(ta, tb, p, sms, st);
+  if (pl.BN == 128) return launch_mma<1, 128, NPA, NPB>(ta, tb, p, sms, st);
+  if (pl.BN == 64) return launch_mma<1, 64, NPA, NPB>(ta, tb, p, sms, st);
+  if constexpr (NPA == 1) return launch_mma<1, 32, 1, 1>(ta, tb, p, sms, st);
+  return GL_ERR_UNSUPPORTED;
 }
 
 static bool aligned16(const void* p, int64_t ld, int esize) {
@@ -422,32 +502,31 @@ int mma_product(const MmaOperand& a, const MmaOperand& b, int64_t M, int64_t N, 
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   const MmaPlan pl = mma_plan(M, N, K, a.planes, b.planes, b.mn, sms);
+  if (pl.splits > 1 && !work) return GL_ERR_WORKSPACE;
   CUtensorMap ta, tb;
   if (int rc = operand_map(&ta, a, M, K, kMmBM)) return rc;
-  if (int rc = operand_map(&tb, b, N, K, pl.BN)) return rc;
+  if (int rc = operand_map(&tb, b, N, K, pl.BN / pl.ctas)) return rc;
   MmaParams p{};
   p.M = M; p.N = N; p.tiles_m = (int)pl.tiles_m; p.tiles_n = (int)pl.tiles_n;
   p.kblocks = (int)((K + kMmBK - 1) / kMmBK); p.chunk = pl.chunk < p.kblocks ? pl.chunk : p.kblocks;
   p.splits = pl.splits; p.split_blocks = pl.split_blocks; p.a_mn = a.mn; p.b_mn = b.mn; p.e = e;
   const int es = e.dtype == GL_DTYPE_F32 || e.accumulate ? 4 : 2;
-  p.vec = aligned16(e.out, e.ldo, es) && aligned16(e.z, e.ldz, es) && aligned16(e.residual, e.ldr, es) &&
-          aligned16(e.bias, 0, es) && aligned16(e.slope, e.lds, 1);
+  const int ss = e.slope_kind == GL_SLOPE_F32 ? 4 : e.slope_kind == GL_SLOPE_I16 ? 2 : 1;
+  const bool vec = aligned16(e.out, e.ldo, es) && aligned16(e.residual, e.ldr, es) && aligned16(e.bias, 0, es) &&
+                   (ss == 1 ? e.slope == nullptr || (((uintptr_t)e.slope | e.lds) & 7) == 0
+                            : aligned16(e.slope, e.lds, ss));
   p.part = pl.splits > 1 ? (float*)work : nullptr;
-  if (pl.splits > 1 && !work) return GL_ERR_WORKSPACE;
+  p.vec = p.part ? N % 4 == 0 : vec;
   int rc = GL_ERR_UNSUPPORTED;
-  if (a.planes == 1 && b.planes == 1) {
-    rc = pl.BN == 256   ? launch_mma<256, 1, 1>(ta, tb, p, sms, st)
-         : pl.BN == 128 ? launch_mma<128, 1, 1>(ta, tb, p, sms, st)
-         : pl.BN == 64  ? launch_mma<64, 1, 1>(ta, tb, p, sms, st)
-                        : launch_mma<32, 1, 1>(ta, tb, p, sms, st);
-  } else if (a.planes == 3 && b.planes == 3) {
-    rc = pl.BN == 128 ? launch_mma<128, 3, 3>(ta, tb, p, sms, st) : launch_mma<64, 3, 3>(ta, tb, p, sms, st);
-  } else if (a.planes == 3 && b.planes == 1) {
-    rc = pl.BN == 128 ? launch_mma<128, 3, 1>(ta, tb, p, sms, st) : launch_mma<64, 3, 1>(ta, tb, p, sms, st);
-  }
+  if (a.planes == 1 && b.planes == 1) rc = launch_shape<1, 1>(pl, ta, tb, p, sms, st);
+  else if (a.planes == 3 && b.planes == 3) rc = launch_shape<3, 3>(pl, ta, tb, p, sms, st);
+  else if (a.planes == 3 && b.planes == 1) rc = launch_shape<3, 1>(pl, ta, tb, p, sms, st);
   if (rc || pl.splits == 1) return rc;
-  const int64_t quads = M * ((N + 3) / 4), need = (quads + 255) / 256;
-  mma_join_kernel<<<(unsigned)(need < 8 * sms ? need : 8 * sms), 256, 0, st>>>(p.part, M, N, pl.splits, e, p.vec);
+  const bool wide = vec && N % 8 == 0;
+  const int64_t units = wide ? M * (N / 8) : M * N, need = (units + 255) / 256, cap = 16ll * sms;
+  const unsigned blocks = (unsigned)(need < cap ? need : cap);
+  if (wide) mma_join_kernel<8><<<blocks, 256, 0, st>>>(p.part, M, N, pl.splits, e);
+  else mma_join_kernel<1><<<blocks, 256, 0, st>>>(p.part, M, N, pl.splits, e);
   const cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return set_cuda_error(err);
   count_launches(1);

@@ -10,15 +10,15 @@
 
 namespace gl {
 
-// What follows the sum over k for an element (m, n).
+// What follows the sum over k for an element (m, n): z = sum + bias, slope = act'(z), out = act(z) + residual; or,
+// with `accumulate`, out (fp32) += sum.
 struct LinEpilogue {
   const void* bias;
   const void* residual;
   void* out;
-  void* z;
-  uint8_t* slope;
-  int64_t ldr, ldo, ldz, lds;
-  int dtype, act, accumulate;
+  void* slope;
+  int64_t ldr, ldo, lds;
+  int dtype, act, accumulate, slope_kind;
 };
 
 // A bf16 operand of `planes` planes `plane` elements apart: element (r, k) at ptr[r ld + k], or ptr[k ld + r] when
@@ -34,128 +34,124 @@ int64_t mma_work_bytes(int64_t M, int64_t N, int64_t K, int a_planes, int b_plan
 int mma_product(const MmaOperand& a, const MmaOperand& b, int64_t M, int64_t N, int64_t K, const LinEpilogue& e,
                 void* work, cudaStream_t st);
 
-__device__ __forceinline__ float ld_dense(const void* p, int64_t i, int dtype) {
-  return dtype == GL_DTYPE_F32 ? reinterpret_cast<const float*>(p)[i]
-                               : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-}
-__device__ __forceinline__ void st_dense(void* p, int64_t i, int dtype, float v) {
-  if (dtype == GL_DTYPE_F32) reinterpret_cast<float*>(p)[i] = v;
-  else reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-}
-
-__device__ __forceinline__ void lin_finish(const LinEpilogue& e, int64_t m, int64_t n, float z) {
-  if (e.accumulate) {
-    reinterpret_cast<float*>(e.out)[m * e.ldo + n] += z;
-    return;
-  }
-  if (e.bias) z += ld_dense(e.bias, n, e.dtype);
-  if (e.z) st_dense(e.z, m * e.ldz + n, e.dtype, z);
-  if (e.slope) e.slope[m * e.lds + n] = (uint8_t)slope_code(dense_slope(e.act, z));
-  float y = dense_act(e.act, z);
-  if (e.residual) y += ld_dense(e.residual, m * e.ldr + n, e.dtype);
-  st_dense(e.out, m * e.ldo + n, e.dtype, y);
-}
-
-// N consecutive elements of row m from n on, all inside the row and 16-byte aligned where they are accessed as
-// vectors (`vec`: every given tensor's base and row stride are).
-template <int N>
-__device__ __forceinline__ void ld_span(const void* p, int64_t i, int dtype, bool vec, float (&v)[N]) {
-  if (!vec) {
+// N elements of type T from p on: as 16-byte vectors where `vec`.
+template <typename T, int N>
+__device__ __forceinline__ void ld_span(const T* p, bool vec, float (&v)[N]) {
+  constexpr int V = kVec16<T>;
+  if constexpr (N % V == 0) {
+    if (vec) {
 #pragma unroll
-    for (int k = 0; k < N; ++k) v[k] = ld_dense(p, i + k, dtype);
-  } else if (dtype == GL_DTYPE_F32) {
+      for (int k = 0; k < N; k += V) {
+        float t[V];
+        load_vec<T, V>(p + k, t);
 #pragma unroll
-    for (int k = 0; k < N; k += 4) {
-      float t[4];
-      load_vec<float, 4>(reinterpret_cast<const float*>(p) + i + k, t);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[k + j] = t[j];
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; k += 8) {
-      float t[8];
-      load_vec<__nv_bfloat16, 8>(reinterpret_cast<const __nv_bfloat16*>(p) + i + k, t);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) v[k + j] = t[j];
+        for (int j = 0; j < V; ++j) v[k + j] = t[j];
+      }
+      return;
     }
   }
+#pragma unroll
+  for (int k = 0; k < N; ++k) v[k] = to_f32<T>(p[k]);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void st_span(T* p, bool vec, const float (&v)[N]) {
+  constexpr int V = kVec16<T>;
+  if constexpr (N % V == 0) {
+    if (vec) {
+#pragma unroll
+      for (int k = 0; k < N; k += V) {
+        float t[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) t[j] = v[k + j];
+        store_vec<T, V>(p + k, t);
+      }
+      return;
+    }
+  }
+#pragma unroll
+  for (int k = 0; k < N; ++k) p[k] = from_f32<T>(v[k]);
 }
 
 template <int N>
-__device__ __forceinline__ void st_span(void* p, int64_t i, int dtype, bool vec, const float (&v)[N]) {
-  if (!vec) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) st_dense(p, i + k, dtype, v[k]);
-  } else if (dtype == GL_DTYPE_F32) {
-#pragma unroll
-    for (int k = 0; k < N; k += 4) {
-      const float t[4] = {v[k], v[k + 1], v[k + 2], v[k + 3]};
-      store_vec<float, 4>(reinterpret_cast<float*>(p) + i + k, t);
-    }
-  } else {
-#pragma unroll
-    for (int k = 0; k < N; k += 8) {
-      const float t[8] = {v[k], v[k + 1], v[k + 2], v[k + 3], v[k + 4], v[k + 5], v[k + 6], v[k + 7]};
-      store_vec<__nv_bfloat16, 8>(reinterpret_cast<__nv_bfloat16*>(p) + i + k, t);
-    }
-  }
-}
-
-// act(z) in place; the branch on the activation is outside the loops.
-template <int N>
-__device__ __forceinline__ void dense_act_all(int act, float (&z)[N]) {
-  if (act == GL_ACT_RELU) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) z[k] = dense_act(GL_ACT_RELU, z[k]);
-  } else if (act == GL_ACT_GELU) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) z[k] = dense_act(GL_ACT_GELU, z[k]);
-  } else if (act == GL_ACT_SILU) {
-#pragma unroll
-    for (int k = 0; k < N; ++k) z[k] = dense_act(GL_ACT_SILU, z[k]);
-  }
-}
-
-// lin_finish for N consecutive columns.
-template <int N>
-__device__ __forceinline__ void lin_finish_span(const LinEpilogue& e, int64_t m, int64_t n, bool vec, float (&z)[N]) {
-  float t[N];
-  if (e.accumulate) {
-    ld_span<N>(e.out, m * e.ldo + n, GL_DTYPE_F32, vec, t);
-#pragma unroll
-    for (int k = 0; k < N; ++k) t[k] += z[k];
-    st_span<N>(e.out, m * e.ldo + n, GL_DTYPE_F32, vec, t);
-    return;
-  }
-  if (e.bias) {
-    ld_span<N>(e.bias, n, e.dtype, vec, t);
-#pragma unroll
-    for (int k = 0; k < N; ++k) z[k] += t[k];
-  }
-  if (e.z) st_span<N>(e.z, m * e.ldz + n, e.dtype, vec, z);
-  if (e.slope) {
-#pragma unroll
-    for (int k = 0; k < N; k += 4) {
-      uint32_t u = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) u |= slope_code(dense_slope(e.act, z[k + j])) << (8 * j);
-      uint8_t* q = e.slope + m * e.lds + n + k;
+__device__ __forceinline__ void st_slope(const LinEpilogue& e, int64_t m, int64_t n, bool vec, const float (&d)[N]) {
+  const int64_t i = m * e.lds + n;
+  if (e.slope_kind == GL_SLOPE_F32) {
+    st_span<float, N>(reinterpret_cast<float*>(e.slope) + i, vec, d);
+  } else if (e.slope_kind == GL_SLOPE_I16) {
+    uint16_t* q = reinterpret_cast<uint16_t*>(e.slope) + i;
+    if constexpr (N == 8) {
       if (vec) {
-        *reinterpret_cast<uint32_t*>(q) = u;
-      } else {
+        uint32_t u[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) q[j] = (uint8_t)(u >> (8 * j));
+        for (int k = 0; k < 4; ++k) u[k] = slope_code16(d[2 * k]) | (slope_code16(d[2 * k + 1]) << 16);
+        *reinterpret_cast<uint4*>(q) = make_uint4(u[0], u[1], u[2], u[3]);
+        return;
       }
     }
+#pragma unroll
+    for (int k = 0; k < N; ++k) q[k] = (uint16_t)slope_code16(d[k]);
+  } else {
+    uint8_t* q = reinterpret_cast<uint8_t*>(e.slope) + i;
+    if constexpr (N == 8) {
+      if (vec) {
+        uint32_t u[2] = {0, 0};
+#pragma unroll
+        for (int k = 0; k < 8; ++k) u[k / 4] |= slope_code(d[k]) << (8 * (k % 4));
+        *reinterpret_cast<uint2*>(q) = make_uint2(u[0], u[1]);
+        return;
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) q[k] = (uint8_t)slope_code(d[k]);
   }
-  dense_act_all<N>(e.act, z);
-  if (e.residual) {
-    ld_span<N>(e.residual, m * e.ldr + n, e.dtype, vec, t);
+}
+
+// N consecutive elements of row m from column n on (inside the row); `vec`: every given tensor's base and row
+// stride is a multiple of 16 bytes (of 8 for a byte slope) and n of N.
+template <typename T, int N>
+__device__ __forceinline__ void lin_finish_as(const LinEpilogue& e, int64_t m, int64_t n, bool vec, float (&z)[N]) {
+  if (e.bias) {
+    float t[N];
+    ld_span<T, N>(reinterpret_cast<const T*>(e.bias) + n, vec, t);
 #pragma unroll
     for (int k = 0; k < N; ++k) z[k] += t[k];
   }
-  st_span<N>(e.out, m * e.ldo + n, e.dtype, vec, z);
+  float r[N];
+  if (e.residual) ld_span<T, N>(reinterpret_cast<const T*>(e.residual) + m * e.ldr + n, vec, r);
+  with_act(e.act, [&](auto tag) {
+    constexpr int ACT = decltype(tag)::value;
+    if (e.slope_kind) {
+      float d[N];
+#pragma unroll
+      for (int k = 0; k < N; ++k) d[k] = dense_slope<ACT, sizeof(T) == 2>(z[k], z[k]);
+      st_slope<N>(e, m, n, vec, d);
+    } else {
+#pragma unroll
+      for (int k = 0; k < N; ++k) z[k] = dense_act<ACT, sizeof(T) == 2>(z[k]);
+    }
+  });
+  if (e.residual) {
+#pragma unroll
+    for (int k = 0; k < N; ++k) z[k] += r[k];
+  }
+  st_span<T, N>(reinterpret_cast<T*>(e.out) + m * e.ldo + n, vec, z);
+}
+
+template <int N>
+__device__ __forceinline__ void lin_finish(const LinEpilogue& e, int64_t m, int64_t n, bool vec, float (&z)[N]) {
+  if (e.accumulate) {
+    float* out = reinterpret_cast<float*>(e.out) + m * e.ldo + n;
+    float t[N];
+    ld_span<float, N>(out, vec, t);
+#pragma unroll
+    for (int k = 0; k < N; ++k) t[k] += z[k];
+    st_span<float, N>(out, vec, t);
+  } else if (e.dtype == GL_DTYPE_F32) {
+    lin_finish_as<float, N>(e, m, n, vec, z);
+  } else {
+    lin_finish_as<__nv_bfloat16, N>(e, m, n, vec, z);
+  }
 }
 
 }  // namespace gl

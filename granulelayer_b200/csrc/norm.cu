@@ -44,7 +44,7 @@ struct NormParams {
   int64_t nseg, npart;  // resident: segments per sample; backward: rows of partial dgamma / dbeta
   int64_t PR;           // positions per CTA (resident) or chunk (streaming)
   int64_t chunks;
-  int ng, cs, R, pdtype, act;
+  int ng, cs, R, pdtype, act;   // act: chosen by the launch (a template argument of the kernels)
   float eps;
 };
 
@@ -145,7 +145,7 @@ __device__ __forceinline__ void norm_barrier(int R) {
 
 
 // ---- resident forward ----
-template <typename T, int N>
+template <typename T, int N, int ACT>
 __global__ void __launch_bounds__(kNormThreads) norm_fwd_resident(NormParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   Raw<T, N>* tile = reinterpret_cast<Raw<T, N>*>(smem);
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_fwd_resident(NormParams p) 
         float f[N];
         unpack<T, N>(tile[q * nv + col], f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = dense_act(p.act, fmaf(f[i] - sub[i], mul[i], bet[i]));
+        for (int i = 0; i < N; ++i) f[i] = dense_act<ACT, sizeof(T) == 2>(fmaf(f[i] - sub[i], mul[i], bet[i]));
         store_vec<T, N>(out + (s * p.P + q0 + q) * p.C + c0 + (int64_t)col * N, f);
       }
     }
@@ -259,7 +259,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_fwd_resident(NormParams p) 
 // ---- backward, resident ----
 // A cluster keeps one segment and walks over samples, adding its dgamma / dbeta in shared memory; one partial
 // row per CTA goes to the join.
-template <typename T, int N, bool CKPT>
+template <typename T, int N, int ACT, bool CKPT>
 __global__ void __launch_bounds__(kNormThreads) norm_bwd_resident(NormParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   const size_t tbytes = ((size_t)p.PR * p.cs * sizeof(T) + 15) & ~(size_t)15;
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_bwd_resident(NormParams p) 
 #pragma unroll
             for (int i = 0; i < N; ++i) {
               const float h = (f[i] - sub[i]) * mul[i];
-              const float du = d[i] * dense_slope(p.act, fmaf(h, gam[i], bet[i]));
+              const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, gam[i], bet[i]));
               aa[i] = fmaf(du, h, aa[i]);
               ab[i] += du;
             }
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_bwd_resident(NormParams p) 
 #pragma unroll
           for (int i = 0; i < N; ++i) {
             const float h = (f[i] - sub[i]) * mul[i];
-            const float du = d[i] * dense_slope(p.act, fmaf(h, gam[i], bet[i]));
+            const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, gam[i], bet[i]));
             f[i] = mul[i] * (fmaf(du, gam[i], -m1[i]) - h * m2[i]);
           }
           store_vec<T, N>(out + (s * p.P + q0 + q) * p.C + c, f);
@@ -498,7 +498,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_stats_join_kernel(NormParam
   }
 }
 
-template <typename T, int N>
+template <typename T, int N, int ACT>
 __global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(NormParams p) {
   const ChunkAt a = chunk_at<N>(p);
   if (!a.live) return;
@@ -516,13 +516,13 @@ __global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(NormParams p) 
     float f[N];
     unpack<T, N>(read_x<T, N, false>(p, a.s, a.q0 + q, a.c), f);
 #pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = dense_act(p.act, fmaf(f[i] - sub[i], mul[i], bet[i]));
+    for (int i = 0; i < N; ++i) f[i] = dense_act<ACT, sizeof(T) == 2>(fmaf(f[i] - sub[i], mul[i], bet[i]));
     store_vec<T, N>(out + (a.s * p.P + a.q0 + q) * p.C + a.c, f);
   }
 }
 
 // Per chunk and channel: dgamma and dbeta partials, part[((s chunks + chunk) 2 + {0, 1}) C + c].
-template <typename T, int N, bool CKPT>
+template <typename T, int N, int ACT, bool CKPT>
 __global__ void __launch_bounds__(kNormThreads) norm_bwd_stats_kernel(NormParams p) {
   __shared__ float r1[kNormThreads * N], r2[kNormThreads * N];
   const ChunkAt a = chunk_at<N>(p);
@@ -545,7 +545,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_bwd_stats_kernel(NormParams
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const float h = (f[i] - sub[i]) * mul[i];
-        const float du = d[i] * dense_slope(p.act, fmaf(h, gam[i], bet[i]));
+        const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, gam[i], bet[i]));
         s1[i] = fmaf(du, h, s1[i]);
         s2[i] += du;
       }
@@ -606,7 +606,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_bwd_join_kernel(NormParams 
   }
 }
 
-template <typename T, int N, bool CKPT>
+template <typename T, int N, int ACT, bool CKPT>
 __global__ void __launch_bounds__(kNormThreads) norm_bwd_apply_kernel(NormParams p, const float* coef) {
   const ChunkAt a = chunk_at<N>(p);
   if (!a.live) return;
@@ -630,7 +630,7 @@ __global__ void __launch_bounds__(kNormThreads) norm_bwd_apply_kernel(NormParams
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const float h = (f[i] - sub[i]) * mul[i];
-      const float du = d[i] * dense_slope(p.act, fmaf(h, gam[i], bet[i]));
+      const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, gam[i], bet[i]));
       f[i] = mul[i] * (fmaf(du, gam[i], -m1[i]) - h * m2[i]);
     }
     store_vec<T, N>(out + (a.s * p.P + a.q0 + q) * p.C + a.c, f);
@@ -765,35 +765,49 @@ static int launched(int n) {
   return GL_OK;
 }
 
-template <typename T, int N>
-static int run_norm_fwd(NormParams& p, const NormPlan& pl, cudaStream_t st) {
-  if (pl.resident) return launch_cluster(norm_fwd_resident<T, N>, p, p.S * pl.nseg * pl.R, pl.R, pl.smem, st);
+template <typename T, int N, int ACT>
+static int run_norm_fwd_act(NormParams& p, const NormPlan& pl, cudaStream_t st) {
+  if (pl.resident) return launch_cluster(norm_fwd_resident<T, N, ACT>, p, p.S * pl.nseg * pl.R, pl.R, pl.smem, st);
   const int64_t segs = (p.C / N + kNormThreads - 1) / kNormThreads, blocks = p.S * pl.chunks * segs;
   if (blocks > 0x7FFFFFFF || p.S * p.G > 0x7FFFFFFF) return GL_ERR_SHAPE;
   norm_stats_kernel<T, N><<<(unsigned)blocks, kNormThreads, 0, st>>>(p);
   norm_stats_join_kernel<<<(unsigned)(p.S * p.G), kNormThreads, 0, st>>>(p);
-  norm_apply_kernel<T, N><<<(unsigned)blocks, kNormThreads, 0, st>>>(p);
+  norm_apply_kernel<T, N, ACT><<<(unsigned)blocks, kNormThreads, 0, st>>>(p);
   return launched(3);
 }
 
-template <typename T, int N, bool CKPT>
-static int run_norm_bwd(NormParams& p, const NormPlan& pl, const GlNormBwdArgs& a, cudaStream_t st) {
+template <typename T, int N>
+static int run_norm_fwd(NormParams& p, const NormPlan& pl, cudaStream_t st) {
+  int rc = GL_ERR_UNSUPPORTED;
+  with_act(p.act, [&](auto tag) { rc = run_norm_fwd_act<T, N, decltype(tag)::value>(p, pl, st); });
+  return rc;
+}
+
+template <typename T, int N, int ACT, bool CKPT>
+static int run_norm_bwd_act(NormParams& p, const NormPlan& pl, const GlNormBwdArgs& a, cudaStream_t st) {
   if (pl.resident) {
-    if (int rc = launch_cluster(norm_bwd_resident<T, N, CKPT>, p, pl.walkers * pl.nseg * pl.R, pl.R, pl.smem, st))
+    if (int rc = launch_cluster(norm_bwd_resident<T, N, ACT, CKPT>, p, pl.walkers * pl.nseg * pl.R, pl.R, pl.smem, st))
       return rc;
   } else {
     const int64_t segs = (p.C / N + kNormThreads - 1) / kNormThreads, blocks = p.S * pl.chunks * segs;
     if (blocks > 0x7FFFFFFF || p.S * p.G > 0x7FFFFFFF) return GL_ERR_SHAPE;
     float* coef = p.part + pl.npart * 2 * p.C;
-    norm_bwd_stats_kernel<T, N, CKPT><<<(unsigned)blocks, kNormThreads, 0, st>>>(p);
+    norm_bwd_stats_kernel<T, N, ACT, CKPT><<<(unsigned)blocks, kNormThreads, 0, st>>>(p);
     norm_bwd_join_kernel<<<(unsigned)(p.S * p.G), kNormThreads, 0, st>>>(p, coef);
-    norm_bwd_apply_kernel<T, N, CKPT><<<(unsigned)blocks, kNormThreads, 0, st>>>(p, coef);
+    norm_bwd_apply_kernel<T, N, ACT, CKPT><<<(unsigned)blocks, kNormThreads, 0, st>>>(p, coef);
     if (int rc = launched(3)) return rc;
   }
   if (!a.dw && !a.db) return GL_OK;
   norm_param_join_kernel<<<(unsigned)((p.C + 31) / 32), 256, 0, st>>>(p.part, pl.npart, p.C, a.dw, a.db, a.pdtype,
                                                                      a.accumulate);
   return launched(1);
+}
+
+template <typename T, int N, bool CKPT>
+static int run_norm_bwd(NormParams& p, const NormPlan& pl, const GlNormBwdArgs& a, cudaStream_t st) {
+  int rc = GL_ERR_UNSUPPORTED;
+  with_act(p.act, [&](auto tag) { rc = run_norm_bwd_act<T, N, decltype(tag)::value, CKPT>(p, pl, a, st); });
+  return rc;
 }
 
 // Zero parameter gradients of an empty batch (nothing is added to accumulated ones).

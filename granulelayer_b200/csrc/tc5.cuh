@@ -78,6 +78,35 @@ __device__ __forceinline__ void t5_commit(uint32_t mbar_smem) {
 __device__ __forceinline__ void t5_fence_before_sync() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void t5_fence_after_sync() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 
+// ---- CTA pairs (cta_group::2): one MMA over the shared and tensor memory of two CTAs of a cluster ----
+__device__ __forceinline__ void t5_tmem_alloc2(uint32_t dst_smem, uint32_t ncols) {
+  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst_smem), "r"(ncols));
+  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::);
+}
+
+__device__ __forceinline__ void t5_tmem_dealloc2(uint32_t taddr, uint32_t ncols) {
+  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols));
+}
+
+// D (M = 256: 128 rows in each CTA's TMEM) = A * B (+ D): each CTA's shared memory holds its 128 rows of A and half of
+// B's N rows, at the same offsets.  One thread of the even CTA issues.
+__device__ __forceinline__ void t5_mma_bf16_pair(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                                 uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}\n" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate));
+}
+
+// Arrive on the mbarrier at this offset in both CTAs once every MMA this thread issued before has completed.
+__device__ __forceinline__ void t5_commit_pair(uint32_t mbar_smem) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+          mbar_smem),
+      "h"((uint16_t)3)
+      : "memory");
+}
+
 // Generic-proxy shared-memory writes become visible to the tensor cores (async proxy).
 __device__ __forceinline__ void t5_fence_smem_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 

@@ -146,10 +146,15 @@ def _returned(p, buf):
 
 # ---- linear ----
 
-def _linear_forward(x2, weight, bias, r2, act, z, slope):
+# act'(z) as the backward pass keeps it: as it is in fp32 layers, in steps of 2^-14 (bf16 would cost the gradient a
+# second rounding to 8 bits) in bf16 ones, in steps of 1/192 in an 8-bit checkpoint
+_SLOPE_DTYPES = {torch.float32: torch.float32, torch.bfloat16: torch.int16}
+
+
+def _linear_forward(x2, weight, bias, r2, act, slope):
     y = torch.empty((x2.shape[0], weight.shape[0]), dtype=x2.dtype, device=x2.device)
     if x2.shape[0]:
-        _native.linear_fwd(x2, weight, bias, r2, y, z, slope, act)
+        _native.linear_fwd(x2, weight, bias, r2, y, slope, act)
     return y
 
 
@@ -159,31 +164,29 @@ class LinearActFunction(torch.autograd.Function):
         M, K, N = x.numel() // x.shape[-1], x.shape[-1], weight.shape[0]
         x2, w2 = _rows(x, K), _rows(weight, K)
         r2 = None if residual is None else _rows(residual, N)
-        z = slope = codes = exps = None
+        slope = codes = exps = None
         if act != 0:
-            if checkpoint == "int8":
-                slope = torch.empty((M, N), dtype=torch.uint8, device=x.device)
-            else:
-                z = torch.empty((M, N), dtype=x.dtype, device=x.device)
-        y = _linear_forward(x2, w2, bias, r2, act, z, slope)
+            slope = torch.empty((M, N), dtype=torch.uint8 if checkpoint == "int8" else _SLOPE_DTYPES[x.dtype],
+                                device=x.device)
+        y = _linear_forward(x2, w2, bias, r2, act, slope)
         if checkpoint == "int8":
             codes, exps = _encode(x2)
-        ctx.save_for_backward(x2 if codes is None else None, codes, exps, weight, bias, z, slope)
-        ctx.act, ctx.xshape = act, x.shape
+        ctx.save_for_backward(x2 if codes is None else None, codes, exps, weight, bias, slope)
+        ctx.xshape = x.shape
         return y.view(*x.shape[:-1], N)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x2, codes, exps, weight, bias, z, slope = ctx.saved_tensors
+        x2, codes, exps, weight, bias, slope = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         N, K = weight.shape
         dx = torch.empty(ctx.xshape, dtype=dy.dtype, device=dy.device) if need_x else None
         (dw, db), main = _grad_buffers((weight, need_w), (bias, need_b))
         if need_x or need_w or need_b:
             w2 = _rows(weight, K) if need_x else None
-            _native.linear_bwd(_rows(dy, N), z, slope, x2, codes, exps, w2, dx.view(-1, K) if need_x else None, dw, db,
-                               K, ctx.act, main)
+            _native.linear_bwd(_rows(dy, N), slope, x2, codes, exps, w2, dx.view(-1, K) if need_x else None, dw, db,
+                               K, main)
         return dx, _returned(weight, dw), _returned(bias, db), dy if need_r else None, None, None
 
 
@@ -212,7 +215,7 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
         return LinearActFunction.apply(x, weight, bias, residual, act, checkpoint)
     K = x.shape[-1]
     y = _linear_forward(_rows(x, K), _rows(weight, K), bias, None if residual is None else _rows(residual, N), act,
-                        None, None)
+                        None)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
 

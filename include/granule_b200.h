@@ -502,31 +502,31 @@ int gl_k16_bwd_t5_f32(const GlK16Args* args, int32_t* status, void* stream);
  * kernels has an iteration limit; a tile whose wait ran out is written as NaN. */
 
 /* Forward of a fused matrix product: y = act(z) + residual, z[m, n] = sum_k x[m, k] w[n, k] + bias[n].
- * `bias` [N], `residual` [M, ldr], `z` and `slope` are optional.  For the backward pass the call also keeps
- * `z` [M, ldz] (dtype) or `slope` [M, lds] (one byte per element: round(192 act'(z)) + 32), as given. */
+ * `bias` [N] and `residual` [M, ldr] are optional.  For the backward pass the call also keeps act'(z) in `slope`
+ * [M, lds] as `slope_kind` says: GL_SLOPE_F32 as it is, GL_SLOPE_I16 round(2^14 act'(z)), GL_SLOPE_U8
+ * round(192 act'(z)) + 32 (both exact at 0 and 1). */
+enum { GL_SLOPE_NONE = 0, GL_SLOPE_F32 = 1, GL_SLOPE_I16 = 2, GL_SLOPE_U8 = 3 };
 typedef struct GlLinearArgs {
   const void* x;            /* [M, ldx] */
   const void* w;            /* [N, ldw] */
   const void* bias;
   const void* residual;
   void* y;                  /* [M, ldy] */
-  void* z;
-  uint8_t* slope;
+  void* slope;
   void* work;
-  int64_t M, N, K, ldx, ldw, ldr, ldy, ldz, lds, work_bytes;
-  int32_t dtype, act;
+  int64_t M, N, K, ldx, ldw, ldr, ldy, lds, work_bytes;
+  int32_t dtype, act, slope_kind, reserved;
 } GlLinearArgs;
 int gl_linear_fwd(const GlLinearArgs* args, void* stream);
 
-/* Backward: dz = dy act'(z) with act' from `z` or `slope` (neither: act is the identity),
+/* Backward: dz = dy act'(z) with act'(z) from `slope` (GL_SLOPE_NONE: act is the identity),
  *   dx = dz w, dw = dz^T x, db = column sums of dz, each where its output is given.
  * x comes as it was (`x`) or as an 8-bit checkpoint (`codes` [M, ldc] and `exps` [M, ceil(K / 32)], gl_act8_*).
  * dx [M, lddx] has the storage type; dw [N, K] and db [N] (contiguous) too, or, with `accumulate`, are fp32 and
  * added to. */
 typedef struct GlLinearBwdArgs {
   const void* dy;           /* [M, lddy] */
-  const void* z;
-  const uint8_t* slope;
+  const void* slope;
   const void* x;
   const int8_t* codes;
   const uint8_t* exps;
@@ -535,8 +535,8 @@ typedef struct GlLinearBwdArgs {
   void* dw;
   void* db;
   void* work;
-  int64_t M, N, K, lddy, ldz, lds, ldx, ldc, ldw, lddx, work_bytes;
-  int32_t dtype, act, accumulate, reserved;
+  int64_t M, N, K, lddy, lds, ldx, ldc, ldw, lddx, work_bytes;
+  int32_t dtype, slope_kind, accumulate, reserved;
 } GlLinearBwdArgs;
 int gl_linear_bwd(const GlLinearBwdArgs* args, void* stream);
 /* `flags`: of GL_LINEAR_*; UNALIGNED where x, or w, has a base or row stride that 16 bytes do not divide (needed for
