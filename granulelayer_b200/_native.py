@@ -715,13 +715,16 @@ def k16_auto_tokens(B: int, S: int, backward: bool) -> int:
 
 # ---- dense operators (dense.py) ----
 # The launches are short, so these helpers keep the host's share small: no device switch when the tensors'
-# device is current, and one call for the workspace size of each new set of sizes.
+# device is current, and one call for the workspace size of each new set of sizes.  dense.py has checked devices
+# and types.
 
 _work_sizes = {}
+_NO_WORK = torch.empty(0, dtype=torch.uint8)   # data_ptr() 0
+_DTYPE_IDS = {torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16}
 
 
 def _work(name: str, dev: torch.device, *sizes):
-    """Scratch of gl_<name>_work_bytes(*sizes) bytes on ``dev`` (None where the call needs none)."""
+    """Scratch of gl_<name>_work_bytes(*sizes) bytes on ``dev`` (an empty tensor where the call needs none)."""
     key = (name, dev.index, sizes)
     n = _work_sizes.get(key)
     if n is None:
@@ -733,7 +736,7 @@ def _work(name: str, dev: torch.device, *sizes):
         if len(_work_sizes) > 4096:
             _work_sizes.clear()
         _work_sizes[key] = n
-    return torch.empty(n, dtype=torch.uint8, device=dev) if n else None
+    return _NO_WORK if n == 0 else torch.empty(n, dtype=torch.uint8, device=dev)
 
 
 def _launch(name: str, a, dev: torch.device):
@@ -762,75 +765,66 @@ _SLOPE_KINDS = {torch.float32: 1, torch.int16: 2, torch.uint8: 3}
 def linear_fwd(x, w, bias, residual, y, slope, act: int):
     """y = act(x w^T + bias) + residual (GlLinearArgs); 2-d tensors with unit column stride.  ``slope`` (optional,
     float32, int16 or uint8 [M, N]) receives act'(z)."""
-    _require_cuda(x, w, bias, residual, y, slope)
     M, K = x.shape
-    N, dt = w.shape[0], _wdtype(w)
-    work = _work("gl_linear_work_bytes", x.device, M, N, K, dt, _unaligned(x, w))
+    N, dt, dev = w.shape[0], _DTYPE_IDS[w.dtype], x.device
+    work = _work("gl_linear_work_bytes", dev, M, N, K, dt, _unaligned(x, w))
     _launch("gl_linear_fwd", GlLinearArgs(
-        x.data_ptr(), w.data_ptr(), _ptr(bias), _ptr(residual), y.data_ptr(), _ptr(slope), _ptr(work),
-        M, N, K, x.stride(0), w.stride(0), residual.stride(0) if residual is not None else 0, y.stride(0),
-        slope.stride(0) if slope is not None else 0, work.numel() if work is not None else 0, dt, act,
-        _SLOPE_KINDS[slope.dtype] if slope is not None else 0, 0), x.device)
+        x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(),
+        0 if residual is None else residual.data_ptr(), y.data_ptr(), 0 if slope is None else slope.data_ptr(),
+        work.data_ptr(), M, N, K, x.stride(0), w.stride(0), 0 if residual is None else residual.stride(0), N,
+        0 if slope is None else N, work.numel(), dt, act, 0 if slope is None else _SLOPE_KINDS[slope.dtype], 0), dev)
 
 
 def linear_bwd(dy, slope, x, codes, exps, w, dx, dw, db, K: int, accumulate: bool):
     """dx, dw, db (each may be None) of linear_fwd for the output gradient dy (GlLinearBwdArgs)."""
-    _require_cuda(dy, slope, x, codes, exps, w, dx, dw, db)
     M, N = dy.shape
-    dt = _wdtype(dy)
-    work = _work("gl_linear_work_bytes", dy.device, M, N, K, dt, 1 | (2 if codes is not None else 0) |
-                 _unaligned(w if dx is not None else None, x if dw is not None else None))
-
-    def ld(t):
-        return t.stride(0) if t is not None else 0
-
+    dt, dev = _DTYPE_IDS[dy.dtype], dy.device
+    work = _work("gl_linear_work_bytes", dev, M, N, K, dt, 1 | (0 if codes is None else 2) |
+                 _unaligned(None if dx is None else w, None if dw is None else x))
     _launch("gl_linear_bwd", GlLinearBwdArgs(
         dy.data_ptr(), _ptr(slope), _ptr(x), _ptr(codes), _ptr(exps), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db),
-        _ptr(work), M, N, K, dy.stride(0), ld(slope), ld(x), ld(codes), ld(w), ld(dx),
-        work.numel() if work is not None else 0, dt, _SLOPE_KINDS[slope.dtype] if slope is not None else 0,
-        int(accumulate), 0), dy.device)
+        work.data_ptr(), M, N, K, dy.stride(0), 0 if slope is None else N, 0 if x is None else x.stride(0),
+        0 if codes is None else codes.stride(0), 0 if w is None else w.stride(0), K, work.numel(), dt,
+        0 if slope is None else _SLOPE_KINDS[slope.dtype], int(accumulate), 0), dev)
 
 
 def _pdtype(*params) -> int:
     """GL_DTYPE_* of the parameters that are given (fp32 when none is)."""
-    return next((_wdtype(p) for p in params if p is not None), DTYPE_F32)
+    for p in params:
+        if p is not None:
+            return _DTYPE_IDS[p.dtype]
+    return DTYPE_F32
 
 
-def norm_fwd(x, w, b, y, mean, rstd, G: int, act: int, eps: float):
-    """y = act(group_norm(x) w + b) of x [S, P, C] (GlNormArgs); mean / rstd [S, G] fp32 are written."""
-    _require_cuda(x, w, b, y, mean, rstd)
+def norm_fwd(x, w, b, y, stats, G: int, act: int, eps: float):
+    """y = act(group_norm(x) w + b) of x [S, P, C] (GlNormArgs); stats [2, S, G] fp32 receives mean and rstd."""
     S, P, C = x.shape
-    dt = _wdtype(x)
-    work = _work("gl_norm_work_bytes", x.device, S, P, C, G, dt, 0)
+    dt, dev, at = _DTYPE_IDS[x.dtype], x.device, stats.data_ptr()
+    work = _work("gl_norm_work_bytes", dev, S, P, C, G, dt, 0)
     _launch("gl_norm_fwd", GlNormArgs(
-        x.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), mean.data_ptr(), rstd.data_ptr(), _ptr(work), S, P, C, G,
-        x.stride(0), x.stride(1), work.numel() if work is not None else 0, dt,
-        _pdtype(w, b), act, eps), x.device)
+        x.data_ptr(), _ptr(w), _ptr(b), y.data_ptr(), at, at + 4 * S * G, work.data_ptr(), S, P, C, G,
+        x.stride(0), x.stride(1), work.numel(), dt, _pdtype(w, b), act, eps), dev)
 
 
-def norm_bwd(dy, x, codes, exps, w, b, mean, rstd, dx, dw, db, G: int, act: int, accumulate: bool):
+def norm_bwd(dy, x, codes, exps, w, b, stats, dx, dw, db, G: int, act: int, accumulate: bool):
     """dx, dw, db (the last two may be None) of norm_fwd (GlNormBwdArgs)."""
-    _require_cuda(dy, x, codes, exps, w, b, mean, rstd, dx, dw, db)
     S, P, C = dy.shape
-    dt = _wdtype(dy)
-    work = _work("gl_norm_work_bytes", dy.device, S, P, C, G, dt, 1)
+    dt, dev, at = _DTYPE_IDS[dy.dtype], dy.device, stats.data_ptr()
+    work = _work("gl_norm_work_bytes", dev, S, P, C, G, dt, 1)
     _launch("gl_norm_bwd", GlNormBwdArgs(
-        dy.data_ptr(), _ptr(x), _ptr(codes), _ptr(exps), _ptr(w), _ptr(b), mean.data_ptr(), rstd.data_ptr(),
-        dx.data_ptr(), _ptr(dw), _ptr(db), _ptr(work), S, P, C, G, x.stride(0) if x is not None else 0,
-        x.stride(1) if x is not None else 0, dy.stride(0), dy.stride(1),
-        codes.stride(0) if codes is not None else 0, work.numel() if work is not None else 0, dt,
-        _pdtype(w, b), act, int(accumulate)), dy.device)
+        dy.data_ptr(), _ptr(x), _ptr(codes), _ptr(exps), _ptr(w), _ptr(b), at, at + 4 * S * G,
+        dx.data_ptr(), _ptr(dw), _ptr(db), work.data_ptr(), S, P, C, G, 0 if x is None else x.stride(0),
+        0 if x is None else x.stride(1), dy.stride(0), dy.stride(1), 0 if codes is None else codes.stride(0),
+        work.numel(), dt, _pdtype(w, b), act, int(accumulate)), dev)
 
 
 def act8_encode(x, codes, exps):
     """int8 codes and exponent bytes of x [rows, C] (GlAct8Args)."""
-    _require_cuda(x, codes, exps)
     _launch("gl_act8_encode", GlAct8Args(x.data_ptr(), 0, codes.data_ptr(), exps.data_ptr(), x.shape[0], x.shape[1],
-                                         x.stride(0), codes.stride(0), _wdtype(x), 0), x.device)
+                                         x.stride(0), codes.stride(0), _DTYPE_IDS[x.dtype], 0), x.device)
 
 
 def act8_decode(codes, exps, out):
     """out [rows, C] = the values of an 8-bit checkpoint (GlAct8Args)."""
-    _require_cuda(codes, exps, out)
     _launch("gl_act8_decode", GlAct8Args(0, out.data_ptr(), codes.data_ptr(), exps.data_ptr(), out.shape[0],
-                                         out.shape[1], out.stride(0), codes.stride(0), _wdtype(out), 0), out.device)
+                                         out.shape[1], out.stride(0), codes.stride(0), _DTYPE_IDS[out.dtype], 0), out.device)

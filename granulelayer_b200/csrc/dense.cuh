@@ -45,6 +45,20 @@ __device__ __forceinline__ void load_vec(const T* p, float (&v)[V]) {
   }
 }
 
+// V elements held as loaded (16 bytes, or one element) until they are used.
+template <typename T, int V>
+struct Vec16 {
+  uint4 v;
+  __device__ __forceinline__ void load(const T* p) { v = __ldg(reinterpret_cast<const uint4*>(p)); }
+  __device__ __forceinline__ void get(float (&f)[V]) const { load_vec<T, V>(reinterpret_cast<const T*>(&v), f); }
+};
+template <typename T>
+struct Vec16<T, 1> {
+  T v;
+  __device__ __forceinline__ void load(const T* p) { v = *p; }
+  __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = to_f32<T>(v); }
+};
+
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);

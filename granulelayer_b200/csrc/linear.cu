@@ -57,190 +57,234 @@ __device__ __forceinline__ void load8(const T* p, int64_t left, bool aligned, fl
   }
 }
 
-// rows x K (row stride ld) -> planes [NP][rows][Kp], Kp = K rounded up to 8.
+// Up to two matrices rows x K (row stride ld) -> planes [NP][rows][K rounded up to 8], in one launch.
+struct PackJob {
+  const void* src;
+  uint16_t* dst;
+  int64_t rows, nk, K, ld;   // nk = ceil(K / 8)
+  int aligned;
+};
+
 template <typename T, int NP>
-__global__ void __launch_bounds__(256) lin_pack_kernel(const T* src, uint16_t* dst, int64_t rows, int64_t K,
-                                                       int64_t ld, int aligned) {
-  const int64_t nk = (K + 7) / 8, total = rows * nk, plane = total * 8;
-  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < total; i += gridDim.x * 256ll) {
-    const int64_t r = i / nk, k = (i - r * nk) * 8;
+__global__ void __launch_bounds__(256) lin_pack_kernel(PackJob j0, PackJob j1) {
+  const int64_t n0 = j0.rows * j0.nk, total = n0 + j1.rows * j1.nk;
+  for (int64_t t = blockIdx.x * 256ll + threadIdx.x; t < total; t += gridDim.x * 256ll) {
+    const bool second = t >= n0;
+    const PackJob& j = second ? j1 : j0;
+    const int64_t i = second ? t - n0 : t, r = i / j.nk, k = (i - r * j.nk) * 8, plane = j.rows * j.nk * 8;
     float v[8];
-    load8<T>(src + r * ld + k, K - k, aligned, v);
+    load8<T>(reinterpret_cast<const T*>(j.src) + r * j.ld + k, j.K - k, j.aligned, v);
     uint4 u[NP];
     bf16_terms<NP>(v, u);
 #pragma unroll
-    for (int j = 0; j < NP; ++j) *reinterpret_cast<uint4*>(dst + j * plane + i * 8) = u[j];
+    for (int q = 0; q < NP; ++q) *reinterpret_cast<uint4*>(j.dst + q * plane + i * 8) = u[q];
   }
 }
 
-constexpr int kDzRows = 64;   // rows of one block of the dz kernel, and of one partial column sum
+constexpr int kDzRows = 32;   // rows of one block of the dz kernel, and of one partial column sum
 
-// Eight saved derivatives from element i of `slope` on (`left` of them inside the row).
 template <int KIND>
-__device__ __forceinline__ void load_slope8(const void* slope, int64_t i, int64_t left, bool aligned, float (&d)[8]) {
+__device__ __forceinline__ float slope_at(const void* slope, int64_t i) {
+  if constexpr (KIND == GL_SLOPE_F32) return reinterpret_cast<const float*>(slope)[i];
+  else if constexpr (KIND == GL_SLOPE_I16) return slope_value16(reinterpret_cast<const uint16_t*>(slope)[i]);
+  else return slope_value(reinterpret_cast<const uint8_t*>(slope)[i]);
+}
+
+// Eight saved derivatives from element i on, as one aligned load (two for fp32).
+template <int KIND>
+__device__ __forceinline__ void slope8(const void* slope, int64_t i, float (&d)[8]) {
   if constexpr (KIND == GL_SLOPE_F32) {
-    load8<float>(reinterpret_cast<const float*>(slope) + i, left, aligned, d);
+    ld_span<float, 8>(reinterpret_cast<const float*>(slope) + i, true, d);
   } else if constexpr (KIND == GL_SLOPE_I16) {
-    const uint16_t* q = reinterpret_cast<const uint16_t*>(slope) + i;
-    if (aligned && left >= 8) {
-      const uint4 t = *reinterpret_cast<const uint4*>(q);
-      const uint32_t u[4] = {t.x, t.y, t.z, t.w};
+    const uint4 t = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(slope) + i);
+    const uint32_t u[4] = {t.x, t.y, t.z, t.w};
 #pragma unroll
-      for (int k = 0; k < 8; ++k) d[k] = slope_value16((u[k / 2] >> (16 * (k & 1))) & 0xFFFF);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) d[k] = k < left ? slope_value16(q[k]) : 0.f;
-    }
+    for (int k = 0; k < 8; ++k) d[k] = slope_value16((u[k / 2] >> (16 * (k & 1))) & 0xFFFF);
   } else {
-    const uint8_t* q = reinterpret_cast<const uint8_t*>(slope) + i;
-    if (aligned && left >= 8) {
-      const uint2 u = *reinterpret_cast<const uint2*>(q);
+    const uint2 u = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(slope) + i);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) d[k] = slope_value(((k < 4 ? u.x : u.y) >> (8 * (k % 4))) & 0xFF);
-    } else {
-#pragma unroll
-      for (int k = 0; k < 8; ++k) d[k] = k < left ? slope_value(q[k]) : 0.f;
-    }
+    for (int k = 0; k < 8; ++k) d[k] = slope_value(((k < 4 ? u.x : u.y) >> (8 * (k % 4))) & 0xFF);
   }
 }
 
 // dz planes [NP][M][Np] (where `dz` is given) and the column sums of each block of kDzRows rows.  A warp spans 256
-// columns, eight per lane; the block's eight warps take every eighth row.
-template <typename T, int NP, int KIND>
-__global__ void __launch_bounds__(256) lin_dz_kernel(const T* dy, const void* slope, uint16_t* dz, float* part,
-                                                     int64_t M, int64_t N, int64_t lddy, int64_t lds, int aligned) {
-  __shared__ float red[8][256 + 8];
+// columns of a row, and the block's eight warps take every eighth row.  VEC: a lane holds eight consecutive
+// columns, in 16-byte accesses; else (rows that are not aligned, or cut) lane + 32 i, in coalesced single ones.
+template <typename T, int NP, int KIND, bool VEC>
+__device__ __forceinline__ void lin_dz_rows(const T* dy, const void* slope, uint16_t* dz, float (&sum)[8], int64_t m0,
+                                            int64_t m1, int64_t n0, int64_t N, int64_t plane, int64_t Np,
+                                            int64_t lddy, int64_t lds) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t segs = (N + 255) / 256, Np = (N + 7) / 8 * 8, plane = M * Np;
-  const int64_t rc = blockIdx.x / segs, n = (blockIdx.x - rc * segs) * 256 + lane * 8, left = N - n;
-  float sum[8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) sum[i] = 0.f;
-  if (left > 0) {
-    const int64_t m1 = min(M, (rc + 1) * kDzRows);
-#pragma unroll 4
-    for (int64_t m = rc * kDzRows + warp; m < m1; m += 8) {
-      float d[8];
-      load8<T>(dy + m * lddy + n, left, aligned, d);
+  for (int h = 0; h < kDzRows / 8; ++h) {
+    const int64_t m = m0 + warp + 8 * h;
+    if (m >= m1) break;
+    float d[8];
+    if constexpr (VEC) {
+      const int64_t n = n0 + lane * 8;
+      ld_span<T, 8>(dy + m * lddy + n, true, d);
       if constexpr (KIND != GL_SLOPE_NONE) {
         float s[8];
-        load_slope8<KIND>(slope, m * lds + n, left, aligned, s);
+        slope8<KIND>(slope, m * lds + n, s);
 #pragma unroll
         for (int i = 0; i < 8; ++i) d[i] *= s[i];
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sum[i] += d[i];
       if (dz) {
         uint4 u[NP];
         bf16_terms<NP>(d, u);
 #pragma unroll
         for (int j = 0; j < NP; ++j) *reinterpret_cast<uint4*>(dz + j * plane + m * Np + n) = u[j];
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int64_t n = n0 + lane + 32 * i;
+        d[i] = n < N ? to_f32<T>(dy[m * lddy + n]) : 0.f;
+        if constexpr (KIND != GL_SLOPE_NONE) d[i] *= n < N ? slope_at<KIND>(slope, m * lds + n) : 0.f;
+      }
+      if (dz) {
+        uint4 u[NP];
+        bf16_terms<NP>(d, u);
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+          const uint32_t q[4] = {u[j].x, u[j].y, u[j].z, u[j].w};
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const int64_t n = n0 + lane + 32 * i;
+            if (n < Np) dz[j * plane + m * Np + n] = (uint16_t)(q[i / 2] >> (16 * (i & 1)));
+          }
+        }
+      }
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) sum[i] += d[i];
   }
+}
+
+template <typename T, int NP, int KIND>
+__global__ void __launch_bounds__(256) lin_dz_kernel(const T* dy, const void* slope, uint16_t* dz, float* part,
+                                                     int64_t M, int64_t N, int64_t lddy, int64_t lds, int aligned) {
+  __shared__ float red[8][256 + 8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t segs = (N + 255) / 256, Np = (N + 7) / 8 * 8, plane = M * Np;
+  const int64_t rc = blockIdx.x / segs, n0 = (blockIdx.x - rc * segs) * 256;
+  const int64_t m0 = rc * kDzRows, m1 = min(M, m0 + kDzRows);
+  const bool vec = aligned && n0 + 256 <= N;
+  float sum[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) sum[i] = 0.f;
+  if (vec) lin_dz_rows<T, NP, KIND, true>(dy, slope, dz, sum, m0, m1, n0, N, plane, Np, lddy, lds);
+  else lin_dz_rows<T, NP, KIND, false>(dy, slope, dz, sum, m0, m1, n0, N, plane, Np, lddy, lds);
   if (part == nullptr) return;
 #pragma unroll
   for (int i = 0; i < 8; ++i) red[warp][lane + 33 * i] = sum[i];
   __syncthreads();
-  const int c = threadIdx.x, src = c / 8 + 33 * (c % 8);   // column c of the block's 256
-  const int64_t col = n - lane * 8 + c;
-  if (col < N) {
+  const int c = threadIdx.x;                                 // column of the block's 256
+  const int src = vec ? c / 8 + 33 * (c % 8) : c % 32 + 33 * (c / 32);
+  if (n0 + c < N) {
     float s = 0.f;
 #pragma unroll
     for (int r = 0; r < 8; ++r) s += red[r][src];
-    part[rc * N + col] = s;
+    part[rc * N + n0 + c] = s;
   }
 }
 
-// db = the partial column sums in block order; 32 columns per block, 8 row lanes.
-__global__ void __launch_bounds__(256) lin_db_kernel(const float* part, int64_t rows, int64_t N, void* db, int dtype,
-                                                     int accumulate) {
-  __shared__ float red[8][33];
-  const int lane = threadIdx.x & 31, r0 = threadIdx.x >> 5;
-  const int64_t n = (int64_t)blockIdx.x * 32 + lane;
-  float s = 0.f;
-  if (n < N) {
-#pragma unroll 4
-    for (int64_t r = r0; r < rows; r += 8) s += part[r * N + n];
-  }
-  red[r0][lane] = s;
-  __syncthreads();
-  if (r0 == 0 && n < N) {
-    s = 0.f;
-#pragma unroll
-    for (int r = 0; r < 8; ++r) s += red[r][lane];
-    if (accumulate) reinterpret_cast<float*>(db)[n] += s;
-    else if (dtype == GL_DTYPE_F32) reinterpret_cast<float*>(db)[n] = s;
-    else reinterpret_cast<__nv_bfloat16*>(db)[n] = __float2bfloat16_rn(s);
-  }
+// db by itself, for calls that want no product.
+__global__ void __launch_bounds__(128) lin_db_kernel(SumRows j) {
+  sum_rows(j, ((int64_t)blockIdx.x * 4 + (threadIdx.x >> 5)) * 32);
 }
 
 // ---- a few rows ----
 
-// One warp per output column n: the warp streams w's row n, four 16-byte loads in flight, against MT rows of x (from
-// L1), fp32 sums, one shuffle reduction.  Bound by reading w.
-template <typename T, int MT, bool ALIGNED>
+// W warps per output column n: each streams its part of w's row n, eight 16-byte loads in flight, against MT rows of
+// x (from L1), fp32 sums, shuffles and one shared-memory step between the W warps.  Bound by reading w; W is
+// chosen so that a warp's part is about eight loads, which keeps all of w's bytes in flight at once.
+template <typename T, int MT, int W, bool ALIGNED>
 __global__ void __launch_bounds__(128) lin_rows_kernel(const T* x, const T* w, int M, int64_t N, int64_t K,
                                                        int64_t ldx, int64_t ldw, LinEpilogue e) {
-  constexpr int V = ALIGNED ? kVec16<T> : 1, U = 4;
-  const int lane = threadIdx.x & 31;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  if (n >= N) return;
-  const T* row = w + n * ldw;
+  constexpr int V = ALIGNED ? kVec16<T> : 1, U = 8;
+  __shared__ float red[4][MT];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % W;
+  const int64_t n = (int64_t)blockIdx.x * (4 / W) + warp / W;
   float acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = 0.f;
-  int64_t k = lane * V;
-  for (; k + (U - 1) * 32 * V + V <= K; k += U * 32 * V) {
-    float wv[U][V];
+  if (n < N) {
+    const T* row = w + n * ldw;
+    constexpr int64_t kStep = (int64_t)W * 32 * V;            // k between a lane's loads
+    int64_t k = (int64_t)(part * 32 + lane) * V;
+    for (; k + (U - 1) * kStep + V <= K; k += U * kStep) {
+      Vec16<T, V> wv[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) load_vec<T, V>(row + k + u * 32 * V, wv[u]);
+      for (int u = 0; u < U; ++u) wv[u].load(row + k + u * kStep);
 #pragma unroll
-    for (int u = 0; u < U; ++u)
+      for (int u = 0; u < U; ++u) {
+        float wf[V];
+        wv[u].get(wf);
 #pragma unroll
-      for (int t = 0; t < MT; ++t) {
-        if (t < M) {
-          float xv[V];
-          load_vec<T, V>(x + t * ldx + k + u * 32 * V, xv);
+        for (int t = 0; t < MT; ++t) {
+          if (t < M) {
+            float xf[V];
+            load_vec<T, V>(x + t * ldx + k + u * kStep, xf);
 #pragma unroll
-          for (int i = 0; i < V; ++i) acc[t] = fmaf(xv[i], wv[u][i], acc[t]);
+            for (int i = 0; i < V; ++i) acc[t] = fmaf(xf[i], wf[i], acc[t]);
+          }
         }
       }
-  }
-  for (; k < K; k += 32 * V) {
+    }
+    for (; k < K; k += kStep) {
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      if (k + i < K) {
-        const float wv = to_f32<T>(row[k + i]);
+      for (int i = 0; i < V; ++i) {
+        if (k + i < K) {
+          const float wf = to_f32<T>(row[k + i]);
 #pragma unroll
-        for (int t = 0; t < MT; ++t)
-          if (t < M) acc[t] = fmaf(to_f32<T>(x[t * ldx + k + i]), wv, acc[t]);
+          for (int t = 0; t < MT; ++t)
+            if (t < M) acc[t] = fmaf(to_f32<T>(x[t * ldx + k + i]), wf, acc[t]);
+        }
       }
     }
+#pragma unroll
+    for (int t = 0; t < MT; ++t)
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) acc[t] += __shfl_xor_sync(kFullMask, acc[t], o);
   }
-#pragma unroll
-  for (int t = 0; t < MT; ++t)
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) acc[t] += __shfl_xor_sync(kFullMask, acc[t], o);
   float z[1] = {acc[0]};
 #pragma unroll
   for (int t = 1; t < MT; ++t)
     if (lane == t) z[0] = acc[t];
-  if (lane < M) lin_finish<1>(e, lane, n, false, z);
+  if constexpr (W > 1) {
+    if (lane < MT) red[warp][lane] = z[0];
+    __syncthreads();
+    if (part != 0) return;
+    if (lane < MT) {
+      z[0] = red[warp][lane];
+#pragma unroll
+      for (int q = 1; q < W; ++q) z[0] += red[warp + q][lane];
+    }
+  }
+  if (n < N && lane < M) lin_finish<1>(e, lane, n, false, z);
 }
 
 // Rows up to which the row kernels run: beyond, w's fp32 splitting or the tensor cores' fixed cost is paid back.
 constexpr int kRowsBf16 = 4, kRowsF32 = 8;
 
+template <typename T, int MT, int W>
+static void launch_rows_w(const GlLinearArgs& a, const LinEpilogue& e, bool aligned, cudaStream_t st) {
+  const unsigned blocks = (unsigned)((a.N + 4 / W - 1) / (4 / W));
+  if (aligned)
+    lin_rows_kernel<T, MT, W, true><<<blocks, 128, 0, st>>>((const T*)a.x, (const T*)a.w, (int)a.M, a.N, a.K, a.ldx,
+                                                            a.ldw, e);
+  else
+    lin_rows_kernel<T, MT, W, false><<<blocks, 128, 0, st>>>((const T*)a.x, (const T*)a.w, (int)a.M, a.N, a.K, a.ldx,
+                                                             a.ldw, e);
+}
+
 template <typename T, int MT>
 static void launch_rows(const GlLinearArgs& a, const LinEpilogue& e, bool aligned, cudaStream_t st) {
-  const unsigned blocks = (unsigned)((a.N + 3) / 4);
-  if (aligned)
-    lin_rows_kernel<T, MT, true><<<blocks, 128, 0, st>>>((const T*)a.x, (const T*)a.w, (int)a.M, a.N, a.K, a.ldx,
-                                                         a.ldw, e);
-  else
-    lin_rows_kernel<T, MT, false><<<blocks, 128, 0, st>>>((const T*)a.x, (const T*)a.w, (int)a.M, a.N, a.K, a.ldx,
-                                                          a.ldw, e);
+  const int64_t loads = a.K * (int64_t)sizeof(T) / 512;       // 16-byte loads of a row, per lane of one warp
+  if (loads <= 8) launch_rows_w<T, MT, 1>(a, e, aligned, st);
+  else if (loads <= 16) launch_rows_w<T, MT, 2>(a, e, aligned, st);
+  else launch_rows_w<T, MT, 4>(a, e, aligned, st);
 }
 
 template <typename T>
@@ -306,33 +350,51 @@ static LinWork lin_bwd_work(int64_t M, int64_t N, int64_t K, int dtype, bool cod
   return w;
 }
 
-// `src` [rows, K] as an operand of the tensor cores: itself where it is aligned bf16, else packed into `dst`.
+// Operands for the tensor cores: a matrix [rows, K] itself where it is aligned bf16, else packed into `dst` by one
+// launch for all of a call's matrices.
 template <typename T>
-static int make_operand(MmaOperand* o, const void* src, int64_t rows, int64_t K, int64_t ld, int mn, void* dst,
-                        int sms, cudaStream_t st) {
-  const bool aligned = rows16(src, ld, sizeof(T));
-  if (sizeof(T) == 2 && aligned) {
-    *o = MmaOperand{src, ld, 0, 1, mn};
+struct Packer {
+  static constexpr int NP = sizeof(T) == 4 ? 3 : 1;
+  PackJob job[2] = {};
+  int n = 0;
+  MmaOperand add(const void* src, int64_t rows, int64_t K, int64_t ld, int mn, void* dst) {
+    const bool aligned = rows16(src, ld, sizeof(T));
+    if (NP == 1 && aligned) return MmaOperand{src, ld, 0, 1, mn};
+    job[n++] = PackJob{src, (uint16_t*)dst, rows, (K + 7) / 8, K, ld, aligned};
+    return MmaOperand{dst, up(K, 8), rows * up(K, 8), NP, mn};
+  }
+  int run(int sms, cudaStream_t st) {
+    if (n == 0) return GL_OK;
+    const int64_t total = job[0].rows * job[0].nk + job[1].rows * job[1].nk, need = (total + 255) / 256;
+    const int64_t cap = 16ll * sms;
+    lin_pack_kernel<T, NP><<<(unsigned)(need < cap ? need : cap), 256, 0, st>>>(job[0], job[1]);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return set_cuda_error(err);
+    count_launches(1);
     return GL_OK;
   }
-  constexpr int NP = sizeof(T) == 4 ? 3 : 1;
-  const int64_t total = rows * ((K + 7) / 8), need = (total + 255) / 256, cap = 16ll * sms;
-  lin_pack_kernel<T, NP><<<(unsigned)(need < cap ? need : cap), 256, 0, st>>>((const T*)src, (uint16_t*)dst, rows, K,
-                                                                           ld, aligned);
-  const cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) return set_cuda_error(err);
-  count_launches(1);
-  *o = MmaOperand{dst, up(K, 8), rows * up(K, 8), NP, mn};
-  return GL_OK;
-}
+};
 
 template <typename T>
 static int run_linear_fwd(const GlLinearArgs& a, const LinEpilogue& e, const LinWork& w, int sms, cudaStream_t st) {
   char* work = (char*)a.work;
-  MmaOperand x, wt;
-  if (int rc = make_operand<T>(&x, a.x, a.M, a.K, a.ldx, 0, work + w.x, sms, st)) return rc;
-  if (int rc = make_operand<T>(&wt, a.w, a.N, a.K, a.ldw, 0, work + w.w, sms, st)) return rc;
-  return mma_product(x, wt, a.M, a.N, a.K, e, work + w.split, st);
+  Packer<T> pack;
+  const MmaOperand x = pack.add(a.x, a.M, a.K, a.ldx, 0, work + w.x);
+  const MmaOperand wt = pack.add(a.w, a.N, a.K, a.ldw, 0, work + w.w);
+  if (int rc = pack.run(sms, st)) return rc;
+  return mma_product(x, wt, a.M, a.N, a.K, e, SumRows{}, work + w.split, st);
+}
+
+template <typename T, int KIND>
+static int launch_dz(const GlLinearBwdArgs& a, uint16_t* dz, float* part, bool aligned, cudaStream_t st) {
+  const int64_t blocks = up(a.M, kDzRows) / kDzRows * ((a.N + 255) / 256);
+  if (blocks > 0x7FFFFFFF) return GL_ERR_SHAPE;
+  lin_dz_kernel<T, sizeof(T) == 4 ? 3 : 1, KIND><<<(unsigned)blocks, 256, 0, st>>>(
+      (const T*)a.dy, a.slope, dz, part, a.M, a.N, a.lddy, a.lds, aligned);
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) return set_cuda_error(err);
+  count_launches(1);
+  return GL_OK;
 }
 
 template <typename T>
@@ -347,54 +409,54 @@ static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, c
   const bool write = !dy_is_dz && (a.dx || a.dw);
   MmaOperand dz{a.dy, a.lddy, 0, 1, 0};
   if (!dy_is_dz) dz = MmaOperand{work + w.dz, up(a.N, 8), a.M * up(a.N, 8), NP, 0};
-  int launches = 0;
   if (write || a.db) {
-    const int64_t rc = up(a.M, kDzRows) / kDzRows, segs = (a.N + 255) / 256;
-    if (rc * segs > 0x7FFFFFFF) return GL_ERR_SHAPE;
+    uint16_t* out = write ? (uint16_t*)(work + w.dz) : nullptr;
     float* part = a.db ? (float*)(work + w.part) : nullptr;
-    const auto kernel = a.slope_kind == GL_SLOPE_NONE  ? lin_dz_kernel<T, NP, GL_SLOPE_NONE>
-                        : a.slope_kind == GL_SLOPE_F32 ? lin_dz_kernel<T, NP, GL_SLOPE_F32>
-                        : a.slope_kind == GL_SLOPE_I16 ? lin_dz_kernel<T, NP, GL_SLOPE_I16>
-                                                       : lin_dz_kernel<T, NP, GL_SLOPE_U8>;
-    kernel<<<(unsigned)(rc * segs), 256, 0, st>>>((const T*)a.dy, a.slope, write ? (uint16_t*)(work + w.dz) : nullptr,
-                                               part, a.M, a.N, a.lddy, a.lds, aligned);
-    ++launches;
-    if (a.db) {
-      lin_db_kernel<<<(unsigned)((a.N + 31) / 32), 256, 0, st>>>(part, rc, a.N, a.db, a.dtype, a.accumulate);
-      ++launches;
-    }
+    const int rc = a.slope_kind == GL_SLOPE_NONE  ? launch_dz<T, GL_SLOPE_NONE>(a, out, part, aligned, st)
+                   : a.slope_kind == GL_SLOPE_F32 ? launch_dz<T, GL_SLOPE_F32>(a, out, part, aligned, st)
+                   : a.slope_kind == GL_SLOPE_I16 ? launch_dz<T, GL_SLOPE_I16>(a, out, part, aligned, st)
+                                                  : launch_dz<T, GL_SLOPE_U8>(a, out, part, aligned, st);
+    if (rc) return rc;
   }
+  SumRows db{};     // done beside the first product
+  if (a.db) db = SumRows{(const float*)(work + w.part), a.db, up(a.M, kDzRows) / kDzRows, a.N, a.dtype, a.accumulate};
+  if (a.db && !a.dx && !a.dw) {
+    lin_db_kernel<<<(unsigned)((a.N + 127) / 128), 128, 0, st>>>(db);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return set_cuda_error(err);
+    count_launches(1);
+    return GL_OK;
+  }
+  Packer<T> pack;
+  MmaOperand wt{}, x{};
+  if (a.dx) wt = pack.add(a.w, a.N, a.K, a.ldw, 1, work + w.w);   // w with its K columns as rows
+  if (a.dw && a.codes) {
+    GlAct8Args d{};
+    d.out = work + w.x;
+    d.codes = const_cast<int8_t*>(a.codes);
+    d.exps = const_cast<uint8_t*>(a.exps);
+    d.rows = a.M; d.C = a.K; d.ldx = up(a.K, 8); d.ldc = a.ldc; d.dtype = GL_DTYPE_BF16;
+    if (int rc = gl_act8_decode(&d, st)) return rc;
+    x = MmaOperand{work + w.x, up(a.K, 8), 0, 1, 1};
+  } else if (a.dw) {
+    x = pack.add(a.x, a.M, a.K, a.ldx, 1, work + w.x);
+  }
+  if (int rc = pack.run(sms, st)) return rc;
   LinEpilogue e{};
   e.dtype = a.dtype;
-  if (a.dx) {   // [M, K] = dz [M, N] w [N, K]: w with its K columns as rows
-    MmaOperand wt;
-    if (int rc = make_operand<T>(&wt, a.w, a.N, a.K, a.ldw, 1, work + w.w, sms, st)) return rc;
+  if (a.dx) {   // [M, K] = dz [M, N] w [N, K]
     e.out = a.dx;
     e.ldo = a.lddx;
-    if (int rc = mma_product(dz, wt, a.M, a.K, a.N, e, work + w.split, st)) return rc;
+    if (int rc = mma_product(dz, wt, a.M, a.K, a.N, e, db, work + w.split, st)) return rc;
+    db = SumRows{};
   }
   if (a.dw) {   // [N, K] = dz^T [N, M] x [M, K]
-    MmaOperand x;
-    if (a.codes) {
-      GlAct8Args d{};
-      d.out = work + w.x;
-      d.codes = const_cast<int8_t*>(a.codes);
-      d.exps = const_cast<uint8_t*>(a.exps);
-      d.rows = a.M; d.C = a.K; d.ldx = up(a.K, 8); d.ldc = a.ldc; d.dtype = GL_DTYPE_BF16;
-      if (int rc = gl_act8_decode(&d, st)) return rc;
-      x = MmaOperand{work + w.x, up(a.K, 8), 0, 1, 1};
-    } else if (int rc = make_operand<T>(&x, a.x, a.M, a.K, a.ldx, 1, work + w.x, sms, st)) {
-      return rc;
-    }
     dz.mn = 1;
     e.out = a.dw;
     e.ldo = a.K;
     e.accumulate = a.accumulate;
-    if (int rc = mma_product(dz, x, a.N, a.K, a.M, e, work + w.split, st)) return rc;
+    if (int rc = mma_product(dz, x, a.N, a.K, a.M, e, db, work + w.split, st)) return rc;
   }
-  const cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) return set_cuda_error(err);
-  count_launches(launches);
   return GL_OK;
 }
 

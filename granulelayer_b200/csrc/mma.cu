@@ -12,11 +12,10 @@
 // its shared memory per 64 k instead of 48 KB, both from L2 and to the tensor core; that traffic, not the MMA
 // rate, bounds the 128 x 256 tile of one CTA.
 //
-// fp32 operands come as three bf16 planes; a slot holds plane i of both and the products of term pairs (i, j),
-// i + j <= 2, run as their slots arrive: (0,0), (0,1) (1,0) (1,1), (0,2) (2,0).  The tensor core's fp32 accumulation
-// truncates, so with several planes a sum over k is cut into chunks of 128: each chunk's accumulator is added to
-// registers in fp32 (rounding to nearest) while the next one runs.  At K = 4096 chunks of 512 were 3.9e-6 off in
-// the 2-norm, chunks of 128 0.8e-6 (plain fp32 products: 1.0e-6).
+// fp32 operands come as three bf16 planes; a slot holds plane i of both, and the products of term pairs (i, j),
+// i + j <= 2, run smallest first.  The tensor core's fp32 accumulation truncates, so with several planes a sum over
+// k is cut into chunks of 128: each chunk's accumulator is added to registers in fp32 (rounding to nearest) while the
+// next one runs.  At K = 4096 chunks of 512 were 3.9e-6 off in the 2-norm (plain fp32 products: 1.0e-6).
 //
 // K-major tiles are one TMA box (64 k wide, all rows of the tile); MN-major tiles are boxes of 64 rows by 64 k, which
 // the matrix descriptor walks with 2048 bytes per 16 k and 8192 bytes per 64 rows.  Edges in every dimension are
@@ -29,7 +28,7 @@
 
 namespace gl {
 
-constexpr int kMmBM = 128, kMmBK = 64, kMmThreads = 320, kMmEpiWarps = 8, kMmMaxSlots = 8;
+constexpr int kMmBM = 128, kMmBK = 64, kMmThreads = 320, kMmEpiWarps = 8, kMmMaxSlots = 9;
 constexpr uint32_t kMmWaitLimit = 1u << 20;
 constexpr uint32_t kMmPlaneA = kMmBM * kMmBK * 2;
 constexpr int kMmPitch = 36;                                   // floats per row of a warp's 32 x 32 epilogue tile
@@ -39,8 +38,10 @@ struct MmaParams {
   int64_t M, N;
   int tiles_m, tiles_n, kblocks, chunk, splits, split_blocks;
   int a_mn, b_mn, vec;
+  uint32_t a_bytes;      // of a plane of A in a slot (a tile of fewer than 128 rows loads fewer)
   float* part;
   LinEpilogue e;
+  SumRows side;
 };
 
 // A slot: a plane of A (128 rows) and of B (this CTA's share of BN rows), 64 k each.
@@ -51,7 +52,7 @@ __host__ __device__ constexpr int mm_slots(int BN, int CTAS) {
 }
 
 struct MmaShared {
-  uint64_t full[kMmMaxSlots], empty[kMmMaxSlots], done[2], free_[2];
+  uint64_t full[kMmMaxSlots], empty[kMmMaxSlots], done[4], free_[4];
   uint32_t tmem;
   int dead;
 };
@@ -183,8 +184,9 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     mma_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const MmaParams p) {
   constexpr int ST = mm_slots(BN, CTAS), BNC = BN / CTAS, BM = kMmBM * CTAS;
   constexpr uint32_t kSlot = mm_slot_bytes(BN, CTAS);
-  constexpr uint32_t kCols = 2 * BN;                 // TMEM columns: two accumulators
   constexpr bool MULTI = NPA > 1;
+  constexpr int NB = MULTI ? 4 : 2;                  // accumulators
+  constexpr uint32_t kCols = NB * BN;                // TMEM columns
   constexpr int HALF = BN >= 64 ? BN / 2 : BN;        // columns per epilogue warp
   constexpr int kEpi = BN >= 64 ? kMmEpiWarps : 4;    // epilogue warps at work
   extern __shared__ unsigned char mm_raw[];
@@ -203,7 +205,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
       t5_mbar_init(t5_smem_u32(&sh.full[i]), 1);
       t5_mbar_init(t5_smem_u32(&sh.empty[i]), 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < NB; ++i) {
       t5_mbar_init(t5_smem_u32(&sh.done[i]), 1);
       t5_mbar_init(t5_smem_u32(&sh.free_[i]), kEpi * CTAS);
     }
@@ -234,7 +236,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             }
             uint32_t bar = t5_smem_u32(&sh.full[r.s]);
             const uint32_t a = smem + r.s * kSlot, b = a + kMmPlaneA;
-            if (rank == 0) mm_expect(bar, CTAS * (i < NPB ? kSlot : kMmPlaneA));
+            if (rank == 0) mm_expect(bar, CTAS * (p.a_bytes + (i < NPB ? kSlot - kMmPlaneA : 0u)));
             if constexpr (CTAS == 2) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(bar) : "r"(bar));
             if (p.a_mn) {
               mm_load<CTAS>(a, &ta, m0, kb * kMmBK, i, bar);
@@ -275,8 +277,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
       for (int64_t item = first; item < items && live; item += step) {
         const MmaTile t = mm_tile(p, item, BM, BN);
         for (int c0 = t.k0; c0 < t.k1 && live; c0 += p.chunk, ++ch) {
-          const int c1 = min(t.k1, c0 + p.chunk), buf = ch & 1;
-          if (ch >= 2 && !mm_wait(sh, sh.free_[buf], ((ch >> 1) - 1) & 1)) {
+          const int c1 = min(t.k1, c0 + p.chunk), buf = ch % NB;
+          if (ch >= NB && !mm_wait(sh, sh.free_[buf], (ch / NB - 1) & 1)) {
             live = false;
             break;
           }
@@ -298,27 +300,29 @@ __global__ void __launch_bounds__(kMmThreads, 1)
 #pragma unroll
             for (int i = 0; i < NPA; ++i, r.next()) {
               slot[i] = r.s;
-              if (!mm_wait(sh, sh.full[r.s], r.round & 1)) {
-                live = false;
-                break;
-              }
-              t5_fence_after_sync();
-              if (i == 0) product(slot[0], slot[0]);
-              if (NPB == 1) {
-                if (i > 0) product(slot[i], slot[0]);
-                if (i > 0 || NPA == 1) commit(sh.empty[slot[i]]);
-              } else if (i == 1) {
-                product(slot[0], slot[1]);
-                product(slot[1], slot[0]);
-                product(slot[1], slot[1]);
-                commit(sh.empty[slot[1]]);
-              } else if (i == 2) {
-                product(slot[0], slot[2]);
-                product(slot[2], slot[0]);
-                commit(sh.empty[slot[2]]);
-              }
-              if (NPA > 1 && i == NPA - 1) commit(sh.empty[slot[0]]);
+              if (live && !mm_wait(sh, sh.full[r.s], r.round & 1)) live = false;
             }
+            if (!live) break;
+            t5_fence_after_sync();
+            if constexpr (NPA == 1) {
+              product(slot[0], slot[0]);
+            } else if constexpr (NPB == 1) {
+              product(slot[2], slot[0]);
+              commit(sh.empty[slot[2]]);
+              product(slot[1], slot[0]);
+              commit(sh.empty[slot[1]]);
+              product(slot[0], slot[0]);
+            } else {
+              product(slot[0], slot[2]);
+              product(slot[2], slot[0]);
+              commit(sh.empty[slot[2]]);
+              product(slot[1], slot[1]);
+              product(slot[0], slot[1]);
+              product(slot[1], slot[0]);
+              commit(sh.empty[slot[1]]);
+              product(slot[0], slot[0]);
+            }
+            commit(sh.empty[slot[0]]);
           }
           if (live) commit(sh.done[buf]);
         }
@@ -328,33 +332,48 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     const int half = warp >> 2;
     const uint32_t lane_base = (uint32_t)(32 * (warp & 3)) << 16;
     float* tile = epi + warp * 32 * kMmPitch;
+    if (p.side.part) {
+      for (int64_t n = ((int64_t)blockIdx.x * kEpi + warp) * 32; n < p.side.N; n += (int64_t)gridDim.x * kEpi * 32)
+        sum_rows(p.side, n);
+    }
     uint32_t ch = 0;
     for (int64_t item = first; item < items; item += step) {
       const MmaTile t = mm_tile(p, item, BM, BN);
       const int64_t m0 = t.m0 + kMmBM * rank + 32 * (warp & 3), n0 = t.n0 + half * HALF;
       float sum[MULTI ? HALF : 1];
       for (int c0 = t.k0; c0 < t.k1; c0 += p.chunk, ++ch) {
-        const int buf = ch & 1;
-        const bool ok = __all_sync(kFullMask, mm_wait(sh, sh.done[buf], (ch >> 1) & 1));
+        const int buf = ch % NB;
+        const bool ok = __all_sync(kFullMask, mm_wait(sh, sh.done[buf], (ch / NB) & 1));
         t5_fence_after_sync();
+        const uint32_t cols = tmem + lane_base + (uint32_t)(buf * BN + half * HALF);
+        if constexpr (MULTI) {   // one load for all of the warp's columns: each waits for the MMAs in flight
+          static_assert(HALF == 32 || HALF == 64, "columns per warp");
+          float v[HALF];
+          if constexpr (HALF == 64) t5_ld64(cols, v);
+          else t5_ld32(cols, v);
+          t5_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mm_arrive<CTAS>(t5_smem_u32(&sh.free_[buf]));
 #pragma unroll
-        for (int q = 0; q < HALF / 32; ++q) {
-          float v[32];
-          t5_ld32(tmem + lane_base + (uint32_t)(buf * BN + half * HALF + 32 * q), v);
-          if (!ok) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7FC00000);
+          for (int i = 0; i < HALF; ++i) {
+            if (!ok) v[i] = __int_as_float(0x7FC00000);
+            sum[i] = c0 == t.k0 ? v[i] : sum[i] + v[i];
           }
-          if (q == HALF / 32 - 1) {                      // the accumulator is read: free it before the stores
-            t5_fence_before_sync();
-            __syncwarp();
-            if (lane == 0) mm_arrive<CTAS>(t5_smem_u32(&sh.free_[buf]));
-          }
-          if constexpr (MULTI) {
+        } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) sum[32 * q + i] = c0 == t.k0 ? v[i] : sum[32 * q + i] + v[i];
-          } else if (m0 < p.M && n0 + 32 * q < p.N) {
-            mm_store_block(p, tile, v, m0, n0 + 32 * q, t.split);
+          for (int q = 0; q < HALF / 32; ++q) {
+            float v[32];
+            t5_ld32(cols + 32 * q, v);
+            if (!ok) {
+#pragma unroll
+              for (int i = 0; i < 32; ++i) v[i] = __int_as_float(0x7FC00000);
+            }
+            if (q == HALF / 32 - 1) {                    // the accumulator is read: free it before the stores
+              t5_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mm_arrive<CTAS>(t5_smem_u32(&sh.free_[buf]));
+            }
+            if (m0 < p.M && n0 + 32 * q < p.N) mm_store_block(p, tile, v, m0, n0 + 32 * q, t.split);
           }
         }
       }
@@ -410,20 +429,21 @@ struct MmaPlan {
 };
 
 // Tile shape and number of splits of k: the least estimated time, in clocks of one SM.  64 k cost the larger of
-// the MMAs (2 BN / ctas clocks a term of 128 x BN) and the loads (about 44 bytes a clock into one SM of many);
-// split sums add their partial tiles' traffic and a second launch.
-static MmaPlan mma_plan(int64_t M, int64_t N, int64_t K, int npa, int npb, bool b_mn, int sms) {
+// the MMAs (2 BN clocks a term) and the loads (about 60 bytes a clock into one SM of many) and four tenths of the
+// smaller; split sums add their partial tiles' traffic and a second launch.
+static MmaPlan mma_search(int64_t M, int64_t N, int64_t K, int npa, int npb, bool b_mn, int sms) {
   MmaPlan best{};
   double best_t = 1e300;
   const int64_t kb = (K + kMmBK - 1) / kMmBK;
   const int terms = npa == 1 ? 1 : (npb == 1 ? 3 : 6);
   struct Shape { int ctas, BN; };
-  for (Shape sh : {Shape{2, 256}, Shape{1, 128}, Shape{1, 64}, Shape{1, 32}}) {
+  for (Shape sh : {Shape{2, 256}, Shape{2, 128}, Shape{1, 128}, Shape{1, 64}, Shape{1, 32}}) {
     if (sh.BN == 32 && (b_mn || npa > 1)) continue;
+    if (sh.BN == 256 && npa > 1) continue;     // four accumulators fill the tensor memory
     const int64_t tm = (M + kMmBM * sh.ctas - 1) / (kMmBM * sh.ctas), tn = (N + sh.BN - 1) / sh.BN, tiles = tm * tn;
-    const double bytes = npa * (double)kMmPlaneA + npb * (double)(sh.BN / sh.ctas) * kMmBK * 2;
-    const double load = bytes / 44.0, mma = terms * 2.0 * sh.BN;
-    const double block = (load > mma ? load : mma) + 20;
+    const double bytes = npa * (double)(M < kMmBM ? M : kMmBM) * kMmBK * 2 + npb * (double)(sh.BN / sh.ctas) * kMmBK * 2;
+    const double load = bytes / 60.0, mma = terms * 2.0 * sh.BN;
+    const double block = load > mma ? load + 0.4 * mma : mma + 0.4 * load;
     const int64_t wide = sms / sh.ctas;
     for (int s = 1; s <= 32 && s <= kb; ++s) {
       const int64_t sb = (kb + s - 1) / s;
@@ -438,6 +458,20 @@ static MmaPlan mma_plan(int64_t M, int64_t N, int64_t K, int npa, int npb, bool 
     }
   }
   return best;
+}
+
+// mma_search with the last plans of this thread at hand: a search costs about as much host time as a launch.
+static MmaPlan mma_plan(int64_t M, int64_t N, int64_t K, int npa, int npb, bool b_mn, int sms) {
+  struct Entry {
+    int64_t M, N, K;
+    int key;
+    MmaPlan plan;
+  };
+  static thread_local Entry cache[64];
+  const int key = 1 + b_mn + 2 * npa + 8 * npb + 32 * sms;
+  Entry& e = cache[(M * 31 + N * 17 + K * 7 + key) & 63];
+  if (e.key != key || e.M != M || e.N != N || e.K != K) e = Entry{M, N, K, key, mma_search(M, N, K, npa, npb, b_mn, sms)};
+  return e.plan;
 }
 
 int64_t mma_work_bytes(int64_t M, int64_t N, int64_t K, int npa, int npb, int sms) {
@@ -506,7 +540,10 @@ static int launch_mma(const CUtensorMap& ta, const CUtensorMap& tb, const MmaPar
 template <int NPA, int NPB>
 static int launch_shape(const MmaPlan& pl, const CUtensorMap& ta, const CUtensorMap& tb, const MmaParams& p, int sms,
                         cudaStream_t st) {
-  if (pl.ctas == 2) return launch_mma<2, 256, NPA, NPB>(ta, tb, p, sms, st);
+  if constexpr (NPA == 1) {
+    if (pl.BN == 256) return launch_mma<2, 256, 1, 1>(ta, tb, p, sms, st);
+  }
+  if (pl.ctas == 2) return launch_mma<2, 128, NPA, NPB>(ta, tb, p, sms, st);
   if (pl.BN == 128) return launch_mma<1, 128, NPA, NPB>(ta, tb, p, sms, st);
   if (pl.BN == 64) return launch_mma<1, 64, NPA, NPB>(ta, tb, p, sms, st);
   if constexpr (NPA == 1) return launch_mma<1, 32, 1, 1>(ta, tb, p, sms, st);
@@ -518,19 +555,23 @@ static bool aligned16(const void* p, int64_t ld, int esize) {
 }
 
 int mma_product(const MmaOperand& a, const MmaOperand& b, int64_t M, int64_t N, int64_t K, const LinEpilogue& e,
-                void* work, cudaStream_t st) {
+                const SumRows& side, void* work, cudaStream_t st) {
   if (M > 0x7FFFFF00 || N > 0x7FFFFF00 || K > 0x7FFFFF00) return GL_ERR_SHAPE;
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   const MmaPlan pl = mma_plan(M, N, K, a.planes, b.planes, b.mn, sms);
   if (pl.splits > 1 && !work) return GL_ERR_WORKSPACE;
   CUtensorMap ta, tb;
-  if (int rc = operand_map(&ta, a, M, K, kMmBM)) return rc;
+  // a tile of fewer rows than 128 (one CTA's only) loads those; the rest of the slot stays as it is, for rows of the
+  // accumulator that nobody reads
+  const int a_rows = M < kMmBM && !a.mn ? (int)(M + 7) / 8 * 8 : kMmBM;
+  if (int rc = operand_map(&ta, a, M, K, a_rows)) return rc;
   if (int rc = operand_map(&tb, b, N, K, pl.BN / pl.ctas)) return rc;
   MmaParams p{};
   p.M = M; p.N = N; p.tiles_m = (int)pl.tiles_m; p.tiles_n = (int)pl.tiles_n;
   p.kblocks = (int)((K + kMmBK - 1) / kMmBK); p.chunk = pl.chunk < p.kblocks ? pl.chunk : p.kblocks;
-  p.splits = pl.splits; p.split_blocks = pl.split_blocks; p.a_mn = a.mn; p.b_mn = b.mn; p.e = e;
+  p.splits = pl.splits; p.split_blocks = pl.split_blocks; p.a_mn = a.mn; p.b_mn = b.mn; p.e = e; p.side = side;
+  p.a_bytes = (uint32_t)a_rows * kMmBK * 2;
   const int es = e.dtype == GL_DTYPE_F32 || e.accumulate ? 4 : 2;
   const int ss = e.slope_kind == GL_SLOPE_F32 ? 4 : e.slope_kind == GL_SLOPE_I16 ? 2 : 1;
   const bool vec = aligned16(e.out, e.ldo, es) && aligned16(e.residual, e.ldr, es) && aligned16(e.bias, 0, es) &&

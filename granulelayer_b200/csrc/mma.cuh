@@ -21,6 +21,35 @@ struct LinEpilogue {
   int dtype, act, accumulate, slope_kind;
 };
 
+// db[n] (=, or += with accumulate) the sum of `rows` partial rows part[r N + n] in row order: work that a product's
+// epilogue warps do while they wait for their first tile.
+struct SumRows {
+  const float* part;
+  void* out;
+  int64_t rows, N;
+  int dtype, accumulate;
+};
+
+// One warp, 32 columns from n0 on.
+__device__ __forceinline__ void sum_rows(const SumRows& j, int64_t n0) {
+  const int64_t n = n0 + (threadIdx.x & 31);
+  if (n >= j.N) return;
+  float s[4] = {0.f, 0.f, 0.f, 0.f};
+  int64_t r = 0;
+  for (; r + 16 <= j.rows; r += 16) {
+    float v[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) v[k] = j.part[(r + k) * j.N + n];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s[k & 3] += v[k];
+  }
+  for (; r < j.rows; ++r) s[0] += j.part[r * j.N + n];
+  const float t = (s[0] + s[1]) + (s[2] + s[3]);
+  if (j.accumulate) reinterpret_cast<float*>(j.out)[n] += t;
+  else if (j.dtype == GL_DTYPE_F32) reinterpret_cast<float*>(j.out)[n] = t;
+  else reinterpret_cast<__nv_bfloat16*>(j.out)[n] = __float2bfloat16_rn(t);
+}
+
 // A bf16 operand of `planes` planes `plane` elements apart: element (r, k) at ptr[r ld + k], or ptr[k ld + r] when
 // `mn`.  ptr 16-byte aligned, ld and plane multiples of 8.
 struct MmaOperand {
@@ -32,7 +61,7 @@ struct MmaOperand {
 // Scratch that mma_product needs (split sums), and the product itself.
 int64_t mma_work_bytes(int64_t M, int64_t N, int64_t K, int a_planes, int b_planes, int sms);
 int mma_product(const MmaOperand& a, const MmaOperand& b, int64_t M, int64_t N, int64_t K, const LinEpilogue& e,
-                void* work, cudaStream_t st);
+                const SumRows& side, void* work, cudaStream_t st);   // side.part NULL: nothing besides
 
 // N elements of type T from p on: as 16-byte vectors where `vec`.
 template <typename T, int N>

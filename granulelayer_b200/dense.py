@@ -20,7 +20,6 @@ from typing import Optional, Tuple
 
 import torch
 from torch import nn
-from torch.autograd.function import once_differentiable
 
 from . import _native
 
@@ -29,11 +28,14 @@ CHECKPOINTS = ("none", "int8")
 _DTYPES = (torch.float32, torch.bfloat16)
 
 
+_ACT_IDS = _native.DENSE_ACT_IDS
+
+
 def _act_id(activation: str) -> int:
-    try:
-        return _native.DENSE_ACT_IDS[activation]
-    except KeyError:
-        raise ValueError(f"activation must be one of {tuple(_native.DENSE_ACT_IDS)}, not {activation!r}") from None
+    act = _ACT_IDS.get(activation)
+    if act is None:
+        raise ValueError(f"activation must be one of {tuple(_ACT_IDS)}, not {activation!r}")
+    return act
 
 
 def _check_checkpoint(checkpoint: str):
@@ -41,20 +43,22 @@ def _check_checkpoint(checkpoint: str):
         raise ValueError(f"checkpoint must be one of {CHECKPOINTS}, not {checkpoint!r}")
 
 
-def _check_tensors(name: str, dtype: torch.dtype, **tensors):
-    """One supported dtype and one device for all tensors that are given."""
-    if dtype not in _DTYPES:
-        raise ValueError(f"{name}: float32 or bfloat16 tensors, not {dtype}")
-    dev = None
+def _check_tensors(name: str, x: torch.Tensor, dtype, **tensors):
+    """``x`` of a supported dtype on a GPU; every other given tensor on its device and, where one is named, of
+    ``dtype``."""
+    if x.dtype not in _DTYPES or dtype not in _DTYPES:
+        raise ValueError(f"{name}: float32 or bfloat16 tensors, not {x.dtype if x.dtype not in _DTYPES else dtype}")
     for k, t in tensors.items():
-        if t is None:
-            continue
-        if t.dtype != dtype:
-            raise ValueError(f"{name}: {k} is {t.dtype}, the input {dtype}")
-        if dev is None:
-            dev = t.device
-        elif t.device != dev:
-            raise ValueError(f"{name}: {k} is on {t.device}, the input on {dev}")
+        if t is not None and t.dtype != dtype:
+            raise ValueError(f"{name}: {k} is {t.dtype}, expected {dtype}")
+        if t is not None and t.device != x.device:
+            raise ValueError(f"{name}: {k} is on {t.device}, the input on {x.device}")
+    _native._require_cuda(x)
+
+
+def _no_double_backward(name: str):
+    if torch.is_grad_enabled():
+        raise RuntimeError(f"{name}: the backward pass is not differentiable (create_graph=True)")
 
 
 def _rows(t: torch.Tensor, width: int) -> torch.Tensor:
@@ -98,8 +102,7 @@ def encode_activation(x: torch.Tensor) -> Activation8:
     """``x`` [..., C] (float32 or bfloat16) in 8 bits."""
     if x.dim() < 1 or x.shape[-1] < 1:
         raise ValueError(f"encode_activation: x needs at least one channel, got shape {tuple(x.shape)}")
-    _check_tensors("encode_activation", x.dtype, x=x)
-    _native._require_cuda(x)
+    _check_tensors("encode_activation", x, x.dtype)
     codes, exps = _encode(_rows(x.detach(), x.shape[-1]))
     return Activation8(codes, exps, tuple(x.shape), x.dtype)
 
@@ -119,29 +122,28 @@ def decode_activation(a: Activation8, dtype: Optional[torch.dtype] = None) -> to
 
 # ---- gradients of parameters ----
 
-def _grad_buffers(*params):
-    """(buffers, accumulate): per (parameter, wanted) the buffer its gradient goes to.  With a ``main_grad`` among
-    them all are fp32 and added to (fresh zeros where a parameter has none), as SparsePoolingLayer's are."""
-    main = any(want and getattr(p, "main_grad", None) is not None for p, want in params if p is not None)
+def _grad_buffers(weight, need_w: bool, bias, need_b: bool):
+    """(weight's buffer, bias's buffer, accumulate): where their gradients go (None: not wanted).  With a ``main_grad``
+    on either, both buffers are fp32 and added to (fresh zeros for one without), as SparsePoolingLayer's are."""
+    need_w, need_b = need_w and weight is not None, need_b and bias is not None
+    main = (need_w and hasattr(weight, "main_grad") and weight.main_grad is not None or
+            need_b and hasattr(bias, "main_grad") and bias.main_grad is not None)
+    if not main:
+        return weight.new_empty(weight.shape) if need_w else None, bias.new_empty(bias.shape) if need_b else None, False
     out = []
-    for p, want in params:
-        if p is None or not want:
-            out.append(None)
-        elif not main:
-            out.append(torch.empty(p.shape, dtype=p.dtype, device=p.device))
-        else:
-            g = getattr(p, "main_grad", None)
-            if g is not None and (g.dtype != torch.float32 or not g.is_contiguous() or g.shape != p.shape):
-                raise ValueError("main_grad must be a contiguous float32 tensor of the parameter's shape")
-            out.append(g if g is not None else torch.zeros(p.shape, dtype=torch.float32, device=p.device))
-    return out, main
+    for p, want in ((weight, need_w), (bias, need_b)):
+        g = getattr(p, "main_grad", None) if want else None
+        if g is not None and (g.dtype != torch.float32 or not g.is_contiguous() or g.shape != p.shape):
+            raise ValueError("main_grad must be a contiguous float32 tensor of the parameter's shape")
+        out.append(g if g is not None or not want else torch.zeros(p.shape, dtype=torch.float32, device=p.device))
+    return out[0], out[1], True
 
 
-def _returned(p, buf):
+def _returned(p, buf, main: bool):
     """What autograd gets for a parameter: None for ``main_grad``, else the buffer in the parameter's dtype."""
-    if buf is None or getattr(p, "main_grad", None) is not None:
-        return None
-    return buf if buf.dtype == p.dtype else buf.to(p.dtype)
+    if buf is None or not main:
+        return buf
+    return None if getattr(p, "main_grad", None) is not None else buf.to(p.dtype)
 
 
 # ---- linear ----
@@ -152,7 +154,7 @@ _SLOPE_DTYPES = {torch.float32: torch.float32, torch.bfloat16: torch.int16}
 
 
 def _linear_forward(x2, weight, bias, r2, act, slope):
-    y = torch.empty((x2.shape[0], weight.shape[0]), dtype=x2.dtype, device=x2.device)
+    y = x2.new_empty((x2.shape[0], weight.shape[0]))
     if x2.shape[0]:
         _native.linear_fwd(x2, weight, bias, r2, y, slope, act)
     return y
@@ -161,33 +163,46 @@ def _linear_forward(x2, weight, bias, r2, act, slope):
 class LinearActFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, checkpoint):
-        M, K, N = x.numel() // x.shape[-1], x.shape[-1], weight.shape[0]
+        N, K = weight.shape
         x2, w2 = _rows(x, K), _rows(weight, K)
-        r2 = None if residual is None else _rows(residual, N)
         slope = codes = exps = None
         if act != 0:
-            slope = torch.empty((M, N), dtype=torch.uint8 if checkpoint == "int8" else _SLOPE_DTYPES[x.dtype],
-                                device=x.device)
-        y = _linear_forward(x2, w2, bias, r2, act, slope)
+            slope = torch.empty((x2.shape[0], N), device=x.device,
+                                dtype=torch.uint8 if checkpoint == "int8" else _SLOPE_DTYPES[x.dtype])
+        y = _linear_forward(x2, w2, bias, None if residual is None else _rows(residual, N), act, slope)
         if checkpoint == "int8":
             codes, exps = _encode(x2)
-        ctx.save_for_backward(x2 if codes is None else None, codes, exps, weight, bias, slope)
+            x2 = None
+        ctx.save_for_backward(x2, codes, exps, weight, bias, slope)
         ctx.xshape = x.shape
-        return y.view(*x.shape[:-1], N)
+        return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
+        _no_double_backward("linear_act")
         x2, codes, exps, weight, bias, slope = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         N, K = weight.shape
-        dx = torch.empty(ctx.xshape, dtype=dy.dtype, device=dy.device) if need_x else None
-        (dw, db), main = _grad_buffers((weight, need_w), (bias, need_b))
-        if need_x or need_w or need_b:
-            w2 = _rows(weight, K) if need_x else None
-            _native.linear_bwd(_rows(dy, N), slope, x2, codes, exps, w2, dx.view(-1, K) if need_x else None, dw, db,
-                               K, main)
-        return dx, _returned(weight, dw), _returned(bias, db), dy if need_r else None, None, None
+        dx = w2 = None
+        if need_x:
+            dx, w2 = dy.new_empty(ctx.xshape), _rows(weight, K)
+        dw, db, main = _grad_buffers(weight, need_w, bias, need_b)
+        if need_x or dw is not None or db is not None:
+            _native.linear_bwd(_rows(dy, N), slope, x2, codes, exps, w2, dx, dw, db, K, main)
+        return dx, _returned(weight, dw, main), _returned(bias, db, main), dy if need_r else None, None, None
+
+
+def _check_linear(x, weight, bias, residual):
+    """Raises for arguments that do not belong together."""
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
+        raise ValueError(f"linear_act: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    N = weight.shape[0]
+    if bias is not None and (bias.shape != (N,) or (N > 1 and bias.stride(0) != 1)):
+        raise ValueError(f"linear_act: bias must be a contiguous [{N}], got {tuple(bias.shape)}")
+    if residual is not None and residual.shape != x.shape[:-1] + (N,):
+        raise ValueError(f"linear_act: residual {tuple(residual.shape)} must have the output's shape "
+                         f"{tuple(x.shape[:-1]) + (N,)}")
+    _check_tensors("linear_act", x, x.dtype, weight=weight, bias=bias, residual=residual)
 
 
 def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
@@ -197,23 +212,16 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
     ``activation``: "identity", "relu", "gelu" (erf form) or "silu".  ``checkpoint="int8"`` keeps the input and the
     activation's derivative in 8 bits for the backward pass.  All tensors share one dtype (float32 or bfloat16;
-    float32 products run as exact three-term bf16 splits on the tensor cores or in fp32).  Parameters with a
-    ``main_grad`` receive their gradients there."""
+    float32 products run as exact three-term bf16 splits on the tensor cores, or in fp32 for a few rows).
+    Parameters with a ``main_grad`` receive their gradients there."""
     act = _act_id(activation)
     _check_checkpoint(checkpoint)
-    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[1] or 0 in weight.shape:
-        raise ValueError(f"linear_act: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
-    N = weight.shape[0]
-    if bias is not None and (bias.shape != (N,) or (N > 1 and bias.stride(0) != 1)):
-        raise ValueError(f"linear_act: bias must be a contiguous [{N}], got {tuple(bias.shape)}")
-    if residual is not None and residual.shape != x.shape[:-1] + (N,):
-        raise ValueError(f"linear_act: residual {tuple(residual.shape)} must have the output's shape "
-                         f"{tuple(x.shape[:-1]) + (N,)}")
-    _check_tensors("linear_act", x.dtype, x=x, weight=weight, bias=bias, residual=residual)
-    _native._require_cuda(x)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    _check_linear(x, weight, bias, residual)
+    if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
+                                    bias is not None and bias.requires_grad or
+                                    residual is not None and residual.requires_grad):
         return LinearActFunction.apply(x, weight, bias, residual, act, checkpoint)
-    K = x.shape[-1]
+    N, K = weight.shape
     y = _linear_forward(_rows(x, K), _rows(weight, K), bias, None if residual is None else _rows(residual, N), act,
                         None)
     return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
@@ -223,54 +231,72 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
 def _positions(t: torch.Tensor, S: int, P: int, C: int) -> torch.Tensor:
     """``t`` [S, ..., C] as [S, P, C] with unit channel stride and positions that do not overlap."""
+    if t.is_contiguous() and C > 1:      # strides of dimensions of size one may still be anything
+        return t.as_strided((S, P, C), (P * C, C, 1))
     t3 = t.reshape(S, P, C)
     if (C > 1 and t3.stride(2) != 1) or (P > 1 and t3.stride(1) < C) or (S > 1 and t3.stride(0) < C):
         t3 = t3.contiguous()
-    if t3.stride(1) < C or t3.stride(0) < C or (C == 1 and t3.stride(2) != 1):   # strides of dimensions of size one
+    if t3.stride(1) < C or t3.stride(0) < C or (C == 1 and t3.stride(2) != 1):
         t3 = t3.as_strided(t3.shape, (t3.stride(0) if S > 1 else P * C, t3.stride(1) if P > 1 else C, 1))
     return t3
 
 
 def _norm_forward(x, num_groups, weight, bias, act, eps):
     S, C = x.shape[0], x.shape[-1]
-    P = x.numel() // (S * C) if S else 0
     y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean, rstd = torch.empty((2, S, num_groups), dtype=torch.float32, device=x.device).unbind(0)
+    stats = torch.empty((2, S, num_groups), dtype=torch.float32, device=x.device)   # mean, rstd
     x3 = None
-    if y.numel():
-        x3 = _positions(x, S, P, C)
-        _native.norm_fwd(x3, weight, bias, y, mean, rstd, num_groups, act, eps)
-    return y, x3, mean, rstd
+    n = x.numel()
+    if n:
+        x3 = _positions(x, S, n // (S * C), C)
+        _native.norm_fwd(x3, weight, bias, y, stats, num_groups, act, eps)
+    return y, x3, stats
 
 
 class GroupNormActFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, num_groups, act, eps, checkpoint):
-        y, x3, mean, rstd = _norm_forward(x, num_groups, weight, bias, act, eps)
+        y, x3, stats = _norm_forward(x, num_groups, weight, bias, act, eps)
         codes = exps = None
         if checkpoint == "int8" and x3 is not None:
             codes, exps = _encode(_rows(x3, x.shape[-1]))
             x3 = None
-        ctx.save_for_backward(x3, codes, exps, weight, bias, mean, rstd)
+        ctx.save_for_backward(x3, codes, exps, weight, bias, stats)
         ctx.act, ctx.groups = act, num_groups
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, dy):
-        x3, codes, exps, weight, bias, mean, rstd = ctx.saved_tensors
+        _no_double_backward("group_norm_act")
+        x3, codes, exps, weight, bias, stats = ctx.saved_tensors
         _, need_w, need_b = ctx.needs_input_grad[:3]
         dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
-        (dw, db), main = _grad_buffers((weight, need_w), (bias, need_b))
+        dw, db, main = _grad_buffers(weight, need_w, bias, need_b)
         S, C = dy.shape[0], dy.shape[-1]
-        if dy.numel():
-            dy3 = _positions(dy, S, dy.numel() // (S * C), C)
-            _native.norm_bwd(dy3, x3, codes, exps, weight, bias, mean, rstd, dx, dw, db, ctx.groups, ctx.act, main)
+        if dx.numel():
+            dy3 = _positions(dy, S, dx.numel() // (S * C), C)
+            _native.norm_bwd(dy3, x3, codes, exps, weight, bias, stats, dx, dw, db, ctx.groups, ctx.act, main)
         elif not main:
             for g in (dw, db):
                 if g is not None:
                     g.zero_()
-        return dx, _returned(weight, dw), _returned(bias, db), None, None, None, None
+        return dx, _returned(weight, dw, main), _returned(bias, db, main), None, None, None, None
+
+
+def _check_norm(x, num_groups, weight, bias, eps):
+    """Raises for arguments that do not belong together."""
+    if x.dim() < 2 or x.shape[-1] < 1:
+        raise ValueError(f"group_norm_act: x must be [samples, ..., channels], got {tuple(x.shape)}")
+    C = x.shape[-1]
+    if num_groups < 1 or C % num_groups:
+        raise ValueError(f"group_norm_act: {C} channels do not split into {num_groups} groups")
+    if not eps > 0:
+        raise ValueError("group_norm_act: eps must be positive")
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is not None and (p.shape != (C,) or (C > 1 and p.stride(0) != 1)):
+            raise ValueError(f"group_norm_act: {name} must be a contiguous [{C}], got {tuple(p.shape)}")
+    ptype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+    _check_tensors("group_norm_act", x, ptype, weight=weight, bias=bias)
 
 
 def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tensor] = None,
@@ -283,24 +309,9 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     dtype for both), whatever x's.  ``activation`` and ``checkpoint`` as in ``linear_act``."""
     act = _act_id(activation)
     _check_checkpoint(checkpoint)
-    if x.dim() < 2 or x.shape[-1] < 1:
-        raise ValueError(f"group_norm_act: x must be [samples, ..., channels], got {tuple(x.shape)}")
-    C = x.shape[-1]
-    if num_groups < 1 or C % num_groups:
-        raise ValueError(f"group_norm_act: {C} channels do not split into {num_groups} groups")
-    if not eps > 0:
-        raise ValueError("group_norm_act: eps must be positive")
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is not None and (p.shape != (C,) or (C > 1 and p.stride(0) != 1)):
-            raise ValueError(f"group_norm_act: {name} must be a contiguous [{C}], got {tuple(p.shape)}")
-        if p is not None and p.device != x.device:
-            raise ValueError(f"group_norm_act: {name} is on {p.device}, the input on {x.device}")
-    _check_tensors("group_norm_act", x.dtype, x=x)
-    ps = [p for p in (weight, bias) if p is not None]
-    if ps:
-        _check_tensors("group_norm_act", ps[0].dtype, weight=weight, bias=bias)
-    _native._require_cuda(x)
-    if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in ps)):
+    _check_norm(x, num_groups, weight, bias, eps)
+    if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad or
+                                    bias is not None and bias.requires_grad):
         return GroupNormActFunction.apply(x, weight, bias, num_groups, act, eps, checkpoint)
     return _norm_forward(x, num_groups, weight, bias, act, eps)[0]
 
