@@ -282,8 +282,8 @@ static void launch_rows_w(const GlLinearArgs& a, const LinEpilogue& e, bool alig
 template <typename T, int MT>
 static void launch_rows(const GlLinearArgs& a, const LinEpilogue& e, bool aligned, cudaStream_t st) {
   const int64_t loads = a.K * (int64_t)sizeof(T) / 512;       // 16-byte loads of a row, per lane of one warp
-  if (loads <= 8) launch_rows_w<T, MT, 1>(a, e, aligned, st);
-  else if (loads <= 16) launch_rows_w<T, MT, 2>(a, e, aligned, st);
+  if (loads <= 16) launch_rows_w<T, MT, 1>(a, e, aligned, st);
+  else if (loads <= 32) launch_rows_w<T, MT, 2>(a, e, aligned, st);
   else launch_rows_w<T, MT, 4>(a, e, aligned, st);
 }
 

@@ -508,10 +508,20 @@ static int operand_map(CUtensorMap* map, const MmaOperand& o, int64_t rows, int6
   const int64_t plane = o.planes > 1 ? o.plane : o.ld * (int64_t)dims[1];
   const cuuint64_t strides[2] = {(cuuint64_t)o.ld * 2, (cuuint64_t)plane * 2};
   const cuuint32_t boxes[3] = {64, (cuuint32_t)(o.mn ? 64 : box), 1}, ones[3] = {1, 1, 1};
-  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.ptr), dims, strides, boxes, ones,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS ? GL_OK : GL_ERR_SHAPE;
+  const auto encode = [&] {
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(o.ptr), dims, strides, boxes, ones,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {   // a thread whose first CUDA call this is: bind its device's context
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaSetDevice(dev);
+    if (e != cudaSuccess) return set_cuda_error(e);
+    r = encode();
+  }
+  return r == CUDA_SUCCESS ? GL_OK : r == CUDA_ERROR_INVALID_VALUE ? GL_ERR_SHAPE : GL_ERR_DEVICE;
 }
 
 template <int CTAS, int BN, int NPA, int NPB>

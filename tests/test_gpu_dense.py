@@ -316,6 +316,26 @@ def test_linear_on_another_stream():
     assert all(torch.equal(g, want) for g in got)
 
 
+def test_linear_as_a_threads_first_cuda_call():
+    """A thread that has not touched the device yet (autograd's, on its first backward) has no current context."""
+    import threading
+
+    x, w = data(64, 128, dtype=BF16, seed=1), data(64, 128, dtype=BF16, seed=2)
+    with torch.no_grad():
+        want = gl.linear_act(x, w)
+    got = []
+
+    def run():
+        with torch.no_grad():
+            got.append(gl.linear_act(x, w))
+
+    t = threading.Thread(target=run)
+    t.start()
+    t.join()
+    torch.cuda.synchronize()
+    assert len(got) == 1 and torch.equal(got[0], want)
+
+
 def test_linear_refusals():
     x, w = data(4, 16), data(8, 16)
     for args, kw in (((x, data(8, 15)), {}), ((x, w, data(7)), {}), ((x, w, None, data(4, 7)), {}),
