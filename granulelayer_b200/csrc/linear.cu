@@ -454,7 +454,11 @@ static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, c
     dz.mn = 1;
     e.out = a.dw;
     e.ldo = a.K;
-    e.accumulate = a.accumulate;
+    if (a.accumulate) {
+      e.residual = a.dw;
+      e.ldr = a.K;
+      e.dtype = GL_DTYPE_F32;
+    }
     if (int rc = mma_product(dz, x, a.N, a.K, a.M, e, db, work + w.split, st)) return rc;
   }
   return GL_OK;
@@ -483,7 +487,7 @@ extern "C" int gl_linear_fwd(const GlLinearArgs* args, void* stream) {
   if (a.M == 0) return GL_OK;
   if (!a.x || !a.w || !a.y || (a.slope_kind && !a.slope)) return GL_ERR_NULL;
   const int es = a.dtype == GL_DTYPE_F32 ? 4 : 2;
-  const LinEpilogue e{a.bias, a.residual, a.y, a.slope, a.ldr, a.ldy, a.lds, a.dtype, a.act, 0, a.slope_kind};
+  const LinEpilogue e{a.bias, a.residual, a.y, a.slope, a.ldr, a.ldy, a.lds, a.dtype, a.act, a.slope_kind};
   const bool aligned = rows16(a.x, a.ldx, es) && rows16(a.w, a.ldw, es);
   cudaStream_t st = (cudaStream_t)stream;
   if (few_rows(a.M, a.dtype))

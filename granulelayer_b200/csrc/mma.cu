@@ -28,9 +28,8 @@
 
 namespace gl {
 
-constexpr int kMmBM = 128, kMmBK = 64, kMmThreads = 320, kMmEpiWarps = 8, kMmMaxSlots = 9;
+constexpr int kMmBM = 128, kMmBK = 64, kMmThreads = 320, kMmEpiWarps = 8, kMmMaxSlots = 20;
 constexpr uint32_t kMmWaitLimit = 1u << 20;
-constexpr uint32_t kMmPlaneA = kMmBM * kMmBK * 2;
 constexpr int kMmPitch = 36;                                   // floats per row of a warp's 32 x 32 epilogue tile
 constexpr uint32_t kMmEpiBytes = kMmEpiWarps * 32 * kMmPitch * 4;
 
@@ -38,18 +37,17 @@ struct MmaParams {
   int64_t M, N;
   int tiles_m, tiles_n, kblocks, chunk, splits, split_blocks;
   int a_mn, b_mn, vec;
-  uint32_t a_bytes;      // of a plane of A in a slot (a tile of fewer than 128 rows loads fewer)
+  uint32_t a_bytes, b_bytes;   // of a plane of A and of B in a slot
+  int slots;
   float* part;
   LinEpilogue e;
   SumRows side;
 };
 
-// A slot: a plane of A (128 rows) and of B (this CTA's share of BN rows), 64 k each.
-__host__ __device__ constexpr uint32_t mm_slot_bytes(int BN, int CTAS) { return kMmPlaneA + (uint32_t)(BN / CTAS) * kMmBK * 2; }
-__host__ __device__ constexpr int mm_slots(int BN, int CTAS) {
-  const int n = (int)((227 * 1024 - 2048 - kMmEpiBytes) / mm_slot_bytes(BN, CTAS));
-  return n > kMmMaxSlots ? kMmMaxSlots : n;
-}
+// A slot: a plane of A (128 rows, or as many as there are) and of B (this CTA's share of BN rows), 64 k each; the ring
+// takes what the epilogue's tiles leave of the shared memory.  (The tensor core reads 128 rows of A whatever a slot
+// holds: the rows past a short A are whatever follows in shared memory, and give accumulator rows nobody reads.)
+constexpr uint32_t kMmRing = 227 * 1024 - 2048 - kMmEpiBytes;
 
 struct MmaShared {
   uint64_t full[kMmMaxSlots], empty[kMmMaxSlots], done[4], free_[4];
@@ -114,12 +112,12 @@ __device__ __forceinline__ bool mm_elect() {
 }
 
 // Position in the ring of slots: index and the parity of its current round.
-template <int ST>
 struct MmaRing {
-  int s = 0;
+  int slots, s = 0;
   uint32_t round = 0;
+  __device__ __forceinline__ explicit MmaRing(int n) : slots(n) {}
   __device__ __forceinline__ void next() {
-    if (++s == ST) {
+    if (++s == slots) {
       s = 0;
       ++round;
     }
@@ -145,45 +143,130 @@ __device__ __forceinline__ MmaTile mm_tile(const MmaParams& p, int64_t item, int
   return t;
 }
 
-// The warp's 32 x 32 block at (m0, n0), lane r holding row r: through shared memory, so that four lanes finish 32
-// columns of a row (or, where rows are not 16-byte aligned or the block is cut, a lane each column).
-__device__ __forceinline__ void mm_store_block(const MmaParams& p, float* tile, const float (&v)[32], int64_t m0,
-                                               int64_t n0, int split) {
+// ---- epilogue of a warp's 32 x 32 block at (m0, n0) ----
+// The accumulator gives lane r row r.  Through shared memory a lane gets, eight values at a time, what lies well in
+// memory: where rows are aligned and the block is whole in n (VEC), columns 8 (lane % 4) .. + 7 of row lane / 4 + 8 h,
+// in 16-byte accesses that fill sectors; else column `lane` of rows 8 h .. 8 h + 7, whose accesses coalesce across
+// lanes.  Eight at a time and not 32: a launch fetches its code from L2, and unrolled epilogues cost small products
+// 2 us.  FULL false (gradients): no bias, activation or slope.
+template <typename T, bool FULL, bool VEC>
+__device__ __forceinline__ void mm_finish8(const LinEpilogue& e, float (&z)[8], int64_t m, int64_t n, int rows) {
+  T* out = reinterpret_cast<T*>(e.out) + m * e.ldo + n;
+  float r[8];
+  if (e.residual) {
+    const T* p = reinterpret_cast<const T*>(e.residual) + m * e.ldr + n;
+    if constexpr (VEC) {
+      ld_span<T, 8>(p, true, r);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) r[i] = i < rows ? to_f32<T>(p[i * e.ldr]) : 0.f;
+    }
+  }
+  if constexpr (FULL) {
+    if (e.bias) {
+      const T* p = reinterpret_cast<const T*>(e.bias) + n;
+      float b[VEC ? 8 : 1];
+      ld_span<T, VEC ? 8 : 1>(p, VEC, b);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] += b[VEC ? i : 0];
+    }
+    with_act(e.act, [&](auto tag) {
+      constexpr int ACT = decltype(tag)::value;
+      if (e.slope_kind) {
+        float d[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) d[i] = dense_slope<ACT, sizeof(T) == 2>(z[i], z[i]);
+        if constexpr (VEC) {
+          st_slope<8>(e, m, n, true, d);
+        } else {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float t[1] = {d[i]};
+            if (i < rows) st_slope<1>(e, m + i, n, false, t);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = dense_act<ACT, sizeof(T) == 2>(z[i]);
+      }
+    });
+  }
+  if (e.residual) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) z[i] += r[i];
+  }
+  if constexpr (VEC) {
+    st_span<T, 8>(out, true, z);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (i < rows) out[i * e.ldo] = from_f32<T>(z[i]);
+  }
+}
+
+template <bool FULL, bool VEC>
+__device__ __forceinline__ void mm_store_rows(const MmaParams& p, const float* tile, int64_t m0, int64_t n0, int split) {
+  const int lane = threadIdx.x & 31, rows = (int)min((int64_t)32, p.M - m0);
+  const int c = VEC ? (lane & 3) * 8 : lane;
+  const int64_t n = n0 + c;
+  if (!VEC && n >= p.N) return;
+#pragma unroll 2
+  for (int h = 0; h < 4; ++h) {
+    const int r = 8 * h + (VEC ? lane >> 2 : 0);
+    if (r >= rows) break;
+    float z[8];
+    if constexpr (VEC) {
+      const float4 a = *reinterpret_cast<const float4*>(tile + r * kMmPitch + c);
+      const float4 b = *reinterpret_cast<const float4*>(tile + r * kMmPitch + c + 4);
+      z[0] = a.x; z[1] = a.y; z[2] = a.z; z[3] = a.w; z[4] = b.x; z[5] = b.y; z[6] = b.z; z[7] = b.w;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) z[i] = tile[(r + i) * kMmPitch + c];
+    }
+    if (p.part) {
+      float* out = p.part + (split * p.M + m0 + r) * p.N + n;
+      if constexpr (VEC) {
+        st_span<float, 8>(out, true, z);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (r + i < rows) out[i * p.N] = z[i];
+      }
+    } else if (p.e.dtype == GL_DTYPE_F32) {
+      mm_finish8<float, FULL, VEC>(p.e, z, m0 + r, n, rows - r);
+    } else {
+      mm_finish8<__nv_bfloat16, FULL, VEC>(p.e, z, m0 + r, n, rows - r);
+    }
+  }
+}
+
+template <bool FULL>
+__device__ __forceinline__ void mm_store_block(const MmaParams& p, float* tile, const float* v, int64_t m0, int64_t n0,
+                                               int split) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int j = 0; j < 32; j += 4)
     *reinterpret_cast<float4*>(tile + lane * kMmPitch + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
   __syncwarp();
-  const int64_t rows = p.M - m0;
-  if (n0 + 32 <= p.N && p.vec) {
-    const int c = (lane & 3) * 8;
-#pragma unroll 2
-    for (int i = 0; i < 4; ++i) {
-      const int r = 8 * i + (lane >> 2);
-      if (r >= rows) break;
-      const float4 a = *reinterpret_cast<const float4*>(tile + r * kMmPitch + c);
-      const float4 b = *reinterpret_cast<const float4*>(tile + r * kMmPitch + c + 4);
-      float z[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-      if (p.part) st_span<float, 8>(p.part + (split * p.M + m0 + r) * p.N + n0 + c, true, z);
-      else lin_finish<8>(p.e, m0 + r, n0 + c, true, z);
-    }
-  } else if (n0 + lane < p.N) {
-    const int n = rows < 32 ? (int)rows : 32;
-#pragma unroll 4
-    for (int r = 0; r < n; ++r) {
-      float z[1] = {tile[r * kMmPitch + lane]};
-      if (p.part) p.part[(split * p.M + m0 + r) * p.N + n0 + lane] = z[0];
-      else lin_finish<1>(p.e, m0 + r, n0 + lane, false, z);
-    }
-  }
+  if (p.vec && n0 + 32 <= p.N) mm_store_rows<FULL, true>(p, tile, m0, n0, split);
+  else mm_store_rows<FULL, false>(p, tile, m0, n0, split);
   __syncwarp();
 }
 
-template <int CTAS, int BN, int NPA, int NPB>
+// Asks L2 for the residual of a warp's rows m0 .. + 31, columns n0 .. + cols - 1, while its accumulator is being made.
+__device__ __forceinline__ void mm_prefetch(const MmaParams& p, int64_t m0, int64_t n0, int cols) {
+  const int lane = threadIdx.x & 31;
+  if (p.part || !p.e.residual || m0 + lane >= p.M) return;
+  const int es = p.e.dtype == GL_DTYPE_F32 ? 4 : 2;
+  const char* row = reinterpret_cast<const char*>(p.e.residual) + (m0 + lane) * p.e.ldr * es;
+  const int64_t end = min(p.N, n0 + cols) * es;
+  for (int64_t b = n0 * es; b < end; b += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + b));
+}
+
+template <int CTAS, int BN, int NPA, int NPB, bool FULL>
 __global__ void __launch_bounds__(kMmThreads, 1)
     mma_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const MmaParams p) {
-  constexpr int ST = mm_slots(BN, CTAS), BNC = BN / CTAS, BM = kMmBM * CTAS;
-  constexpr uint32_t kSlot = mm_slot_bytes(BN, CTAS);
+  constexpr int BNC = BN / CTAS, BM = kMmBM * CTAS;
   constexpr bool MULTI = NPA > 1;
   constexpr int NB = MULTI ? 4 : 2;                  // accumulators
   constexpr uint32_t kCols = NB * BN;                // TMEM columns
@@ -193,7 +276,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
   __shared__ MmaShared sh;
   const uint32_t pad = ((t5_smem_u32(mm_raw) + 1023u) & ~1023u) - t5_smem_u32(mm_raw);
   const uint32_t smem = t5_smem_u32(mm_raw) + pad;
-  float* epi = reinterpret_cast<float*>(mm_raw + pad + ST * kSlot);
+  float* epi = reinterpret_cast<float*>(mm_raw + pad + kMmRing / 1024 * 1024);
+  const uint32_t slot_bytes = p.a_bytes + p.b_bytes;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1);
   if (warp == 9) {
@@ -201,7 +285,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     else t5_tmem_alloc2(t5_smem_u32(&sh.tmem), kCols);
   }
   if (tid == 0) {
-    for (int i = 0; i < ST; ++i) {
+    for (int i = 0; i < p.slots; ++i) {
       t5_mbar_init(t5_smem_u32(&sh.full[i]), 1);
       t5_mbar_init(t5_smem_u32(&sh.empty[i]), 1);
     }
@@ -222,7 +306,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
 
   if (warp == 8) {
     if (mm_elect()) {
-      MmaRing<ST> r;
+      MmaRing r(p.slots);
       bool live = true;
       for (int64_t item = first; item < items && live; item += step) {
         const MmaTile t = mm_tile(p, item, BM, BN);
@@ -235,8 +319,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
               break;
             }
             uint32_t bar = t5_smem_u32(&sh.full[r.s]);
-            const uint32_t a = smem + r.s * kSlot, b = a + kMmPlaneA;
-            if (rank == 0) mm_expect(bar, CTAS * (p.a_bytes + (i < NPB ? kSlot - kMmPlaneA : 0u)));
+            const uint32_t a = smem + r.s * slot_bytes, b = a + p.a_bytes;
+            if (rank == 0) mm_expect(bar, CTAS * (p.a_bytes + (i < NPB ? p.b_bytes : 0u)));
             if constexpr (CTAS == 2) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(bar) : "r"(bar));
             if (p.a_mn) {
               mm_load<CTAS>(a, &ta, m0, kb * kMmBK, i, bar);
@@ -257,9 +341,9 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         }
       }
       if (!live && rank == 0) {   // the copies in flight must land before the shared memory goes away
-        const uint32_t it = r.round * ST + r.s;
-        for (uint32_t j = it > ST ? it - ST : 0; j < it; ++j)
-          t5_mbar_wait(t5_smem_u32(&sh.full[j % ST]), (j / ST) & 1, kMmWaitLimit);
+        const uint32_t n = (uint32_t)p.slots, it = r.round * n + r.s;
+        for (uint32_t j = it > n ? it - n : 0; j < it; ++j)
+          t5_mbar_wait(t5_smem_u32(&sh.full[j % n]), (j / n) & 1, kMmWaitLimit);
       }
     }
   } else if (warp == 9) {
@@ -267,7 +351,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
       const uint32_t idesc = t5_idesc_bf16(BM, BN, p.a_mn, p.b_mn);
       const uint32_t ka = (p.a_mn ? 2048u : 32u) >> 4, kb_ = (p.b_mn ? 2048u : 32u) >> 4;   // 16-byte units per 16 k
       const uint64_t desc = t5_desc_sw128(smem, 8192, 1024);   // of A in slot 0; the address field counts 16 bytes
-      MmaRing<ST> r;
+      MmaRing r(p.slots);
       uint32_t ch = 0;
       bool live = true;
       auto commit = [&](uint64_t& bar) {
@@ -286,8 +370,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
           const uint32_t d = tmem + buf * BN;
           uint32_t acc = 0;
           auto product = [&](int sa, int sb) {   // the plane of A in slot sa by the plane of B in slot sb
-            const uint64_t ad = desc + (uint32_t)(sa * (int)(kSlot >> 4));
-            const uint64_t bd = desc + (uint32_t)(sb * (int)(kSlot >> 4) + (int)(kMmPlaneA >> 4));
+            const uint64_t ad = desc + sa * (slot_bytes >> 4);
+            const uint64_t bd = desc + (sb * slot_bytes + p.a_bytes >> 4);
 #pragma unroll
             for (int k = 0; k < kMmBK / 16; ++k) {
               if constexpr (CTAS == 1) t5_mma_bf16(d, ad + k * ka, bd + k * kb_, idesc, acc);
@@ -341,6 +425,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
       const MmaTile t = mm_tile(p, item, BM, BN);
       const int64_t m0 = t.m0 + kMmBM * rank + 32 * (warp & 3), n0 = t.n0 + half * HALF;
       float sum[MULTI ? HALF : 1];
+      mm_prefetch(p, m0, n0, HALF);
       for (int c0 = t.k0; c0 < t.k1; c0 += p.chunk, ++ch) {
         const int buf = ch % NB;
         const bool ok = __all_sync(kFullMask, mm_wait(sh, sh.done[buf], (ch / NB) & 1));
@@ -373,17 +458,14 @@ __global__ void __launch_bounds__(kMmThreads, 1)
               __syncwarp();
               if (lane == 0) mm_arrive<CTAS>(t5_smem_u32(&sh.free_[buf]));
             }
-            if (m0 < p.M && n0 + 32 * q < p.N) mm_store_block(p, tile, v, m0, n0 + 32 * q, t.split);
+            if (m0 < p.M && n0 + 32 * q < p.N) mm_store_block<FULL>(p, tile, v, m0, n0 + 32 * q, t.split);
           }
         }
       }
       if constexpr (MULTI) {
 #pragma unroll
         for (int q = 0; q < HALF / 32; ++q) {
-          float v[32];
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = sum[32 * q + i];
-          if (m0 < p.M && n0 + 32 * q < p.N) mm_store_block(p, tile, v, m0, n0 + 32 * q, t.split);
+          if (m0 < p.M && n0 + 32 * q < p.N) mm_store_block<FULL>(p, tile, sum + 32 * q, m0, n0 + 32 * q, t.split);
         }
       }
     }
@@ -524,10 +606,10 @@ static int operand_map(CUtensorMap* map, const MmaOperand& o, int64_t rows, int6
   return r == CUDA_SUCCESS ? GL_OK : r == CUDA_ERROR_INVALID_VALUE ? GL_ERR_SHAPE : GL_ERR_DEVICE;
 }
 
-template <int CTAS, int BN, int NPA, int NPB>
+template <int CTAS, int BN, int NPA, int NPB, bool FULL>
 static int launch_mma(const CUtensorMap& ta, const CUtensorMap& tb, const MmaParams& p, int sms, cudaStream_t st) {
-  const auto kernel = mma_kernel<CTAS, BN, NPA, NPB>;
-  const size_t smem = mm_slots(BN, CTAS) * mm_slot_bytes(BN, CTAS) + kMmEpiBytes + 1024;
+  const auto kernel = mma_kernel<CTAS, BN, NPA, NPB, FULL>;
+  const size_t smem = kMmRing + kMmEpiBytes + 1024;
   if (int rc = ensure_dynamic_smem((const void*)kernel, smem)) return rc;
   const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits, most = sms / CTAS;
   cudaLaunchConfig_t cfg{};
@@ -547,17 +629,16 @@ static int launch_mma(const CUtensorMap& ta, const CUtensorMap& tb, const MmaPar
   return GL_OK;
 }
 
-template <int NPA, int NPB>
+template <int NPA, int NPB, bool FULL>
 static int launch_shape(const MmaPlan& pl, const CUtensorMap& ta, const CUtensorMap& tb, const MmaParams& p, int sms,
                         cudaStream_t st) {
   if constexpr (NPA == 1) {
-    if (pl.BN == 256) return launch_mma<2, 256, 1, 1>(ta, tb, p, sms, st);
+    if (pl.BN == 256) return launch_mma<2, 256, 1, 1, FULL>(ta, tb, p, sms, st);
+    if (pl.BN == 32) return launch_mma<1, 32, 1, 1, FULL>(ta, tb, p, sms, st);
   }
-  if (pl.ctas == 2) return launch_mma<2, 128, NPA, NPB>(ta, tb, p, sms, st);
-  if (pl.BN == 128) return launch_mma<1, 128, NPA, NPB>(ta, tb, p, sms, st);
-  if (pl.BN == 64) return launch_mma<1, 64, NPA, NPB>(ta, tb, p, sms, st);
-  if constexpr (NPA == 1) return launch_mma<1, 32, 1, 1>(ta, tb, p, sms, st);
-  return GL_ERR_UNSUPPORTED;
+  if (pl.ctas == 2) return launch_mma<2, 128, NPA, NPB, FULL>(ta, tb, p, sms, st);
+  if (pl.BN == 128) return launch_mma<1, 128, NPA, NPB, FULL>(ta, tb, p, sms, st);
+  return launch_mma<1, 64, NPA, NPB, FULL>(ta, tb, p, sms, st);
 }
 
 static bool aligned16(const void* p, int64_t ld, int esize) {
@@ -582,17 +663,24 @@ int mma_product(const MmaOperand& a, const MmaOperand& b, int64_t M, int64_t N, 
   p.kblocks = (int)((K + kMmBK - 1) / kMmBK); p.chunk = pl.chunk < p.kblocks ? pl.chunk : p.kblocks;
   p.splits = pl.splits; p.split_blocks = pl.split_blocks; p.a_mn = a.mn; p.b_mn = b.mn; p.e = e; p.side = side;
   p.a_bytes = (uint32_t)a_rows * kMmBK * 2;
-  const int es = e.dtype == GL_DTYPE_F32 || e.accumulate ? 4 : 2;
+  p.b_bytes = (uint32_t)(pl.BN / pl.ctas) * kMmBK * 2;
+  p.slots = (int)(kMmRing / 1024 * 1024 / (p.a_bytes + p.b_bytes));
+  if (p.slots > kMmMaxSlots) p.slots = kMmMaxSlots;
+  const int es = e.dtype == GL_DTYPE_F32 ? 4 : 2;
   const int ss = e.slope_kind == GL_SLOPE_F32 ? 4 : e.slope_kind == GL_SLOPE_I16 ? 2 : 1;
   const bool vec = aligned16(e.out, e.ldo, es) && aligned16(e.residual, e.ldr, es) && aligned16(e.bias, 0, es) &&
                    (ss == 1 ? e.slope == nullptr || (((uintptr_t)e.slope | e.lds) & 7) == 0
                             : aligned16(e.slope, e.lds, ss));
   p.part = pl.splits > 1 ? (float*)work : nullptr;
   p.vec = p.part ? N % 4 == 0 : vec;
+  const bool full = !p.part && (e.bias || e.act != GL_ACT_IDENTITY || e.slope_kind);
   int rc = GL_ERR_UNSUPPORTED;
-  if (a.planes == 1 && b.planes == 1) rc = launch_shape<1, 1>(pl, ta, tb, p, sms, st);
-  else if (a.planes == 3 && b.planes == 3) rc = launch_shape<3, 3>(pl, ta, tb, p, sms, st);
-  else if (a.planes == 3 && b.planes == 1) rc = launch_shape<3, 1>(pl, ta, tb, p, sms, st);
+  if (a.planes == 1 && b.planes == 1)
+    rc = full ? launch_shape<1, 1, true>(pl, ta, tb, p, sms, st) : launch_shape<1, 1, false>(pl, ta, tb, p, sms, st);
+  else if (a.planes == 3 && b.planes == 3)
+    rc = full ? launch_shape<3, 3, true>(pl, ta, tb, p, sms, st) : launch_shape<3, 3, false>(pl, ta, tb, p, sms, st);
+  else if (a.planes == 3 && b.planes == 1 && !full)   // only weight gradients meet a checkpoint
+    rc = launch_shape<3, 1, false>(pl, ta, tb, p, sms, st);
   if (rc || pl.splits == 1) return rc;
   const bool wide = vec && N % 8 == 0;
   const int64_t units = wide ? M * (N / 8) : M * N, need = (units + 255) / 256, cap = 16ll * sms;

@@ -10,15 +10,15 @@
 
 namespace gl {
 
-// What follows the sum over k for an element (m, n): z = sum + bias, slope = act'(z), out = act(z) + residual; or,
-// with `accumulate`, out (fp32) += sum.
+// What follows the sum over k for an element (m, n): z = sum + bias, slope = act'(z), out = act(z) + residual, all in
+// storage type `dtype`.  (Adding to an fp32 gradient is a residual that is the output itself.)
 struct LinEpilogue {
   const void* bias;
   const void* residual;
   void* out;
   void* slope;
   int64_t ldr, ldo, lds;
-  int dtype, act, accumulate, slope_kind;
+  int dtype, act, slope_kind;
 };
 
 // db[n] (=, or += with accumulate) the sum of `rows` partial rows part[r N + n] in row order: work that a product's
@@ -169,18 +169,8 @@ __device__ __forceinline__ void lin_finish_as(const LinEpilogue& e, int64_t m, i
 
 template <int N>
 __device__ __forceinline__ void lin_finish(const LinEpilogue& e, int64_t m, int64_t n, bool vec, float (&z)[N]) {
-  if (e.accumulate) {
-    float* out = reinterpret_cast<float*>(e.out) + m * e.ldo + n;
-    float t[N];
-    ld_span<float, N>(out, vec, t);
-#pragma unroll
-    for (int k = 0; k < N; ++k) t[k] += z[k];
-    st_span<float, N>(out, vec, t);
-  } else if (e.dtype == GL_DTYPE_F32) {
-    lin_finish_as<float, N>(e, m, n, vec, z);
-  } else {
-    lin_finish_as<__nv_bfloat16, N>(e, m, n, vec, z);
-  }
+  if (e.dtype == GL_DTYPE_F32) lin_finish_as<float, N>(e, m, n, vec, z);
+  else lin_finish_as<__nv_bfloat16, N>(e, m, n, vec, z);
 }
 
 }  // namespace gl
