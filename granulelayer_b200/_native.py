@@ -779,7 +779,8 @@ def linear_bwd(dy, slope, x, codes, exps, w, dx, dw, db, K: int, accumulate: boo
     """dx, dw, db (each may be None) of linear_fwd for the output gradient dy (GlLinearBwdArgs)."""
     M, N = dy.shape
     dt, dev = _DTYPE_IDS[dy.dtype], dy.device
-    work = _work("gl_linear_work_bytes", dev, M, N, K, dt, 1 | (0 if codes is None else 2) |
+    work = _work("gl_linear_work_bytes", dev, M, N, K, dt,
+                 1 | (0 if codes is None else 2) | (0 if dx is None else 8) | (0 if dw is None else 16) |
                  _unaligned(None if dx is None else w, None if dw is None else x))
     _launch("gl_linear_bwd", GlLinearBwdArgs(
         dy.data_ptr(), _ptr(slope), _ptr(x), _ptr(codes), _ptr(exps), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db),

@@ -333,11 +333,13 @@ static LinWork lin_fwd_work(int64_t M, int64_t N, int64_t K, int dtype, bool una
     w.x = w.take(np * M * up(K, 8) * 2);
     w.w = w.take(np * N * up(K, 8) * 2);
   }
-  w.split = w.take(mma_work_bytes(M, N, K, np, np, sms));
+  const MmaSize size{M, N, K, np, np, 0};
+  w.split = w.take(mma_work_bytes(&size, 1, sms));
   return w;
 }
 
-static LinWork lin_bwd_work(int64_t M, int64_t N, int64_t K, int dtype, bool codes, bool unaligned, int sms) {
+// `want`: GL_LINEAR_DX / GL_LINEAR_DW, the products of the call.
+static LinWork lin_bwd_work(int64_t M, int64_t N, int64_t K, int dtype, bool codes, bool unaligned, int want, int sms) {
   LinWork w;
   if (M == 0) return w;
   const int np = dtype == GL_DTYPE_F32 ? 3 : 1, npx = codes ? 1 : np;
@@ -345,8 +347,11 @@ static LinWork lin_bwd_work(int64_t M, int64_t N, int64_t K, int dtype, bool cod
   w.dz = w.take(np * M * up(N, 8) * 2);
   if (np == 3 || unaligned) w.w = w.take(np * N * up(K, 8) * 2);
   if (np == 3 || unaligned || codes) w.x = w.take(npx * M * up(K, 8) * 2);
-  const int64_t s1 = mma_work_bytes(M, K, N, np, np, sms), s2 = mma_work_bytes(N, K, M, np, npx, sms);
-  w.split = w.take(s1 > s2 ? s1 : s2);
+  MmaSize size[2];
+  int n = 0;
+  if (want & GL_LINEAR_DX) size[n++] = MmaSize{M, K, N, np, np, 1};
+  if (want & GL_LINEAR_DW) size[n++] = MmaSize{N, K, M, np, npx, 1};
+  w.split = w.take(n ? mma_work_bytes(size, n, sms) : 0);
   return w;
 }
 
@@ -382,7 +387,8 @@ static int run_linear_fwd(const GlLinearArgs& a, const LinEpilogue& e, const Lin
   const MmaOperand x = pack.add(a.x, a.M, a.K, a.ldx, 0, work + w.x);
   const MmaOperand wt = pack.add(a.w, a.N, a.K, a.ldw, 0, work + w.w);
   if (int rc = pack.run(sms, st)) return rc;
-  return mma_product(x, wt, a.M, a.N, a.K, e, SumRows{}, work + w.split, st);
+  const MmaJob job{x, wt, a.M, a.N, a.K, e};
+  return mma_run(&job, 1, SumRows{}, work + w.split, st);
 }
 
 template <typename T, int KIND>
@@ -418,7 +424,7 @@ static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, c
                                                   : launch_dz<T, GL_SLOPE_U8>(a, out, part, aligned, st);
     if (rc) return rc;
   }
-  SumRows db{};     // done beside the first product
+  SumRows db{};     // done beside the products
   if (a.db) db = SumRows{(const float*)(work + w.part), a.db, up(a.M, kDzRows) / kDzRows, a.N, a.dtype, a.accumulate};
   if (a.db && !a.dx && !a.dw) {
     lin_db_kernel<<<(unsigned)((a.N + 127) / 128), 128, 0, st>>>(db);
@@ -442,16 +448,18 @@ static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, c
     x = pack.add(a.x, a.M, a.K, a.ldx, 1, work + w.x);
   }
   if (int rc = pack.run(sms, st)) return rc;
-  LinEpilogue e{};
-  e.dtype = a.dtype;
+  MmaJob jobs[2];
+  int n = 0;
   if (a.dx) {   // [M, K] = dz [M, N] w [N, K]
+    LinEpilogue e{};
+    e.dtype = a.dtype;
     e.out = a.dx;
     e.ldo = a.lddx;
-    if (int rc = mma_product(dz, wt, a.M, a.K, a.N, e, db, work + w.split, st)) return rc;
-    db = SumRows{};
+    jobs[n++] = MmaJob{dz, wt, a.M, a.K, a.N, e};
   }
   if (a.dw) {   // [N, K] = dz^T [N, M] x [M, K]
-    dz.mn = 1;
+    LinEpilogue e{};
+    e.dtype = a.dtype;
     e.out = a.dw;
     e.ldo = a.K;
     if (a.accumulate) {
@@ -459,9 +467,10 @@ static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, c
       e.ldr = a.K;
       e.dtype = GL_DTYPE_F32;
     }
-    if (int rc = mma_product(dz, x, a.N, a.K, a.M, e, db, work + w.split, st)) return rc;
+    dz.mn = 1;
+    jobs[n++] = MmaJob{dz, x, a.N, a.K, a.M, e};
   }
-  return GL_OK;
+  return mma_run(jobs, n, db, work + w.split, st);
 }
 
 }  // namespace gl
@@ -473,7 +482,8 @@ extern "C" int64_t gl_linear_work_bytes(int64_t M, int64_t N, int64_t K, int32_t
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   const bool unaligned = (flags & GL_LINEAR_UNALIGNED) != 0;
-  if (flags & GL_LINEAR_BACKWARD) return lin_bwd_work(M, N, K, dtype, (flags & GL_LINEAR_CODES) != 0, unaligned, sms).total;
+  if (flags & GL_LINEAR_BACKWARD)
+    return lin_bwd_work(M, N, K, dtype, (flags & GL_LINEAR_CODES) != 0, unaligned, flags, sms).total;
   return lin_fwd_work(M, N, K, dtype, unaligned, sms).total;
 }
 
@@ -528,7 +538,8 @@ extern "C" int gl_linear_bwd(const GlLinearBwdArgs* args, void* stream) {
   const bool aligned = (!a.dx || rows16(a.w, a.ldw, es)) && (!a.dw || codes || rows16(a.x, a.ldx, es));
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
-  const LinWork w = lin_bwd_work(a.M, a.N, a.K, a.dtype, codes, !aligned, sms);
+  const int want = (a.dx ? GL_LINEAR_DX : 0) | (a.dw ? GL_LINEAR_DW : 0);
+  const LinWork w = lin_bwd_work(a.M, a.N, a.K, a.dtype, codes, !aligned, want, sms);
   if (w.total > 0 && (!a.work || a.work_bytes < w.total)) return GL_ERR_WORKSPACE;
   if ((uintptr_t)a.work & 255) return GL_ERR_ALIGN;
   return a.dtype == GL_DTYPE_F32 ? run_linear_bwd<float>(a, w, sms, st) : run_linear_bwd<__nv_bfloat16>(a, w, sms, st);

@@ -33,14 +33,19 @@ constexpr uint32_t kMmWaitLimit = 1u << 20;
 constexpr int kMmPitch = 36;                                   // floats per row of a warp's 32 x 32 epilogue tile
 constexpr uint32_t kMmEpiBytes = kMmEpiWarps * 32 * kMmPitch * 4;
 
-struct MmaParams {
+struct MmaOne {
   int64_t M, N;
-  int tiles_m, tiles_n, kblocks, chunk, splits, split_blocks;
-  int a_mn, b_mn, vec;
-  uint32_t a_bytes, b_bytes;   // of a plane of A and of B in a slot
-  int slots;
+  int tiles_m, tiles_n, kblocks, splits, split_blocks;
+  int a_mn, b_mn, vec, npb;
+  uint32_t a_bytes;            // of a plane of A as loaded
   float* part;
   LinEpilogue e;
+};
+struct MmaParams {
+  MmaOne job[2];
+  int64_t items0, items;       // work items of job 0, of all
+  int chunk, slots;
+  uint32_t a_slot, b_bytes;    // bytes of a slot for A, for B
   SumRows side;
 };
 
@@ -126,20 +131,23 @@ struct MmaRing {
 
 struct MmaTile {
   int64_t m0, n0;
-  int k0, k1, split;
+  int k0, k1, split, job;
 };
 
-// Work item -> tile and k range.  Tiles run in bands of 8 rows of tiles so that concurrent CTAs share operands in L2.
+// Work item -> job, tile and k range.  Tiles run in bands of 8 rows of tiles so that concurrent CTAs share operands in L2.
+template <int JOBS>
 __device__ __forceinline__ MmaTile mm_tile(const MmaParams& p, int64_t item, int BM, int BN) {
   MmaTile t;
-  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-  t.split = (int)(item / tiles);
-  const int64_t i = item - t.split * tiles, band = i / (8ll * p.tiles_n), first = band * 8;
-  const int64_t rows = min((int64_t)8, p.tiles_m - first), j = i - band * 8 * p.tiles_n;
+  t.job = JOBS == 1 ? 0 : item >= p.items0;   // one job: its parameters are constants of the launch
+  const MmaOne& o = p.job[JOBS == 1 ? 0 : t.job];
+  const int64_t tiles = (int64_t)o.tiles_m * o.tiles_n, it = t.job ? item - p.items0 : item;
+  t.split = (int)(it / tiles);
+  const int64_t i = it - t.split * tiles, band = i / (8ll * o.tiles_n), first = band * 8;
+  const int64_t rows = min((int64_t)8, o.tiles_m - first), j = i - band * 8 * o.tiles_n;
   t.m0 = (first + j % rows) * BM;
   t.n0 = (j / rows) * BN;
-  t.k0 = t.split * p.split_blocks;
-  t.k1 = min(p.kblocks, t.k0 + p.split_blocks);
+  t.k0 = t.split * o.split_blocks;
+  t.k1 = min(o.kblocks, t.k0 + o.split_blocks);
   return t;
 }
 
@@ -205,7 +213,7 @@ __device__ __forceinline__ void mm_finish8(const LinEpilogue& e, float (&z)[8], 
 }
 
 template <bool FULL, bool VEC>
-__device__ __forceinline__ void mm_store_rows(const MmaParams& p, const float* tile, int64_t m0, int64_t n0, int split) {
+__device__ __forceinline__ void mm_store_rows(const MmaOne& p, const float* tile, int64_t m0, int64_t n0, int split) {
   const int lane = threadIdx.x & 31, rows = (int)min((int64_t)32, p.M - m0);
   const int c = VEC ? (lane & 3) * 8 : lane;
   const int64_t n = n0 + c;
@@ -241,7 +249,7 @@ __device__ __forceinline__ void mm_store_rows(const MmaParams& p, const float* t
 }
 
 template <bool FULL>
-__device__ __forceinline__ void mm_store_block(const MmaParams& p, float* tile, const float* v, int64_t m0, int64_t n0,
+__device__ __forceinline__ void mm_store_block(const MmaOne& p, float* tile, const float* v, int64_t m0, int64_t n0,
                                                int split) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
@@ -254,7 +262,7 @@ __device__ __forceinline__ void mm_store_block(const MmaParams& p, float* tile, 
 }
 
 // Asks L2 for the residual of a warp's rows m0 .. + 31, columns n0 .. + cols - 1, while its accumulator is being made.
-__device__ __forceinline__ void mm_prefetch(const MmaParams& p, int64_t m0, int64_t n0, int cols) {
+__device__ __forceinline__ void mm_prefetch(const MmaOne& p, int64_t m0, int64_t n0, int cols) {
   const int lane = threadIdx.x & 31;
   if (p.part || !p.e.residual || m0 + lane >= p.M) return;
   const int es = p.e.dtype == GL_DTYPE_F32 ? 4 : 2;
@@ -263,9 +271,11 @@ __device__ __forceinline__ void mm_prefetch(const MmaParams& p, int64_t m0, int6
   for (int64_t b = n0 * es; b < end; b += 128) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + b));
 }
 
-template <int CTAS, int BN, int NPA, int NPB, bool FULL>
+template <int CTAS, int BN, int NPA, bool FULL, int JOBS>
 __global__ void __launch_bounds__(kMmThreads, 1)
-    mma_kernel(const __grid_constant__ CUtensorMap ta, const __grid_constant__ CUtensorMap tb, const MmaParams p) {
+    mma_kernel(const __grid_constant__ CUtensorMap ta0, const __grid_constant__ CUtensorMap tb0,
+               const __grid_constant__ CUtensorMap ta1, const __grid_constant__ CUtensorMap tb1,
+               const __grid_constant__ MmaParams p) {
   constexpr int BNC = BN / CTAS, BM = kMmBM * CTAS;
   constexpr bool MULTI = NPA > 1;
   constexpr int NB = MULTI ? 4 : 2;                  // accumulators
@@ -277,7 +287,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
   const uint32_t pad = ((t5_smem_u32(mm_raw) + 1023u) & ~1023u) - t5_smem_u32(mm_raw);
   const uint32_t smem = t5_smem_u32(mm_raw) + pad;
   float* epi = reinterpret_cast<float*>(mm_raw + pad + kMmRing / 1024 * 1024);
-  const uint32_t slot_bytes = p.a_bytes + p.b_bytes;
+  const uint32_t slot_bytes = p.a_slot + p.b_bytes;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = CTAS == 1 ? 0 : (int)(blockIdx.x & 1);
   if (warp == 9) {
@@ -301,7 +311,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
   else asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   t5_fence_after_sync();
   const uint32_t tmem = sh.tmem;
-  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+  const int64_t items = p.items;
   const int64_t first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (warp == 8) {
@@ -309,7 +319,12 @@ __global__ void __launch_bounds__(kMmThreads, 1)
       MmaRing r(p.slots);
       bool live = true;
       for (int64_t item = first; item < items && live; item += step) {
-        const MmaTile t = mm_tile(p, item, BM, BN);
+        const MmaTile t = mm_tile<JOBS>(p, item, BM, BN);
+        const MmaOne& o = p.job[JOBS == 1 ? 0 : t.job];
+        const CUtensorMap* ta = JOBS == 1 || !t.job ? &ta0 : &ta1;
+        const CUtensorMap* tb = JOBS == 1 || !t.job ? &tb0 : &tb1;
+        const int a_mn = o.a_mn, b_mn = o.b_mn, npb = o.npb;
+        const uint32_t a_bytes = o.a_bytes;
         const int m0 = (int)t.m0 + kMmBM * rank, n0 = (int)t.n0 + BNC * rank;
         for (int kb = t.k0; kb < t.k1 && live; ++kb) {
 #pragma unroll
@@ -319,22 +334,22 @@ __global__ void __launch_bounds__(kMmThreads, 1)
               break;
             }
             uint32_t bar = t5_smem_u32(&sh.full[r.s]);
-            const uint32_t a = smem + r.s * slot_bytes, b = a + p.a_bytes;
-            if (rank == 0) mm_expect(bar, CTAS * (p.a_bytes + (i < NPB ? p.b_bytes : 0u)));
+            const uint32_t a = smem + r.s * slot_bytes, b = a + p.a_slot;
+            if (rank == 0) mm_expect(bar, CTAS * (a_bytes + (i < npb ? p.b_bytes : 0u)));
             if constexpr (CTAS == 2) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(bar) : "r"(bar));
-            if (p.a_mn) {
-              mm_load<CTAS>(a, &ta, m0, kb * kMmBK, i, bar);
-              mm_load<CTAS>(a + 8192, &ta, m0 + 64, kb * kMmBK, i, bar);
+            if (a_mn) {
+              mm_load<CTAS>(a, ta, m0, kb * kMmBK, i, bar);
+              mm_load<CTAS>(a + 8192, ta, m0 + 64, kb * kMmBK, i, bar);
             } else {
-              mm_load<CTAS>(a, &ta, kb * kMmBK, m0, i, bar);
+              mm_load<CTAS>(a, ta, kb * kMmBK, m0, i, bar);
             }
-            if (i < NPB) {
-              if (BNC >= 64 && p.b_mn) {
+            if (i < npb) {
+              if (BNC >= 64 && b_mn) {
 #pragma unroll
                 for (int h = 0; h < BNC / 64; ++h)
-                  mm_load<CTAS>(b + h * 8192, &tb, n0 + 64 * h, kb * kMmBK, i, bar);
+                  mm_load<CTAS>(b + h * 8192, tb, n0 + 64 * h, kb * kMmBK, i, bar);
               } else {
-                mm_load<CTAS>(b, &tb, kb * kMmBK, n0, i, bar);
+                mm_load<CTAS>(b, tb, kb * kMmBK, n0, i, bar);
               }
             }
           }
@@ -348,8 +363,6 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     }
   } else if (warp == 9) {
     if (rank == 0 && mm_elect()) {
-      const uint32_t idesc = t5_idesc_bf16(BM, BN, p.a_mn, p.b_mn);
-      const uint32_t ka = (p.a_mn ? 2048u : 32u) >> 4, kb_ = (p.b_mn ? 2048u : 32u) >> 4;   // 16-byte units per 16 k
       const uint64_t desc = t5_desc_sw128(smem, 8192, 1024);   // of A in slot 0; the address field counts 16 bytes
       MmaRing r(p.slots);
       uint32_t ch = 0;
@@ -359,7 +372,11 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         else t5_commit_pair(t5_smem_u32(&bar));
       };
       for (int64_t item = first; item < items && live; item += step) {
-        const MmaTile t = mm_tile(p, item, BM, BN);
+        const MmaTile t = mm_tile<JOBS>(p, item, BM, BN);
+        const MmaOne& o = p.job[JOBS == 1 ? 0 : t.job];
+        const uint32_t idesc = t5_idesc_bf16(BM, BN, 0, 0) | ((uint32_t)o.a_mn << 15) | ((uint32_t)o.b_mn << 16);
+        const int npb = o.npb;
+        const uint32_t ka = (o.a_mn ? 2048u : 32u) >> 4, kb_ = (o.b_mn ? 2048u : 32u) >> 4;   // 16-byte units per 16 k
         for (int c0 = t.k0; c0 < t.k1 && live; c0 += p.chunk, ++ch) {
           const int c1 = min(t.k1, c0 + p.chunk), buf = ch % NB;
           if (ch >= NB && !mm_wait(sh, sh.free_[buf], (ch / NB - 1) & 1)) {
@@ -371,7 +388,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
           uint32_t acc = 0;
           auto product = [&](int sa, int sb) {   // the plane of A in slot sa by the plane of B in slot sb
             const uint64_t ad = desc + sa * (slot_bytes >> 4);
-            const uint64_t bd = desc + (sb * slot_bytes + p.a_bytes >> 4);
+            const uint64_t bd = desc + (sb * slot_bytes + p.a_slot >> 4);
 #pragma unroll
             for (int k = 0; k < kMmBK / 16; ++k) {
               if constexpr (CTAS == 1) t5_mma_bf16(d, ad + k * ka, bd + k * kb_, idesc, acc);
@@ -390,7 +407,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
             t5_fence_after_sync();
             if constexpr (NPA == 1) {
               product(slot[0], slot[0]);
-            } else if constexpr (NPB == 1) {
+            } else if (npb == 1) {
               product(slot[2], slot[0]);
               commit(sh.empty[slot[2]]);
               product(slot[1], slot[0]);
@@ -422,10 +439,11 @@ __global__ void __launch_bounds__(kMmThreads, 1)
     }
     uint32_t ch = 0;
     for (int64_t item = first; item < items; item += step) {
-      const MmaTile t = mm_tile(p, item, BM, BN);
+      const MmaTile t = mm_tile<JOBS>(p, item, BM, BN);
+      const MmaOne& o = p.job[JOBS == 1 ? 0 : t.job];
       const int64_t m0 = t.m0 + kMmBM * rank + 32 * (warp & 3), n0 = t.n0 + half * HALF;
       float sum[MULTI ? HALF : 1];
-      mm_prefetch(p, m0, n0, HALF);
+      mm_prefetch(o, m0, n0, HALF);
       for (int c0 = t.k0; c0 < t.k1; c0 += p.chunk, ++ch) {
         const int buf = ch % NB;
         const bool ok = __all_sync(kFullMask, mm_wait(sh, sh.done[buf], (ch / NB) & 1));
@@ -458,14 +476,14 @@ __global__ void __launch_bounds__(kMmThreads, 1)
               __syncwarp();
               if (lane == 0) mm_arrive<CTAS>(t5_smem_u32(&sh.free_[buf]));
             }
-            if (m0 < p.M && n0 + 32 * q < p.N) mm_store_block<FULL>(p, tile, v, m0, n0 + 32 * q, t.split);
+            if (m0 < o.M && n0 + 32 * q < o.N) mm_store_block<FULL>(o, tile, v, m0, n0 + 32 * q, t.split);
           }
         }
       }
       if constexpr (MULTI) {
 #pragma unroll
         for (int q = 0; q < HALF / 32; ++q) {
-          if (m0 < p.M && n0 + 32 * q < p.N) mm_store_block<FULL>(p, tile, sum + 32 * q, m0, n0 + 32 * q, t.split);
+          if (m0 < o.M && n0 + 32 * q < o.N) mm_store_block<FULL>(o, tile, sum + 32 * q, m0, n0 + 32 * q, t.split);
         }
       }
     }
@@ -506,64 +524,107 @@ __global__ void __launch_bounds__(256) mma_join_kernel(const float* part, int64_
 
 // ---- host ----
 struct MmaPlan {
-  int ctas, BN, splits, split_blocks, chunk;
-  int64_t tiles_m, tiles_n;
+  int ctas, BN;
+  int splits[2], split_blocks[2];
 };
 
-// Tile shape and number of splits of k: the least estimated time, in clocks of one SM.  64 k cost the larger of
-// the MMAs (2 BN clocks a term) and the loads (about 60 bytes a clock into one SM of many) and four tenths of the
-// smaller; split sums add their partial tiles' traffic and a second launch.
-static MmaPlan mma_search(int64_t M, int64_t N, int64_t K, int npa, int npb, bool b_mn, int sms) {
+// Tile shape and splits of k: the least estimated time, in clocks of one SM, fitted to measured products (256 x 256
+// pairs 610 clocks per 64 k, 128 x 32 tiles 400 however few bytes, epilogues 37 clocks a column).  64 k cost the
+// larger of the MMAs (2 BN clocks a term) and the loads (60 bytes a clock into one SM of many), a fifth of the smaller
+// and a hand-over; an epilogue runs beside the next item's sum; split sums add their partial tiles' traffic and a
+// launch.
+static MmaPlan mma_search(const MmaSize* z, int n, int sms) {
   MmaPlan best{};
   double best_t = 1e300;
-  const int64_t kb = (K + kMmBK - 1) / kMmBK;
-  const int terms = npa == 1 ? 1 : (npb == 1 ? 3 : 6);
   struct Shape { int ctas, BN; };
+  static const int kSplits[] = {1, 2, 3, 4, 5, 6, 8, 10, 12, 16, 24, 32};
   for (Shape sh : {Shape{2, 256}, Shape{2, 128}, Shape{1, 128}, Shape{1, 64}, Shape{1, 32}}) {
-    if (sh.BN == 32 && (b_mn || npa > 1)) continue;
-    if (sh.BN == 256 && npa > 1) continue;     // four accumulators fill the tensor memory
-    const int64_t tm = (M + kMmBM * sh.ctas - 1) / (kMmBM * sh.ctas), tn = (N + sh.BN - 1) / sh.BN, tiles = tm * tn;
-    const double bytes = npa * (double)(M < kMmBM ? M : kMmBM) * kMmBK * 2 + npb * (double)(sh.BN / sh.ctas) * kMmBK * 2;
-    const double load = bytes / 60.0, mma = terms * 2.0 * sh.BN;
-    const double block = load > mma ? load + 0.4 * mma : mma + 0.4 * load;
-    const int64_t wide = sms / sh.ctas;
-    for (int s = 1; s <= 32 && s <= kb; ++s) {
-      const int64_t sb = (kb + s - 1) / s;
-      if ((kb + sb - 1) / sb != s) continue;
-      const int64_t waves = (tiles * s + wide - 1) / wide;
-      double t = (double)waves * sb * block + 3000.0 + (double)sh.BN * 12 + 500.0 * (sh.ctas - 1);
-      if (s > 1) t += 4000.0 + (double)M * N * (s + 1) * 4 / 2500.0;
-      if (t < best_t) {
-        best_t = t;
-        best = MmaPlan{sh.ctas, sh.BN, s, (int)sb, npa > 1 ? 2 : 1 << 30, tm, tn};
+    bool fits = true;
+    for (int j = 0; j < n; ++j) {
+      if (sh.BN == 32 && (z[j].b_mn || z[j].npa > 1)) fits = false;
+      if (sh.BN == 256 && z[j].npa > 1) fits = false;          // four accumulators fill the tensor memory
+    }
+    if (!fits) continue;
+    const double wide = sms / sh.ctas, epilogue = 800 + sh.BN * 37.0;
+    double tiles[2] = {0, 0}, block[2] = {0, 0}, out[2] = {0, 0};
+    int64_t kb[2] = {1, 1};
+    for (int j = 0; j < n; ++j) {
+      const int64_t bm = kMmBM * sh.ctas;
+      const int terms = z[j].npa == 1 ? 1 : (z[j].npb == 1 ? 3 : 6);
+      const double bytes = z[j].npa * (double)(z[j].M < kMmBM ? z[j].M : kMmBM) * kMmBK * 2 +
+                           z[j].npb * (double)(sh.BN / sh.ctas) * kMmBK * 2;
+      const double load = bytes / 60.0, mma = terms * 2.0 * sh.BN;
+      tiles[j] = (double)((z[j].M + bm - 1) / bm) * (double)((z[j].N + sh.BN - 1) / sh.BN);
+      block[j] = (load > mma ? load + 0.2 * mma : mma + 0.2 * load) + 50;
+      if (block[j] < 400) block[j] = 400;
+      kb[j] = (z[j].K + kMmBK - 1) / kMmBK;
+      out[j] = (double)z[j].M * z[j].N;
+    }
+    for (int s0 : kSplits) {
+      if (s0 > kb[0]) break;
+      for (int s1 : kSplits) {
+        if (s1 > 1 && (n < 2 || s1 > kb[1])) break;
+        const int s[2] = {s0, s1};
+        double sum = 0, longest = 0, extra = 0, items = 0;
+        for (int j = 0; j < n; ++j) {
+          double t = (double)((kb[j] + s[j] - 1) / s[j]) * block[j];
+          if (t < epilogue) t = epilogue;
+          sum += tiles[j] * s[j] * t;
+          items += tiles[j] * s[j];
+          if (t > longest) longest = t;
+          if (s[j] > 1) extra += 5000.0 + out[j] * (s[j] + 1) * 4 / 2500.0;
+        }
+        const double waves = (double)(int64_t)((items + wide - 1) / wide);
+        const double even = sum / items * waves;                 // every CTA the same number of items
+        const double t = (even > longest ? even : longest) + epilogue + extra + 500.0 * (sh.ctas - 1);
+        if (t < best_t) {
+          best_t = t;
+          best = MmaPlan{sh.ctas, sh.BN, {s0, s1}, {1, 1}};
+          for (int j = 0; j < n; ++j) best.split_blocks[j] = (int)((kb[j] + s[j] - 1) / s[j]);
+        }
       }
     }
+  }
+  for (int j = 0; j < n; ++j) {   // no empty splits
+    const int64_t kb = (z[j].K + kMmBK - 1) / kMmBK;
+    best.splits[j] = (int)((kb + best.split_blocks[j] - 1) / best.split_blocks[j]);
   }
   return best;
 }
 
-// mma_search with the last plans of this thread at hand: a search costs about as much host time as a launch.
-static MmaPlan mma_plan(int64_t M, int64_t N, int64_t K, int npa, int npb, bool b_mn, int sms) {
+// mma_search with the last plans of this thread at hand: a search costs more host time than a launch.
+static MmaPlan mma_plan(const MmaSize* z, int n, int sms) {
   struct Entry {
-    int64_t M, N, K;
-    int key;
+    MmaSize z[2];
+    int n, sms;
     MmaPlan plan;
   };
   static thread_local Entry cache[64];
-  const int key = 1 + b_mn + 2 * npa + 8 * npb + 32 * sms;
-  Entry& e = cache[(M * 31 + N * 17 + K * 7 + key) & 63];
-  if (e.key != key || e.M != M || e.N != N || e.K != K) e = Entry{M, N, K, key, mma_search(M, N, K, npa, npb, b_mn, sms)};
+  int64_t h = n;
+  for (int j = 0; j < n; ++j) h = h * 31 + z[j].M * 17 + z[j].N * 7 + z[j].K * 3 + z[j].npa + 2 * z[j].npb + z[j].b_mn;
+  Entry& e = cache[h & 63];
+  bool hit = e.n == n && e.sms == sms;
+  for (int j = 0; j < n && hit; ++j)
+    hit = e.z[j].M == z[j].M && e.z[j].N == z[j].N && e.z[j].K == z[j].K && e.z[j].npa == z[j].npa &&
+          e.z[j].npb == z[j].npb && e.z[j].b_mn == z[j].b_mn;
+  if (!hit) {
+    e.n = n;
+    e.sms = sms;
+    for (int j = 0; j < n; ++j) e.z[j] = z[j];
+    e.plan = mma_search(z, n, sms);
+  }
   return e.plan;
 }
 
-int64_t mma_work_bytes(int64_t M, int64_t N, int64_t K, int npa, int npb, int sms) {
-  int64_t most = 0;
-  for (int b_mn = 0; b_mn < 2; ++b_mn) {
-    const MmaPlan pl = mma_plan(M, N, K, npa, npb, b_mn, sms);
-    const int64_t n = pl.splits > 1 ? 4 * pl.splits * M * N : 0;
-    if (n > most) most = n;
-  }
-  return most;
+static int64_t split_bytes(const MmaSize& z, int splits) {
+  return splits > 1 ? (4 * splits * z.M * z.N + 255) / 256 * 256 : 0;
+}
+
+int64_t mma_work_bytes(const MmaSize* z, int n, int sms) {
+  const MmaPlan pl = mma_plan(z, n, sms);
+  int64_t bytes = 0;
+  for (int j = 0; j < n; ++j) bytes += split_bytes(z[j], pl.splits[j]);
+  return bytes;
 }
 
 typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -606,14 +667,14 @@ static int operand_map(CUtensorMap* map, const MmaOperand& o, int64_t rows, int6
   return r == CUDA_SUCCESS ? GL_OK : r == CUDA_ERROR_INVALID_VALUE ? GL_ERR_SHAPE : GL_ERR_DEVICE;
 }
 
-template <int CTAS, int BN, int NPA, int NPB, bool FULL>
-static int launch_mma(const CUtensorMap& ta, const CUtensorMap& tb, const MmaParams& p, int sms, cudaStream_t st) {
-  const auto kernel = mma_kernel<CTAS, BN, NPA, NPB, FULL>;
+template <int CTAS, int BN, int NPA, bool FULL, int JOBS>
+static int launch_mma(const CUtensorMap (&map)[4], const MmaParams& p, int sms, cudaStream_t st) {
+  const auto kernel = mma_kernel<CTAS, BN, NPA, FULL, JOBS>;
   const size_t smem = kMmRing + kMmEpiBytes + 1024;
   if (int rc = ensure_dynamic_smem((const void*)kernel, smem)) return rc;
-  const int64_t items = (int64_t)p.tiles_m * p.tiles_n * p.splits, most = sms / CTAS;
+  const int64_t most = sms / CTAS;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((items < most ? items : most) * CTAS));
+  cfg.gridDim = dim3((unsigned)((p.items < most ? p.items : most) * CTAS));
   cfg.blockDim = dim3(kMmThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -623,73 +684,110 @@ static int launch_mma(const CUtensorMap& ta, const CUtensorMap& tb, const MmaPar
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
   cfg.numAttrs = CTAS > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, ta, tb, p);
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, map[0], map[1], map[2], map[3], p);
   if (e != cudaSuccess) return set_cuda_error(e);
   count_launches(1);
   return GL_OK;
 }
 
-template <int NPA, int NPB, bool FULL>
-static int launch_shape(const MmaPlan& pl, const CUtensorMap& ta, const CUtensorMap& tb, const MmaParams& p, int sms,
-                        cudaStream_t st) {
+template <int NPA, bool FULL, int JOBS>
+static int launch_shape(const MmaPlan& pl, const CUtensorMap (&map)[4], const MmaParams& p, int sms, cudaStream_t st) {
   if constexpr (NPA == 1) {
-    if (pl.BN == 256) return launch_mma<2, 256, 1, 1, FULL>(ta, tb, p, sms, st);
-    if (pl.BN == 32) return launch_mma<1, 32, 1, 1, FULL>(ta, tb, p, sms, st);
+    if (pl.BN == 256) return launch_mma<2, 256, 1, FULL, JOBS>(map, p, sms, st);
+    if constexpr (JOBS == 1)                                       // an MN-major B has no 32-wide tiles
+      if (pl.BN == 32) return launch_mma<1, 32, 1, FULL, JOBS>(map, p, sms, st);
   }
-  if (pl.ctas == 2) return launch_mma<2, 128, NPA, NPB, FULL>(ta, tb, p, sms, st);
-  if (pl.BN == 128) return launch_mma<1, 128, NPA, NPB, FULL>(ta, tb, p, sms, st);
-  return launch_mma<1, 64, NPA, NPB, FULL>(ta, tb, p, sms, st);
+  if (pl.ctas == 2) return launch_mma<2, 128, NPA, FULL, JOBS>(map, p, sms, st);
+  if (pl.BN == 128) return launch_mma<1, 128, NPA, FULL, JOBS>(map, p, sms, st);
+  return launch_mma<1, 64, NPA, FULL, JOBS>(map, p, sms, st);
+}
+
+template <int NPA>
+static int launch_jobs(const MmaPlan& pl, const CUtensorMap (&map)[4], const MmaParams& p, int n, bool full, int sms,
+                       cudaStream_t st) {
+  if (n == 2) return launch_shape<NPA, false, 2>(pl, map, p, sms, st);   // gradients: no activation
+  return full ? launch_shape<NPA, true, 1>(pl, map, p, sms, st) : launch_shape<NPA, false, 1>(pl, map, p, sms, st);
 }
 
 static bool aligned16(const void* p, int64_t ld, int esize) {
   return p == nullptr || (((uintptr_t)p & 15) == 0 && (ld * esize) % 16 == 0);
 }
 
-int mma_product(const MmaOperand& a, const MmaOperand& b, int64_t M, int64_t N, int64_t K, const LinEpilogue& e,
-                const SumRows& side, void* work, cudaStream_t st) {
-  if (M > 0x7FFFFF00 || N > 0x7FFFFF00 || K > 0x7FFFFF00) return GL_ERR_SHAPE;
-  int sms = 0;
-  if (int rc = device_sm_count(&sms)) return rc;
-  const MmaPlan pl = mma_plan(M, N, K, a.planes, b.planes, b.mn, sms);
-  if (pl.splits > 1 && !work) return GL_ERR_WORKSPACE;
-  CUtensorMap ta, tb;
-  // a tile of fewer rows than 128 (one CTA's only) loads those; the rest of the slot stays as it is, for rows of the
-  // accumulator that nobody reads
-  const int a_rows = M < kMmBM && !a.mn ? (int)(M + 7) / 8 * 8 : kMmBM;
-  if (int rc = operand_map(&ta, a, M, K, a_rows)) return rc;
-  if (int rc = operand_map(&tb, b, N, K, pl.BN / pl.ctas)) return rc;
-  MmaParams p{};
-  p.M = M; p.N = N; p.tiles_m = (int)pl.tiles_m; p.tiles_n = (int)pl.tiles_n;
-  p.kblocks = (int)((K + kMmBK - 1) / kMmBK); p.chunk = pl.chunk < p.kblocks ? pl.chunk : p.kblocks;
-  p.splits = pl.splits; p.split_blocks = pl.split_blocks; p.a_mn = a.mn; p.b_mn = b.mn; p.e = e; p.side = side;
-  p.a_bytes = (uint32_t)a_rows * kMmBK * 2;
-  p.b_bytes = (uint32_t)(pl.BN / pl.ctas) * kMmBK * 2;
-  p.slots = (int)(kMmRing / 1024 * 1024 / (p.a_bytes + p.b_bytes));
-  if (p.slots > kMmMaxSlots) p.slots = kMmMaxSlots;
+// Every tensor of an epilogue can be accessed in 16-byte pieces.
+static bool epilogue_vec(const LinEpilogue& e) {
   const int es = e.dtype == GL_DTYPE_F32 ? 4 : 2;
   const int ss = e.slope_kind == GL_SLOPE_F32 ? 4 : e.slope_kind == GL_SLOPE_I16 ? 2 : 1;
-  const bool vec = aligned16(e.out, e.ldo, es) && aligned16(e.residual, e.ldr, es) && aligned16(e.bias, 0, es) &&
-                   (ss == 1 ? e.slope == nullptr || (((uintptr_t)e.slope | e.lds) & 7) == 0
-                            : aligned16(e.slope, e.lds, ss));
-  p.part = pl.splits > 1 ? (float*)work : nullptr;
-  p.vec = p.part ? N % 4 == 0 : vec;
-  const bool full = !p.part && (e.bias || e.act != GL_ACT_IDENTITY || e.slope_kind);
-  int rc = GL_ERR_UNSUPPORTED;
-  if (a.planes == 1 && b.planes == 1)
-    rc = full ? launch_shape<1, 1, true>(pl, ta, tb, p, sms, st) : launch_shape<1, 1, false>(pl, ta, tb, p, sms, st);
-  else if (a.planes == 3 && b.planes == 3)
-    rc = full ? launch_shape<3, 3, true>(pl, ta, tb, p, sms, st) : launch_shape<3, 3, false>(pl, ta, tb, p, sms, st);
-  else if (a.planes == 3 && b.planes == 1 && !full)   // only weight gradients meet a checkpoint
-    rc = launch_shape<3, 1, false>(pl, ta, tb, p, sms, st);
-  if (rc || pl.splits == 1) return rc;
-  const bool wide = vec && N % 8 == 0;
-  const int64_t units = wide ? M * (N / 8) : M * N, need = (units + 255) / 256, cap = 16ll * sms;
-  const unsigned blocks = (unsigned)(need < cap ? need : cap);
-  if (wide) mma_join_kernel<8><<<blocks, 256, 0, st>>>(p.part, M, N, pl.splits, e);
-  else mma_join_kernel<1><<<blocks, 256, 0, st>>>(p.part, M, N, pl.splits, e);
-  const cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) return set_cuda_error(err);
-  count_launches(1);
+  return aligned16(e.out, e.ldo, es) && aligned16(e.residual, e.ldr, es) && aligned16(e.bias, 0, es) &&
+         (ss == 1 ? e.slope == nullptr || (((uintptr_t)e.slope | e.lds) & 7) == 0 : aligned16(e.slope, e.lds, ss));
+}
+
+int mma_run(const MmaJob* jobs, int n, const SumRows& side, void* work, cudaStream_t st) {
+  int sms = 0;
+  if (int rc = device_sm_count(&sms)) return rc;
+  MmaSize z[2];
+  for (int j = 0; j < n; ++j) {
+    const MmaJob& q = jobs[j];
+    if (q.M > 0x7FFFFF00 || q.N > 0x7FFFFF00 || q.K > 0x7FFFFF00) return GL_ERR_SHAPE;
+    z[j] = MmaSize{q.M, q.N, q.K, q.a.planes, q.b.planes, q.b.mn};
+  }
+  const MmaPlan pl = mma_plan(z, n, sms);
+  CUtensorMap map[4];
+  MmaParams p{};
+  bool full = false;
+  char* scratch = (char*)work;
+  for (int j = 0; j < n; ++j) {
+    const MmaJob& q = jobs[j];
+    MmaOne& o = p.job[j];
+    // a tile of fewer rows than 128 loads those; the rest of the slot stays as it is, for rows of the accumulator that
+    // nobody reads
+    const int a_rows = q.M < kMmBM && !q.a.mn ? (int)(q.M + 7) / 8 * 8 : kMmBM;
+    if (int rc = operand_map(&map[2 * j], q.a, q.M, q.K, a_rows)) return rc;
+    if (int rc = operand_map(&map[2 * j + 1], q.b, q.N, q.K, pl.BN / pl.ctas)) return rc;
+    o.M = q.M;
+    o.N = q.N;
+    o.tiles_m = (int)((q.M + kMmBM * pl.ctas - 1) / (kMmBM * pl.ctas));
+    o.tiles_n = (int)((q.N + pl.BN - 1) / pl.BN);
+    o.kblocks = (int)((q.K + kMmBK - 1) / kMmBK);
+    o.splits = pl.splits[j];
+    o.split_blocks = pl.split_blocks[j];
+    o.a_mn = q.a.mn;
+    o.b_mn = q.b.mn;
+    o.npb = q.b.planes;
+    o.a_bytes = (uint32_t)a_rows * kMmBK * 2;
+    o.e = q.e;
+    o.vec = epilogue_vec(q.e);
+    if (o.splits > 1) {
+      if (!work) return GL_ERR_WORKSPACE;
+      o.part = (float*)scratch;
+      scratch += split_bytes(z[j], o.splits);
+      o.vec = q.N % 4 == 0;
+    } else if (q.e.bias || q.e.act != GL_ACT_IDENTITY || q.e.slope_kind) {
+      full = true;
+    }
+    p.items += (int64_t)o.tiles_m * o.tiles_n * o.splits;
+    if (j == 0) p.items0 = p.items;
+    if (o.a_bytes > p.a_slot) p.a_slot = o.a_bytes;
+  }
+  if (n == 1) map[2] = map[3] = map[0];
+  p.chunk = z[0].npa > 1 ? 2 : 1 << 30;   // one chunk; k block numbers stay below 2^25
+  p.b_bytes = (uint32_t)(pl.BN / pl.ctas) * kMmBK * 2;
+  p.slots = (int)(kMmRing / 1024 * 1024 / (p.a_slot + p.b_bytes));
+  if (p.slots > kMmMaxSlots) p.slots = kMmMaxSlots;
+  p.side = side;
+  const int rc = z[0].npa == 1 ? launch_jobs<1>(pl, map, p, n, full, sms, st) : launch_jobs<3>(pl, map, p, n, full, sms, st);
+  if (rc) return rc;
+  for (int j = 0; j < n; ++j) {
+    if (pl.splits[j] == 1) continue;
+    const MmaJob& q = jobs[j];
+    const bool wide = epilogue_vec(q.e) && q.N % 8 == 0;
+    const int64_t units = wide ? q.M * (q.N / 8) : q.M * q.N, need = (units + 255) / 256, cap = 16ll * sms;
+    const unsigned blocks = (unsigned)(need < cap ? need : cap);
+    if (wide) mma_join_kernel<8><<<blocks, 256, 0, st>>>(p.job[j].part, q.M, q.N, pl.splits[j], q.e);
+    else mma_join_kernel<1><<<blocks, 256, 0, st>>>(p.job[j].part, q.M, q.N, pl.splits[j], q.e);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return set_cuda_error(err);
+    count_launches(1);
+  }
   return GL_OK;
 }
 

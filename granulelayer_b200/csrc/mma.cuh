@@ -58,10 +58,20 @@ struct MmaOperand {
   int planes, mn;
 };
 
-// Scratch that mma_product needs (split sums), and the product itself.
-int64_t mma_work_bytes(int64_t M, int64_t N, int64_t K, int a_planes, int b_planes, int sms);
-int mma_product(const MmaOperand& a, const MmaOperand& b, int64_t M, int64_t N, int64_t K, const LinEpilogue& e,
-                const SumRows& side, void* work, cudaStream_t st);   // side.part NULL: nothing besides
+// One product, and up to two in one launch (the gradients of a layer's input and weight: their tiles share the
+// machine's waves, and a launch is saved).
+struct MmaJob {
+  MmaOperand a, b;
+  int64_t M, N, K;
+  LinEpilogue e;
+};
+struct MmaSize {
+  int64_t M, N, K;
+  int npa, npb, b_mn;   // planes of A and B, B MN-major
+};
+
+int64_t mma_work_bytes(const MmaSize* sizes, int n, int sms);   // scratch for split sums
+int mma_run(const MmaJob* jobs, int n, const SumRows& side, void* work, cudaStream_t st);   // side.part NULL: none
 
 // N elements of type T from p on: as 16-byte vectors where `vec`.
 template <typename T, int N>

@@ -540,8 +540,9 @@ typedef struct GlLinearBwdArgs {
 } GlLinearBwdArgs;
 int gl_linear_bwd(const GlLinearBwdArgs* args, void* stream);
 /* `flags`: of GL_LINEAR_*; UNALIGNED where x, or w, has a base or row stride that 16 bytes do not divide (needed for
- * bf16 only), CODES for a backward call on a checkpoint.  `work` itself is 256-byte aligned. */
-enum { GL_LINEAR_BACKWARD = 1, GL_LINEAR_CODES = 2, GL_LINEAR_UNALIGNED = 4 };
+ * bf16 only); for a backward call BACKWARD, with CODES on a checkpoint and DX, DW for the outputs that it has.  `work`
+ * itself is 256-byte aligned. */
+enum { GL_LINEAR_BACKWARD = 1, GL_LINEAR_CODES = 2, GL_LINEAR_UNALIGNED = 4, GL_LINEAR_DX = 8, GL_LINEAR_DW = 16 };
 int64_t gl_linear_work_bytes(int64_t M, int64_t N, int64_t K, int32_t dtype, int32_t flags);
 
 /* Group norm with an affine map and an activation, channels last: x [S, P, C] (sample stride sx, position
