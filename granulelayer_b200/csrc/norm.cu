@@ -6,18 +6,20 @@
 //   backward: du = dy act'(u), q = du gamma,
 //   dx = rstd (q - mean(q) - h mean(q h)), dgamma = sum du h, dbeta = sum du
 //
-// Bound by HBM: forward 2, backward 3 elements of traffic per element, when every input is read once.
-// Two families:
-//  * resident kernels: a cluster of R <= 8 CTAs owns one (sample, segment of whole groups); each CTA keeps its
-//    positions of the segment in shared memory, so the data comes from HBM once, and the group sums cross the
-//    cluster through distributed shared memory.  The variance is a second pass over the resident data
-//    (sum (x - mu)^2), not a difference of squares.
-//  * streaming kernels, for samples that do not fit a cluster's shared memory: per-channel partial statistics of
-//    chunks of positions (shifted by the chunk's first value, merged with Chan's formula), a join, and an
-//    elementwise pass; x is read twice.
-// A thread owns whole 16-byte vectors of channels and walks over positions, so all sums are first per channel:
-// group boundaries need no alignment, and with A_c = sum du h, B_c = sum du the backward's group means are
-// sum gamma_c A_c / m and sum gamma_c B_c / m.  No atomics: every sum has one order.
+// Bound by HBM where the data comes from there: forward 2, backward 3 elements of traffic per element if every input
+// is read once; arithmetic (about 16 and 40 instructions an element with an activation) is not far behind.
+// Three families:
+//  * row kernels (P = 1: tokens, each with its own statistics; groups that a warp can hold): L lanes keep a
+//    group in registers, reductions are shuffles, no barrier at all; several samples per warp are in flight.
+//  * resident kernels: a cluster of R <= 8 CTAs owns one (sample, segment of whole groups) in shared memory, so the
+//    data comes from HBM once; the group sums cross the cluster through distributed shared memory.
+//  * streaming kernels: chunks of positions give partial statistics (per channel shifted by the chunk's first value,
+//    merged with Chan's formula), and an elementwise pass merges those of its groups; x is read twice, the second
+//    time from L2 where it fits, and no block waits for another.
+// Variances are sums of squared deviations, never differences of squares.  Outside the row kernels a thread owns whole
+// 16-byte vectors of channels and walks over positions, so all sums are first per channel: group boundaries need no
+// alignment, and with A_c = sum du h, B_c = sum du the backward's group means are sum gamma_c A_c / m and
+// sum gamma_c B_c / m.  No atomics: every sum has one order.
 #include <cooperative_groups.h>
 
 #include "dense.cuh"
@@ -26,7 +28,6 @@ namespace cg = cooperative_groups;
 
 namespace gl {
 
-constexpr int kNormThreads = 256;
 constexpr int kNormMaxCluster = 8;
 
 struct NormParams {
@@ -37,14 +38,18 @@ struct NormParams {
   const int8_t* codes;
   const uint8_t* exps;
   void* out;            // y or dx (contiguous)
+  void* dw;             // streaming backward: joined beside the elementwise pass
+  void* db;
   float* mean;          // [S, G]
   float* rstd;
-  float* part;          // workspace
+  float* part;          // workspace: partial dgamma / dbeta rows [npart][2][C] (backward)
+  float* gpart;         // streaming: per (sample, chunk, group) statistics or sums [S][chunks][G][2]
   int64_t S, P, C, G, cpg, sx, px, sdy, pdy, ldc, nblk;
-  int64_t nseg, npart;  // resident: segments per sample; backward: rows of partial dgamma / dbeta
+  int64_t nseg, npart;  // segments per sample; rows of part
   int64_t PR;           // positions per CTA (resident) or chunk (streaming)
-  int64_t chunks;
-  int ng, cs, R, pdtype, act;   // act: chosen by the launch (a template argument of the kernels)
+  int64_t chunks, blocks;
+  int ng, cs, R, pdtype, accumulate;
+  int nsub, subc;       // streaming, groups too wide for a block: parts of a group, channels of a part (ng = 1)
   float eps;
 };
 
@@ -106,21 +111,80 @@ __device__ __forceinline__ Raw<T, N> read_dy(const NormParams& p, int64_t s, int
   return *reinterpret_cast<const Raw<T, N>*>(reinterpret_cast<const T*>(p.dy) + s * p.sdy + q * p.pdy + c);
 }
 
-// gs[g] = sum over the group's channels and the TY rows of red[row * cs + c], for the CTA's ngl groups: a warp
-// per group where there is enough to add, else a thread.
+// ---- what a CTA of the resident and streaming kernels works on ----
+// A segment of ngl whole groups, or a part of one (csl channels from c0 on, cpg to a group, nv vectors) of sample s,
+// positions q0 .. q0 + np - 1; thread (tx, ty) owns vector columns tx, tx + TX, .. and every TY-th position.
+template <int N, int NT>
+struct Slab {
+  int64_t s, c0, q0;
+  int g0, ngl, csl, cpg, nv, np, TX, TY, tx, ty, rows;
+  __device__ __forceinline__ Slab(const NormParams& p, int64_t s_, int64_t seg, int64_t part) {
+    s = s_;
+    if (p.nsub == 1) {
+      g0 = (int)seg * p.ng;
+      ngl = min(p.ng, (int)p.G - g0);
+      cpg = (int)p.cpg;
+      csl = ngl * cpg;
+      c0 = (int64_t)g0 * p.cpg;
+    } else {
+      g0 = (int)(seg / p.nsub);
+      const int64_t at = (seg - (int64_t)g0 * p.nsub) * p.subc;
+      ngl = 1;
+      cpg = csl = (int)min((int64_t)p.subc, p.cpg - at);
+      c0 = (int64_t)g0 * p.cpg + at;
+    }
+    nv = csl / N;
+    q0 = part * p.PR;
+    np = (int)max((int64_t)0, min(p.PR, p.P - q0));
+    TX = min(nv, NT);
+    TY = NT / TX;
+    tx = (int)threadIdx.x % TX;
+    ty = (int)threadIdx.x / TX;
+    rows = 32 % TX == 0 ? NT / 32 : TY;
+  }
+  __device__ __forceinline__ bool live() const { return ty < TY; }
+  // A column's sums to red[row csl + channel], one row per warp where a warp's lanes share columns, else per ty.
+  __device__ __forceinline__ void put(float (&acc)[N], float* red, int col) const {
+    if (32 % TX == 0) {
+      for (int o = TX; o < 32; o *= 2)
+#pragma unroll
+        for (int i = 0; i < N; ++i) acc[i] += __shfl_xor_sync(kFullMask, acc[i], o);
+      if ((int)(threadIdx.x & 31) < TX) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) red[(threadIdx.x >> 5) * csl + col * N + i] = acc[i];
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) red[ty * csl + col * N + i] = acc[i];
+    }
+  }
+};
+
+// Floats of one `red` array: rows * csl is at most NT * N, or cs where a segment is wider than a row of threads.
+__host__ __device__ inline int64_t norm_red(int64_t cs, int N, int NT) { return cs > (int64_t)NT * N ? cs : (int64_t)NT * N; }
+
+// gs[g] = sum over the group's channels and the rows of red[row * cs + c]: a warp per group where there is enough to
+// add, else a thread.
+template <int NT>
 __device__ __forceinline__ void group_sums(const float* red, int cs, int rows, int ngl, int cpg, float* gs) {
   const int tid = threadIdx.x, lane = tid & 31;
   if (cpg * rows >= 64) {
-    for (int g = tid >> 5; g < ngl; g += kNormThreads / 32) {
+    for (int g = tid >> 5; g < ngl; g += NT / 32) {
       float s = 0.f;
-      for (int r = 0; r < rows; ++r)
-        for (int c = lane; c < cpg; c += 32) s += red[r * cs + g * cpg + c];
+      if (cpg >= 32) {
+        for (int r = 0; r < rows; ++r)
+          for (int c = lane; c < cpg; c += 32) s += red[r * cs + g * cpg + c];
+      } else {
+        const int per = 32 / cpg, c = lane % cpg;            // rows at a time
+        if (lane < per * cpg)
+          for (int r = lane / cpg; r < rows; r += per) s += red[r * cs + g * cpg + c];
+      }
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(kFullMask, s, o);
       if (lane == 0) gs[g] = s;
     }
   } else {
-    for (int g = tid; g < ngl; g += kNormThreads) {
+    for (int g = tid; g < ngl; g += NT) {
       float s = 0.f;
       for (int r = 0; r < rows; ++r)
         for (int c = 0; c < cpg; ++c) s += red[r * cs + g * cpg + c];
@@ -143,66 +207,73 @@ __device__ __forceinline__ void norm_barrier(int R) {
   else cg::this_cluster().sync();
 }
 
+// A vector of channels' constants: (x - sub) mul = h, and gamma, beta.
+template <int N>
+struct ChanConst {
+  float mul[N], sub[N], gam[N], bet[N];
+  template <typename F>
+  __device__ __forceinline__ void load(const NormParams& p, int64_t c, F stat) {   // stat(i, mean, rstd)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      stat(i, sub[i], mul[i]);
+      gam[i] = ld_param(p.w, c + i, p.pdtype, 1.f);
+      bet[i] = ld_param(p.b, c + i, p.pdtype, 0.f);
+    }
+  }
+};
 
 // ---- resident forward ----
-template <typename T, int N, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_fwd_resident(NormParams p) {
+template <typename T, int N, int NT, int ACT>
+__global__ void __launch_bounds__(NT) norm_fwd_resident(NormParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   Raw<T, N>* tile = reinterpret_cast<Raw<T, N>*>(smem);
   const int tid = threadIdx.x, R = p.R, rank = blockIdx.x % R, cpg = (int)p.cpg;
   const int64_t item = blockIdx.x / R, s = item / p.nseg;
-  const int g0 = (int)(item - s * p.nseg) * p.ng;
-  const int ngl = min(p.ng, (int)p.G - g0), csl = ngl * cpg, nv = csl / N;
-  const int64_t c0 = (int64_t)g0 * cpg;
+  const Slab<N, NT> a(p, s, item - s * p.nseg, rank);
   float* red = reinterpret_cast<float*>(smem + (((size_t)p.PR * p.cs * sizeof(T) + 15) & ~(size_t)15));
-  float* gs = red + max(p.cs, kNormThreads * N);       // [2][ng]
+  float* gs = red + norm_red(p.cs, N, NT);             // [2][ng]
   float* stat = gs + 2 * p.ng;                         // [2][ng]: mean, rstd
-  const int TX = min(nv, kNormThreads), TY = kNormThreads / TX;
-  const int tx = tid % TX, ty = tid / TX;
-  const int64_t q0 = rank * p.PR;
-  const int np = (int)max((int64_t)0, min(p.PR, p.P - q0));
   const float inv_m = 1.f / ((float)p.P * (float)cpg);
 
-  if (ty < TY) {
-    for (int col = tx; col < nv; col += TX) {
+  if (a.live()) {
+    for (int col = a.tx; col < a.nv; col += a.TX) {
       float acc[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) acc[i] = 0.f;
-      const int64_t c = c0 + (int64_t)col * N;
-      int q = ty;
-      for (; q + 3 * TY < np; q += 4 * TY) {           // four loads in flight
+      const int64_t c = a.c0 + (int64_t)col * N;
+      int q = a.ty;
+      for (; q + 3 * a.TY < a.np; q += 4 * a.TY) {     // four loads in flight
         Raw<T, N> r[4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) r[k] = read_x<T, N, false>(p, s, q0 + q + k * TY, c);
+        for (int k = 0; k < 4; ++k) r[k] = read_x<T, N, false>(p, s, a.q0 + q + k * a.TY, c);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          tile[(q + k * TY) * nv + col] = r[k];
+          tile[(q + k * a.TY) * a.nv + col] = r[k];
           float f[N];
           unpack<T, N>(r[k], f);
 #pragma unroll
           for (int i = 0; i < N; ++i) acc[i] += f[i];
         }
       }
-      for (; q < np; q += TY) {
-        const Raw<T, N> r = read_x<T, N, false>(p, s, q0 + q, c);
-        tile[q * nv + col] = r;
+      for (; q < a.np; q += a.TY) {
+        const Raw<T, N> r = read_x<T, N, false>(p, s, a.q0 + q, c);
+        tile[q * a.nv + col] = r;
         float f[N];
         unpack<T, N>(r, f);
 #pragma unroll
         for (int i = 0; i < N; ++i) acc[i] += f[i];
       }
-#pragma unroll
-      for (int i = 0; i < N; ++i) red[ty * csl + col * N + i] = acc[i];
+      a.put(acc, red, col);
     }
   }
   __syncthreads();
-  group_sums(red, csl, TY, ngl, cpg, gs);
+  group_sums<NT>(red, a.csl, a.rows, a.ngl, cpg, gs);
   norm_barrier(R);
-  for (int g = tid; g < ngl; g += kNormThreads) stat[g] = cluster_total(gs, g, R) * inv_m;
+  for (int g = tid; g < a.ngl; g += NT) stat[g] = cluster_total(gs, g, R) * inv_m;
   __syncthreads();
 
-  if (ty < TY) {
-    for (int col = tx; col < nv; col += TX) {
+  if (a.live()) {
+    for (int col = a.tx; col < a.nv; col += a.TX) {
       float acc[N], mu[N];
 #pragma unroll
       for (int i = 0; i < N; ++i) {
@@ -210,454 +281,398 @@ __global__ void __launch_bounds__(kNormThreads) norm_fwd_resident(NormParams p) 
         mu[i] = stat[(col * N + i) / cpg];
       }
 #pragma unroll 4
-      for (int q = ty; q < np; q += TY) {
+      for (int q = a.ty; q < a.np; q += a.TY) {
         float f[N];
-        unpack<T, N>(tile[q * nv + col], f);
+        unpack<T, N>(tile[q * a.nv + col], f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) acc[i] += (f[i] - mu[i]) * (f[i] - mu[i]);
+        for (int i = 0; i < N; ++i) acc[i] = fmaf(f[i] - mu[i], f[i] - mu[i], acc[i]);
       }
-#pragma unroll
-      for (int i = 0; i < N; ++i) red[ty * csl + col * N + i] = acc[i];
+      a.put(acc, red, col);
     }
   }
   __syncthreads();
-  group_sums(red, csl, TY, ngl, cpg, gs + p.ng);
+  group_sums<NT>(red, a.csl, a.rows, a.ngl, cpg, gs + p.ng);
   norm_barrier(R);
-  for (int g = tid; g < ngl; g += kNormThreads) {
+  for (int g = tid; g < a.ngl; g += NT) {
     const float rs = 1.f / sqrtf(cluster_total(gs + p.ng, g, R) * inv_m + p.eps);
     stat[p.ng + g] = rs;
     if (rank == 0) {
-      p.mean[s * p.G + g0 + g] = stat[g];
-      p.rstd[s * p.G + g0 + g] = rs;
+      p.mean[s * p.G + a.g0 + g] = stat[g];
+      p.rstd[s * p.G + a.g0 + g] = rs;
     }
   }
   norm_barrier(R);                                     // peers are done with this CTA's gs; stat is visible
 
-  if (ty < TY) {
+  if (a.live()) {
     T* out = reinterpret_cast<T*>(p.out);
-    for (int col = tx; col < nv; col += TX) {
-      float mul[N], sub[N], bet[N];
+    for (int col = a.tx; col < a.nv; col += a.TX) {
+      ChanConst<N> k;
+      const int64_t c = a.c0 + (int64_t)col * N;
+      k.load(p, c, [&](int i, float& mean, float& rstd) {
+        const int g = (col * N + i) / cpg;
+        mean = stat[g];
+        rstd = stat[p.ng + g];
+      });
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const int cl = col * N + i, g = cl / cpg;
-        mul[i] = stat[p.ng + g] * ld_param(p.w, c0 + cl, p.pdtype, 1.f);
-        sub[i] = stat[g];
-        bet[i] = ld_param(p.b, c0 + cl, p.pdtype, 0.f);
-      }
+      for (int i = 0; i < N; ++i) k.mul[i] *= k.gam[i];
 #pragma unroll 2
-      for (int q = ty; q < np; q += TY) {
+      for (int q = a.ty; q < a.np; q += a.TY) {
         float f[N];
-        unpack<T, N>(tile[q * nv + col], f);
+        unpack<T, N>(tile[q * a.nv + col], f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = dense_act<ACT, sizeof(T) == 2>(fmaf(f[i] - sub[i], mul[i], bet[i]));
-        store_vec<T, N>(out + (s * p.P + q0 + q) * p.C + c0 + (int64_t)col * N, f);
+        for (int i = 0; i < N; ++i) f[i] = dense_act<ACT, sizeof(T) == 2>(fmaf(f[i] - k.sub[i], k.mul[i], k.bet[i]));
+        store_vec<T, N>(out + (s * p.P + a.q0 + q) * p.C + c, f);
       }
     }
   }
 }
 
-// ---- backward, resident ----
+// ---- resident backward ----
 // A cluster keeps one segment and walks over samples, adding its dgamma / dbeta in shared memory; one partial
 // row per CTA goes to the join.
-template <typename T, int N, int ACT, bool CKPT>
-__global__ void __launch_bounds__(kNormThreads) norm_bwd_resident(NormParams p) {
+template <typename T, int N, int NT, int ACT, bool CKPT>
+__global__ void __launch_bounds__(NT) norm_bwd_resident(NormParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   const size_t tbytes = ((size_t)p.PR * p.cs * sizeof(T) + 15) & ~(size_t)15;
   Raw<T, N>* xt = reinterpret_cast<Raw<T, N>*>(smem);
   Raw<T, N>* dt = reinterpret_cast<Raw<T, N>*>(smem + tbytes);
   const int tid = threadIdx.x, R = p.R, rank = blockIdx.x % R, cpg = (int)p.cpg;
   const int64_t cluster = blockIdx.x / R, walkers = (gridDim.x / R) / p.nseg, walker = cluster / p.nseg;
-  const int g0 = (int)(cluster - walker * p.nseg) * p.ng;
-  const int ngl = min(p.ng, (int)p.G - g0), csl = ngl * cpg, nv = csl / N;
-  const int64_t c0 = (int64_t)g0 * cpg;
-  const int rf = max(p.cs, kNormThreads * N);
+  const int64_t rf = norm_red(p.cs, N, NT);
   float* ra = reinterpret_cast<float*>(smem + 2 * tbytes);   // sum du h per channel
   float* rb = ra + rf;                                       // sum du per channel
   float* da = rb + rf;                                       // dgamma, dbeta of this CTA
   float* db = da + p.cs;
   float* gs = db + p.cs;                                     // [2 parities][2][ng]
   float* stat = gs + 4 * p.ng;                               // [2][ng]: mean(q), mean(q h)
-  const int TX = min(nv, kNormThreads), TY = kNormThreads / TX;
-  const int tx = tid % TX, ty = tid / TX;
-  const int64_t q0 = rank * p.PR;
-  const int np = (int)max((int64_t)0, min(p.PR, p.P - q0));
   const float inv_m = 1.f / ((float)p.P * (float)cpg);
-  for (int c = tid; c < csl; c += kNormThreads) da[c] = db[c] = 0.f;
+  const Slab<N, NT> a(p, walker, cluster - walker * p.nseg, rank);
+  for (int c = tid; c < a.csl; c += NT) da[c] = db[c] = 0.f;
   int par = 0;
   for (int64_t s = walker; s < p.S; s += walkers, par ^= 1) {
     float* gsp = gs + par * 2 * p.ng;
-    if (ty < TY) {
-      for (int col = tx; col < nv; col += TX) {
-        float aa[N], ab[N], mul[N], sub[N], gam[N], bet[N];
-        const int64_t c = c0 + (int64_t)col * N;
+    if (a.live()) {
+      for (int col = a.tx; col < a.nv; col += a.TX) {
+        float aa[N], ab[N];
+        ChanConst<N> k;
+        const int64_t c = a.c0 + (int64_t)col * N;
+        k.load(p, c, [&](int i, float& mean, float& rstd) {
+          const int64_t g = s * p.G + a.g0 + (col * N + i) / cpg;
+          mean = p.mean[g];
+          rstd = p.rstd[g];
+        });
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int64_t g = s * p.G + g0 + (col * N + i) / cpg;
-          aa[i] = ab[i] = 0.f;
-          mul[i] = p.rstd[g];
-          sub[i] = p.mean[g];
-          gam[i] = ld_param(p.w, c + i, p.pdtype, 1.f);
-          bet[i] = ld_param(p.b, c + i, p.pdtype, 0.f);
-        }
-        for (int q = ty; q < np; q += 2 * TY) {
+        for (int i = 0; i < N; ++i) aa[i] = ab[i] = 0.f;
+        for (int q = a.ty; q < a.np; q += 2 * a.TY) {
           Raw<T, N> rx[2], rd[2];
-          const bool two = q + TY < np;
-          rx[0] = read_x<T, N, CKPT>(p, s, q0 + q, c);
-          rd[0] = read_dy<T, N>(p, s, q0 + q, c);
+          const bool two = q + a.TY < a.np;
+          rx[0] = read_x<T, N, CKPT>(p, s, a.q0 + q, c);
+          rd[0] = read_dy<T, N>(p, s, a.q0 + q, c);
           if (two) {
-            rx[1] = read_x<T, N, CKPT>(p, s, q0 + q + TY, c);
-            rd[1] = read_dy<T, N>(p, s, q0 + q + TY, c);
+            rx[1] = read_x<T, N, CKPT>(p, s, a.q0 + q + a.TY, c);
+            rd[1] = read_dy<T, N>(p, s, a.q0 + q + a.TY, c);
           }
 #pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            if (k == 1 && !two) break;
-            xt[(q + k * TY) * nv + col] = rx[k];
-            dt[(q + k * TY) * nv + col] = rd[k];
+          for (int j = 0; j < 2; ++j) {
+            if (j == 1 && !two) break;
+            xt[(q + j * a.TY) * a.nv + col] = rx[j];
+            dt[(q + j * a.TY) * a.nv + col] = rd[j];
             float f[N], d[N];
-            unpack<T, N>(rx[k], f);
-            unpack<T, N>(rd[k], d);
+            unpack<T, N>(rx[j], f);
+            unpack<T, N>(rd[j], d);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-              const float h = (f[i] - sub[i]) * mul[i];
-              const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, gam[i], bet[i]));
+              const float h = (f[i] - k.sub[i]) * k.mul[i];
+              const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, k.gam[i], k.bet[i]));
               aa[i] = fmaf(du, h, aa[i]);
               ab[i] += du;
             }
           }
         }
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          ra[ty * csl + col * N + i] = aa[i];
-          rb[ty * csl + col * N + i] = ab[i];
-        }
+        a.put(aa, ra, col);
+        a.put(ab, rb, col);
       }
     }
     __syncthreads();
-    for (int c = tid; c < csl; c += kNormThreads) {
-      float a = 0.f, b = 0.f;
-      for (int r = 0; r < TY; ++r) {
-        a += ra[r * csl + c];
-        b += rb[r * csl + c];
+    for (int c = tid; c < a.csl; c += NT) {
+      float va = 0.f, vb = 0.f;
+      for (int r = 0; r < a.rows; ++r) {
+        va += ra[r * a.csl + c];
+        vb += rb[r * a.csl + c];
       }
-      da[c] += a;
-      db[c] += b;
-      const float gam = ld_param(p.w, c0 + c, p.pdtype, 1.f);
-      ra[c] = a * gam;
-      rb[c] = b * gam;
+      da[c] += va;
+      db[c] += vb;
+      const float gam = ld_param(p.w, a.c0 + c, p.pdtype, 1.f);
+      ra[c] = va * gam;
+      rb[c] = vb * gam;
     }
     __syncthreads();
-    group_sums(rb, csl, 1, ngl, cpg, gsp);
-    group_sums(ra, csl, 1, ngl, cpg, gsp + p.ng);
+    group_sums<NT>(rb, a.csl, 1, a.ngl, cpg, gsp);
+    group_sums<NT>(ra, a.csl, 1, a.ngl, cpg, gsp + p.ng);
     norm_barrier(R);
-    for (int g = tid; g < 2 * ngl; g += kNormThreads) {
-      const int k = g / ngl, gg = g - k * ngl;
-      stat[k * p.ng + gg] = cluster_total(gsp + k * p.ng, gg, R) * inv_m;
+    for (int g = tid; g < 2 * a.ngl; g += NT) {
+      const int j = g / a.ngl, gg = g - j * a.ngl;
+      stat[j * p.ng + gg] = cluster_total(gsp + j * p.ng, gg, R) * inv_m;
     }
     __syncthreads();
-    if (ty < TY) {
+    if (a.live()) {
       T* out = reinterpret_cast<T*>(p.out);
-      for (int col = tx; col < nv; col += TX) {
-        float mul[N], sub[N], gam[N], bet[N], m1[N], m2[N];
-        const int64_t c = c0 + (int64_t)col * N;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const int gl_ = (col * N + i) / cpg;
-          const int64_t g = s * p.G + g0 + gl_;
-          mul[i] = p.rstd[g];
-          sub[i] = p.mean[g];
-          gam[i] = ld_param(p.w, c + i, p.pdtype, 1.f);
-          bet[i] = ld_param(p.b, c + i, p.pdtype, 0.f);
-          m1[i] = stat[gl_];
-          m2[i] = stat[p.ng + gl_];
-        }
-        for (int q = ty; q < np; q += TY) {
+      for (int col = a.tx; col < a.nv; col += a.TX) {
+        float m1[N], m2[N];
+        ChanConst<N> k;
+        const int64_t c = a.c0 + (int64_t)col * N;
+        k.load(p, c, [&](int i, float& mean, float& rstd) {
+          const int g = (col * N + i) / cpg;
+          mean = p.mean[s * p.G + a.g0 + g];
+          rstd = p.rstd[s * p.G + a.g0 + g];
+          m1[i] = stat[g];
+          m2[i] = stat[p.ng + g];
+        });
+#pragma unroll 2
+        for (int q = a.ty; q < a.np; q += a.TY) {
           float f[N], d[N];
-          unpack<T, N>(xt[q * nv + col], f);
-          unpack<T, N>(dt[q * nv + col], d);
+          unpack<T, N>(xt[q * a.nv + col], f);
+          unpack<T, N>(dt[q * a.nv + col], d);
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            const float h = (f[i] - sub[i]) * mul[i];
-            const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, gam[i], bet[i]));
-            f[i] = mul[i] * (fmaf(du, gam[i], -m1[i]) - h * m2[i]);
+            const float h = (f[i] - k.sub[i]) * k.mul[i];
+            const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, k.gam[i], k.bet[i]));
+            f[i] = k.mul[i] * (fmaf(du, k.gam[i], -m1[i]) - h * m2[i]);
           }
-          store_vec<T, N>(out + (s * p.P + q0 + q) * p.C + c, f);
+          store_vec<T, N>(out + (s * p.P + a.q0 + q) * p.C + c, f);
         }
       }
     }
     __syncthreads();                                   // ra / rb / stat / tiles free; gs alternates by parity
   }
-  float* row = p.part + ((walker * R + rank) * 2) * p.C + c0;
-  for (int c = tid; c < csl; c += kNormThreads) {
+  float* row = p.part + ((walker * R + rank) * 2) * p.C + a.c0;
+  for (int c = tid; c < a.csl; c += NT) {
     row[c] = da[c];
     row[p.C + c] = db[c];
   }
   norm_barrier(R);                                     // no CTA leaves while a peer may still read its gs
 }
 
-// ---- streaming kernels ----
-// Thread mapping of a chunk: blockDim 256 = TX vectors x TY positions; channel segments of 256 vectors.
-struct ChunkAt {
-  int64_t s, q0, c;
-  int np, TY, ty, tx, TX;
-  bool live;
-};
-
-template <int N>
-__device__ __forceinline__ ChunkAt chunk_at(const NormParams& p) {
-  ChunkAt a;
-  const int64_t nv = p.C / N, segs = (nv + kNormThreads - 1) / kNormThreads;
-  const int64_t seg = blockIdx.x % segs, sc = blockIdx.x / segs;
-  a.s = sc / p.chunks;
-  a.q0 = (sc - a.s * p.chunks) * p.PR;
-  a.np = (int)min(p.PR, p.P - a.q0);
-  const int64_t left = nv - seg * kNormThreads;
-  a.TX = (int)min((int64_t)kNormThreads, left);
-  a.TY = kNormThreads / a.TX;
-  a.tx = threadIdx.x % a.TX;
-  a.ty = threadIdx.x / a.TX;
-  a.c = (seg * kNormThreads + a.tx) * N;
-  a.live = a.ty < a.TY;
-  return a;
+// ---- streaming kernels: a block per (sample, chunk of positions, segment) ----
+template <int N, int NT>
+__device__ __forceinline__ Slab<N, NT> chunk_slab(const NormParams& p) {
+  const int64_t seg = blockIdx.x % p.nseg, sc = blockIdx.x / p.nseg, s = sc / p.chunks;
+  return Slab<N, NT>(p, s, seg, sc - s * p.chunks);
 }
 
-// part[(s chunks + chunk) C + c] = (mean, sum of squared deviations) of the chunk's values of channel c.
-template <typename T, int N>
-__global__ void __launch_bounds__(kNormThreads) norm_stats_kernel(NormParams p) {
-  __shared__ float r1[kNormThreads * N], r2[kNormThreads * N];
-  const ChunkAt a = chunk_at<N>(p);
-  float k0[N], s1[N], s2[N];
-  if (a.live) {
-    unpack<T, N>(read_x<T, N, false>(p, a.s, a.q0, a.c), k0);
+// This block's first entry in a chunk's row of gpart, and the number of elements behind entry (chunk, part).
+__device__ __forceinline__ int64_t entry0(const NormParams& p, int g0) {
+  return p.nsub == 1 ? g0 : (int64_t)(blockIdx.x % p.nseg);
+}
+__device__ __forceinline__ float entry_count(const NormParams& p, int64_t ch, int64_t part) {
+  const int64_t c = p.nsub == 1 ? p.cpg : min((int64_t)p.subc, p.cpg - part * p.subc);
+  return (float)min(p.PR, p.P - ch * p.PR) * (float)c;
+}
+
+// gpart[((s chunks + chunk) G + g) nsub + part] = (mean, sum of squared deviations) of the chunk's values of the group,
+// or of its part.
+template <typename T, int N, int NT>
+__global__ void __launch_bounds__(NT) norm_stats_kernel(NormParams p) {
+  extern __shared__ float sf[];
+  const Slab<N, NT> a = chunk_slab<N, NT>(p);
+  const int64_t rf = norm_red(p.cs, N, NT);
+  float* r1 = sf;
+  float* r2 = sf + rf;
+  float* gm = r2 + rf;                                  // [ng]
+  float* gv = gm + p.ng;
+  const int cpg = a.cpg;
+  const float n = (float)a.np;
+  if (a.live()) {
+    for (int col = a.tx; col < a.nv; col += a.TX) {
+      float k0[N], s1[N], s2[N];
+      const int64_t c = a.c0 + (int64_t)col * N;
+      unpack<T, N>(read_x<T, N, false>(p, a.s, a.q0, c), k0);
 #pragma unroll
-    for (int i = 0; i < N; ++i) s1[i] = s2[i] = 0.f;
+      for (int i = 0; i < N; ++i) s1[i] = s2[i] = 0.f;
+#pragma unroll 8
+      for (int q = a.ty; q < a.np; q += a.TY) {
+        float f[N];
+        unpack<T, N>(read_x<T, N, false>(p, a.s, a.q0 + q, c), f);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const float d = f[i] - k0[i];
+          s1[i] += d;
+          s2[i] = fmaf(d, d, s2[i]);
+        }
+      }
+      a.put(s1, r1, col);
+      a.put(s2, r2, col);
+    }
+  }
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.csl; c += NT) {       // channel c: mean and squared deviations
+    float t1 = 0.f, t2 = 0.f;
+    for (int r = 0; r < a.rows; ++r) {
+      t1 += r1[r * a.csl + c];
+      t2 += r2[r * a.csl + c];
+    }
+    const float dm = t1 / n;
+    const float k0 = to_f32<T>(reinterpret_cast<const T*>(p.x)[a.s * p.sx + a.q0 * p.px + a.c0 + c]);
+    r1[c] = k0 + dm;
+    r2[c] = fmaxf(t2 - dm * t1, 0.f);
+  }
+  __syncthreads();
+  group_sums<NT>(r1, a.csl, 1, a.ngl, cpg, gm);
+  __syncthreads();
+  for (int c = threadIdx.x; c < a.csl; c += NT) {       // Chan: n (mean_c - mean_g)^2 joins the deviations
+    const float d = r1[c] - gm[c / cpg] / (float)cpg;
+    r2[c] = fmaf(n * d, d, r2[c]);
+  }
+  __syncthreads();
+  group_sums<NT>(r2, a.csl, 1, a.ngl, cpg, gv);
+  __syncthreads();
+  float2* out = reinterpret_cast<float2*>(p.gpart) + (a.s * p.chunks + a.q0 / p.PR) * p.G * p.nsub + entry0(p, a.g0);
+  for (int g = threadIdx.x; g < a.ngl; g += NT) out[g] = make_float2(gm[g] / (float)cpg, gv[g]);
+}
+
+// The groups' statistics from the chunks' (every block the same sums), then act(h gamma + beta).
+template <typename T, int N, int NT, int ACT>
+__global__ void __launch_bounds__(NT) norm_apply_kernel(NormParams p) {
+  extern __shared__ float sf[];
+  const Slab<N, NT> a = chunk_slab<N, NT>(p);
+  const int cpg = a.cpg, lane = threadIdx.x & 31;
+  float* mean = sf;                                     // [ng]
+  float* rstd = sf + p.ng;
+  const float2* part = reinterpret_cast<const float2*>(p.gpart) + (a.s * p.chunks * p.G + a.g0) * p.nsub;
+  const float m = (float)p.P * (float)p.cpg;
+  for (int g = threadIdx.x >> 5; g < a.ngl; g += NT / 32) {
+    float v = 0.f;
+    for (int64_t j = lane; j < p.chunks * p.nsub; j += 32) {
+      const int64_t ch = j / p.nsub;
+      v = fmaf(part[(ch * p.G + g) * p.nsub + (j - ch * p.nsub)].x, entry_count(p, ch, j - ch * p.nsub), v);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+    const float mu = v / m;
+    v = 0.f;
+    for (int64_t j = lane; j < p.chunks * p.nsub; j += 32) {
+      const int64_t ch = j / p.nsub;
+      const float2 t = part[(ch * p.G + g) * p.nsub + (j - ch * p.nsub)];
+      v += fmaf((t.x - mu) * (t.x - mu), entry_count(p, ch, j - ch * p.nsub), t.y);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+    if (lane == 0) {
+      const float rs = 1.f / sqrtf(v / m + p.eps);
+      mean[g] = mu;
+      rstd[g] = rs;
+      if (a.q0 == 0 && a.c0 == a.g0 * p.cpg) {       // the group's first block
+        p.mean[a.s * p.G + a.g0 + g] = mu;
+        p.rstd[a.s * p.G + a.g0 + g] = rs;
+      }
+    }
+  }
+  __syncthreads();
+  if (!a.live()) return;
+  T* out = reinterpret_cast<T*>(p.out);
+  for (int col = a.tx; col < a.nv; col += a.TX) {
+    ChanConst<N> k;
+    const int64_t c = a.c0 + (int64_t)col * N;
+    k.load(p, c, [&](int i, float& m, float& r) {
+      const int g = (col * N + i) / cpg;
+      m = mean[g];
+      r = rstd[g];
+    });
+#pragma unroll
+    for (int i = 0; i < N; ++i) k.mul[i] *= k.gam[i];
 #pragma unroll 4
     for (int q = a.ty; q < a.np; q += a.TY) {
       float f[N];
-      unpack<T, N>(read_x<T, N, false>(p, a.s, a.q0 + q, a.c), f);
+      unpack<T, N>(read_x<T, N, false>(p, a.s, a.q0 + q, c), f);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float d = f[i] - k0[i];
-        s1[i] += d;
-        s2[i] = fmaf(d, d, s2[i]);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      r1[(a.ty * a.TX + a.tx) * N + i] = s1[i];
-      r2[(a.ty * a.TX + a.tx) * N + i] = s2[i];
-    }
-  }
-  __syncthreads();
-  if (a.live && a.ty == 0) {
-    float2* out = reinterpret_cast<float2*>(p.part) + (a.s * p.chunks + a.q0 / p.PR) * p.C + a.c;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float t1 = 0.f, t2 = 0.f;
-      for (int r = 0; r < a.TY; ++r) {
-        t1 += r1[(r * a.TX + a.tx) * N + i];
-        t2 += r2[(r * a.TX + a.tx) * N + i];
-      }
-      const float dm = t1 / (float)a.np;
-      out[i] = make_float2(k0[i] + dm, fmaxf(t2 - dm * t1, 0.f));
+      for (int i = 0; i < N; ++i) f[i] = dense_act<ACT, sizeof(T) == 2>(fmaf(f[i] - k.sub[i], k.mul[i], k.bet[i]));
+      store_vec<T, N>(out + (a.s * p.P + a.q0 + q) * p.C + c, f);
     }
   }
 }
 
-// mean and rstd of each (sample, group) from the chunks' channel statistics (one block each).
-__global__ void __launch_bounds__(kNormThreads) norm_stats_join_kernel(NormParams p) {
-  __shared__ float red[kNormThreads / 32 + 1];
-  const int64_t s = blockIdx.x / p.G, g = blockIdx.x % p.G, n = p.chunks * p.cpg;
-  const float2* part = reinterpret_cast<const float2*>(p.part) + s * p.chunks * p.C + g * p.cpg;
-  const float m = (float)p.P * (float)p.cpg;
-  auto total = [&](float v) {
-    __syncthreads();
+// Per chunk: dgamma and dbeta partial rows, and each group's sums of q and q h in gpart.
+template <typename T, int N, int NT, int ACT, bool CKPT>
+__global__ void __launch_bounds__(NT) norm_bwd_stats_kernel(NormParams p) {
+  extern __shared__ float sf[];
+  const Slab<N, NT> a = chunk_slab<N, NT>(p);
+  const int64_t rf = norm_red(p.cs, N, NT);
+  float* ra = sf;
+  float* rb = sf + rf;
+  float* ga = rb + rf;
+  float* gb = ga + p.ng;
+  const int cpg = a.cpg;
+  if (a.live()) {
+    for (int col = a.tx; col < a.nv; col += a.TX) {
+      float aa[N], ab[N];
+      ChanConst<N> k;
+      const int64_t c = a.c0 + (int64_t)col * N;
+      k.load(p, c, [&](int i, float& mean, float& rstd) {
+        const int64_t g = a.s * p.G + a.g0 + (col * N + i) / cpg;
+        mean = p.mean[g];
+        rstd = p.rstd[g];
+      });
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
-    __syncthreads();
-    float t = 0.f;
-    for (int i = 0; i < kNormThreads / 32; ++i) t += red[i];
-    return t;
-  };
-  float v = 0.f;
-  for (int64_t i = threadIdx.x; i < n; i += kNormThreads) {
-    const int64_t ch = i / p.cpg;
-    v += part[ch * p.C + (i - ch * p.cpg)].x * (float)min(p.PR, p.P - ch * p.PR);
-  }
-  const float mu = total(v) / m;
-  v = 0.f;
-  for (int64_t i = threadIdx.x; i < n; i += kNormThreads) {
-    const int64_t ch = i / p.cpg;
-    const float2 t = part[ch * p.C + (i - ch * p.cpg)];
-    v += t.y + (t.x - mu) * (t.x - mu) * (float)min(p.PR, p.P - ch * p.PR);
-  }
-  const float var = total(v) / m;
-  if (threadIdx.x == 0) {
-    p.mean[blockIdx.x] = mu;
-    p.rstd[blockIdx.x] = 1.f / sqrtf(var + p.eps);
-  }
-}
-
-template <typename T, int N, int ACT>
-__global__ void __launch_bounds__(kNormThreads) norm_apply_kernel(NormParams p) {
-  const ChunkAt a = chunk_at<N>(p);
-  if (!a.live) return;
-  float mul[N], sub[N], bet[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int64_t g = a.s * p.G + (a.c + i) / p.cpg;
-    mul[i] = p.rstd[g] * ld_param(p.w, a.c + i, p.pdtype, 1.f);
-    sub[i] = p.mean[g];
-    bet[i] = ld_param(p.b, a.c + i, p.pdtype, 0.f);
-  }
-  T* out = reinterpret_cast<T*>(p.out);
-#pragma unroll 4
-  for (int q = a.ty; q < a.np; q += a.TY) {
-    float f[N];
-    unpack<T, N>(read_x<T, N, false>(p, a.s, a.q0 + q, a.c), f);
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = dense_act<ACT, sizeof(T) == 2>(fmaf(f[i] - sub[i], mul[i], bet[i]));
-    store_vec<T, N>(out + (a.s * p.P + a.q0 + q) * p.C + a.c, f);
-  }
-}
-
-// Per chunk and channel: dgamma and dbeta partials, part[((s chunks + chunk) 2 + {0, 1}) C + c].
-template <typename T, int N, int ACT, bool CKPT>
-__global__ void __launch_bounds__(kNormThreads) norm_bwd_stats_kernel(NormParams p) {
-  __shared__ float r1[kNormThreads * N], r2[kNormThreads * N];
-  const ChunkAt a = chunk_at<N>(p);
-  if (a.live) {
-    float s1[N], s2[N], mul[N], sub[N], gam[N], bet[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const int64_t g = a.s * p.G + (a.c + i) / p.cpg;
-      s1[i] = s2[i] = 0.f;
-      mul[i] = p.rstd[g];
-      sub[i] = p.mean[g];
-      gam[i] = ld_param(p.w, a.c + i, p.pdtype, 1.f);
-      bet[i] = ld_param(p.b, a.c + i, p.pdtype, 0.f);
-    }
+      for (int i = 0; i < N; ++i) aa[i] = ab[i] = 0.f;
 #pragma unroll 2
-    for (int q = a.ty; q < a.np; q += a.TY) {
-      float f[N], d[N];
-      unpack<T, N>(read_x<T, N, CKPT>(p, a.s, a.q0 + q, a.c), f);
-      unpack<T, N>(read_dy<T, N>(p, a.s, a.q0 + q, a.c), d);
+      for (int q = a.ty; q < a.np; q += a.TY) {
+        float f[N], d[N];
+        unpack<T, N>(read_x<T, N, CKPT>(p, a.s, a.q0 + q, c), f);
+        unpack<T, N>(read_dy<T, N>(p, a.s, a.q0 + q, c), d);
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        const float h = (f[i] - sub[i]) * mul[i];
-        const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, gam[i], bet[i]));
-        s1[i] = fmaf(du, h, s1[i]);
-        s2[i] += du;
+        for (int i = 0; i < N; ++i) {
+          const float h = (f[i] - k.sub[i]) * k.mul[i];
+          const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, k.gam[i], k.bet[i]));
+          aa[i] = fmaf(du, h, aa[i]);
+          ab[i] += du;
+        }
       }
-    }
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      r1[(a.ty * a.TX + a.tx) * N + i] = s1[i];
-      r2[(a.ty * a.TX + a.tx) * N + i] = s2[i];
+      a.put(aa, ra, col);
+      a.put(ab, rb, col);
     }
   }
   __syncthreads();
-  if (a.live && a.ty == 0) {
-    float* out = p.part + (a.s * p.chunks + a.q0 / p.PR) * 2 * p.C + a.c;
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float t1 = 0.f, t2 = 0.f;
-      for (int r = 0; r < a.TY; ++r) {
-        t1 += r1[(r * a.TX + a.tx) * N + i];
-        t2 += r2[(r * a.TX + a.tx) * N + i];
-      }
-      out[i] = t1;
-      out[p.C + i] = t2;
+  const int64_t chunk = a.s * p.chunks + a.q0 / p.PR;
+  float* row = p.part + chunk * 2 * p.C + a.c0;
+  for (int c = threadIdx.x; c < a.csl; c += NT) {
+    float va = 0.f, vb = 0.f;
+    for (int r = 0; r < a.rows; ++r) {
+      va += ra[r * a.csl + c];
+      vb += rb[r * a.csl + c];
     }
-  }
-}
-
-// coef[(s G + g) 2] = mean(q), mean(q h) of each (sample, group); coef follows the partials.
-__global__ void __launch_bounds__(kNormThreads) norm_bwd_join_kernel(NormParams p, float* coef) {
-  __shared__ float red[2 * (kNormThreads / 32)];
-  const int64_t s = blockIdx.x / p.G, g = blockIdx.x % p.G, n = p.chunks * p.cpg;
-  const float m = (float)p.P * (float)p.cpg;
-  float va = 0.f, vb = 0.f;
-  for (int64_t i = threadIdx.x; i < n; i += kNormThreads) {
-    const int64_t ch = i / p.cpg, c = g * p.cpg + (i - ch * p.cpg);
-    const float* row = p.part + (s * p.chunks + ch) * 2 * p.C + c;
-    const float gam = ld_param(p.w, c, p.pdtype, 1.f);
-    va = fmaf(row[0], gam, va);
-    vb = fmaf(row[p.C], gam, vb);
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    va += __shfl_xor_sync(kFullMask, va, o);
-    vb += __shfl_xor_sync(kFullMask, vb, o);
-  }
-  if ((threadIdx.x & 31) == 0) {
-    red[threadIdx.x >> 5] = va;
-    red[kNormThreads / 32 + (threadIdx.x >> 5)] = vb;
+    row[c] = va;
+    row[p.C + c] = vb;
+    const float gam = ld_param(p.w, a.c0 + c, p.pdtype, 1.f);
+    ra[c] = va * gam;
+    rb[c] = vb * gam;
   }
   __syncthreads();
-  if (threadIdx.x == 0) {
-    va = vb = 0.f;
-    for (int i = 0; i < kNormThreads / 32; ++i) {
-      va += red[i];
-      vb += red[kNormThreads / 32 + i];
-    }
-    coef[blockIdx.x * 2] = vb / m;
-    coef[blockIdx.x * 2 + 1] = va / m;
-  }
+  group_sums<NT>(ra, a.csl, 1, a.ngl, cpg, ga);
+  group_sums<NT>(rb, a.csl, 1, a.ngl, cpg, gb);
+  __syncthreads();
+  float2* out = reinterpret_cast<float2*>(p.gpart) + chunk * p.G * p.nsub + entry0(p, a.g0);
+  for (int g = threadIdx.x; g < a.ngl; g += NT) out[g] = make_float2(gb[g], ga[g]);
 }
 
-template <typename T, int N, int ACT, bool CKPT>
-__global__ void __launch_bounds__(kNormThreads) norm_bwd_apply_kernel(NormParams p, const float* coef) {
-  const ChunkAt a = chunk_at<N>(p);
-  if (!a.live) return;
-  float mul[N], sub[N], gam[N], bet[N], m1[N], m2[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int64_t g = a.s * p.G + (a.c + i) / p.cpg;
-    mul[i] = p.rstd[g];
-    sub[i] = p.mean[g];
-    m1[i] = coef[2 * g];
-    m2[i] = coef[2 * g + 1];
-    gam[i] = ld_param(p.w, a.c + i, p.pdtype, 1.f);
-    bet[i] = ld_param(p.b, a.c + i, p.pdtype, 0.f);
-  }
-  T* out = reinterpret_cast<T*>(p.out);
-#pragma unroll 2
-  for (int q = a.ty; q < a.np; q += a.TY) {
-    float f[N], d[N];
-    unpack<T, N>(read_x<T, N, CKPT>(p, a.s, a.q0 + q, a.c), f);
-    unpack<T, N>(read_dy<T, N>(p, a.s, a.q0 + q, a.c), d);
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float h = (f[i] - sub[i]) * mul[i];
-      const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, gam[i], bet[i]));
-      f[i] = mul[i] * (fmaf(du, gam[i], -m1[i]) - h * m2[i]);
-    }
-    store_vec<T, N>(out + (a.s * p.P + a.q0 + q) * p.C + a.c, f);
-  }
-}
-
-// dgamma / dbeta = the partial rows' sums in row order; 32 channels per block, 8 row lanes.
-__global__ void __launch_bounds__(256) norm_param_join_kernel(const float* part, int64_t rows, int64_t C, void* dw,
-                                                              void* db, int pdtype, int accumulate) {
-  __shared__ float red[8][2][33];
+// dgamma / dbeta of 32 channels = the partial rows' sums in a fixed order: by `warps` row lanes.
+__device__ __forceinline__ void param_join(const float* part, int64_t rows, int64_t C, int64_t c0, void* dw, void* db,
+                                           int pdtype, int accumulate, float* red, int warps) {
   const int lane = threadIdx.x & 31, r0 = threadIdx.x >> 5;
-  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  const int64_t c = c0 + lane;
   float a = 0.f, b = 0.f;
   if (c < C) {
-#pragma unroll 4
-    for (int64_t r = r0; r < rows; r += 8) {
+#pragma unroll 8
+    for (int64_t r = r0; r < rows; r += warps) {
       a += part[r * 2 * C + c];
       b += part[r * 2 * C + C + c];
     }
   }
-  red[r0][0][lane] = a;
-  red[r0][1][lane] = b;
+  red[(r0 * 2) * 33 + lane] = a;
+  red[(r0 * 2 + 1) * 33 + lane] = b;
   __syncthreads();
   if (r0 < 2 && c < C) {
     float t = 0.f;
-#pragma unroll
-    for (int r = 0; r < 8; ++r) t += red[r][r0][lane];
+    for (int r = 0; r < warps; ++r) t += red[(r * 2 + r0) * 33 + lane];
     void* out = r0 == 0 ? dw : db;
     if (out != nullptr) {
       if (accumulate) reinterpret_cast<float*>(out)[c] += t;
@@ -667,62 +682,354 @@ __global__ void __launch_bounds__(256) norm_param_join_kernel(const float* part,
   }
 }
 
+__global__ void __launch_bounds__(512) norm_param_join_kernel(const float* part, int64_t rows, int64_t C, void* dw,
+                                                              void* db, int pdtype, int accumulate) {
+  __shared__ float red[16 * 2 * 33];
+  param_join(part, rows, C, (int64_t)blockIdx.x * 32, dw, db, pdtype, accumulate, red, 16);
+}
+
+// The groups' means of q and q h from the chunks', then dx; blocks past p.blocks join dgamma / dbeta.
+template <typename T, int N, int NT, int ACT, bool CKPT>
+__global__ void __launch_bounds__(NT) norm_bwd_apply_kernel(NormParams p) {
+  extern __shared__ float sf[];
+  if ((int64_t)blockIdx.x >= p.blocks) {
+    param_join(p.part, p.npart, p.C, ((int64_t)blockIdx.x - p.blocks) * 32, p.dw, p.db, p.pdtype, p.accumulate, sf,
+               NT / 32);
+    return;
+  }
+  const Slab<N, NT> a = chunk_slab<N, NT>(p);
+  const int cpg = a.cpg, lane = threadIdx.x & 31;
+  float* s1 = sf;                                       // [ng] mean(q), mean(q h)
+  float* s2 = sf + p.ng;
+  const float2* part = reinterpret_cast<const float2*>(p.gpart) + (a.s * p.chunks * p.G + a.g0) * p.nsub;
+  for (int g = threadIdx.x >> 5; g < a.ngl; g += NT / 32) {
+    float v1 = 0.f, v2 = 0.f;
+    for (int64_t j = lane; j < p.chunks * p.nsub; j += 32) {
+      const int64_t ch = j / p.nsub;
+      const float2 t = part[(ch * p.G + g) * p.nsub + (j - ch * p.nsub)];
+      v1 += t.x;
+      v2 += t.y;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      v1 += __shfl_xor_sync(kFullMask, v1, o);
+      v2 += __shfl_xor_sync(kFullMask, v2, o);
+    }
+    if (lane == 0) {
+      const float m = (float)p.P * (float)p.cpg;
+      s1[g] = v1 / m;
+      s2[g] = v2 / m;
+    }
+  }
+  __syncthreads();
+  if (!a.live()) return;
+  T* out = reinterpret_cast<T*>(p.out);
+  for (int col = a.tx; col < a.nv; col += a.TX) {
+    float m1[N], m2[N];
+    ChanConst<N> k;
+    const int64_t c = a.c0 + (int64_t)col * N;
+    k.load(p, c, [&](int i, float& mean, float& rstd) {
+      const int g = (col * N + i) / cpg;
+      mean = p.mean[a.s * p.G + a.g0 + g];
+      rstd = p.rstd[a.s * p.G + a.g0 + g];
+      m1[i] = s1[g];
+      m2[i] = s2[g];
+    });
+#pragma unroll 2
+    for (int q = a.ty; q < a.np; q += a.TY) {
+      float f[N], d[N];
+      unpack<T, N>(read_x<T, N, CKPT>(p, a.s, a.q0 + q, c), f);
+      unpack<T, N>(read_dy<T, N>(p, a.s, a.q0 + q, c), d);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float h = (f[i] - k.sub[i]) * k.mul[i];
+        const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, k.gam[i], k.bet[i]));
+        f[i] = k.mul[i] * (fmaf(du, k.gam[i], -m1[i]) - h * m2[i]);
+      }
+      store_vec<T, N>(out + (a.s * p.P + a.q0 + q) * p.C + c, f);
+    }
+  }
+}
+
+// ---- row kernels (P = 1) ----
+// L lanes (a power of two) hold a group of cpg = nvg N channels, V vectors each (lane l: vectors l, l + L, ..); a warp
+// holds 32 / L neighbouring groups.  Eight warps of a block share the groups and take different samples.
+constexpr int kRowWarps = 8;
+
+struct RowAt {
+  int g, l;        // group, lane within it
+  bool live;
+};
+template <int L>
+__device__ __forceinline__ RowAt row_at(const NormParams& p) {
+  const int lane = threadIdx.x & 31;
+  RowAt a;
+  a.g = (int)blockIdx.x % (int)p.nseg * (32 / L) + lane / L;
+  a.l = lane % L;
+  a.live = a.g < (int)p.G;
+  if (!a.live) a.g = (int)p.G - 1;
+  return a;
+}
+
+template <int L>
+__device__ __forceinline__ float lanes_sum(float v) {
+#pragma unroll
+  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+  return v;
+}
+
+// U samples of a warp at a time, so that U V loads are in flight.
+template <typename T, int N, int L, int V, int ACT>
+__global__ void __launch_bounds__(32 * kRowWarps) norm_fwd_rows(NormParams p) {
+  constexpr int U = V >= 4 ? 1 : 4 / V;
+  const RowAt a = row_at<L>(p);
+  const int nvg = (int)p.cpg / N, warp = threadIdx.x >> 5;
+  const int64_t c0 = (int64_t)a.g * p.cpg;
+  const float inv = 1.f / (float)p.cpg;
+  const int64_t step = (int64_t)(gridDim.x / p.nseg) * kRowWarps * U;
+  for (int64_t s0 = ((int64_t)(blockIdx.x / p.nseg) * kRowWarps + warp) * U; s0 < p.S; s0 += step) {
+    Raw<T, N> r[U][V];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int v = 0; v < V; ++v)
+        if (s0 + u < p.S && a.l + v * L < nvg) r[u][v] = read_x<T, N, false>(p, s0 + u, 0, c0 + (a.l + v * L) * N);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (s0 + u >= p.S) break;                            // the same for the whole warp
+      float t = 0.f, f[N];
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (a.l + v * L < nvg) {
+          unpack<T, N>(r[u][v], f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) t += f[i];
+        }
+      }
+      const float mu = lanes_sum<L>(t) * inv;
+      t = 0.f;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (a.l + v * L < nvg) {
+          unpack<T, N>(r[u][v], f);
+#pragma unroll
+          for (int i = 0; i < N; ++i) t = fmaf(f[i] - mu, f[i] - mu, t);
+        }
+      }
+      const float rs = 1.f / sqrtf(lanes_sum<L>(t) * inv + p.eps);
+      if (a.live && a.l == 0) {
+        p.mean[(s0 + u) * p.G + a.g] = mu;
+        p.rstd[(s0 + u) * p.G + a.g] = rs;
+      }
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if (a.live && a.l + v * L < nvg) {
+          const int64_t c = c0 + (a.l + v * L) * N;
+          unpack<T, N>(r[u][v], f);
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            f[i] = dense_act<ACT, sizeof(T) == 2>(fmaf(f[i] - mu, rs * ld_param(p.w, c + i, p.pdtype, 1.f),
+                                                       ld_param(p.b, c + i, p.pdtype, 0.f)));
+          store_vec<T, N>(reinterpret_cast<T*>(p.out) + (s0 + u) * p.C + c, f);
+        }
+      }
+    }
+  }
+}
+
+// A lane adds its channels' dgamma / dbeta over the samples of its warp; the block's warps are summed at the end into
+// one partial row per block of samples.
+template <typename T, int N, int L, int V, int ACT, bool CKPT>
+__global__ void __launch_bounds__(32 * kRowWarps) norm_bwd_rows(NormParams p) {
+  extern __shared__ float sf[];                            // [warps][2][32 V N]
+  const RowAt a = row_at<L>(p);
+  const int nvg = (int)p.cpg / N, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c0 = (int64_t)a.g * p.cpg, walker = blockIdx.x / p.nseg, walkers = gridDim.x / p.nseg;
+  const float inv = 1.f / (float)p.cpg;
+  float gam[V][N], bet[V][N], da[V][N], db[V][N];
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const bool in = a.l + v * L < nvg;
+      gam[v][i] = in ? ld_param(p.w, c0 + (a.l + v * L) * N + i, p.pdtype, 1.f) : 0.f;
+      bet[v][i] = in ? ld_param(p.b, c0 + (a.l + v * L) * N + i, p.pdtype, 0.f) : 0.f;
+      da[v][i] = db[v][i] = 0.f;
+    }
+  Raw<T, N> rx[V], rd[V];
+  float mu = 0.f, rs = 0.f;
+  const auto load = [&](int64_t s) {
+    mu = p.mean[s * p.G + a.g];
+    rs = p.rstd[s * p.G + a.g];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (a.l + v * L < nvg) {
+        rx[v] = read_x<T, N, CKPT>(p, s, 0, c0 + (a.l + v * L) * N);
+        rd[v] = read_dy<T, N>(p, s, 0, c0 + (a.l + v * L) * N);
+      }
+    }
+  };
+  int64_t s = walker * kRowWarps + warp;
+  if (s < p.S) load(s);
+  while (s < p.S) {
+    float h[V][N], du[V][N], t1 = 0.f, t2 = 0.f;
+    const float r = rs;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (a.l + v * L < nvg) {
+        unpack<T, N>(rx[v], h[v]);
+        unpack<T, N>(rd[v], du[v]);
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          h[v][i] = (h[v][i] - mu) * r;
+          du[v][i] *= dense_slope<ACT, sizeof(T) == 2>(fmaf(h[v][i], gam[v][i], bet[v][i]));
+          da[v][i] = fmaf(du[v][i], h[v][i], da[v][i]);
+          db[v][i] += du[v][i];
+          t1 = fmaf(du[v][i], gam[v][i], t1);
+          t2 = fmaf(du[v][i] * gam[v][i], h[v][i], t2);
+        }
+      }
+    }
+    const int64_t cur = s;
+    s += walkers * kRowWarps;
+    if (s < p.S) load(s);                                  // the next sample's loads run under this one's reduction
+    t1 = lanes_sum<L>(t1) * inv;
+    t2 = lanes_sum<L>(t2) * inv;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      if (a.live && a.l + v * L < nvg) {
+        float f[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) f[i] = r * (fmaf(du[v][i], gam[v][i], -t1) - h[v][i] * t2);
+        store_vec<T, N>(reinterpret_cast<T*>(p.out) + cur * p.C + c0 + (a.l + v * L) * N, f);
+      }
+    }
+  }
+  constexpr int W = 32 * V * N;
+#pragma unroll
+  for (int v = 0; v < V; ++v)
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      sf[(warp * 2) * W + (v * N + i) * 32 + lane] = da[v][i];
+      sf[(warp * 2 + 1) * W + (v * N + i) * 32 + lane] = db[v][i];
+    }
+  __syncthreads();
+  // thread -> (which, vector element, lane): sums over the warps, written by the lane's owner pattern
+  for (int j = threadIdx.x; j < 2 * W; j += 32 * kRowWarps) {
+    const int which = j / W, e = j - which * W, ln = e % 32, vi = e / 32, v = vi / N, i = vi - v * N;
+    const int g = (int)blockIdx.x % (int)p.nseg * (32 / L) + ln / L, vec = ln % L + v * L;
+    if (g >= (int)p.G || vec >= nvg) continue;
+    float t = 0.f;
+#pragma unroll
+    for (int w = 0; w < kRowWarps; ++w) t += sf[(w * 2 + which) * W + e];
+    p.part[(walker * 2 + which) * p.C + (int64_t)g * p.cpg + vec * N + i] = t;
+  }
+}
+
 // ---- host ----
+enum { kNormRows, kNormResident, kNormStream };
 struct NormPlan {
-  bool resident;
-  int N, ng, cs, R;
-  int64_t nseg, PR, chunks, walkers, npart;
+  int kind, N, NT, ng, cs, R, L, V, nsub, subc;
+  int64_t nseg, PR, chunks, walkers, npart, gparts;   // gparts: floats of gpart
   size_t smem;
 };
 
-// Segments of whole groups, cluster size and positions per CTA; falls back to streaming where a segment does
-// not fit kNormMaxCluster CTAs.  A segment is at least 128 bytes of channels (a full line per position), wider
-// while there are more than four segments for each SM, and its vectors must not straddle segments.
+// Which family, and its sizes.
+//  rows       P = 1, aligned, a group of at most 8 vectors a lane (measured at 1024 x 4096 fp32 in 64 groups: forward
+//             and backward 36 + 79 us resident, without it)
+//  resident   a segment fits a cluster, and either its CTAs are many or the tensor is too large for the streaming
+//             kernels' second read to come from L2.  A segment is at least 128 bytes of channels (a full line per
+//             position), wider while there are more than four segments for each SM; vectors do not straddle segments.
+//  streaming  otherwise
 static NormPlan norm_plan(int64_t S, int64_t P, int64_t C, int64_t G, int esize, bool vec, bool bwd, int sms,
                           int smem_max) {
   NormPlan pl{};
   const int64_t cpg = C / G;
   pl.N = vec ? 16 / esize : 1;
+  pl.nsub = 1;
+  if (P == 1 && vec && cpg % pl.N == 0 && G < (1 << 30)) {
+    const int64_t nvg = cpg / pl.N;
+    int L = 1;
+    while (L < 32 && L < nvg) L *= 2;
+    int V = 1;
+    while (V * L < nvg) V *= 2;
+    if (V <= (bwd ? 4 : 8)) {
+      pl.kind = kNormRows;
+      pl.L = L;
+      pl.V = V;
+      pl.nseg = (G + 32 / L - 1) / (32 / L);
+      const int64_t per = kRowWarps * (bwd ? 1 : (V >= 4 ? 1 : 4 / V));   // samples of a block at a time
+      const int64_t most = (S + per - 1) / per, want = (sms * (bwd ? 4 : 8) + pl.nseg - 1) / pl.nseg;
+      pl.walkers = most < want ? most : want;
+      pl.npart = pl.walkers;
+      pl.smem = bwd ? (size_t)kRowWarps * 2 * 32 * V * pl.N * 4 : 0;
+      return pl;
+    }
+  }
   const int tiles = bwd ? 2 : 1;
-  auto fixed = [&](int64_t cs, int64_t ng) -> int64_t {      // floats beside the tiles
-    const int64_t red = cs > kNormThreads * pl.N ? cs : (int64_t)kNormThreads * pl.N;
-    return 4 * (bwd ? 2 * red + 2 * cs + 6 * ng : red + 4 * ng) + 32;
-  };
   int64_t ng = 1;
   while (ng < G && (ng * cpg) % pl.N) ++ng;
   const int64_t unit = ng;
   while (ng + unit <= G && ng * cpg * esize < 128) ng += unit;
   if (ng > G || (ng * cpg) % pl.N) ng = G;
   while (ng * 2 <= G && S * ((G + 2 * ng - 1) / (2 * ng)) >= 4 * sms && P * ng * 2 * cpg * esize * tiles <= 32768) ng *= 2;
-  for (int64_t cap : {(int64_t)(smem_max / 2 - 1024), (int64_t)smem_max}) {
-    for (int R = 1; R <= kNormMaxCluster; R *= 2) {
-      const int64_t PR = (P + R - 1) / R, cs = ng * cpg;
-      if (cs > (1 << 20) || PR > (1 << 20)) continue;
-      const int64_t bytes = tiles * ((PR * cs * esize + 15) / 16 * 16) + fixed(cs, ng);
-      if (bytes > cap) continue;
-      pl.resident = true;
-      pl.ng = (int)ng;
-      pl.cs = (int)cs;
-      pl.R = R;
-      pl.PR = PR;
-      pl.nseg = (G + ng - 1) / ng;
-      pl.smem = (size_t)bytes;
-      const int64_t per_sm = cap == smem_max ? 1 : (smem_max + 1024) / (bytes + 1024) > 8 ? 8 : (smem_max + 1024) / (bytes + 1024);
-      const int64_t want = (sms * per_sm + R * pl.nseg - 1) / (R * pl.nseg);
-      pl.walkers = S < want ? S : want;
-      pl.npart = pl.walkers * R;
-      return pl;
+  pl.ng = (int)ng;
+  const int64_t cs = ng * cpg;
+  pl.nseg = (G + ng - 1) / ng;
+  const bool large = S * P * C * esize * tiles > (int64_t)48 << 20;
+  if (cs <= (1 << 20)) {
+    pl.cs = (int)cs;
+    for (int64_t cap : {(int64_t)(smem_max / 2 - 1024), (int64_t)smem_max}) {
+      for (int R = 1; R <= kNormMaxCluster; R *= 2) {
+        const int64_t PR = (P + R - 1) / R, tile = tiles * ((PR * cs * esize + 15) / 16 * 16);
+        if (PR > (1 << 20) || tile > cap) continue;
+        const int NT = vec && tile > 32768 ? 512 : 256;
+        const int64_t red = norm_red(cs, pl.N, NT);
+        const int64_t bytes = tile + 4 * (bwd ? 2 * red + 2 * cs + 6 * ng : red + 4 * ng) + 32;
+        if (bytes > cap) continue;
+        if (R > 1 && !large) break;               // a cluster's barriers cost more than a second read from L2
+        pl.kind = kNormResident;
+        pl.R = R;
+        pl.PR = PR;
+        pl.NT = NT;
+        pl.smem = (size_t)bytes;
+        int64_t per_sm = (smem_max + 1024) / (bytes + 1024);
+        if (per_sm > 2048 / NT) per_sm = 2048 / NT;
+        const int64_t want = (sms * per_sm + R * pl.nseg - 1) / (R * pl.nseg);
+        pl.walkers = S < want ? S : want;
+        pl.npart = pl.walkers * R;
+        return pl;
+      }
     }
   }
-  // streaming: about 8 blocks per SM, at least 32 positions each
-  const int64_t segs = (C / pl.N + kNormThreads - 1) / kNormThreads;
-  int64_t chunks = (8 * (int64_t)sms + S * segs - 1) / (S * segs);
-  const int64_t most = (P + 31) / 32;
+  // streaming: about 6 blocks per SM, at least 16 positions each where there are that many; groups too wide for a
+  // block's sums in parts of 4096 channels
+  pl.kind = kNormStream;
+  pl.NT = 256;
+  pl.cs = (int)cs;
+  if (cs > 16384) {
+    if (cpg % pl.N) pl.N = 1;      // parts start where groups do
+    ng = 1;
+    pl.subc = 4096;
+    pl.nsub = (int)((cpg + pl.subc - 1) / pl.subc);
+    pl.cs = pl.nsub > 1 ? pl.subc : (int)cpg;
+    pl.ng = 1;
+    pl.nseg = G * pl.nsub;
+  }
+  int64_t chunks = (6 * (int64_t)sms + S * pl.nseg - 1) / (S * pl.nseg);
+  const int64_t most = (P + 15) / 16;
   if (chunks > most) chunks = most;
   pl.PR = (P + chunks - 1) / chunks;
   pl.chunks = (P + pl.PR - 1) / pl.PR;
   pl.npart = S * pl.chunks;
+  pl.gparts = S * pl.chunks * G * pl.nsub * 2;
+  pl.smem = (size_t)(4 * (2 * norm_red(pl.cs, pl.N, 256) + 2 * ng));
   return pl;
+}
+
+// Floats of workspace.
+static int64_t norm_floats(const NormPlan& pl, int64_t C, bool bwd) {
+  return (bwd ? pl.npart * 2 * C : 0) + pl.gparts;
 }
 
 static int norm_checks(int64_t S, int64_t P, int64_t C, int64_t G, int dtype, int pdtype, int act) {
@@ -738,12 +1045,12 @@ static bool vec_rows(const void* p, int64_t a, int64_t b, int64_t C, int esize) 
 }
 
 template <typename K>
-static int launch_cluster(K kernel, const NormParams& p, int64_t blocks, int R, size_t smem, cudaStream_t st) {
+static int launch_cluster(K kernel, const NormParams& p, int64_t blocks, int threads, int R, size_t smem, cudaStream_t st) {
   if (blocks > 0x7FFFFFFF) return GL_ERR_SHAPE;
   if (int rc = ensure_dynamic_smem((const void*)kernel, smem)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3(kNormThreads);
+  cfg.blockDim = dim3((unsigned)threads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at{};
@@ -751,62 +1058,98 @@ static int launch_cluster(K kernel, const NormParams& p, int64_t blocks, int R, 
   at.val.clusterDim.x = (unsigned)R;
   at.val.clusterDim.y = at.val.clusterDim.z = 1;
   cfg.attrs = &at;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = R > 1 ? 1 : 0;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
   if (e != cudaSuccess) return set_cuda_error(e);
   count_launches(1);
   return GL_OK;
 }
 
-static int launched(int n) {
-  const cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return set_cuda_error(e);
-  count_launches(n);
-  return GL_OK;
+// f(ActTag L, ActTag V) for a row plan (the tags carry plain integers).
+template <int MAXV, typename F>
+static void with_row_shape(int L, int V, F f) {
+  const auto pick_v = [&](auto l) {
+    if (V == 1) f(l, ActTag<1>());
+    if constexpr (decltype(l)::value == 32) {      // more than one vector a lane only with all 32 lanes
+      if (V == 2) f(l, ActTag<2>());
+      if (V == 4) f(l, ActTag<4>());
+      if constexpr (MAXV >= 8)
+        if (V == 8) f(l, ActTag<8>());
+    }
+  };
+  switch (L) {
+    case 1: pick_v(ActTag<1>()); break;
+    case 2: pick_v(ActTag<2>()); break;
+    case 4: pick_v(ActTag<4>()); break;
+    case 8: pick_v(ActTag<8>()); break;
+    case 16: pick_v(ActTag<16>()); break;
+    default: pick_v(ActTag<32>()); break;
+  }
 }
 
 template <typename T, int N, int ACT>
 static int run_norm_fwd_act(NormParams& p, const NormPlan& pl, cudaStream_t st) {
-  if (pl.resident) return launch_cluster(norm_fwd_resident<T, N, ACT>, p, p.S * pl.nseg * pl.R, pl.R, pl.smem, st);
-  const int64_t segs = (p.C / N + kNormThreads - 1) / kNormThreads, blocks = p.S * pl.chunks * segs;
-  if (blocks > 0x7FFFFFFF || p.S * p.G > 0x7FFFFFFF) return GL_ERR_SHAPE;
-  norm_stats_kernel<T, N><<<(unsigned)blocks, kNormThreads, 0, st>>>(p);
-  norm_stats_join_kernel<<<(unsigned)(p.S * p.G), kNormThreads, 0, st>>>(p);
-  norm_apply_kernel<T, N, ACT><<<(unsigned)blocks, kNormThreads, 0, st>>>(p);
-  return launched(3);
+  if constexpr (N > 1) {
+    if (pl.kind == kNormRows) {
+      int rc = GL_ERR_UNSUPPORTED;
+      with_row_shape<8>(pl.L, pl.V, [&](auto l, auto v) {
+        rc = launch_cluster(norm_fwd_rows<T, N, decltype(l)::value, decltype(v)::value, ACT>, p, pl.nseg * pl.walkers,
+                            32 * kRowWarps, 1, 0, st);
+      });
+      return rc;
+    }
+    if (pl.kind == kNormResident && pl.NT == 512)
+      return launch_cluster(norm_fwd_resident<T, N, 512, ACT>, p, p.S * pl.nseg * pl.R, 512, pl.R, pl.smem, st);
+  }
+  if (pl.kind == kNormResident)
+    return launch_cluster(norm_fwd_resident<T, N, 256, ACT>, p, p.S * pl.nseg * pl.R, 256, pl.R, pl.smem, st);
+  const int64_t blocks = p.S * pl.chunks * pl.nseg;
+  if (int rc = launch_cluster(norm_stats_kernel<T, N, 256>, p, blocks, 256, 1, pl.smem, st)) return rc;
+  return launch_cluster(norm_apply_kernel<T, N, 256, ACT>, p, blocks, 256, 1, pl.smem, st);
 }
 
 template <typename T, int N>
-static int run_norm_fwd(NormParams& p, const NormPlan& pl, cudaStream_t st) {
+static int run_norm_fwd(NormParams& p, int act, const NormPlan& pl, cudaStream_t st) {
   int rc = GL_ERR_UNSUPPORTED;
-  with_act(p.act, [&](auto tag) { rc = run_norm_fwd_act<T, N, decltype(tag)::value>(p, pl, st); });
+  with_act(act, [&](auto tag) { rc = run_norm_fwd_act<T, N, decltype(tag)::value>(p, pl, st); });
   return rc;
 }
 
 template <typename T, int N, int ACT, bool CKPT>
-static int run_norm_bwd_act(NormParams& p, const NormPlan& pl, const GlNormBwdArgs& a, cudaStream_t st) {
-  if (pl.resident) {
-    if (int rc = launch_cluster(norm_bwd_resident<T, N, ACT, CKPT>, p, pl.walkers * pl.nseg * pl.R, pl.R, pl.smem, st))
-      return rc;
-  } else {
-    const int64_t segs = (p.C / N + kNormThreads - 1) / kNormThreads, blocks = p.S * pl.chunks * segs;
-    if (blocks > 0x7FFFFFFF || p.S * p.G > 0x7FFFFFFF) return GL_ERR_SHAPE;
-    float* coef = p.part + pl.npart * 2 * p.C;
-    norm_bwd_stats_kernel<T, N, ACT, CKPT><<<(unsigned)blocks, kNormThreads, 0, st>>>(p);
-    norm_bwd_join_kernel<<<(unsigned)(p.S * p.G), kNormThreads, 0, st>>>(p, coef);
-    norm_bwd_apply_kernel<T, N, ACT, CKPT><<<(unsigned)blocks, kNormThreads, 0, st>>>(p, coef);
-    if (int rc = launched(3)) return rc;
+static int run_norm_bwd_act(NormParams& p, const NormPlan& pl, cudaStream_t st) {
+  const int64_t joins = p.dw || p.db ? (p.C + 31) / 32 : 0;
+  int rc = GL_ERR_UNSUPPORTED;
+  if (pl.kind == kNormStream) {
+    p.blocks = p.S * pl.chunks * pl.nseg;
+    const size_t smem = pl.smem < 8 * 2 * 33 * 4 ? 8 * 2 * 33 * 4 : pl.smem;
+    rc = launch_cluster(norm_bwd_stats_kernel<T, N, 256, ACT, CKPT>, p, p.blocks, 256, 1, pl.smem, st);
+    if (rc) return rc;
+    return launch_cluster(norm_bwd_apply_kernel<T, N, 256, ACT, CKPT>, p, p.blocks + joins, 256, 1, smem, st);
   }
-  if (!a.dw && !a.db) return GL_OK;
-  norm_param_join_kernel<<<(unsigned)((p.C + 31) / 32), 256, 0, st>>>(p.part, pl.npart, p.C, a.dw, a.db, a.pdtype,
-                                                                     a.accumulate);
-  return launched(1);
+  if constexpr (N > 1) {
+    if (pl.kind == kNormRows) {
+      with_row_shape<4>(pl.L, pl.V, [&](auto l, auto v) {
+        rc = launch_cluster(norm_bwd_rows<T, N, decltype(l)::value, decltype(v)::value, ACT, CKPT>, p,
+                            pl.nseg * pl.walkers, 32 * kRowWarps, 1, pl.smem, st);
+      });
+    } else if (pl.NT == 512) {
+      rc = launch_cluster(norm_bwd_resident<T, N, 512, ACT, CKPT>, p, pl.walkers * pl.nseg * pl.R, 512, pl.R, pl.smem, st);
+    }
+  }
+  if (pl.kind == kNormResident && pl.NT == 256)
+    rc = launch_cluster(norm_bwd_resident<T, N, 256, ACT, CKPT>, p, pl.walkers * pl.nseg * pl.R, 256, pl.R, pl.smem, st);
+  if (rc || !joins) return rc;
+  norm_param_join_kernel<<<(unsigned)joins, 512, 0, st>>>(p.part, pl.npart, p.C, p.dw, p.db, p.pdtype, p.accumulate);
+  const cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return set_cuda_error(e);
+  count_launches(1);
+  return GL_OK;
 }
 
 template <typename T, int N, bool CKPT>
-static int run_norm_bwd(NormParams& p, const NormPlan& pl, const GlNormBwdArgs& a, cudaStream_t st) {
+static int run_norm_bwd(NormParams& p, int act, const NormPlan& pl, cudaStream_t st) {
   int rc = GL_ERR_UNSUPPORTED;
-  with_act(p.act, [&](auto tag) { rc = run_norm_bwd_act<T, N, decltype(tag)::value, CKPT>(p, pl, a, st); });
+  with_act(act, [&](auto tag) { rc = run_norm_bwd_act<T, N, decltype(tag)::value, CKPT>(p, pl, st); });
   return rc;
 }
 
@@ -838,8 +1181,7 @@ extern "C" int64_t gl_norm_work_bytes(int64_t S, int64_t P, int64_t C, int64_t G
   for (int vec = 0; vec < 2; ++vec) {     // the call's alignment decides which of the two plans runs
     if (vec && (C * esize) % 16) continue;
     const NormPlan pl = norm_plan(S, P, C, G, esize, vec, backward != 0, sms, smem);
-    const int64_t n = backward ? 4 * (pl.npart * 2 * C + (pl.resident ? 0 : 2 * S * G))
-                               : (pl.resident ? 0 : 8 * S * pl.chunks * C);
+    const int64_t n = 4 * norm_floats(pl, C, backward != 0);
     if (n > most) most = n;
   }
   return most;
@@ -858,15 +1200,16 @@ extern "C" int gl_norm_fwd(const GlNormArgs* args, void* stream) {
   const int esize = a.dtype == GL_DTYPE_F32 ? 4 : 2;
   const bool vec = vec_rows(a.x, a.sx, a.px, a.C, esize) && vec_rows(a.y, 0, 0, a.C, esize);
   const NormPlan pl = norm_plan(a.S, a.P, a.C, a.G, esize, vec, false, sms, smem);
-  if (!pl.resident && (!a.work || a.work_bytes < 8 * a.S * pl.chunks * a.C)) return GL_ERR_WORKSPACE;
+  if (pl.gparts > 0 && (!a.work || a.work_bytes < 4 * pl.gparts)) return GL_ERR_WORKSPACE;
   NormParams p{};
-  p.x = a.x; p.w = a.w; p.b = a.b; p.out = a.y; p.mean = a.mean; p.rstd = a.rstd; p.part = (float*)a.work;
+  p.x = a.x; p.w = a.w; p.b = a.b; p.out = a.y; p.mean = a.mean; p.rstd = a.rstd; p.gpart = (float*)a.work;
   p.S = a.S; p.P = a.P; p.C = a.C; p.G = a.G; p.cpg = a.C / a.G; p.sx = a.sx; p.px = a.px;
   p.nseg = pl.nseg; p.PR = pl.PR; p.chunks = pl.chunks; p.ng = pl.ng; p.cs = pl.cs; p.R = pl.R;
-  p.pdtype = a.pdtype; p.act = a.act; p.eps = a.eps;
+  p.nsub = pl.nsub; p.subc = pl.subc;
+  p.pdtype = a.pdtype; p.eps = a.eps;
   cudaStream_t st = (cudaStream_t)stream;
-  if (a.dtype == GL_DTYPE_F32) return vec ? run_norm_fwd<float, 4>(p, pl, st) : run_norm_fwd<float, 1>(p, pl, st);
-  return vec ? run_norm_fwd<__nv_bfloat16, 8>(p, pl, st) : run_norm_fwd<__nv_bfloat16, 1>(p, pl, st);
+  if (a.dtype == GL_DTYPE_F32) return pl.N > 1 ? run_norm_fwd<float, 4>(p, a.act, pl, st) : run_norm_fwd<float, 1>(p, a.act, pl, st);
+  return pl.N > 1 ? run_norm_fwd<__nv_bfloat16, 8>(p, a.act, pl, st) : run_norm_fwd<__nv_bfloat16, 1>(p, a.act, pl, st);
 }
 
 extern "C" int gl_norm_bwd(const GlNormBwdArgs* args, void* stream) {
@@ -888,18 +1231,20 @@ extern "C" int gl_norm_bwd(const GlNormBwdArgs* args, void* stream) {
   const bool vec = (ckpt || vec_rows(a.x, a.sx, a.px, a.C, esize)) && vec_rows(a.dy, a.sdy, a.pdy, a.C, esize) &&
                    vec_rows(a.dx, 0, 0, a.C, esize);
   const NormPlan pl = norm_plan(a.S, a.P, a.C, a.G, esize, vec, true, sms, smem);
-  if (a.work_bytes < 4 * (pl.npart * 2 * a.C + (pl.resident ? 0 : 2 * a.S * a.G))) return GL_ERR_WORKSPACE;
+  if (a.work_bytes < 4 * norm_floats(pl, a.C, true)) return GL_ERR_WORKSPACE;
   NormParams p{};
   p.x = a.x; p.dy = a.dy; p.w = a.w; p.b = a.b; p.codes = a.codes; p.exps = a.exps; p.out = a.dx;
   p.mean = const_cast<float*>(a.mean); p.rstd = const_cast<float*>(a.rstd); p.part = (float*)a.work;
+  p.gpart = p.part + pl.npart * 2 * a.C; p.dw = a.dw; p.db = a.db; p.accumulate = a.accumulate;
   p.S = a.S; p.P = a.P; p.C = a.C; p.G = a.G; p.cpg = a.C / a.G; p.sx = a.sx; p.px = a.px; p.sdy = a.sdy;
   p.pdy = a.pdy; p.ldc = a.ldc; p.nblk = nblk; p.nseg = pl.nseg; p.npart = pl.npart; p.PR = pl.PR;
-  p.chunks = pl.chunks; p.ng = pl.ng; p.cs = pl.cs; p.R = pl.R; p.pdtype = a.pdtype; p.act = a.act;
+  p.chunks = pl.chunks; p.ng = pl.ng; p.cs = pl.cs; p.R = pl.R;
+  p.nsub = pl.nsub; p.subc = pl.subc; p.pdtype = a.pdtype;
   if (a.dtype == GL_DTYPE_F32) {
-    if (ckpt) return vec ? run_norm_bwd<float, 4, true>(p, pl, a, st) : run_norm_bwd<float, 1, true>(p, pl, a, st);
-    return vec ? run_norm_bwd<float, 4, false>(p, pl, a, st) : run_norm_bwd<float, 1, false>(p, pl, a, st);
+    if (ckpt) return pl.N > 1 ? run_norm_bwd<float, 4, true>(p, a.act, pl, st) : run_norm_bwd<float, 1, true>(p, a.act, pl, st);
+    return pl.N > 1 ? run_norm_bwd<float, 4, false>(p, a.act, pl, st) : run_norm_bwd<float, 1, false>(p, a.act, pl, st);
   }
   using B = __nv_bfloat16;
-  if (ckpt) return vec ? run_norm_bwd<B, 8, true>(p, pl, a, st) : run_norm_bwd<B, 1, true>(p, pl, a, st);
-  return vec ? run_norm_bwd<B, 8, false>(p, pl, a, st) : run_norm_bwd<B, 1, false>(p, pl, a, st);
+  if (ckpt) return pl.N > 1 ? run_norm_bwd<B, 8, true>(p, a.act, pl, st) : run_norm_bwd<B, 1, true>(p, a.act, pl, st);
+  return pl.N > 1 ? run_norm_bwd<B, 8, false>(p, a.act, pl, st) : run_norm_bwd<B, 1, false>(p, a.act, pl, st);
 }
