@@ -18,70 +18,92 @@ struct Act8Params {
   int64_t rows, C, ldx, ldc, nblk;
 };
 
-// One warp per (row, segment of 32 lanes); LANE_CH channels per lane, 32 / LANE_CH lanes per block.  VEC is
-// LANE_CH where a row's 16-byte vectors are aligned, else 1 (element accesses).
+// A warp takes U = 4 segments of 32 lanes at a time, so that four loads are in flight; N channels per lane, L = 32 / N
+// lanes per block.  ALIGNED: rows' 16-byte vectors are, else elements are accessed one by one.
 template <typename T, bool ENCODE, bool ALIGNED>
 __global__ void __launch_bounds__(256) act8_kernel(Act8Params p) {
-  constexpr int N = kVec16<T>;
-  constexpr int L = kActBlock / N;          // lanes per block
+  constexpr int N = kVec16<T>, L = kActBlock / N, U = 4;
   const int lane = threadIdx.x & 31;
-  const int64_t segs = (p.nblk * L + 31) / 32;
+  const int64_t segs = (p.nblk * L + 31) / 32, total = p.rows * segs;
   const int64_t warps = (int64_t)gridDim.x * (blockDim.x >> 5);
-  for (int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < p.rows * segs; w += warps) {
-    const int64_t row = w / segs, c = ((w - row * segs) * 32 + lane) * N;
-    const int64_t blk = c / kActBlock;
-    const bool whole = c + N <= p.C;
-    float v[N];
+  for (int64_t w = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5); w < total; w += warps * U) {
+    int64_t row[U], c[U];
+    bool live[U];                               // the lane's block exists
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int64_t k = w + u * warps;
+      row[u] = total < (1ll << 31) ? (int64_t)((unsigned)k / (unsigned)segs) : k / segs;
+      c[u] = ((k - row[u] * segs) * 32 + lane) * N;
+      live[u] = k < total && c[u] < p.nblk * kActBlock;
+    }
     if constexpr (ENCODE) {
-      const T* src = reinterpret_cast<const T*>(p.x) + row * p.ldx + c;
-      if (ALIGNED && whole) {
-        load_vec<T, N>(src, v);
-      } else {
+      float v[U][N];
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = c + i < p.C ? to_f32<T>(src[i]) : 0.f;
+      for (int u = 0; u < U; ++u) {
+        const T* src = reinterpret_cast<const T*>(p.x) + row[u] * p.ldx + c[u];
+        if (ALIGNED && live[u] && c[u] + N <= p.C) {
+          load_vec<T, N>(src, v[u]);
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i) v[u][i] = live[u] && c[u] + i < p.C ? to_f32<T>(src[i]) : 0.f;
+        }
       }
-      int m = 0;                            // |v| ordered by its bits: a NaN is above every number
 #pragma unroll
-      for (int i = 0; i < N; ++i) m = max(m, __float_as_int(v[i]) & 0x7FFFFFFF);
+      for (int u = 0; u < U; ++u) {
+        int m = 0;                              // |v| ordered by its bits: a NaN is above every number
 #pragma unroll
-      for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, o));
-      if (blk < p.nblk) {
+        for (int i = 0; i < N; ++i) m = max(m, __float_as_int(v[u][i]) & 0x7FFFFFFF);
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(kFullMask, m, o));
+        if (!live[u]) continue;
         const int byte = act8_exponent(__int_as_float(m));
         const float inv = byte == 255 ? 0.f : act8_inverse(byte);
         const int most = byte == 249 ? 63 : 127;   // 64 * 2^122 would read back as an infinity
         uint32_t q[N / 4];
 #pragma unroll
         for (int i = 0; i < N; i += 4) {
-          uint32_t u = 0;
+          uint32_t b = 0;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) u |= (uint32_t)(max(min(__float2int_rn(v[i + j] * inv), most), -most) & 0xFF) << (8 * j);
-          q[i / 4] = u;
+          for (int j = 0; j < 4; ++j)
+            b |= (uint32_t)(max(min(__float2int_rn(v[u][i + j] * inv), most), -most) & 0xFF) << (8 * j);
+          q[i / 4] = b;
         }
-        int8_t* dst = p.codes + row * p.ldc + c;
+        int8_t* dst = p.codes + row[u] * p.ldc + c[u];
         if constexpr (N == 4) *reinterpret_cast<uint32_t*>(dst) = q[0];
         else *reinterpret_cast<uint2*>(dst) = make_uint2(q[0], q[1]);
-        if (lane % L == 0) p.exps[row * p.nblk + blk] = (uint8_t)byte;
+        if (lane % L == 0) p.exps[row[u] * p.nblk + c[u] / kActBlock] = (uint8_t)byte;
       }
-    } else if (c < p.C) {
-      const float s = act8_scale(p.exps[row * p.nblk + blk]);
-      const int8_t* src = p.codes + row * p.ldc + c;
-      uint32_t q[N / 4];
-      if constexpr (N == 4) {
-        q[0] = *reinterpret_cast<const uint32_t*>(src);
-      } else {
-        const uint2 u = *reinterpret_cast<const uint2*>(src);
-        q[0] = u.x;
-        q[N / 4 - 1] = u.y;
+    } else {
+      uint32_t q[U][N / 4];
+      uint8_t e[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        if (!live[u]) continue;
+        e[u] = p.exps[row[u] * p.nblk + c[u] / kActBlock];
+        const int8_t* src = p.codes + row[u] * p.ldc + c[u];
+        if constexpr (N == 4) {
+          q[u][0] = *reinterpret_cast<const uint32_t*>(src);
+        } else {
+          const uint2 t = *reinterpret_cast<const uint2*>(src);
+          q[u][0] = t.x;
+          q[u][N / 4 - 1] = t.y;
+        }
       }
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = (float)(int8_t)(q[i / 4] >> (8 * (i % 4))) * s;
-      T* dst = reinterpret_cast<T*>(p.out) + row * p.ldx + c;
-      if (ALIGNED && whole) {
-        store_vec<T, N>(dst, v);
-      } else {
+      for (int u = 0; u < U; ++u) {
+        if (!live[u] || c[u] >= p.C) continue;
+        const float s = act8_scale(e[u]);
+        float v[N];
 #pragma unroll
-        for (int i = 0; i < N; ++i)
-          if (c + i < p.C) dst[i] = from_f32<T>(v[i]);
+        for (int i = 0; i < N; ++i) v[i] = (float)(int8_t)(q[u][i / 4] >> (8 * (i % 4))) * s;
+        T* dst = reinterpret_cast<T*>(p.out) + row[u] * p.ldx + c[u];
+        if (ALIGNED && c[u] + N <= p.C) {
+          store_vec<T, N>(dst, v);
+        } else {
+#pragma unroll
+          for (int i = 0; i < N; ++i)
+            if (c[u] + i < p.C) dst[i] = from_f32<T>(v[i]);
+        }
       }
     }
   }
@@ -95,7 +117,7 @@ static int launch_act8(const GlAct8Args& a, cudaStream_t st) {
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   const int64_t segs = (p.nblk * (kActBlock / kVec16<T>) + 31) / 32;
-  const int64_t need = (a.rows * segs + 7) / 8, cap = (int64_t)sms * 32;
+  const int64_t need = (a.rows * segs + 7) / 8, cap = (int64_t)sms * 8;
   const unsigned blocks = (unsigned)(need < cap ? need : cap);
   if (aligned) act8_kernel<T, ENCODE, true><<<blocks, 256, 0, st>>>(p);
   else act8_kernel<T, ENCODE, false><<<blocks, 256, 0, st>>>(p);

@@ -83,14 +83,26 @@ __device__ __forceinline__ void store_vec(T* p, const float (&v)[V]) {
 // the normal distribution's tail by Abramowitz & Stegun 7.1.26, erfc(t) = (a1 s + .. + a5 s^5) e^(-t^2) with
 // s = 1 / (1 + 0.3275911 t), whose error is at most 1.5e-7 (a bf16 step is 4e-3) and whose exponential is also
 // the density that act' needs.  With erff and expf the backward kernels were bound by arithmetic, not memory.
+__device__ __forceinline__ float ex2_approx(float x) {   // 2^x; denormals are 0
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+  float r;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 template <bool FAST>
 __device__ __forceinline__ void normal_cdf_pdf(float z, float& cdf, float& pdf) {
   if constexpr (FAST) {
-    const float e = __expf(-0.5f * z * z), t = fabsf(z) * 0.7071067811865476f;
-    const float s = __fdividef(1.f, fmaf(0.3275911f, t, 1.f));
-    const float q = s * fmaf(s, fmaf(s, fmaf(s, fmaf(s, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f),
-                             0.254829592f);
-    const float tail = 0.5f * q * e;
+    const float e = ex2_approx(z * z * (-0.5f * 1.4426950408889634f));       // e^(-z^2 / 2)
+    const float s = rcp_approx(fmaf(fabsf(z), 0.3275911f * 0.7071067811865476f, 1.f));
+    // half of the published coefficients: the tail is erfc / 2
+    const float q = s * fmaf(s, fmaf(s, fmaf(s, fmaf(s, 0.5307027145f, -0.7265760135f), 0.7107068705f), -0.142248368f),
+                             0.127414796f);
+    const float tail = q * e;
     cdf = z < 0.f ? tail : 1.f - tail;
     pdf = 0.3989422804014327f * e;
   } else {
@@ -101,7 +113,7 @@ __device__ __forceinline__ void normal_cdf_pdf(float z, float& cdf, float& pdf) 
 
 template <bool FAST>
 __device__ __forceinline__ float logistic(float z) {
-  if constexpr (FAST) return __fdividef(1.f, 1.f + __expf(-z));
+  if constexpr (FAST) return rcp_approx(1.f + ex2_approx(z * -1.4426950408889634f));
   else return 1.f / (1.f + expf(-z));
 }
 

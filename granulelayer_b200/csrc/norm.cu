@@ -11,24 +11,20 @@
 // Three families:
 //  * row kernels (P = 1: tokens, each with its own statistics; groups that a warp can hold): L lanes keep a
 //    group in registers, reductions are shuffles, no barrier at all; several samples per warp are in flight.
-//  * resident kernels: a cluster of R <= 8 CTAs owns one (sample, segment of whole groups) in shared memory, so the
-//    data comes from HBM once; the group sums cross the cluster through distributed shared memory.
+//  * resident kernels, for small samples: a block owns one (sample, segment of whole groups) in shared memory, one
+//    launch, x read once.
 //  * streaming kernels: chunks of positions give partial statistics (per channel shifted by the chunk's first value,
-//    merged with Chan's formula), and an elementwise pass merges those of its groups; x is read twice, the second
-//    time from L2 where it fits, and no block waits for another.
+//    merged with Chan's formula), and an elementwise pass, in the opposite block order, merges those of its groups;
+//    x is read twice, the second time from L2 as far as it fits, and no block waits for another.  (Clusters of 8 blocks
+//    that kept 64-channel segments of such samples in distributed shared memory read them once, but in 128-byte
+//    pieces between cluster barriers: 69 + 160 us forward and backward at 16 x 4096 x 512 bf16.)
 // Variances are sums of squared deviations, never differences of squares.  Outside the row kernels a thread owns whole
 // 16-byte vectors of channels and walks over positions, so all sums are first per channel: group boundaries need no
 // alignment, and with A_c = sum du h, B_c = sum du the backward's group means are sum gamma_c A_c / m and
 // sum gamma_c B_c / m.  No atomics: every sum has one order.
-#include <cooperative_groups.h>
-
 #include "dense.cuh"
 
-namespace cg = cooperative_groups;
-
 namespace gl {
-
-constexpr int kNormMaxCluster = 8;
 
 struct NormParams {
   const void* x;
@@ -46,9 +42,9 @@ struct NormParams {
   float* gpart;         // streaming: per (sample, chunk, group) statistics or sums [S][chunks][G][2]
   int64_t S, P, C, G, cpg, sx, px, sdy, pdy, ldc, nblk;
   int64_t nseg, npart;  // segments per sample; rows of part
-  int64_t PR;           // positions per CTA (resident) or chunk (streaming)
+  int64_t PR;           // positions per chunk (resident: all)
   int64_t chunks, blocks;
-  int ng, cs, R, pdtype, accumulate;
+  int ng, cs, pdtype, accumulate;
   int nsub, subc;       // streaming, groups too wide for a block: parts of a group, channels of a part (ng = 1)
   float eps;
 };
@@ -57,6 +53,25 @@ __device__ __forceinline__ float ld_param(const void* p, int64_t i, int dtype, f
   if (p == nullptr) return none;
   return dtype == GL_DTYPE_F32 ? reinterpret_cast<const float*>(p)[i]
                                : __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+}
+
+// N parameters from channel c on; whole vectors where they are 16-byte aligned.
+template <int N>
+__device__ __forceinline__ void ld_params(const void* p, int64_t c, int dtype, float none, float (&v)[N]) {
+  if (N > 1 && p != nullptr && (((uintptr_t)p | c * (dtype == GL_DTYPE_F32 ? 4 : 2)) & 15) == 0 && N * (dtype == GL_DTYPE_F32 ? 4 : 2) % 16 == 0) {
+    if (dtype == GL_DTYPE_F32) {
+#pragma unroll
+      for (int k = 0; k + 4 <= N; k += 4) {
+        const float4 a = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + c + k);
+        v[k] = a.x; v[k + 1] = a.y; v[k + 2] = a.z; v[k + 3] = a.w;
+      }
+    } else if constexpr (N == 8) {
+      load_vec<__nv_bfloat16, 8>(reinterpret_cast<const __nv_bfloat16*>(p) + c, v);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) v[i] = ld_param(p, c + i, dtype, none);
 }
 
 // N raw elements (16 bytes, or one element).
@@ -116,7 +131,7 @@ __device__ __forceinline__ Raw<T, N> read_dy(const NormParams& p, int64_t s, int
 // positions q0 .. q0 + np - 1; thread (tx, ty) owns vector columns tx, tx + TX, .. and every TY-th position.
 template <int N, int NT>
 struct Slab {
-  int64_t s, c0, q0;
+  int64_t s, c0, q0, at;   // at: position range (rank or chunk)
   int g0, ngl, csl, cpg, nv, np, TX, TY, tx, ty, rows;
   __device__ __forceinline__ Slab(const NormParams& p, int64_t s_, int64_t seg, int64_t part) {
     s = s_;
@@ -128,12 +143,13 @@ struct Slab {
       c0 = (int64_t)g0 * p.cpg;
     } else {
       g0 = (int)(seg / p.nsub);
-      const int64_t at = (seg - (int64_t)g0 * p.nsub) * p.subc;
+      const int64_t off = (seg - (int64_t)g0 * p.nsub) * p.subc;
       ngl = 1;
-      cpg = csl = (int)min((int64_t)p.subc, p.cpg - at);
-      c0 = (int64_t)g0 * p.cpg + at;
+      cpg = csl = (int)min((int64_t)p.subc, p.cpg - off);
+      c0 = (int64_t)g0 * p.cpg + off;
     }
     nv = csl / N;
+    at = part;
     q0 = part * p.PR;
     np = (int)max((int64_t)0, min(p.PR, p.P - q0));
     TX = min(nv, NT);
@@ -193,31 +209,22 @@ __device__ __forceinline__ void group_sums(const float* red, int cs, int rows, i
   }
 }
 
-// Sum of gs[g] over the cluster's CTAs, in rank order (every CTA computes the same value).
-__device__ __forceinline__ float cluster_total(float* gs, int g, int R) {
-  if (R == 1) return gs[g];
-  cg::cluster_group cl = cg::this_cluster();
-  float s = 0.f;
-  for (int r = 0; r < R; ++r) s += cl.map_shared_rank(gs, r)[g];
-  return s;
-}
-
-__device__ __forceinline__ void norm_barrier(int R) {
-  if (R == 1) __syncthreads();
-  else cg::this_cluster().sync();
-}
-
-// A vector of channels' constants: (x - sub) mul = h, and gamma, beta.
-template <int N>
+// A vector of channels' constants: (x - sub) mul = h, and gamma, beta.  With FAST (bf16 x, whose own rounding is 2^15
+// times larger) h is x mul + sub with sub = -mean mul: one operation instead of two.
+template <int N, bool FAST>
 struct ChanConst {
   float mul[N], sub[N], gam[N], bet[N];
+  __device__ __forceinline__ float h(float x, int i) const {
+    return FAST ? fmaf(x, mul[i], sub[i]) : (x - sub[i]) * mul[i];
+  }
   template <typename F>
   __device__ __forceinline__ void load(const NormParams& p, int64_t c, F stat) {   // stat(i, mean, rstd)
+    ld_params<N>(p.w, c, p.pdtype, 1.f, gam);
+    ld_params<N>(p.b, c, p.pdtype, 0.f, bet);
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       stat(i, sub[i], mul[i]);
-      gam[i] = ld_param(p.w, c + i, p.pdtype, 1.f);
-      bet[i] = ld_param(p.b, c + i, p.pdtype, 0.f);
+      if (FAST) sub[i] *= -mul[i];
     }
   }
 };
@@ -227,9 +234,9 @@ template <typename T, int N, int NT, int ACT>
 __global__ void __launch_bounds__(NT) norm_fwd_resident(NormParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   Raw<T, N>* tile = reinterpret_cast<Raw<T, N>*>(smem);
-  const int tid = threadIdx.x, R = p.R, rank = blockIdx.x % R, cpg = (int)p.cpg;
-  const int64_t item = blockIdx.x / R, s = item / p.nseg;
-  const Slab<N, NT> a(p, s, item - s * p.nseg, rank);
+  const int tid = threadIdx.x, cpg = (int)p.cpg;
+  const int64_t s = blockIdx.x / (unsigned)p.nseg;
+  const Slab<N, NT> a(p, s, blockIdx.x % (unsigned)p.nseg, 0);
   float* red = reinterpret_cast<float*>(smem + (((size_t)p.PR * p.cs * sizeof(T) + 15) & ~(size_t)15));
   float* gs = red + norm_red(p.cs, N, NT);             // [2][ng]
   float* stat = gs + 2 * p.ng;                         // [2][ng]: mean, rstd
@@ -268,8 +275,8 @@ __global__ void __launch_bounds__(NT) norm_fwd_resident(NormParams p) {
   }
   __syncthreads();
   group_sums<NT>(red, a.csl, a.rows, a.ngl, cpg, gs);
-  norm_barrier(R);
-  for (int g = tid; g < a.ngl; g += NT) stat[g] = cluster_total(gs, g, R) * inv_m;
+  __syncthreads();
+  for (int g = tid; g < a.ngl; g += NT) stat[g] = gs[g] * inv_m;
   __syncthreads();
 
   if (a.live()) {
@@ -292,35 +299,31 @@ __global__ void __launch_bounds__(NT) norm_fwd_resident(NormParams p) {
   }
   __syncthreads();
   group_sums<NT>(red, a.csl, a.rows, a.ngl, cpg, gs + p.ng);
-  norm_barrier(R);
+  __syncthreads();
   for (int g = tid; g < a.ngl; g += NT) {
-    const float rs = 1.f / sqrtf(cluster_total(gs + p.ng, g, R) * inv_m + p.eps);
+    const float rs = 1.f / sqrtf(gs[p.ng + g] * inv_m + p.eps);
     stat[p.ng + g] = rs;
-    if (rank == 0) {
-      p.mean[s * p.G + a.g0 + g] = stat[g];
-      p.rstd[s * p.G + a.g0 + g] = rs;
-    }
+    p.mean[s * p.G + a.g0 + g] = stat[g];
+    p.rstd[s * p.G + a.g0 + g] = rs;
   }
-  norm_barrier(R);                                     // peers are done with this CTA's gs; stat is visible
+  __syncthreads();
 
   if (a.live()) {
     T* out = reinterpret_cast<T*>(p.out);
     for (int col = a.tx; col < a.nv; col += a.TX) {
-      ChanConst<N> k;
+      ChanConst<N, sizeof(T) == 2> k;
       const int64_t c = a.c0 + (int64_t)col * N;
       k.load(p, c, [&](int i, float& mean, float& rstd) {
         const int g = (col * N + i) / cpg;
         mean = stat[g];
         rstd = stat[p.ng + g];
       });
-#pragma unroll
-      for (int i = 0; i < N; ++i) k.mul[i] *= k.gam[i];
 #pragma unroll 2
       for (int q = a.ty; q < a.np; q += a.TY) {
         float f[N];
         unpack<T, N>(tile[q * a.nv + col], f);
 #pragma unroll
-        for (int i = 0; i < N; ++i) f[i] = dense_act<ACT, sizeof(T) == 2>(fmaf(f[i] - k.sub[i], k.mul[i], k.bet[i]));
+        for (int i = 0; i < N; ++i) f[i] = dense_act<ACT, sizeof(T) == 2>(fmaf(k.h(f[i], i), k.gam[i], k.bet[i]));
         store_vec<T, N>(out + (s * p.P + a.q0 + q) * p.C + c, f);
       }
     }
@@ -328,33 +331,31 @@ __global__ void __launch_bounds__(NT) norm_fwd_resident(NormParams p) {
 }
 
 // ---- resident backward ----
-// A cluster keeps one segment and walks over samples, adding its dgamma / dbeta in shared memory; one partial
-// row per CTA goes to the join.
+// A block keeps one segment and walks over samples, adding its dgamma / dbeta in shared memory; one partial row per
+// block goes to the join.
 template <typename T, int N, int NT, int ACT, bool CKPT>
 __global__ void __launch_bounds__(NT) norm_bwd_resident(NormParams p) {
   extern __shared__ __align__(16) unsigned char smem[];
   const size_t tbytes = ((size_t)p.PR * p.cs * sizeof(T) + 15) & ~(size_t)15;
   Raw<T, N>* xt = reinterpret_cast<Raw<T, N>*>(smem);
   Raw<T, N>* dt = reinterpret_cast<Raw<T, N>*>(smem + tbytes);
-  const int tid = threadIdx.x, R = p.R, rank = blockIdx.x % R, cpg = (int)p.cpg;
-  const int64_t cluster = blockIdx.x / R, walkers = (gridDim.x / R) / p.nseg, walker = cluster / p.nseg;
+  const int tid = threadIdx.x, cpg = (int)p.cpg;
+  const int64_t walkers = gridDim.x / (unsigned)p.nseg, walker = blockIdx.x / (unsigned)p.nseg;
   const int64_t rf = norm_red(p.cs, N, NT);
   float* ra = reinterpret_cast<float*>(smem + 2 * tbytes);   // sum du h per channel
   float* rb = ra + rf;                                       // sum du per channel
   float* da = rb + rf;                                       // dgamma, dbeta of this CTA
   float* db = da + p.cs;
-  float* gs = db + p.cs;                                     // [2 parities][2][ng]
-  float* stat = gs + 4 * p.ng;                               // [2][ng]: mean(q), mean(q h)
+  float* gs = db + p.cs;                                     // [2][ng]
+  float* stat = gs + 2 * p.ng;                               // [2][ng]: mean(q), mean(q h)
   const float inv_m = 1.f / ((float)p.P * (float)cpg);
-  const Slab<N, NT> a(p, walker, cluster - walker * p.nseg, rank);
+  const Slab<N, NT> a(p, walker, blockIdx.x % (unsigned)p.nseg, 0);
   for (int c = tid; c < a.csl; c += NT) da[c] = db[c] = 0.f;
-  int par = 0;
-  for (int64_t s = walker; s < p.S; s += walkers, par ^= 1) {
-    float* gsp = gs + par * 2 * p.ng;
+  for (int64_t s = walker; s < p.S; s += walkers) {
     if (a.live()) {
       for (int col = a.tx; col < a.nv; col += a.TX) {
         float aa[N], ab[N];
-        ChanConst<N> k;
+        ChanConst<N, sizeof(T) == 2> k;
         const int64_t c = a.c0 + (int64_t)col * N;
         k.load(p, c, [&](int i, float& mean, float& rstd) {
           const int64_t g = s * p.G + a.g0 + (col * N + i) / cpg;
@@ -382,7 +383,7 @@ __global__ void __launch_bounds__(NT) norm_bwd_resident(NormParams p) {
             unpack<T, N>(rd[j], d);
 #pragma unroll
             for (int i = 0; i < N; ++i) {
-              const float h = (f[i] - k.sub[i]) * k.mul[i];
+              const float h = k.h(f[i], i);
               const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, k.gam[i], k.bet[i]));
               aa[i] = fmaf(du, h, aa[i]);
               ab[i] += du;
@@ -407,19 +408,19 @@ __global__ void __launch_bounds__(NT) norm_bwd_resident(NormParams p) {
       rb[c] = vb * gam;
     }
     __syncthreads();
-    group_sums<NT>(rb, a.csl, 1, a.ngl, cpg, gsp);
-    group_sums<NT>(ra, a.csl, 1, a.ngl, cpg, gsp + p.ng);
-    norm_barrier(R);
-    for (int g = tid; g < 2 * a.ngl; g += NT) {
-      const int j = g / a.ngl, gg = g - j * a.ngl;
-      stat[j * p.ng + gg] = cluster_total(gsp + j * p.ng, gg, R) * inv_m;
+    group_sums<NT>(rb, a.csl, 1, a.ngl, cpg, gs);
+    group_sums<NT>(ra, a.csl, 1, a.ngl, cpg, gs + p.ng);
+    __syncthreads();
+    for (int g = tid; g < a.ngl; g += NT) {
+      stat[g] = gs[g] * inv_m;
+      stat[p.ng + g] = gs[p.ng + g] * inv_m;
     }
     __syncthreads();
     if (a.live()) {
       T* out = reinterpret_cast<T*>(p.out);
       for (int col = a.tx; col < a.nv; col += a.TX) {
         float m1[N], m2[N];
-        ChanConst<N> k;
+        ChanConst<N, sizeof(T) == 2> k;
         const int64_t c = a.c0 + (int64_t)col * N;
         k.load(p, c, [&](int i, float& mean, float& rstd) {
           const int g = (col * N + i) / cpg;
@@ -435,7 +436,7 @@ __global__ void __launch_bounds__(NT) norm_bwd_resident(NormParams p) {
           unpack<T, N>(dt[q * a.nv + col], d);
 #pragma unroll
           for (int i = 0; i < N; ++i) {
-            const float h = (f[i] - k.sub[i]) * k.mul[i];
+            const float h = k.h(f[i], i);
             const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, k.gam[i], k.bet[i]));
             f[i] = k.mul[i] * (fmaf(du, k.gam[i], -m1[i]) - h * m2[i]);
           }
@@ -443,26 +444,99 @@ __global__ void __launch_bounds__(NT) norm_bwd_resident(NormParams p) {
         }
       }
     }
-    __syncthreads();                                   // ra / rb / stat / tiles free; gs alternates by parity
+    __syncthreads();                                   // shared memory is free for the next sample
   }
-  float* row = p.part + ((walker * R + rank) * 2) * p.C + a.c0;
+  float* row = p.part + walker * 2 * p.C + a.c0;
   for (int c = tid; c < a.csl; c += NT) {
     row[c] = da[c];
     row[p.C + c] = db[c];
   }
-  norm_barrier(R);                                     // no CTA leaves while a peer may still read its gs
 }
 
 // ---- streaming kernels: a block per (sample, chunk of positions, segment) ----
+// Blocks of 256 threads, kStatBlocks / kBwdBlocks to an SM (the registers of U loads in flight and the channels'
+// constants), and two whole waves of them.
+constexpr int kFwdBlocks = 4, kBwdBlocks = 3;
+
+// A thread's column of a [positions][channels] operand: element vectors `step` positions apart.
+template <typename T, int N>
+struct Column {
+  const T* p;
+  int64_t step;
+  __device__ __forceinline__ Column(const void* base, int64_t s, int64_t q, int64_t c, int64_t ss, int64_t ps, int TY)
+      : p(reinterpret_cast<const T*>(base) + s * ss + q * ps + c), step(ps * TY) {}
+  __device__ __forceinline__ Raw<T, N> at(int k) const { return *reinterpret_cast<const Raw<T, N>*>(p + k * step); }
+  __device__ __forceinline__ void next(int u) { p += u * step; }
+};
+// x, or its checkpoint.
+template <typename T, int N, bool CKPT>
+struct XColumn : Column<T, N> {
+  __device__ __forceinline__ XColumn(const NormParams& p, int64_t s, int64_t q, int64_t c, int TY)
+      : Column<T, N>(p.x, s, q, c, p.sx, p.px, TY) {}
+};
+template <typename T, int N>
+struct XColumn<T, N, true> {
+  const NormParams& p;
+  int64_t row, c;
+  int TY;
+  __device__ __forceinline__ XColumn(const NormParams& p_, int64_t s, int64_t q, int64_t c_, int TY_)
+      : p(p_), row(s * p_.P + q), c(c_), TY(TY_) {}
+  __device__ __forceinline__ Raw<T, N> at(int k) const { return read_codes<T, N>(p, row + k * TY, c); }
+  __device__ __forceinline__ void next(int u) { row += u * TY; }
+};
+
+// f(x values[, dy values], index of the position in the block) for every position of the thread's column, U positions'
+// loads in flight.
+template <int U, typename T, int N, typename X, typename F>
+__device__ __forceinline__ void walk(const Slab<N, 256>& a, X x, F f) {
+  for (int q = a.ty; q < a.np; q += U * a.TY, x.next(U)) {
+    Raw<T, N> r[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k)
+      if (q + k * a.TY < a.np) r[k] = x.at(k);
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (q + k * a.TY < a.np) {
+        float v[N];
+        unpack<T, N>(r[k], v);
+        f(v, q + k * a.TY);
+      }
+    }
+  }
+}
+template <int U, typename T, int N, typename X, typename D, typename F>
+__device__ __forceinline__ void walk(const Slab<N, 256>& a, X x, D d, F f) {
+  for (int q = a.ty; q < a.np; q += U * a.TY, x.next(U), d.next(U)) {
+    Raw<T, N> r[U], e[U];
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (q + k * a.TY < a.np) {
+        r[k] = x.at(k);
+        e[k] = d.at(k);
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      if (q + k * a.TY < a.np) {
+        float v[N], w[N];
+        unpack<T, N>(r[k], v);
+        unpack<T, N>(e[k], w);
+        f(v, w, q + k * a.TY);
+      }
+    }
+  }
+}
+
 template <int N, int NT>
-__device__ __forceinline__ Slab<N, NT> chunk_slab(const NormParams& p) {
-  const int64_t seg = blockIdx.x % p.nseg, sc = blockIdx.x / p.nseg, s = sc / p.chunks;
-  return Slab<N, NT>(p, s, seg, sc - s * p.chunks);
+__device__ __forceinline__ Slab<N, NT> chunk_slab(const NormParams& p, unsigned block) {
+  const unsigned nseg = (unsigned)p.nseg, chunks = (unsigned)p.chunks;   // 32-bit divisions: block numbers are
+  const unsigned sc = block / nseg, s = sc / chunks;
+  return Slab<N, NT>(p, s, block - sc * nseg, sc - s * chunks);
 }
 
 // This block's first entry in a chunk's row of gpart, and the number of elements behind entry (chunk, part).
-__device__ __forceinline__ int64_t entry0(const NormParams& p, int g0) {
-  return p.nsub == 1 ? g0 : (int64_t)(blockIdx.x % p.nseg);
+__device__ __forceinline__ int64_t entry0(const NormParams& p, int g0) {   // of the statistics kernels
+  return p.nsub == 1 ? g0 : (int64_t)(blockIdx.x % (unsigned)p.nseg);
 }
 __device__ __forceinline__ float entry_count(const NormParams& p, int64_t ch, int64_t part) {
   const int64_t c = p.nsub == 1 ? p.cpg : min((int64_t)p.subc, p.cpg - part * p.subc);
@@ -472,9 +546,9 @@ __device__ __forceinline__ float entry_count(const NormParams& p, int64_t ch, in
 // gpart[((s chunks + chunk) G + g) nsub + part] = (mean, sum of squared deviations) of the chunk's values of the group,
 // or of its part.
 template <typename T, int N, int NT>
-__global__ void __launch_bounds__(NT) norm_stats_kernel(NormParams p) {
+__global__ void __launch_bounds__(NT, kFwdBlocks) norm_stats_kernel(NormParams p) {
   extern __shared__ float sf[];
-  const Slab<N, NT> a = chunk_slab<N, NT>(p);
+  const Slab<N, NT> a = chunk_slab<N, NT>(p, blockIdx.x);
   const int64_t rf = norm_red(p.cs, N, NT);
   float* r1 = sf;
   float* r2 = sf + rf;
@@ -489,17 +563,14 @@ __global__ void __launch_bounds__(NT) norm_stats_kernel(NormParams p) {
       unpack<T, N>(read_x<T, N, false>(p, a.s, a.q0, c), k0);
 #pragma unroll
       for (int i = 0; i < N; ++i) s1[i] = s2[i] = 0.f;
-#pragma unroll 8
-      for (int q = a.ty; q < a.np; q += a.TY) {
-        float f[N];
-        unpack<T, N>(read_x<T, N, false>(p, a.s, a.q0 + q, c), f);
+      walk<4, T, N>(a, XColumn<T, N, false>(p, a.s, a.q0 + a.ty, c, a.TY), [&](const float (&f)[N], int) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
           const float d = f[i] - k0[i];
           s1[i] += d;
           s2[i] = fmaf(d, d, s2[i]);
         }
-      }
+      });
       a.put(s1, r1, col);
       a.put(s2, r2, col);
     }
@@ -526,33 +597,34 @@ __global__ void __launch_bounds__(NT) norm_stats_kernel(NormParams p) {
   __syncthreads();
   group_sums<NT>(r2, a.csl, 1, a.ngl, cpg, gv);
   __syncthreads();
-  float2* out = reinterpret_cast<float2*>(p.gpart) + (a.s * p.chunks + a.q0 / p.PR) * p.G * p.nsub + entry0(p, a.g0);
+  float2* out = reinterpret_cast<float2*>(p.gpart) + (a.s * p.chunks + a.at) * p.G * p.nsub + entry0(p, a.g0);
   for (int g = threadIdx.x; g < a.ngl; g += NT) out[g] = make_float2(gm[g] / (float)cpg, gv[g]);
 }
 
 // The groups' statistics from the chunks' (every block the same sums), then act(h gamma + beta).
 template <typename T, int N, int NT, int ACT>
-__global__ void __launch_bounds__(NT) norm_apply_kernel(NormParams p) {
+__global__ void __launch_bounds__(NT, kFwdBlocks) norm_apply_kernel(NormParams p) {
   extern __shared__ float sf[];
-  const Slab<N, NT> a = chunk_slab<N, NT>(p);
+  const Slab<N, NT> a = chunk_slab<N, NT>(p, gridDim.x - 1 - blockIdx.x);
   const int cpg = a.cpg, lane = threadIdx.x & 31;
   float* mean = sf;                                     // [ng]
   float* rstd = sf + p.ng;
   const float2* part = reinterpret_cast<const float2*>(p.gpart) + (a.s * p.chunks * p.G + a.g0) * p.nsub;
   const float m = (float)p.P * (float)p.cpg;
+  const int entries = (int)(p.chunks * p.nsub);
   for (int g = threadIdx.x >> 5; g < a.ngl; g += NT / 32) {
     float v = 0.f;
-    for (int64_t j = lane; j < p.chunks * p.nsub; j += 32) {
-      const int64_t ch = j / p.nsub;
-      v = fmaf(part[(ch * p.G + g) * p.nsub + (j - ch * p.nsub)].x, entry_count(p, ch, j - ch * p.nsub), v);
+    for (int j = lane; j < entries; j += 32) {
+      const int ch = j / p.nsub;
+      v = fmaf(part[((int64_t)ch * p.G + g) * p.nsub + (j - ch * p.nsub)].x, entry_count(p, ch, j - ch * p.nsub), v);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
     const float mu = v / m;
     v = 0.f;
-    for (int64_t j = lane; j < p.chunks * p.nsub; j += 32) {
-      const int64_t ch = j / p.nsub;
-      const float2 t = part[(ch * p.G + g) * p.nsub + (j - ch * p.nsub)];
+    for (int j = lane; j < entries; j += 32) {
+      const int ch = j / p.nsub;
+      const float2 t = part[((int64_t)ch * p.G + g) * p.nsub + (j - ch * p.nsub)];
       v += fmaf((t.x - mu) * (t.x - mu), entry_count(p, ch, j - ch * p.nsub), t.y);
     }
 #pragma unroll
@@ -571,31 +643,34 @@ __global__ void __launch_bounds__(NT) norm_apply_kernel(NormParams p) {
   if (!a.live()) return;
   T* out = reinterpret_cast<T*>(p.out);
   for (int col = a.tx; col < a.nv; col += a.TX) {
-    ChanConst<N> k;
+    // u = (x - sub) mul + add, with the mean folded into add for bf16 x (one operation less; its own rounding is 2^15
+    // times larger than what that costs)
+    float mul[N], sub[N], add[N], gam[N];
     const int64_t c = a.c0 + (int64_t)col * N;
-    k.load(p, c, [&](int i, float& m, float& r) {
+    ld_params<N>(p.w, c, p.pdtype, 1.f, gam);
+    ld_params<N>(p.b, c, p.pdtype, 0.f, add);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
       const int g = (col * N + i) / cpg;
-      m = mean[g];
-      r = rstd[g];
-    });
-#pragma unroll
-    for (int i = 0; i < N; ++i) k.mul[i] *= k.gam[i];
-#pragma unroll 4
-    for (int q = a.ty; q < a.np; q += a.TY) {
-      float f[N];
-      unpack<T, N>(read_x<T, N, false>(p, a.s, a.q0 + q, c), f);
-#pragma unroll
-      for (int i = 0; i < N; ++i) f[i] = dense_act<ACT, sizeof(T) == 2>(fmaf(f[i] - k.sub[i], k.mul[i], k.bet[i]));
-      store_vec<T, N>(out + (a.s * p.P + a.q0 + q) * p.C + c, f);
+      mul[i] = rstd[g] * gam[i];
+      sub[i] = mean[g];
+      if constexpr (sizeof(T) == 2) add[i] = fmaf(-sub[i], mul[i], add[i]);
     }
+    T* to = out + (a.s * p.P + a.q0) * p.C + c;
+    walk<4, T, N>(a, XColumn<T, N, false>(p, a.s, a.q0 + a.ty, c, a.TY), [&](float (&f)[N], int q) {
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        f[i] = dense_act<ACT, sizeof(T) == 2>(fmaf(sizeof(T) == 2 ? f[i] : f[i] - sub[i], mul[i], add[i]));
+      store_vec<T, N>(to + q * p.C, f);
+    });
   }
 }
 
 // Per chunk: dgamma and dbeta partial rows, and each group's sums of q and q h in gpart.
 template <typename T, int N, int NT, int ACT, bool CKPT>
-__global__ void __launch_bounds__(NT) norm_bwd_stats_kernel(NormParams p) {
+__global__ void __launch_bounds__(NT, kBwdBlocks) norm_bwd_stats_kernel(NormParams p) {
   extern __shared__ float sf[];
-  const Slab<N, NT> a = chunk_slab<N, NT>(p);
+  const Slab<N, NT> a = chunk_slab<N, NT>(p, blockIdx.x);
   const int64_t rf = norm_red(p.cs, N, NT);
   float* ra = sf;
   float* rb = sf + rf;
@@ -604,35 +679,38 @@ __global__ void __launch_bounds__(NT) norm_bwd_stats_kernel(NormParams p) {
   const int cpg = a.cpg;
   if (a.live()) {
     for (int col = a.tx; col < a.nv; col += a.TX) {
-      float aa[N], ab[N];
-      ChanConst<N> k;
+      // xc = x - mean, u = xc mul gamma + beta; sum du xc is scaled by rstd at the end
+      float aa[N], ab[N], sub[N], ga[N], bet[N], mul[N];
       const int64_t c = a.c0 + (int64_t)col * N;
-      k.load(p, c, [&](int i, float& mean, float& rstd) {
-        const int64_t g = a.s * p.G + a.g0 + (col * N + i) / cpg;
-        mean = p.mean[g];
-        rstd = p.rstd[g];
-      });
+      ld_params<N>(p.w, c, p.pdtype, 1.f, ga);
+      ld_params<N>(p.b, c, p.pdtype, 0.f, bet);
 #pragma unroll
-      for (int i = 0; i < N; ++i) aa[i] = ab[i] = 0.f;
-#pragma unroll 2
-      for (int q = a.ty; q < a.np; q += a.TY) {
-        float f[N], d[N];
-        unpack<T, N>(read_x<T, N, CKPT>(p, a.s, a.q0 + q, c), f);
-        unpack<T, N>(read_dy<T, N>(p, a.s, a.q0 + q, c), d);
+      for (int i = 0; i < N; ++i) {
+        const int64_t g = a.s * p.G + a.g0 + (col * N + i) / cpg;
+        sub[i] = p.mean[g];
+        mul[i] = p.rstd[g];
+        ga[i] *= mul[i];
+        aa[i] = ab[i] = 0.f;
+      }
+      walk<2, T, N>(a, XColumn<T, N, CKPT>(p, a.s, a.q0 + a.ty, c, a.TY),
+                    Column<T, N>(p.dy, a.s, a.q0 + a.ty, c, p.sdy, p.pdy, a.TY),
+                    [&](const float (&f)[N], const float (&d)[N], int) {
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const float h = (f[i] - k.sub[i]) * k.mul[i];
-          const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, k.gam[i], k.bet[i]));
-          aa[i] = fmaf(du, h, aa[i]);
+          const float xc = f[i] - sub[i];
+          const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(xc, ga[i], bet[i]));
+          aa[i] = fmaf(du, xc, aa[i]);
           ab[i] += du;
         }
-      }
+      });
+#pragma unroll
+      for (int i = 0; i < N; ++i) aa[i] *= mul[i];
       a.put(aa, ra, col);
       a.put(ab, rb, col);
     }
   }
   __syncthreads();
-  const int64_t chunk = a.s * p.chunks + a.q0 / p.PR;
+  const int64_t chunk = a.s * p.chunks + a.at;
   float* row = p.part + chunk * 2 * p.C + a.c0;
   for (int c = threadIdx.x; c < a.csl; c += NT) {
     float va = 0.f, vb = 0.f;
@@ -690,23 +768,24 @@ __global__ void __launch_bounds__(512) norm_param_join_kernel(const float* part,
 
 // The groups' means of q and q h from the chunks', then dx; blocks past p.blocks join dgamma / dbeta.
 template <typename T, int N, int NT, int ACT, bool CKPT>
-__global__ void __launch_bounds__(NT) norm_bwd_apply_kernel(NormParams p) {
+__global__ void __launch_bounds__(NT, kBwdBlocks) norm_bwd_apply_kernel(NormParams p) {
   extern __shared__ float sf[];
   if ((int64_t)blockIdx.x >= p.blocks) {
     param_join(p.part, p.npart, p.C, ((int64_t)blockIdx.x - p.blocks) * 32, p.dw, p.db, p.pdtype, p.accumulate, sf,
                NT / 32);
     return;
   }
-  const Slab<N, NT> a = chunk_slab<N, NT>(p);
+  const Slab<N, NT> a = chunk_slab<N, NT>(p, (unsigned)p.blocks - 1 - blockIdx.x);
   const int cpg = a.cpg, lane = threadIdx.x & 31;
   float* s1 = sf;                                       // [ng] mean(q), mean(q h)
   float* s2 = sf + p.ng;
   const float2* part = reinterpret_cast<const float2*>(p.gpart) + (a.s * p.chunks * p.G + a.g0) * p.nsub;
+  const int entries = (int)(p.chunks * p.nsub);
   for (int g = threadIdx.x >> 5; g < a.ngl; g += NT / 32) {
     float v1 = 0.f, v2 = 0.f;
-    for (int64_t j = lane; j < p.chunks * p.nsub; j += 32) {
-      const int64_t ch = j / p.nsub;
-      const float2 t = part[(ch * p.G + g) * p.nsub + (j - ch * p.nsub)];
+    for (int j = lane; j < entries; j += 32) {
+      const int ch = j / p.nsub;
+      const float2 t = part[((int64_t)ch * p.G + g) * p.nsub + (j - ch * p.nsub)];
       v1 += t.x;
       v2 += t.y;
     }
@@ -725,29 +804,32 @@ __global__ void __launch_bounds__(NT) norm_bwd_apply_kernel(NormParams p) {
   if (!a.live()) return;
   T* out = reinterpret_cast<T*>(p.out);
   for (int col = a.tx; col < a.nv; col += a.TX) {
-    float m1[N], m2[N];
-    ChanConst<N> k;
+    // xc = x - mean, u = xc ga + beta with ga = rstd gamma, dx = du ga - xc rstd^2 mean(q h) - rstd mean(q)
+    float sub[N], ga[N], bet[N], bx[N], cc[N];
     const int64_t c = a.c0 + (int64_t)col * N;
-    k.load(p, c, [&](int i, float& mean, float& rstd) {
+    ld_params<N>(p.w, c, p.pdtype, 1.f, ga);
+    ld_params<N>(p.b, c, p.pdtype, 0.f, bet);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
       const int g = (col * N + i) / cpg;
-      mean = p.mean[a.s * p.G + a.g0 + g];
-      rstd = p.rstd[a.s * p.G + a.g0 + g];
-      m1[i] = s1[g];
-      m2[i] = s2[g];
-    });
-#pragma unroll 2
-    for (int q = a.ty; q < a.np; q += a.TY) {
-      float f[N], d[N];
-      unpack<T, N>(read_x<T, N, CKPT>(p, a.s, a.q0 + q, c), f);
-      unpack<T, N>(read_dy<T, N>(p, a.s, a.q0 + q, c), d);
+      const float rs = p.rstd[a.s * p.G + a.g0 + g];
+      sub[i] = p.mean[a.s * p.G + a.g0 + g];
+      ga[i] *= rs;
+      bx[i] = -rs * rs * s2[g];
+      cc[i] = -rs * s1[g];
+    }
+    T* to = out + (a.s * p.P + a.q0) * p.C + c;
+    walk<2, T, N>(a, XColumn<T, N, CKPT>(p, a.s, a.q0 + a.ty, c, a.TY),
+                  Column<T, N>(p.dy, a.s, a.q0 + a.ty, c, p.sdy, p.pdy, a.TY),
+                  [&](float (&f)[N], const float (&d)[N], int q) {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        const float h = (f[i] - k.sub[i]) * k.mul[i];
-        const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(h, k.gam[i], k.bet[i]));
-        f[i] = k.mul[i] * (fmaf(du, k.gam[i], -m1[i]) - h * m2[i]);
+        const float xc = f[i] - sub[i];
+        const float du = d[i] * dense_slope<ACT, sizeof(T) == 2>(fmaf(xc, ga[i], bet[i]));
+        f[i] = fmaf(du, ga[i], fmaf(xc, bx[i], cc[i]));
       }
-      store_vec<T, N>(out + (a.s * p.P + a.q0 + q) * p.C + c, f);
-    }
+      store_vec<T, N>(to + q * p.C, f);
+    });
   }
 }
 
@@ -929,7 +1011,7 @@ __global__ void __launch_bounds__(32 * kRowWarps) norm_bwd_rows(NormParams p) {
 // ---- host ----
 enum { kNormRows, kNormResident, kNormStream };
 struct NormPlan {
-  int kind, N, NT, ng, cs, R, L, V, nsub, subc;
+  int kind, N, NT, ng, cs, L, V, nsub, subc;
   int64_t nseg, PR, chunks, walkers, npart, gparts;   // gparts: floats of gpart
   size_t smem;
 };
@@ -937,9 +1019,9 @@ struct NormPlan {
 // Which family, and its sizes.
 //  rows       P = 1, aligned, a group of at most 8 vectors a lane (measured at 1024 x 4096 fp32 in 64 groups: forward
 //             and backward 36 + 79 us resident, without it)
-//  resident   a segment fits a cluster, and either its CTAs are many or the tensor is too large for the streaming
-//             kernels' second read to come from L2.  A segment is at least 128 bytes of channels (a full line per
-//             position), wider while there are more than four segments for each SM; vectors do not straddle segments.
+//  resident   a segment's positions fit a block's shared memory.  A segment is at least 128 bytes of channels (a full
+//             line per position), wider while there are more than four segments for each SM; vectors do not straddle
+//             segments.
 //  streaming  otherwise
 static NormPlan norm_plan(int64_t S, int64_t P, int64_t C, int64_t G, int esize, bool vec, bool bwd, int sms,
                           int smem_max) {
@@ -976,38 +1058,34 @@ static NormPlan norm_plan(int64_t S, int64_t P, int64_t C, int64_t G, int esize,
   pl.ng = (int)ng;
   const int64_t cs = ng * cpg;
   pl.nseg = (G + ng - 1) / ng;
-  const bool large = S * P * C * esize * tiles > (int64_t)48 << 20;
-  if (cs <= (1 << 20)) {
+  if (cs <= (1 << 20) && P <= (1 << 20)) {
     pl.cs = (int)cs;
-    for (int64_t cap : {(int64_t)(smem_max / 2 - 1024), (int64_t)smem_max}) {
-      for (int R = 1; R <= kNormMaxCluster; R *= 2) {
-        const int64_t PR = (P + R - 1) / R, tile = tiles * ((PR * cs * esize + 15) / 16 * 16);
-        if (PR > (1 << 20) || tile > cap) continue;
-        const int NT = vec && tile > 32768 ? 512 : 256;
-        const int64_t red = norm_red(cs, pl.N, NT);
-        const int64_t bytes = tile + 4 * (bwd ? 2 * red + 2 * cs + 6 * ng : red + 4 * ng) + 32;
-        if (bytes > cap) continue;
-        if (R > 1 && !large) break;               // a cluster's barriers cost more than a second read from L2
-        pl.kind = kNormResident;
-        pl.R = R;
-        pl.PR = PR;
-        pl.NT = NT;
-        pl.smem = (size_t)bytes;
-        int64_t per_sm = (smem_max + 1024) / (bytes + 1024);
-        if (per_sm > 2048 / NT) per_sm = 2048 / NT;
-        const int64_t want = (sms * per_sm + R * pl.nseg - 1) / (R * pl.nseg);
-        pl.walkers = S < want ? S : want;
-        pl.npart = pl.walkers * R;
-        return pl;
-      }
+    const int64_t tile = tiles * ((P * cs * esize + 15) / 16 * 16);
+    const int NT = vec && tile > 32768 ? 512 : 256;
+    const int64_t red = norm_red(cs, pl.N, NT);
+    const int64_t bytes = tile + 4 * (bwd ? 2 * red + 2 * cs + 4 * ng : red + 4 * ng) + 32;
+    if (tile <= smem_max && bytes <= smem_max) {
+      pl.kind = kNormResident;
+      pl.PR = P;
+      pl.NT = NT;
+      pl.smem = (size_t)bytes;
+      int64_t per_sm = (smem_max + 1024) / (bytes + 1024);
+      if (per_sm > 2048 / NT) per_sm = 2048 / NT;
+      const int64_t want = (sms * per_sm + pl.nseg - 1) / pl.nseg;
+      pl.walkers = S < want ? S : want;
+      pl.npart = pl.walkers;
+      return pl;
     }
   }
-  // streaming: about 6 blocks per SM, at least 16 positions each where there are that many; groups too wide for a
-  // block's sums in parts of 4096 channels
+  // streaming: two waves of blocks, at least 16 positions each where there are that many; groups too wide for a block's
+  // sums in parts of 4096 channels
   pl.kind = kNormStream;
   pl.NT = 256;
-  pl.cs = (int)cs;
-  if (cs > 16384) {
+  while (ng + unit <= G && (ng + unit) * cpg <= 256 * pl.N) ng += unit;   // whole rows where they fit a row of threads
+  pl.ng = (int)ng;
+  pl.cs = (int)(ng * cpg);
+  pl.nseg = (G + ng - 1) / ng;
+  if (ng * cpg > 16384) {
     if (cpg % pl.N) pl.N = 1;      // parts start where groups do
     ng = 1;
     pl.subc = 4096;
@@ -1016,7 +1094,8 @@ static NormPlan norm_plan(int64_t S, int64_t P, int64_t C, int64_t G, int esize,
     pl.ng = 1;
     pl.nseg = G * pl.nsub;
   }
-  int64_t chunks = (6 * (int64_t)sms + S * pl.nseg - 1) / (S * pl.nseg);
+  int64_t chunks = 2 * (int64_t)sms * (bwd ? kBwdBlocks : kFwdBlocks) / (S * pl.nseg);
+  if (chunks < 1) chunks = 1;
   const int64_t most = (P + 15) / 16;
   if (chunks > most) chunks = most;
   pl.PR = (P + chunks - 1) / chunks;
@@ -1045,21 +1124,11 @@ static bool vec_rows(const void* p, int64_t a, int64_t b, int64_t C, int esize) 
 }
 
 template <typename K>
-static int launch_cluster(K kernel, const NormParams& p, int64_t blocks, int threads, int R, size_t smem, cudaStream_t st) {
+static int launch_norm(K kernel, const NormParams& p, int64_t blocks, int threads, size_t smem, cudaStream_t st) {
   if (blocks > 0x7FFFFFFF) return GL_ERR_SHAPE;
   if (int rc = ensure_dynamic_smem((const void*)kernel, smem)) return rc;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)blocks);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim.x = (unsigned)R;
-  at.val.clusterDim.y = at.val.clusterDim.z = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = R > 1 ? 1 : 0;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+  kernel<<<(unsigned)blocks, (unsigned)threads, smem, st>>>(p);
+  const cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return set_cuda_error(e);
   count_launches(1);
   return GL_OK;
@@ -1093,19 +1162,19 @@ static int run_norm_fwd_act(NormParams& p, const NormPlan& pl, cudaStream_t st) 
     if (pl.kind == kNormRows) {
       int rc = GL_ERR_UNSUPPORTED;
       with_row_shape<8>(pl.L, pl.V, [&](auto l, auto v) {
-        rc = launch_cluster(norm_fwd_rows<T, N, decltype(l)::value, decltype(v)::value, ACT>, p, pl.nseg * pl.walkers,
-                            32 * kRowWarps, 1, 0, st);
+        rc = launch_norm(norm_fwd_rows<T, N, decltype(l)::value, decltype(v)::value, ACT>, p, pl.nseg * pl.walkers,
+                         32 * kRowWarps, 0, st);
       });
       return rc;
     }
     if (pl.kind == kNormResident && pl.NT == 512)
-      return launch_cluster(norm_fwd_resident<T, N, 512, ACT>, p, p.S * pl.nseg * pl.R, 512, pl.R, pl.smem, st);
+      return launch_norm(norm_fwd_resident<T, N, 512, ACT>, p, p.S * pl.nseg, 512, pl.smem, st);
   }
   if (pl.kind == kNormResident)
-    return launch_cluster(norm_fwd_resident<T, N, 256, ACT>, p, p.S * pl.nseg * pl.R, 256, pl.R, pl.smem, st);
+    return launch_norm(norm_fwd_resident<T, N, 256, ACT>, p, p.S * pl.nseg, 256, pl.smem, st);
   const int64_t blocks = p.S * pl.chunks * pl.nseg;
-  if (int rc = launch_cluster(norm_stats_kernel<T, N, 256>, p, blocks, 256, 1, pl.smem, st)) return rc;
-  return launch_cluster(norm_apply_kernel<T, N, 256, ACT>, p, blocks, 256, 1, pl.smem, st);
+  if (int rc = launch_norm(norm_stats_kernel<T, N, 256>, p, blocks, 256, pl.smem, st)) return rc;
+  return launch_norm(norm_apply_kernel<T, N, 256, ACT>, p, blocks, 256, pl.smem, st);
 }
 
 template <typename T, int N>
@@ -1122,22 +1191,22 @@ static int run_norm_bwd_act(NormParams& p, const NormPlan& pl, cudaStream_t st) 
   if (pl.kind == kNormStream) {
     p.blocks = p.S * pl.chunks * pl.nseg;
     const size_t smem = pl.smem < 8 * 2 * 33 * 4 ? 8 * 2 * 33 * 4 : pl.smem;
-    rc = launch_cluster(norm_bwd_stats_kernel<T, N, 256, ACT, CKPT>, p, p.blocks, 256, 1, pl.smem, st);
+    rc = launch_norm(norm_bwd_stats_kernel<T, N, 256, ACT, CKPT>, p, p.blocks, 256, pl.smem, st);
     if (rc) return rc;
-    return launch_cluster(norm_bwd_apply_kernel<T, N, 256, ACT, CKPT>, p, p.blocks + joins, 256, 1, smem, st);
+    return launch_norm(norm_bwd_apply_kernel<T, N, 256, ACT, CKPT>, p, p.blocks + joins, 256, smem, st);
   }
   if constexpr (N > 1) {
     if (pl.kind == kNormRows) {
       with_row_shape<4>(pl.L, pl.V, [&](auto l, auto v) {
-        rc = launch_cluster(norm_bwd_rows<T, N, decltype(l)::value, decltype(v)::value, ACT, CKPT>, p,
-                            pl.nseg * pl.walkers, 32 * kRowWarps, 1, pl.smem, st);
+        rc = launch_norm(norm_bwd_rows<T, N, decltype(l)::value, decltype(v)::value, ACT, CKPT>, p,
+                            pl.nseg * pl.walkers, 32 * kRowWarps, pl.smem, st);
       });
     } else if (pl.NT == 512) {
-      rc = launch_cluster(norm_bwd_resident<T, N, 512, ACT, CKPT>, p, pl.walkers * pl.nseg * pl.R, 512, pl.R, pl.smem, st);
+      rc = launch_norm(norm_bwd_resident<T, N, 512, ACT, CKPT>, p, pl.walkers * pl.nseg, 512, pl.smem, st);
     }
   }
   if (pl.kind == kNormResident && pl.NT == 256)
-    rc = launch_cluster(norm_bwd_resident<T, N, 256, ACT, CKPT>, p, pl.walkers * pl.nseg * pl.R, 256, pl.R, pl.smem, st);
+    rc = launch_norm(norm_bwd_resident<T, N, 256, ACT, CKPT>, p, pl.walkers * pl.nseg, 256, pl.smem, st);
   if (rc || !joins) return rc;
   norm_param_join_kernel<<<(unsigned)joins, 512, 0, st>>>(p.part, pl.npart, p.C, p.dw, p.db, p.pdtype, p.accumulate);
   const cudaError_t e = cudaGetLastError();
@@ -1204,7 +1273,7 @@ extern "C" int gl_norm_fwd(const GlNormArgs* args, void* stream) {
   NormParams p{};
   p.x = a.x; p.w = a.w; p.b = a.b; p.out = a.y; p.mean = a.mean; p.rstd = a.rstd; p.gpart = (float*)a.work;
   p.S = a.S; p.P = a.P; p.C = a.C; p.G = a.G; p.cpg = a.C / a.G; p.sx = a.sx; p.px = a.px;
-  p.nseg = pl.nseg; p.PR = pl.PR; p.chunks = pl.chunks; p.ng = pl.ng; p.cs = pl.cs; p.R = pl.R;
+  p.nseg = pl.nseg; p.PR = pl.PR; p.chunks = pl.chunks; p.ng = pl.ng; p.cs = pl.cs;
   p.nsub = pl.nsub; p.subc = pl.subc;
   p.pdtype = a.pdtype; p.eps = a.eps;
   cudaStream_t st = (cudaStream_t)stream;
@@ -1238,7 +1307,7 @@ extern "C" int gl_norm_bwd(const GlNormBwdArgs* args, void* stream) {
   p.gpart = p.part + pl.npart * 2 * a.C; p.dw = a.dw; p.db = a.db; p.accumulate = a.accumulate;
   p.S = a.S; p.P = a.P; p.C = a.C; p.G = a.G; p.cpg = a.C / a.G; p.sx = a.sx; p.px = a.px; p.sdy = a.sdy;
   p.pdy = a.pdy; p.ldc = a.ldc; p.nblk = nblk; p.nseg = pl.nseg; p.npart = pl.npart; p.PR = pl.PR;
-  p.chunks = pl.chunks; p.ng = pl.ng; p.cs = pl.cs; p.R = pl.R;
+  p.chunks = pl.chunks; p.ng = pl.ng; p.cs = pl.cs;
   p.nsub = pl.nsub; p.subc = pl.subc; p.pdtype = a.pdtype;
   if (a.dtype == GL_DTYPE_F32) {
     if (ckpt) return pl.N > 1 ? run_norm_bwd<float, 4, true>(p, a.act, pl, st) : run_norm_bwd<float, 1, true>(p, a.act, pl, st);

@@ -91,8 +91,8 @@ class Activation8:
 def _encode(x2: torch.Tensor):
     rows, C = x2.shape
     nblk = -(-C // BLOCK)
-    codes = torch.empty((rows, nblk * BLOCK), dtype=torch.int8, device=x2.device)
-    exps = torch.empty((rows, nblk), dtype=torch.uint8, device=x2.device)
+    codes = x2.new_empty((rows, nblk * BLOCK), dtype=torch.int8)
+    exps = x2.new_empty((rows, nblk), dtype=torch.uint8)
     if rows:
         _native.act8_encode(x2, codes, exps)
     return codes, exps
@@ -167,8 +167,7 @@ class LinearActFunction(torch.autograd.Function):
         x2, w2 = _rows(x, K), _rows(weight, K)
         slope = codes = exps = None
         if act != 0:
-            slope = torch.empty((x2.shape[0], N), device=x.device,
-                                dtype=torch.uint8 if checkpoint == "int8" else _SLOPE_DTYPES[x.dtype])
+            slope = x2.new_empty((x2.shape[0], N), dtype=torch.uint8 if checkpoint == "int8" else _SLOPE_DTYPES[x.dtype])
         y = _linear_forward(x2, w2, bias, None if residual is None else _rows(residual, N), act, slope)
         if checkpoint == "int8":
             codes, exps = _encode(x2)
@@ -214,9 +213,17 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
     activation's derivative in 8 bits for the backward pass.  All tensors share one dtype (float32 or bfloat16;
     float32 products run as exact three-term bf16 splits on the tensor cores, or in fp32 for a few rows).
     Parameters with a ``main_grad`` receive their gradients there."""
-    act = _act_id(activation)
-    _check_checkpoint(checkpoint)
-    _check_linear(x, weight, bias, residual)
+    act = _ACT_IDS.get(activation)
+    xs, ws, dt, dev = x.shape, weight.shape, x.dtype, x.device
+    # one expression for what is right; the exact complaint is _check_linear's
+    if not (act is not None and checkpoint in CHECKPOINTS and dt in _DTYPES and x.is_cuda and len(ws) == 2 and
+            len(xs) > 0 and xs[-1] == ws[1] and 0 not in ws and weight.dtype == dt and weight.device == dev and
+            (bias is None or bias.shape == ws[:1] and bias.dtype == dt and bias.device == dev and bias.is_contiguous())
+            and (residual is None or residual.shape == xs[:-1] + ws[:1] and residual.dtype == dt and
+                 residual.device == dev)):
+        _act_id(activation)
+        _check_checkpoint(checkpoint)
+        _check_linear(x, weight, bias, residual)
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or
                                     bias is not None and bias.requires_grad or
                                     residual is not None and residual.requires_grad):
@@ -243,8 +250,8 @@ def _positions(t: torch.Tensor, S: int, P: int, C: int) -> torch.Tensor:
 
 def _norm_forward(x, num_groups, weight, bias, act, eps):
     S, C = x.shape[0], x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, S, num_groups), dtype=torch.float32, device=x.device)   # mean, rstd
+    y = x.new_empty(x.shape)
+    stats = x.new_empty((2, S, num_groups), dtype=torch.float32)   # mean, rstd
     x3 = None
     n = x.numel()
     if n:
@@ -270,7 +277,7 @@ class GroupNormActFunction(torch.autograd.Function):
         _no_double_backward("group_norm_act")
         x3, codes, exps, weight, bias, stats = ctx.saved_tensors
         _, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = torch.empty(dy.shape, dtype=dy.dtype, device=dy.device)
+        dx = dy.new_empty(dy.shape)
         dw, db, main = _grad_buffers(weight, need_w, bias, need_b)
         S, C = dy.shape[0], dy.shape[-1]
         if dx.numel():
@@ -307,9 +314,18 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
     Statistics (mean, biased variance) run over a sample's positions and each of ``num_groups`` groups of
     consecutive channels; with x [S, C] that is per token.  ``weight`` and ``bias`` [C] are float32 or bfloat16 (one
     dtype for both), whatever x's.  ``activation`` and ``checkpoint`` as in ``linear_act``."""
-    act = _act_id(activation)
-    _check_checkpoint(checkpoint)
-    _check_norm(x, num_groups, weight, bias, eps)
+    act = _ACT_IDS.get(activation)
+    xs, dev = x.shape, x.device
+    ptype = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
+    # one expression for what is right; the exact complaint is _check_norm's
+    if not (act is not None and checkpoint in CHECKPOINTS and x.dtype in _DTYPES and ptype in _DTYPES and x.is_cuda and
+            len(xs) > 1 and num_groups > 0 and xs[-1] > 0 and xs[-1] % num_groups == 0 and eps > 0 and
+            (weight is None or weight.shape == xs[-1:] and weight.device == dev and weight.is_contiguous()) and
+            (bias is None or bias.shape == xs[-1:] and bias.dtype == ptype and bias.device == dev and
+             bias.is_contiguous())):
+        _act_id(activation)
+        _check_checkpoint(checkpoint)
+        _check_norm(x, num_groups, weight, bias, eps)
     if torch.is_grad_enabled() and (x.requires_grad or weight is not None and weight.requires_grad or
                                     bias is not None and bias.requires_grad):
         return GroupNormActFunction.apply(x, weight, bias, num_groups, act, eps, checkpoint)
