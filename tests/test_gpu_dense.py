@@ -553,3 +553,22 @@ def test_norm_refusals():
             gl.group_norm_act(*args, **kw)
     with pytest.raises(_native.NativeLibraryError):
         gl.group_norm_act(x.cpu(), 4)
+
+
+# ---- together ----
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_block_trains_with_and_without_checkpoints(dtype):
+    """norm -> linear -> sparse pooling -> linear + residual: with either form of saved activations steps of the
+    optimizer descend, and the first loss, before any gradient, is the same."""
+    import importlib.util
+    from pathlib import Path
+
+    spec = importlib.util.spec_from_file_location("dense_block", Path(__file__).resolve().parent.parent / "examples" /
+                                                  "dense_block.py")
+    mod = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(mod)
+    plain = mod.train("none", dtype, steps=12)
+    kept = mod.train("int8", dtype, steps=12)
+    assert plain[-1] < plain[0] and kept[-1] < kept[0]
+    assert kept[0] == plain[0]                                  # the forward pass does not change
