@@ -13,9 +13,11 @@
 // rate, bounds the 128 x 256 tile of one CTA.
 //
 // fp32 operands come as three bf16 planes; a slot holds plane i of both, and the products of term pairs (i, j),
-// i + j <= 2, run smallest first.  The tensor core's fp32 accumulation truncates, so with several planes a sum over
-// k is cut into chunks of 128: each chunk's accumulator is added to registers in fp32 (rounding to nearest) while the
-// next one runs.  At K = 4096 chunks of 512 were 3.9e-6 off in the 2-norm (plain fp32 products: 1.0e-6).
+// i + j <= 2, run as their slots arrive.  The tensor core's fp32 accumulation truncates, so the pair (0, 0) has an
+// accumulator of its own that the five small pairs (2^-8 of its size and less) do not disturb, and a sum over k is
+// cut into chunks of 512: each chunk's accumulators are added to registers in fp32 (rounding to nearest) while the
+// next one runs.  (One accumulator for all pairs needed chunks of 128 for 0.8e-6 in the 2-norm at K = 4096, where plain
+// fp32 products are 1.0e-6 off, and reading it that often cost a fifth of the time.)
 //
 // K-major tiles are one TMA box (64 k wide, all rows of the tile); MN-major tiles are boxes of 64 rows by 64 k, which
 // the matrix descriptor walks with 2048 bytes per 16 k and 8192 bytes per 64 rows.  Edges in every dimension are
@@ -108,8 +110,14 @@ __device__ __forceinline__ bool mm_wait(MmaShared& sh, uint64_t& bar, uint32_t p
   return false;
 }
 
+// For a whole warp: the same answer in every lane.
+__device__ __forceinline__ bool mm_wait_warp(MmaShared& sh, uint64_t& bar, uint32_t parity) {
+  return __all_sync(kFullMask, mm_wait(sh, bar, parity));
+}
+
 // One lane of a converged warp.  elect.sync rather than lane == 0: the compiler then knows that one thread issues the
-// tensor instructions and need not loop over the active ones (8192 x 4096 x 4096: 254 -> 210 us).
+// tensor instructions and need not loop over the active ones (8192 x 4096 x 4096: 254 -> 210 us).  The whole warp runs
+// the loops around them, so that addresses and descriptors stay in uniform registers.
 __device__ __forceinline__ bool mm_elect() {
   uint32_t p;
   asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
@@ -278,8 +286,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                const __grid_constant__ MmaParams p) {
   constexpr int BNC = BN / CTAS, BM = kMmBM * CTAS;
   constexpr bool MULTI = NPA > 1;
-  constexpr int NB = MULTI ? 4 : 2;                  // accumulators
-  constexpr uint32_t kCols = NB * BN;                // TMEM columns
+  constexpr int NB = 2;                              // accumulator buffers, of one or (MULTI) two accumulators
+  constexpr uint32_t kCols = NB * (MULTI ? 2 : 1) * BN;   // TMEM columns
   constexpr int HALF = BN >= 64 ? BN / 2 : BN;        // columns per epilogue warp
   constexpr int kEpi = BN >= 64 ? kMmEpiWarps : 4;    // epilogue warps at work
   extern __shared__ unsigned char mm_raw[];
@@ -315,7 +323,8 @@ __global__ void __launch_bounds__(kMmThreads, 1)
   const int64_t first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (warp == 8) {
-    if (mm_elect()) {
+    {
+      const bool lead = mm_elect();
       MmaRing r(p.slots);
       bool live = true;
       for (int64_t item = first; item < items && live; item += step) {
@@ -329,29 +338,33 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         for (int kb = t.k0; kb < t.k1 && live; ++kb) {
 #pragma unroll
           for (int i = 0; i < NPA; ++i, r.next()) {
-            if (r.round && !mm_wait(sh, sh.empty[r.s], (r.round - 1) & 1)) {
+            if (r.round && !mm_wait_warp(sh, sh.empty[r.s], (r.round - 1) & 1)) {
               live = false;
               break;
             }
-            uint32_t bar = t5_smem_u32(&sh.full[r.s]);
+            const uint32_t bar = t5_smem_u32(&sh.full[r.s]);
+            uint32_t rbar = bar;
             const uint32_t a = smem + r.s * slot_bytes, b = a + p.a_slot;
+            if constexpr (CTAS == 2) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(rbar) : "r"(bar));
+            if (lead) {
             if (rank == 0) mm_expect(bar, CTAS * (a_bytes + (i < npb ? p.b_bytes : 0u)));
-            if constexpr (CTAS == 2) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(bar) : "r"(bar));
             if (a_mn) {
-              mm_load<CTAS>(a, ta, m0, kb * kMmBK, i, bar);
-              mm_load<CTAS>(a + 8192, ta, m0 + 64, kb * kMmBK, i, bar);
+              mm_load<CTAS>(a, ta, m0, kb * kMmBK, i, rbar);
+              mm_load<CTAS>(a + 8192, ta, m0 + 64, kb * kMmBK, i, rbar);
             } else {
-              mm_load<CTAS>(a, ta, kb * kMmBK, m0, i, bar);
+              mm_load<CTAS>(a, ta, kb * kMmBK, m0, i, rbar);
             }
             if (i < npb) {
               if (BNC >= 64 && b_mn) {
 #pragma unroll
                 for (int h = 0; h < BNC / 64; ++h)
-                  mm_load<CTAS>(b + h * 8192, tb, n0 + 64 * h, kb * kMmBK, i, bar);
+                  mm_load<CTAS>(b + h * 8192, tb, n0 + 64 * h, kb * kMmBK, i, rbar);
               } else {
-                mm_load<CTAS>(b, tb, kb * kMmBK, n0, i, bar);
+                mm_load<CTAS>(b, tb, kb * kMmBK, n0, i, rbar);
               }
             }
+            }
+            __syncwarp();
           }
         }
       }
@@ -362,14 +375,19 @@ __global__ void __launch_bounds__(kMmThreads, 1)
       }
     }
   } else if (warp == 9) {
-    if (rank == 0 && mm_elect()) {
+    if (rank == 0) {
+      const bool lead = mm_elect();
       const uint64_t desc = t5_desc_sw128(smem, 8192, 1024);   // of A in slot 0; the address field counts 16 bytes
       MmaRing r(p.slots);
       uint32_t ch = 0;
       bool live = true;
       auto commit = [&](uint64_t& bar) {
-        if constexpr (CTAS == 1) t5_commit(t5_smem_u32(&bar));
-        else t5_commit_pair(t5_smem_u32(&bar));
+        const uint32_t a = t5_smem_u32(&bar);
+        if (lead) {
+          if constexpr (CTAS == 1) t5_commit(a);
+          else t5_commit_pair(a);
+        }
+        __syncwarp();
       };
       for (int64_t item = first; item < items && live; item += step) {
         const MmaTile t = mm_tile<JOBS>(p, item, BM, BN);
@@ -379,51 +397,52 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         const uint32_t ka = (o.a_mn ? 2048u : 32u) >> 4, kb_ = (o.b_mn ? 2048u : 32u) >> 4;   // 16-byte units per 16 k
         for (int c0 = t.k0; c0 < t.k1 && live; c0 += p.chunk, ++ch) {
           const int c1 = min(t.k1, c0 + p.chunk), buf = ch % NB;
-          if (ch >= NB && !mm_wait(sh, sh.free_[buf], (ch / NB - 1) & 1)) {
+          if (ch >= NB && !mm_wait_warp(sh, sh.free_[buf], (ch / NB - 1) & 1)) {
             live = false;
             break;
           }
           t5_fence_after_sync();
-          const uint32_t d = tmem + buf * BN;
-          uint32_t acc = 0;
-          auto product = [&](int sa, int sb) {   // the plane of A in slot sa by the plane of B in slot sb
+          // one plane: accumulator buf; several: the leading products into one, all others into another
+          const uint32_t d = tmem + buf * (MULTI ? 2 : 1) * BN;
+          uint32_t acc[2] = {0, 0};
+          auto product = [&](int which, int sa, int sb) {   // the plane of A in slot sa by the plane of B in slot sb
             const uint64_t ad = desc + sa * (slot_bytes >> 4);
             const uint64_t bd = desc + (sb * slot_bytes + p.a_slot >> 4);
+            if (lead) {
 #pragma unroll
-            for (int k = 0; k < kMmBK / 16; ++k) {
-              if constexpr (CTAS == 1) t5_mma_bf16(d, ad + k * ka, bd + k * kb_, idesc, acc);
-              else t5_mma_bf16_pair(d, ad + k * ka, bd + k * kb_, idesc, acc);
-              acc = 1;
+              for (int k = 0; k < kMmBK / 16; ++k) {
+                if constexpr (CTAS == 1) t5_mma_bf16(d + which * BN, ad + k * ka, bd + k * kb_, idesc, acc[which] | k);
+                else t5_mma_bf16_pair(d + which * BN, ad + k * ka, bd + k * kb_, idesc, acc[which] | k);
+              }
             }
+            acc[which] = 1;
           };
           for (int kb = c0; kb < c1 && live; ++kb) {
             int slot[NPA];
 #pragma unroll
             for (int i = 0; i < NPA; ++i, r.next()) {
               slot[i] = r.s;
-              if (live && !mm_wait(sh, sh.full[r.s], r.round & 1)) live = false;
+              if (live && !mm_wait_warp(sh, sh.full[r.s], r.round & 1)) live = false;
+              if (!live) continue;
+              t5_fence_after_sync();
+              if constexpr (NPA == 1) {
+                product(0, slot[0], slot[0]);
+              } else if (i == 0) {
+                product(0, slot[0], slot[0]);
+              } else if (i == 1) {
+                product(1, slot[1], slot[0]);
+                if (npb > 1) {
+                  product(1, slot[0], slot[1]);
+                  product(1, slot[1], slot[1]);
+                }
+                commit(sh.empty[slot[1]]);
+              } else {
+                product(1, slot[2], slot[0]);
+                if (npb > 1) product(1, slot[0], slot[2]);
+                commit(sh.empty[slot[2]]);
+              }
             }
-            if (!live) break;
-            t5_fence_after_sync();
-            if constexpr (NPA == 1) {
-              product(slot[0], slot[0]);
-            } else if (npb == 1) {
-              product(slot[2], slot[0]);
-              commit(sh.empty[slot[2]]);
-              product(slot[1], slot[0]);
-              commit(sh.empty[slot[1]]);
-              product(slot[0], slot[0]);
-            } else {
-              product(slot[0], slot[2]);
-              product(slot[2], slot[0]);
-              commit(sh.empty[slot[2]]);
-              product(slot[1], slot[1]);
-              product(slot[0], slot[1]);
-              product(slot[1], slot[0]);
-              commit(sh.empty[slot[1]]);
-              product(slot[0], slot[0]);
-            }
-            commit(sh.empty[slot[0]]);
+            if (live) commit(sh.empty[slot[0]]);
           }
           if (live) commit(sh.done[buf]);
         }
@@ -446,21 +465,26 @@ __global__ void __launch_bounds__(kMmThreads, 1)
       mm_prefetch(o, m0, n0, HALF);
       for (int c0 = t.k0; c0 < t.k1; c0 += p.chunk, ++ch) {
         const int buf = ch % NB;
-        const bool ok = __all_sync(kFullMask, mm_wait(sh, sh.done[buf], (ch / NB) & 1));
+        const bool ok = mm_wait_warp(sh, sh.done[buf], (ch / NB) & 1);
         t5_fence_after_sync();
-        const uint32_t cols = tmem + lane_base + (uint32_t)(buf * BN + half * HALF);
+        const uint32_t cols = tmem + lane_base + (uint32_t)(buf * (MULTI ? 2 : 1) * BN + half * HALF);
         if constexpr (MULTI) {   // one load for all of the warp's columns: each waits for the MMAs in flight
           static_assert(HALF == 32 || HALF == 64, "columns per warp");
-          float v[HALF];
-          if constexpr (HALF == 64) t5_ld64(cols, v);
-          else t5_ld32(cols, v);
-          t5_fence_before_sync();
-          __syncwarp();
-          if (lane == 0) mm_arrive<CTAS>(t5_smem_u32(&sh.free_[buf]));
 #pragma unroll
-          for (int i = 0; i < HALF; ++i) {
-            if (!ok) v[i] = __int_as_float(0x7FC00000);
-            sum[i] = c0 == t.k0 ? v[i] : sum[i] + v[i];
+          for (int which = 1; which >= 0; --which) {
+            float v[HALF];
+            if constexpr (HALF == 64) t5_ld64(cols + which * BN, v);
+            else t5_ld32(cols + which * BN, v);
+            if (which == 0) {
+              t5_fence_before_sync();
+              __syncwarp();
+              if (lane == 0) mm_arrive<CTAS>(t5_smem_u32(&sh.free_[buf]));
+            }
+#pragma unroll
+            for (int i = 0; i < HALF; ++i) {
+              if (!ok) v[i] = __int_as_float(0x7FC00000);
+              sum[i] = which == 1 && c0 == t.k0 ? v[i] : sum[i] + v[i];
+            }
           }
         } else {
 #pragma unroll
@@ -769,7 +793,7 @@ int mma_run(const MmaJob* jobs, int n, const SumRows& side, void* work, cudaStre
     if (o.a_bytes > p.a_slot) p.a_slot = o.a_bytes;
   }
   if (n == 1) map[2] = map[3] = map[0];
-  p.chunk = z[0].npa > 1 ? 2 : 1 << 30;   // one chunk; k block numbers stay below 2^25
+  p.chunk = z[0].npa > 1 ? 8 : 1 << 30;   // one chunk; k block numbers stay below 2^25
   p.b_bytes = (uint32_t)(pl.BN / pl.ctas) * kMmBK * 2;
   p.slots = (int)(kMmRing / 1024 * 1024 / (p.a_slot + p.b_bytes));
   if (p.slots > kMmMaxSlots) p.slots = kMmMaxSlots;
