@@ -455,7 +455,7 @@ __global__ void __launch_bounds__(NT) norm_bwd_resident(NormParams p) {
 
 // ---- streaming kernels: a block per (sample, chunk of positions, segment) ----
 // Blocks of 256 threads, kStatBlocks / kBwdBlocks to an SM (the registers of U loads in flight and the channels'
-// constants), and two whole waves of them.
+// constants), and one whole wave of them: a block's statistics and merges cost as much as several positions.
 constexpr int kFwdBlocks = 4, kBwdBlocks = 3;
 
 // A thread's column of a [positions][channels] operand: element vectors `step` positions apart.
@@ -532,6 +532,15 @@ __device__ __forceinline__ Slab<N, NT> chunk_slab(const NormParams& p, unsigned 
   const unsigned nseg = (unsigned)p.nseg, chunks = (unsigned)p.chunks;   // 32-bit divisions: block numbers are
   const unsigned sc = block / nseg, s = sc / chunks;
   return Slab<N, NT>(p, s, block - sc * nseg, sc - s * chunks);
+}
+
+// Lanes (a power of two, at most a warp) that merge one group's chunks in the elementwise kernels: all groups of a block
+// at once where they fit, since every merge is a chain of loads.
+template <int NT>
+__device__ __forceinline__ int group_lanes(int ngl) {
+  int l = 32;
+  while (l > 1 && NT / l < ngl) l >>= 1;
+  return l;
 }
 
 // This block's first entry in a chunk's row of gpart, and the number of elements behind entry (chunk, part).
@@ -611,25 +620,27 @@ __global__ void __launch_bounds__(NT, kFwdBlocks) norm_apply_kernel(NormParams p
   float* rstd = sf + p.ng;
   const float2* part = reinterpret_cast<const float2*>(p.gpart) + (a.s * p.chunks * p.G + a.g0) * p.nsub;
   const float m = (float)p.P * (float)p.cpg;
-  const int entries = (int)(p.chunks * p.nsub);
-  for (int g = threadIdx.x >> 5; g < a.ngl; g += NT / 32) {
+  const int entries = (int)(p.chunks * p.nsub), gl = group_lanes<NT>(a.ngl), l = lane % gl;
+  for (int g = threadIdx.x / gl; g < (a.ngl + 31) / 32 * 32; g += NT / gl) {   // whole warps: shuffles below
+    const bool in = g < a.ngl;
     float v = 0.f;
-    for (int j = lane; j < entries; j += 32) {
-      const int ch = j / p.nsub;
-      v = fmaf(part[((int64_t)ch * p.G + g) * p.nsub + (j - ch * p.nsub)].x, entry_count(p, ch, j - ch * p.nsub), v);
+#pragma unroll 4
+    for (int j = l; j < entries; j += gl) {
+      const int ch = p.nsub == 1 ? j : j / p.nsub;
+      if (in) v = fmaf(part[((int64_t)ch * p.G + g) * p.nsub + (j - ch * p.nsub)].x, entry_count(p, ch, j - ch * p.nsub), v);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+    for (int o = gl / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
     const float mu = v / m;
     v = 0.f;
-    for (int j = lane; j < entries; j += 32) {
-      const int ch = j / p.nsub;
+#pragma unroll 4
+    for (int j = l; j < entries; j += gl) {
+      const int ch = p.nsub == 1 ? j : j / p.nsub;
+      if (!in) continue;
       const float2 t = part[((int64_t)ch * p.G + g) * p.nsub + (j - ch * p.nsub)];
       v += fmaf((t.x - mu) * (t.x - mu), entry_count(p, ch, j - ch * p.nsub), t.y);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
-    if (lane == 0) {
+    for (int o = gl / 2; o > 0; o >>= 1) v += __shfl_xor_sync(kFullMask, v, o);
+    if (in && l == 0) {
       const float rs = 1.f / sqrtf(v / m + p.eps);
       mean[g] = mu;
       rstd[g] = rs;
@@ -780,21 +791,23 @@ __global__ void __launch_bounds__(NT, kBwdBlocks) norm_bwd_apply_kernel(NormPara
   float* s1 = sf;                                       // [ng] mean(q), mean(q h)
   float* s2 = sf + p.ng;
   const float2* part = reinterpret_cast<const float2*>(p.gpart) + (a.s * p.chunks * p.G + a.g0) * p.nsub;
-  const int entries = (int)(p.chunks * p.nsub);
-  for (int g = threadIdx.x >> 5; g < a.ngl; g += NT / 32) {
+  const int entries = (int)(p.chunks * p.nsub), gl = group_lanes<NT>(a.ngl), l = lane % gl;
+  for (int g = threadIdx.x / gl; g < (a.ngl + 31) / 32 * 32; g += NT / gl) {
+    const bool in = g < a.ngl;
     float v1 = 0.f, v2 = 0.f;
-    for (int j = lane; j < entries; j += 32) {
-      const int ch = j / p.nsub;
+#pragma unroll 4
+    for (int j = l; j < entries; j += gl) {
+      const int ch = p.nsub == 1 ? j : j / p.nsub;
+      if (!in) continue;
       const float2 t = part[((int64_t)ch * p.G + g) * p.nsub + (j - ch * p.nsub)];
       v1 += t.x;
       v2 += t.y;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
+    for (int o = gl / 2; o > 0; o >>= 1) {
       v1 += __shfl_xor_sync(kFullMask, v1, o);
       v2 += __shfl_xor_sync(kFullMask, v2, o);
     }
-    if (lane == 0) {
+    if (in && l == 0) {
       const float m = (float)p.P * (float)p.cpg;
       s1[g] = v1 / m;
       s2[g] = v2 / m;
@@ -1077,7 +1090,7 @@ static NormPlan norm_plan(int64_t S, int64_t P, int64_t C, int64_t G, int esize,
       return pl;
     }
   }
-  // streaming: two waves of blocks, at least 16 positions each where there are that many; groups too wide for a block's
+  // streaming: one wave of blocks, at least 16 positions each where there are that many; groups too wide for a block's
   // sums in parts of 4096 channels
   pl.kind = kNormStream;
   pl.NT = 256;
@@ -1094,7 +1107,7 @@ static NormPlan norm_plan(int64_t S, int64_t P, int64_t C, int64_t G, int esize,
     pl.ng = 1;
     pl.nseg = G * pl.nsub;
   }
-  int64_t chunks = 2 * (int64_t)sms * (bwd ? kBwdBlocks : kFwdBlocks) / (S * pl.nseg);
+  int64_t chunks = (int64_t)sms * (bwd ? kBwdBlocks : kFwdBlocks) / (S * pl.nseg);
   if (chunks < 1) chunks = 1;
   const int64_t most = (P + 15) / 16;
   if (chunks > most) chunks = most;

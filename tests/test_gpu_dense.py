@@ -186,7 +186,8 @@ def test_linear_optional_inputs(dtype, bias, residual):
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("M,K,N", [(1, 4096, 512), (2, 1001, 77), (4, 256, 1000), (7, 512, 96), (8, 333, 130),
-                                   (9, 640, 64), (16, 2048, 200), (37, 1024, 520), (2000, 64, 16)])
+                                   (9, 640, 64), (16, 2048, 200), (37, 1024, 520), (2000, 64, 16), (60, 8192, 42),
+                                   (130, 8192, 72), (1, 8192, 33), (4, 2056, 264)])
 def test_linear_without_gradients(M, K, N, dtype):
     """The serving calls (no saved tensors), one token to many."""
     x, w, b, r, _ = linear_case(M, K, N, dtype, "silu", "none", seed=9)
@@ -316,6 +317,37 @@ def test_linear_on_another_stream():
     assert all(torch.equal(g, want) for g in got)
 
 
+def test_in_a_cuda_graph():
+    """Forward calls captured on a stream replay on new contents of the same tensors."""
+    x, w, b, r, _ = linear_case(200, 320, 264, BF16, "gelu", "none", seed=4)
+    gam = 1 + data(264, dtype=BF16, seed=5, scale=0.1)
+
+    def call():
+        return gl.group_norm_act(gl.linear_act(x, w, b, r, activation="gelu"), 8, gam, activation="silu")
+
+    with torch.no_grad():
+        s = torch.cuda.Stream()
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            call()
+        torch.cuda.current_stream().wait_stream(s)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = call()
+        x.copy_(data(200, 320, dtype=BF16, seed=77))
+        want = call()
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, want)
+
+
+def test_second_derivatives_are_refused():
+    x = data(8, 32, seed=1).requires_grad_(True)
+    for y in (gl.linear_act(x, data(16, 32, seed=2), activation="gelu"), gl.group_norm_act(x, 4)):
+        with pytest.raises(RuntimeError, match="not differentiable"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
 def test_linear_as_a_threads_first_cuda_call():
     """A thread that has not touched the device yet (autograd's, on its first backward) has no current context."""
     import threading
@@ -402,6 +434,12 @@ def check_norm(x, G, w, b, dy, act="silu", ckpt="none", eps=1e-5):
 NORM_SIZES = [((1, 1), 1), ((1, 8), 8), ((3, 40), 4), ((1, 4096), 32), ((300, 512), 8), ((2, 5, 24), 3),
               ((2, 3, 7, 33), 11), ((4, 1000, 64), 8), ((3, 129, 1000), 8), ((2, 64, 64, 512), 32), ((1, 70000, 8), 2),
               ((5, 1, 1, 96), 96), ((2, 2000, 1001), 7), ((1, 3, 40000), 2), ((1, 1, 200001), 3)]
+
+
+# token rows: groups of one vector, of as many as lanes, of several a lane, of no power of two; samples past a block's
+# walk; and groups too wide for a block's sums
+NORM_SIZES += [((7, 4096), 1), ((7, 2048), 1), ((130, 1024), 1), ((5, 800), 5), ((3, 96), 12), ((9, 160), 8),
+               ((5000, 64), 4), ((2, 3, 65536), 1), ((1, 40, 131072), 2)]
 
 
 @pytest.mark.parametrize("dtype", [F32, BF16])
