@@ -120,6 +120,11 @@ def decode_activation(a: Activation8, dtype: Optional[torch.dtype] = None) -> to
     return out
 
 
+def _empty_as(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous uninitialised memory of ``t``'s shape and type (empty_like is the cheapest call for it)."""
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
+
+
 # ---- gradients of parameters ----
 
 def _grad_buffers(weight, need_w: bool, bias, need_b: bool):
@@ -129,7 +134,7 @@ def _grad_buffers(weight, need_w: bool, bias, need_b: bool):
     main = (need_w and hasattr(weight, "main_grad") and weight.main_grad is not None or
             need_b and hasattr(bias, "main_grad") and bias.main_grad is not None)
     if not main:
-        return weight.new_empty(weight.shape) if need_w else None, bias.new_empty(bias.shape) if need_b else None, False
+        return _empty_as(weight) if need_w else None, _empty_as(bias) if need_b else None, False
     out = []
     for p, want in ((weight, need_w), (bias, need_b)):
         g = getattr(p, "main_grad", None) if want else None
@@ -250,7 +255,7 @@ def _positions(t: torch.Tensor, S: int, P: int, C: int) -> torch.Tensor:
 
 def _norm_forward(x, num_groups, weight, bias, act, eps):
     S, C = x.shape[0], x.shape[-1]
-    y = x.new_empty(x.shape)
+    y = _empty_as(x)
     stats = x.new_empty((2, S, num_groups), dtype=torch.float32)   # mean, rstd
     x3 = None
     n = x.numel()
@@ -277,7 +282,7 @@ class GroupNormActFunction(torch.autograd.Function):
         _no_double_backward("group_norm_act")
         x3, codes, exps, weight, bias, stats = ctx.saved_tensors
         _, need_w, need_b = ctx.needs_input_grad[:3]
-        dx = dy.new_empty(dy.shape)
+        dx = _empty_as(dy)
         dw, db, main = _grad_buffers(weight, need_w, bias, need_b)
         S, C = dy.shape[0], dy.shape[-1]
         if dx.numel():
