@@ -196,16 +196,23 @@ __global__ void __launch_bounds__(128) lin_db_kernel(SumRows j) {
 
 // ---- a few rows ----
 
-// W warps per output column n: each streams its part of w's row n, eight 16-byte loads in flight, against MT rows of
-// x (from L1), fp32 sums, shuffles and one shared-memory step between the W warps.  Bound by reading w; W is
-// chosen so that a warp's part is about eight loads, which keeps all of w's bytes in flight at once.
+// W warps per output column n: each streams its part of w's row n, four 16-byte loads in flight, against MT rows of x
+// (from L1), fp32 sums, shuffles and one shared-memory step between the W warps.  Bound by reading w; W grows with the
+// row, so that the machine has enough of it in flight (4096 -> 2048 fp32, one token: W = 1 10.2 us, W = 2 7.2 us,
+// 4.7 TB/s; 4096 -> 4096 bf16 W = 1 8.1 us, W = 2 8.8 us, eight loads 10.3 us).
 template <typename T, int MT, int W, bool ALIGNED>
 __global__ void __launch_bounds__(128) lin_rows_kernel(const T* x, const T* w, int M, int64_t N, int64_t K,
                                                        int64_t ldx, int64_t ldw, LinEpilogue e) {
-  constexpr int V = ALIGNED ? kVec16<T> : 1, U = 8;
+  constexpr int V = ALIGNED ? kVec16<T> : 1, U = 4;
   __shared__ float red[4][MT];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % W;
   const int64_t n = (int64_t)blockIdx.x * (4 / W) + warp / W;
+  // lane t finishes row t: its bias and residual are on the way while w is read
+  float bias = 0.f, residual = 0.f;
+  if (part == 0 && n < N && lane < M) {
+    if (e.bias) bias = to_f32<T>(reinterpret_cast<const T*>(e.bias)[n]);
+    if (e.residual) residual = to_f32<T>(reinterpret_cast<const T*>(e.residual)[lane * e.ldr + n]);
+  }
   float acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = 0.f;
@@ -262,11 +269,24 @@ __global__ void __launch_bounds__(128) lin_rows_kernel(const T* x, const T* w, i
       for (int q = 1; q < W; ++q) z[0] += red[warp + q][lane];
     }
   }
-  if (n < N && lane < M) lin_finish<1>(e, lane, n, false, z);
+  if (n < N && lane < M) {
+    z[0] += bias;
+    with_act(e.act, [&](auto tag) {
+      constexpr int ACT = decltype(tag)::value;
+      if (e.slope_kind) {
+        const float d[1] = {dense_slope<ACT, sizeof(T) == 2>(z[0], z[0])};
+        st_slope<1>(e, lane, n, false, d);
+      } else {
+        z[0] = dense_act<ACT, sizeof(T) == 2>(z[0]);
+      }
+    });
+    reinterpret_cast<T*>(e.out)[lane * e.ldo + n] = from_f32<T>(z[0] + residual);
+  }
 }
 
 // Rows up to which the row kernels run: beyond, w's fp32 splitting or the tensor cores' fixed cost is paid back.
-constexpr int kRowsBf16 = 4, kRowsF32 = 8;
+template <typename T>
+constexpr int kRows = sizeof(T) == 4 ? 8 : 4;
 
 template <typename T, int MT, int W>
 static void launch_rows_w(const GlLinearArgs& a, const LinEpilogue& e, bool aligned, cudaStream_t st) {
@@ -291,8 +311,8 @@ template <typename T>
 static int run_rows(const GlLinearArgs& a, const LinEpilogue& e, bool aligned, cudaStream_t st) {
   if (a.M == 1) launch_rows<T, 1>(a, e, aligned, st);
   else if (a.M == 2) launch_rows<T, 2>(a, e, aligned, st);
-  else if (a.M <= 4) launch_rows<T, 4>(a, e, aligned, st);
-  else launch_rows<T, 8>(a, e, aligned, st);
+  else if (kRows<T> == 4 || a.M <= 4) launch_rows<T, 4>(a, e, aligned, st);
+  else launch_rows<T, kRows<T>>(a, e, aligned, st);
   const cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return set_cuda_error(err);
   count_launches(1);
@@ -323,7 +343,9 @@ struct LinWork {
   }
 };
 
-static bool few_rows(int64_t M, int dtype) { return M <= (dtype == GL_DTYPE_F32 ? kRowsF32 : kRowsBf16); }
+static bool few_rows(int64_t M, int dtype) {
+  return M <= (dtype == GL_DTYPE_F32 ? kRows<float> : kRows<__nv_bfloat16>);
+}
 
 static LinWork lin_fwd_work(int64_t M, int64_t N, int64_t K, int dtype, bool unaligned, int sms) {
   LinWork w;

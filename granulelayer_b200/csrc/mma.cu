@@ -2,8 +2,8 @@
 //
 // A persistent CTA, or a pair of CTAs, takes output tiles of 128 (256) x BN and, with split sums, ranges of k.  Ten
 // warps per CTA:
-//   producer (one lane)  TMA loads of 64 k of a plane of A and of B into a ring of 128-byte-swizzled slots
-//   issuer (one lane; of a pair, the even CTA's)  tcgen05.mma per 16 k and term pair, two accumulators in TMEM
+//   producer  TMA loads of 64 k of a plane of A and of B into a ring of 128-byte-swizzled slots
+//   issuer (of a pair, the even CTA's)  tcgen05.mma per 16 k and term pair, two accumulators in TMEM
 //   eight epilogue warps TMEM -> registers -> shared memory -> bias, activation, residual -> memory, row by row in
 //                        whole sectors, while the next tile runs
 // handing over through mbarriers: full / empty per slot, done / free per accumulator.
@@ -323,30 +323,29 @@ __global__ void __launch_bounds__(kMmThreads, 1)
   const int64_t first = blockIdx.x / CTAS, step = gridDim.x / CTAS;
 
   if (warp == 8) {
-    {
-      const bool lead = mm_elect();
-      MmaRing r(p.slots);
-      bool live = true;
-      for (int64_t item = first; item < items && live; item += step) {
-        const MmaTile t = mm_tile<JOBS>(p, item, BM, BN);
-        const MmaOne& o = p.job[JOBS == 1 ? 0 : t.job];
-        const CUtensorMap* ta = JOBS == 1 || !t.job ? &ta0 : &ta1;
-        const CUtensorMap* tb = JOBS == 1 || !t.job ? &tb0 : &tb1;
-        const int a_mn = o.a_mn, b_mn = o.b_mn, npb = o.npb;
-        const uint32_t a_bytes = o.a_bytes;
-        const int m0 = (int)t.m0 + kMmBM * rank, n0 = (int)t.n0 + BNC * rank;
-        for (int kb = t.k0; kb < t.k1 && live; ++kb) {
+    const bool lead = mm_elect();
+    MmaRing r(p.slots);
+    bool live = true;
+    for (int64_t item = first; item < items && live; item += step) {
+      const MmaTile t = mm_tile<JOBS>(p, item, BM, BN);
+      const MmaOne& o = p.job[JOBS == 1 ? 0 : t.job];
+      const CUtensorMap* ta = JOBS == 1 || !t.job ? &ta0 : &ta1;
+      const CUtensorMap* tb = JOBS == 1 || !t.job ? &tb0 : &tb1;
+      const int a_mn = o.a_mn, b_mn = o.b_mn, npb = o.npb;
+      const uint32_t a_bytes = o.a_bytes;
+      const int m0 = (int)t.m0 + kMmBM * rank, n0 = (int)t.n0 + BNC * rank;
+      for (int kb = t.k0; kb < t.k1 && live; ++kb) {
 #pragma unroll
-          for (int i = 0; i < NPA; ++i, r.next()) {
-            if (r.round && !mm_wait_warp(sh, sh.empty[r.s], (r.round - 1) & 1)) {
-              live = false;
-              break;
-            }
-            const uint32_t bar = t5_smem_u32(&sh.full[r.s]);
-            uint32_t rbar = bar;
-            const uint32_t a = smem + r.s * slot_bytes, b = a + p.a_slot;
-            if constexpr (CTAS == 2) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(rbar) : "r"(bar));
-            if (lead) {
+        for (int i = 0; i < NPA; ++i, r.next()) {
+          if (r.round && !mm_wait_warp(sh, sh.empty[r.s], (r.round - 1) & 1)) {
+            live = false;
+            break;
+          }
+          const uint32_t bar = t5_smem_u32(&sh.full[r.s]);
+          uint32_t rbar = bar;                           // the even CTA's barrier of this slot
+          const uint32_t a = smem + r.s * slot_bytes, b = a + p.a_slot;
+          if constexpr (CTAS == 2) asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(rbar) : "r"(bar));
+          if (lead) {
             if (rank == 0) mm_expect(bar, CTAS * (a_bytes + (i < npb ? p.b_bytes : 0u)));
             if (a_mn) {
               mm_load<CTAS>(a, ta, m0, kb * kMmBK, i, rbar);
@@ -363,16 +362,15 @@ __global__ void __launch_bounds__(kMmThreads, 1)
                 mm_load<CTAS>(b, tb, kb * kMmBK, n0, i, rbar);
               }
             }
-            }
-            __syncwarp();
           }
+          __syncwarp();
         }
       }
-      if (!live && rank == 0) {   // the copies in flight must land before the shared memory goes away
-        const uint32_t n = (uint32_t)p.slots, it = r.round * n + r.s;
-        for (uint32_t j = it > n ? it - n : 0; j < it; ++j)
-          t5_mbar_wait(t5_smem_u32(&sh.full[j % n]), (j / n) & 1, kMmWaitLimit);
-      }
+    }
+    if (!live && rank == 0) {   // the copies in flight must land before the shared memory goes away
+      const uint32_t n = (uint32_t)p.slots, it = r.round * n + r.s;
+      for (uint32_t j = it > n ? it - n : 0; j < it; ++j)
+        t5_mbar_wait(t5_smem_u32(&sh.full[j % n]), (j / n) & 1, kMmWaitLimit);
     }
   } else if (warp == 9) {
     if (rank == 0) {
