@@ -207,12 +207,8 @@ __global__ void __launch_bounds__(128) lin_rows_kernel(const T* x, const T* w, i
   __shared__ float red[4][MT];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, part = warp % W;
   const int64_t n = (int64_t)blockIdx.x * (4 / W) + warp / W;
-  // lane t finishes row t: its bias and residual are on the way while w is read
-  float bias = 0.f, residual = 0.f;
-  if (part == 0 && n < N && lane < M) {
-    if (e.bias) bias = to_f32<T>(reinterpret_cast<const T*>(e.bias)[n]);
-    if (e.residual) residual = to_f32<T>(reinterpret_cast<const T*>(e.residual)[lane * e.ldr + n]);
-  }
+  if (part == 0 && n < N && lane < M && e.residual)          // lane t finishes row t
+    asm volatile("prefetch.global.L2 [%0];" ::"l"(reinterpret_cast<const T*>(e.residual) + lane * e.ldr + n));
   float acc[MT];
 #pragma unroll
   for (int t = 0; t < MT; ++t) acc[t] = 0.f;
@@ -269,19 +265,7 @@ __global__ void __launch_bounds__(128) lin_rows_kernel(const T* x, const T* w, i
       for (int q = 1; q < W; ++q) z[0] += red[warp + q][lane];
     }
   }
-  if (n < N && lane < M) {
-    z[0] += bias;
-    with_act(e.act, [&](auto tag) {
-      constexpr int ACT = decltype(tag)::value;
-      if (e.slope_kind) {
-        const float d[1] = {dense_slope<ACT, sizeof(T) == 2>(z[0], z[0])};
-        st_slope<1>(e, lane, n, false, d);
-      } else {
-        z[0] = dense_act<ACT, sizeof(T) == 2>(z[0]);
-      }
-    });
-    reinterpret_cast<T*>(e.out)[lane * e.ldo + n] = from_f32<T>(z[0] + residual);
-  }
+  if (n < N && lane < M) lin_finish<1>(e, lane, n, false, z);
 }
 
 // Rows up to which the row kernels run: beyond, w's fp32 splitting or the tensor cores' fixed cost is paid back.
