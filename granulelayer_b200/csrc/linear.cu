@@ -66,9 +66,9 @@ struct PackJob {
 };
 
 template <typename T, int NP>
-__global__ void __launch_bounds__(256) lin_pack_kernel(PackJob j0, PackJob j1) {
+__device__ __forceinline__ void lin_pack(const PackJob& j0, const PackJob& j1, unsigned block, unsigned blocks) {
   const int64_t n0 = j0.rows * j0.nk, total = n0 + j1.rows * j1.nk;
-  for (int64_t t = blockIdx.x * 256ll + threadIdx.x; t < total; t += gridDim.x * 256ll) {
+  for (int64_t t = block * 256ll + threadIdx.x; t < total; t += blocks * 256ll) {
     const bool second = t >= n0;
     const PackJob& j = second ? j1 : j0;
     const int64_t i = second ? t - n0 : t, r = i / j.nk, k = (i - r * j.nk) * 8, plane = j.rows * j.nk * 8;
@@ -79,6 +79,11 @@ __global__ void __launch_bounds__(256) lin_pack_kernel(PackJob j0, PackJob j1) {
 #pragma unroll
     for (int q = 0; q < NP; ++q) *reinterpret_cast<uint4*>(j.dst + q * plane + i * 8) = u[q];
   }
+}
+
+template <typename T, int NP>
+__global__ void __launch_bounds__(256) lin_pack_kernel(PackJob j0, PackJob j1) {
+  lin_pack<T, NP>(j0, j1, blockIdx.x, gridDim.x);
 }
 
 constexpr int kDzRows = 32;   // rows of one block of the dz kernel, and of one partial column sum
@@ -161,10 +166,16 @@ __device__ __forceinline__ void lin_dz_rows(const T* dy, const void* slope, uint
   }
 }
 
+// Blocks past dz_blocks pack the products' other operands (a launch less).
 template <typename T, int NP, int KIND>
 __global__ void __launch_bounds__(256) lin_dz_kernel(const T* dy, const void* slope, uint16_t* dz, float* part,
-                                                     int64_t M, int64_t N, int64_t lddy, int64_t lds, int aligned) {
+                                                     int64_t M, int64_t N, int64_t lddy, int64_t lds, int aligned,
+                                                     unsigned dz_blocks, PackJob j0, PackJob j1) {
   __shared__ float red[8][256 + 8];
+  if (blockIdx.x >= dz_blocks) {
+    lin_pack<T, NP>(j0, j1, blockIdx.x - dz_blocks, gridDim.x - dz_blocks);
+    return;
+  }
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t segs = (N + 255) / 256, Np = (N + 7) / 8 * 8, plane = M * Np;
   const int64_t rc = blockIdx.x / segs, n0 = (blockIdx.x - rc * segs) * 256;
@@ -374,11 +385,14 @@ struct Packer {
     job[n++] = PackJob{src, (uint16_t*)dst, rows, (K + 7) / 8, K, ld, aligned};
     return MmaOperand{dst, up(K, 8), rows * up(K, 8), NP, mn};
   }
-  int run(int sms, cudaStream_t st) {
-    if (n == 0) return GL_OK;
+  unsigned blocks(int sms) const {
     const int64_t total = job[0].rows * job[0].nk + job[1].rows * job[1].nk, need = (total + 255) / 256;
     const int64_t cap = 16ll * sms;
-    lin_pack_kernel<T, NP><<<(unsigned)(need < cap ? need : cap), 256, 0, st>>>(job[0], job[1]);
+    return (unsigned)(need < cap ? need : cap);
+  }
+  int run(int sms, cudaStream_t st) {
+    if (n == 0) return GL_OK;
+    lin_pack_kernel<T, NP><<<blocks(sms), 256, 0, st>>>(job[0], job[1]);
     const cudaError_t err = cudaGetLastError();
     if (err != cudaSuccess) return set_cuda_error(err);
     count_launches(1);
@@ -398,11 +412,13 @@ static int run_linear_fwd(const GlLinearArgs& a, const LinEpilogue& e, const Lin
 }
 
 template <typename T, int KIND>
-static int launch_dz(const GlLinearBwdArgs& a, uint16_t* dz, float* part, bool aligned, cudaStream_t st) {
+static int launch_dz(const GlLinearBwdArgs& a, uint16_t* dz, float* part, bool aligned, const Packer<T>& pack, int sms,
+                     cudaStream_t st) {
   const int64_t blocks = up(a.M, kDzRows) / kDzRows * ((a.N + 255) / 256);
-  if (blocks > 0x7FFFFFFF) return GL_ERR_SHAPE;
-  lin_dz_kernel<T, sizeof(T) == 4 ? 3 : 1, KIND><<<(unsigned)blocks, 256, 0, st>>>(
-      (const T*)a.dy, a.slope, dz, part, a.M, a.N, a.lddy, a.lds, aligned);
+  const unsigned more = pack.n ? pack.blocks(sms) : 0;
+  if (blocks + more > 0x7FFFFFFF) return GL_ERR_SHAPE;
+  lin_dz_kernel<T, sizeof(T) == 4 ? 3 : 1, KIND><<<(unsigned)blocks + more, 256, 0, st>>>(
+      (const T*)a.dy, a.slope, dz, part, a.M, a.N, a.lddy, a.lds, aligned, (unsigned)blocks, pack.job[0], pack.job[1]);
   const cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return set_cuda_error(err);
   count_launches(1);
@@ -421,24 +437,6 @@ static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, c
   const bool write = !dy_is_dz && (a.dx || a.dw);
   MmaOperand dz{a.dy, a.lddy, 0, 1, 0};
   if (!dy_is_dz) dz = MmaOperand{work + w.dz, up(a.N, 8), a.M * up(a.N, 8), NP, 0};
-  if (write || a.db) {
-    uint16_t* out = write ? (uint16_t*)(work + w.dz) : nullptr;
-    float* part = a.db ? (float*)(work + w.part) : nullptr;
-    const int rc = a.slope_kind == GL_SLOPE_NONE  ? launch_dz<T, GL_SLOPE_NONE>(a, out, part, aligned, st)
-                   : a.slope_kind == GL_SLOPE_F32 ? launch_dz<T, GL_SLOPE_F32>(a, out, part, aligned, st)
-                   : a.slope_kind == GL_SLOPE_I16 ? launch_dz<T, GL_SLOPE_I16>(a, out, part, aligned, st)
-                                                  : launch_dz<T, GL_SLOPE_U8>(a, out, part, aligned, st);
-    if (rc) return rc;
-  }
-  SumRows db{};     // done beside the products
-  if (a.db) db = SumRows{(const float*)(work + w.part), a.db, up(a.M, kDzRows) / kDzRows, a.N, a.dtype, a.accumulate};
-  if (a.db && !a.dx && !a.dw) {
-    lin_db_kernel<<<(unsigned)((a.N + 127) / 128), 128, 0, st>>>(db);
-    const cudaError_t err = cudaGetLastError();
-    if (err != cudaSuccess) return set_cuda_error(err);
-    count_launches(1);
-    return GL_OK;
-  }
   Packer<T> pack;
   MmaOperand wt{}, x{};
   if (a.dx) wt = pack.add(a.w, a.N, a.K, a.ldw, 1, work + w.w);   // w with its K columns as rows
@@ -453,7 +451,26 @@ static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, c
   } else if (a.dw) {
     x = pack.add(a.x, a.M, a.K, a.ldx, 1, work + w.x);
   }
-  if (int rc = pack.run(sms, st)) return rc;
+  if (write || a.db) {
+    uint16_t* out = write ? (uint16_t*)(work + w.dz) : nullptr;
+    float* part = a.db ? (float*)(work + w.part) : nullptr;
+    const int rc = a.slope_kind == GL_SLOPE_NONE  ? launch_dz<T, GL_SLOPE_NONE>(a, out, part, aligned, pack, sms, st)
+                   : a.slope_kind == GL_SLOPE_F32 ? launch_dz<T, GL_SLOPE_F32>(a, out, part, aligned, pack, sms, st)
+                   : a.slope_kind == GL_SLOPE_I16 ? launch_dz<T, GL_SLOPE_I16>(a, out, part, aligned, pack, sms, st)
+                                                  : launch_dz<T, GL_SLOPE_U8>(a, out, part, aligned, pack, sms, st);
+    if (rc) return rc;
+  } else if (int rc = pack.run(sms, st)) {
+    return rc;
+  }
+  SumRows db{};     // done beside the products
+  if (a.db) db = SumRows{(const float*)(work + w.part), a.db, up(a.M, kDzRows) / kDzRows, a.N, a.dtype, a.accumulate};
+  if (a.db && !a.dx && !a.dw) {
+    lin_db_kernel<<<(unsigned)((a.N + 127) / 128), 128, 0, st>>>(db);
+    const cudaError_t err = cudaGetLastError();
+    if (err != cudaSuccess) return set_cuda_error(err);
+    count_launches(1);
+    return GL_OK;
+  }
   MmaJob jobs[2];
   int n = 0;
   if (a.dx) {   // [M, K] = dz [M, N] w [N, K]
