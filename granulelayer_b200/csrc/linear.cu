@@ -279,7 +279,8 @@ __global__ void __launch_bounds__(128) lin_rows_kernel(const T* x, const T* w, i
   if (n < N && lane < M) lin_finish<1>(e, lane, n, false, z);
 }
 
-// Rows up to which the row kernels run: beyond, w's fp32 splitting or the tensor cores' fixed cost is paid back.
+// Rows up to which the row kernels run.  4096 -> 4096, bf16: 4 rows 12.5 us here, 13.7 us on the tensor cores (which the
+// rows' number hardly changes); fp32: 8 rows 27 us here, 16 rows 73 us through the split of w.
 template <typename T>
 constexpr int kRows = sizeof(T) == 4 ? 8 : 4;
 
