@@ -13,12 +13,14 @@
 //    group in registers, reductions are shuffles, no barrier at all; several samples per warp are in flight.
 //  * resident kernels, for small samples: a block owns one (sample, segment of whole groups) in shared memory, one
 //    launch, x read once.
-//  * streaming kernels: chunks of positions give partial statistics (per channel shifted by the chunk's first value,
-//    merged with Chan's formula), and an elementwise pass, in the opposite block order, merges those of its groups;
+//  * streaming kernels: chunks of positions give partial statistics, and an elementwise pass, in the opposite block
+//    order, merges those of its groups;
 //    x is read twice, the second time from L2 as far as it fits, and no block waits for another.  (Clusters of 8 blocks
 //    that kept 64-channel segments of such samples in distributed shared memory read them once, but in 128-byte
 //    pieces between cluster barriers: 69 + 160 us forward and backward at 16 x 4096 x 512 bf16.)
-// Variances are sums of squared deviations, never differences of squares.  Outside the row kernels a thread owns whole
+// Variances are sums of squared deviations, never differences of squares: the row and resident kernels take the mean
+// first; the streaming ones take both of four positions at a time and merge such pairs (RunningStats), so that no value,
+// wherever it stands, is a shift for the others.  Outside the row kernels a thread owns whole
 // 16-byte vectors of channels and walks over positions, so all sums are first per channel: group boundaries need no
 // alignment, and with A_c = sum du h, B_c = sum du the backward's group means are sum gamma_c A_c / m and
 // sum gamma_c B_c / m.  No atomics: every sum has one order.
@@ -552,6 +554,71 @@ __device__ __forceinline__ float entry_count(const NormParams& p, int64_t ch, in
   return (float)min(p.PR, p.P - ch * p.PR) * (float)c;
 }
 
+// Mean and sum of squared deviations of the values seen so far, N channels.  Two sets a and b make one by
+//   mean = mean_a + d n_b / n, m2 = m2_a + m2_b + d^2 n_a n_b / n, d = mean_b - mean_a, n = n_a + n_b
+// (Chan, Golub and LeVeque), all of m2's terms positive.  lo holds what the mean's rounding left of the last steps: over a
+// thread's column the mean would otherwise drift by the square root of its length in roundings.  Differences from the
+// chunk's first value, their sum and sum of squares, took 20.1 instead of 22.4 us at 16 x 4096 x 512 bf16, but where that
+// value stands far off they cancel: a channel 1000 deviations off at position 0 of 600 x 4096 x 64 fp32 put the variance off
+// by up to 1.5e-2.
+template <typename T, int N>
+struct RunningStats {
+  float mean[N], lo[N], m2[N], n;
+  __device__ __forceinline__ RunningStats() : n(0.f) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) mean[i] = lo[i] = m2[i] = 0.f;
+  }
+  static __device__ __forceinline__ float element(const Raw<T, N>& r, int i) {   // one, so that 32 need no registers at once
+    if constexpr (N == 1) {
+      return to_f32<T>(r.v);
+    } else {
+      const uint32_t u[4] = {r.v.x, r.v.y, r.v.z, r.v.w};
+      if constexpr (sizeof(T) == 4) return __uint_as_float(u[i]);
+      else return __uint_as_float(i & 1 ? u[i / 2] & 0xFFFF0000u : u[i / 2] << 16);
+    }
+  }
+  // A channel's mean mb and squared deviations q of more values, w = n_b / n and cw = n_a n_b / n.
+  __device__ __forceinline__ void merge(int i, float mb, float q, float w, float cw) {
+    const float d = (mb - mean[i]) - lo[i], t = fmaf(d, w, lo[i]), to = mean[i] + t;
+    m2[i] = fmaf(d * d, cw, m2[i] + q);
+    lo[i] = t - (to - mean[i]);
+    mean[i] = to;
+  }
+  __device__ __forceinline__ void add4(const Raw<T, N> (&r)[4]) {
+    const float w = 4.f / (n + 4.f), cw = n * w;
+    n += 4.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      float a = element(r[0], i), b = element(r[1], i), c = element(r[2], i), d = element(r[3], i);
+      const float mb = 0.25f * ((a + b) + (c + d));
+      a -= mb;
+      b -= mb;
+      c -= mb;
+      d -= mb;
+      merge(i, mb, fmaf(a, a, fmaf(b, b, fmaf(c, c, d * d))), w, cw);
+    }
+  }
+  __device__ __forceinline__ void add(const Raw<T, N>& r) {
+    const float w = 1.f / (n + 1.f), cw = n * w;
+    n += 1.f;
+#pragma unroll
+    for (int i = 0; i < N; ++i) merge(i, element(r, i), 0.f, w, cw);
+  }
+  // The sets of the lanes TX, 2 TX, .. apart, in all of them.
+  __device__ __forceinline__ void merge_lanes(int TX) {
+    for (int o = TX; o < 32; o *= 2) {
+      const float nb = __shfl_xor_sync(kFullMask, n, o), w = nb > 0.f ? nb / (n + nb) : 0.f, cw = n * w;
+      n += nb;
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float d = __shfl_xor_sync(kFullMask, mean[i], o) - mean[i];
+        m2[i] = fmaf(d * d, cw, m2[i] + __shfl_xor_sync(kFullMask, m2[i], o));
+        mean[i] = fmaf(d, w, mean[i]);
+      }
+    }
+  }
+};
+
 // gpart[((s chunks + chunk) G + g) nsub + part] = (mean, sum of squared deviations) of the chunk's values of the group,
 // or of its part.
 template <typename T, int N, int NT>
@@ -559,42 +626,56 @@ __global__ void __launch_bounds__(NT, kFwdBlocks) norm_stats_kernel(NormParams p
   extern __shared__ float sf[];
   const Slab<N, NT> a = chunk_slab<N, NT>(p, blockIdx.x);
   const int64_t rf = norm_red(p.cs, N, NT);
-  float* r1 = sf;
-  float* r2 = sf + rf;
+  float* r1 = sf;                                       // [rows][csl] means
+  float* r2 = sf + rf;                                  // and squared deviations
   float* gm = r2 + rf;                                  // [ng]
   float* gv = gm + p.ng;
   const int cpg = a.cpg;
   const float n = (float)a.np;
+  const bool lanes = 32 % a.TX == 0;                    // a warp's lanes share columns (all of them are live)
   if (a.live()) {
     for (int col = a.tx; col < a.nv; col += a.TX) {
-      float k0[N], s1[N], s2[N];
       const int64_t c = a.c0 + (int64_t)col * N;
-      unpack<T, N>(read_x<T, N, false>(p, a.s, a.q0, c), k0);
+      RunningStats<T, N> st;
+      XColumn<T, N, false> x(p, a.s, a.q0 + a.ty, c, a.TY);
+      int q = a.ty;
+      for (; q + 3 * a.TY < a.np; q += 4 * a.TY, x.next(4)) {
+        const Raw<T, N> r[4] = {x.at(0), x.at(1), x.at(2), x.at(3)};
+        st.add4(r);
+      }
+      Raw<T, N> r[3];
 #pragma unroll
-      for (int i = 0; i < N; ++i) s1[i] = s2[i] = 0.f;
-      walk<4, T, N>(a, XColumn<T, N, false>(p, a.s, a.q0 + a.ty, c, a.TY), [&](const float (&f)[N], int) {
+      for (int k = 0; k < 3; ++k)
+        if (q + k * a.TY < a.np) r[k] = x.at(k);
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+        if (q + k * a.TY < a.np) st.add(r[k]);
+      if (lanes) st.merge_lanes(a.TX);
+      if (!lanes || (int)(threadIdx.x & 31) < a.TX) {
+        const int row = (lanes ? (int)threadIdx.x >> 5 : a.ty) * a.csl + col * N;
 #pragma unroll
         for (int i = 0; i < N; ++i) {
-          const float d = f[i] - k0[i];
-          s1[i] += d;
-          s2[i] = fmaf(d, d, s2[i]);
+          r1[row + i] = st.mean[i];
+          r2[row + i] = st.m2[i];
         }
-      });
-      a.put(s1, r1, col);
-      a.put(s2, r2, col);
+      }
     }
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < a.csl; c += NT) {       // channel c: mean and squared deviations
-    float t1 = 0.f, t2 = 0.f;
+  // Positions behind row r: of the `per` threads of its column, those from r per on.
+  const int per = lanes ? 32 / a.TX : 1, whole = a.np / a.TY, rest = a.np - whole * a.TY;
+  const auto behind = [&](int r) { return (float)(whole * per + min(max(rest - r * per, 0), per)); };
+  for (int c = threadIdx.x; c < a.csl; c += NT) {       // channel c: mean and squared deviations (row 0 has values)
+    const float m0 = r1[c];
+    float t = 0.f, v = 0.f;
+    for (int r = 1; r < a.rows; ++r) t = fmaf(behind(r), r1[r * a.csl + c] - m0, t);
+    const float mean = m0 + t / n;
     for (int r = 0; r < a.rows; ++r) {
-      t1 += r1[r * a.csl + c];
-      t2 += r2[r * a.csl + c];
+      const float k = behind(r), d = r1[r * a.csl + c] - mean;
+      if (k > 0.f) v += fmaf(k * d, d, r2[r * a.csl + c]);
     }
-    const float dm = t1 / n;
-    const float k0 = to_f32<T>(reinterpret_cast<const T*>(p.x)[a.s * p.sx + a.q0 * p.px + a.c0 + c]);
-    r1[c] = k0 + dm;
-    r2[c] = fmaxf(t2 - dm * t1, 0.f);
+    r1[c] = mean;
+    r2[c] = v;
   }
   __syncthreads();
   group_sums<NT>(r1, a.csl, 1, a.ngl, cpg, gm);

@@ -1,0 +1,49 @@
+"""Inputs at which the dense operators could come out wrong though ordinary draws do not show it: outliers where a
+chunk of the norm's statistics begins, non-finite values in the backward passes, fp32 values past bf16's range."""
+import pytest
+import torch
+
+import granulelayer_b200 as gl
+from granulelayer_b200 import dense
+
+pytestmark = pytest.mark.gpu
+F32, BF16 = torch.float32, torch.bfloat16
+
+
+def data(*shape, dtype=F32, seed=0, scale=1.0):
+    gen = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=gen, device="cuda") * scale).to(dtype)
+
+
+# ---- group norm: statistics ----
+
+@pytest.mark.parametrize("rest", ["normal", "constant"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("shape,G", [((64, 4096, 512), 32), ((600, 4096, 64), 8), ((16, 4096, 512), 32),
+                                     ((300, 5000, 24), 3)])
+def test_norm_statistics_with_an_outlier_at_the_first_position(shape, G, dtype, rest):
+    """One channel of every group is 1000 at position 0, the other positions are N(0, 1) or all alike.  A thread sums
+    squared deviations, all positive, over at most 256 positions of its column, two roundings for four positions; some 60 more
+    follow where threads, channels and chunks meet: (2 * 64 + 64) 2^-24 = 1.1e-5 < 2^-16."""
+    S, P, C = shape
+    x = data(*shape, seed=1) if rest == "normal" else torch.full(shape, 0.5, device="cuda")
+    x[:, 0, :: C // G] = 1000.0
+    x = x.to(dtype)
+    _, _, stats = dense._norm_forward(x, G, None, None, 0, 1e-5)
+    var, mean = torch.var_mean(x.double().reshape(S, P, G, C // G), dim=(1, 3), correction=0)
+    got_var = stats[1].double() ** -2 - 1e-5
+    assert float(((got_var - var).abs() / (var + 1e-5)).max()) < 2.0 ** -16
+    assert float(((stats[0].double() - mean).abs() / (mean.abs() + var.sqrt())).max()) < 2.0 ** -16
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_norm_non_finite_values_in_long_samples(dtype):
+    """A NaN and an infinity, at a chunk's first position and inside, reach their groups only."""
+    x = data(2, 70000, 16, dtype=dtype, seed=2)
+    clean = gl.group_norm_act(x, 4)
+    x[0, 0, 1], x[1, 0, 6], x[1, 33333, 15] = float("nan"), float("inf"), -float("inf")
+    y = gl.group_norm_act(x, 4)
+    hit = torch.zeros(2, 1, 16, dtype=torch.bool, device="cuda")
+    hit[0, :, 0:4] = hit[1, :, 4:8] = hit[1, :, 12:16] = True
+    hit = hit.expand(x.shape)
+    assert torch.equal(y[~hit], clean[~hit]) and bool(torch.isnan(y[hit]).all())
