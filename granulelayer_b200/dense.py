@@ -140,6 +140,8 @@ def _grad_buffers(weight, need_w: bool, bias, need_b: bool):
         g = getattr(p, "main_grad", None) if want else None
         if g is not None and (g.dtype != torch.float32 or not g.is_contiguous() or g.shape != p.shape):
             raise ValueError("main_grad must be a contiguous float32 tensor of the parameter's shape")
+        if g is not None and g.device != p.device:      # the kernels take its address
+            raise ValueError(f"main_grad is on device {g.device}, its parameter on {p.device}")
         out.append(g if g is not None or not want else torch.zeros(p.shape, dtype=torch.float32, device=p.device))
     return out[0], out[1], True
 
@@ -340,6 +342,17 @@ def group_norm_act(x: torch.Tensor, num_groups: int, weight: Optional[torch.Tens
 # ---- modules ----
 
 class _MainGradModule(nn.Module):
+    def _apply(self, fn, recurse=True):
+        """Moves ``main_grad`` to where its parameter goes (to(), cuda()); its type stays fp32."""
+        kept = {n: getattr(p, "main_grad", None) for n, p in self._parameters.items()}
+        super()._apply(fn, recurse)
+        for n, p in self._parameters.items():
+            g = kept[n]
+            if g is not None:
+                p.main_grad = (g if g.device == p.device else torch.zeros(g.shape, dtype=g.dtype, device=p.device)
+                               if g.is_meta else g.to(p.device))
+        return self
+
     def enable_main_grad(self):
         """Accumulate parameter gradients into persistent FP32 ``main_grad`` buffers (autograd then returns None
         for them), as SparsePoolingLayer.enable_main_grad."""
