@@ -165,7 +165,8 @@ static int check_act8(const GlAct8Args* a, bool encode) {
   if (a->dtype != GL_DTYPE_F32 && a->dtype != GL_DTYPE_BF16) return GL_ERR_UNSUPPORTED;
   if (a->rows == 0) return GL_OK;
   if (!(encode ? a->x : (const void*)a->out) || !a->codes || !a->exps) return GL_ERR_NULL;
-  if ((uintptr_t)a->codes & 15) return GL_ERR_ALIGN;
+  if (off_type(a->dtype == GL_DTYPE_F32 ? 4 : 2, encode ? a->x : (const void*)a->out) || off_type(16, a->codes))
+    return GL_ERR_ALIGN;
   return GL_OK;
 }
 

@@ -23,6 +23,12 @@ __device__ __forceinline__ float from_f32<float>(float v) { return v; }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
+// Host: any of the given pointers (NULL: absent) is no multiple of `bytes`.
+template <typename... P>
+inline bool off_type(int bytes, P... p) {
+  return ((reinterpret_cast<uintptr_t>(p) | ...) & (uintptr_t)(bytes - 1)) != 0;
+}
+
 // V consecutive elements as fp32; V * sizeof(T) = 16 bytes (aligned) or V = 1.
 template <typename T>
 constexpr int kVec16 = 16 / (int)sizeof(T);

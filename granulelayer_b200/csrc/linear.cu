@@ -320,6 +320,7 @@ static int run_rows(const GlLinearArgs& a, const LinEpilogue& e, bool aligned, c
 static bool rows16(const void* p, int64_t ld, int esize) {
   return ((uintptr_t)p & 15) == 0 && (ld * esize) % 16 == 0;
 }
+static int slope_bytes(int kind) { return kind == GL_SLOPE_F32 ? 4 : kind == GL_SLOPE_I16 ? 2 : 1; }
 static int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
 static int lin_checks(int64_t M, int64_t N, int64_t K, int dtype, int act) {
@@ -430,7 +431,7 @@ template <typename T>
 static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, cudaStream_t st) {
   constexpr int NP = sizeof(T) == 4 ? 3 : 1;
   char* work = (char*)a.work;
-  const int ss = a.slope_kind == GL_SLOPE_F32 ? 4 : 2;
+  const int ss = slope_bytes(a.slope_kind);
   const bool aligned = rows16(a.dy, a.lddy, sizeof(T)) &&
                        (a.slope_kind == GL_SLOPE_NONE ||
                         (a.slope_kind == GL_SLOPE_U8 ? (((uintptr_t)a.slope | a.lds) & 7) == 0 : rows16(a.slope, a.lds, ss)));
@@ -521,6 +522,8 @@ extern "C" int gl_linear_fwd(const GlLinearArgs* args, void* stream) {
   if (a.M == 0) return GL_OK;
   if (!a.x || !a.w || !a.y || (a.slope_kind && !a.slope)) return GL_ERR_NULL;
   const int es = a.dtype == GL_DTYPE_F32 ? 4 : 2;
+  if (off_type(es, a.x, a.w, a.bias, a.residual, a.y) || off_type(slope_bytes(a.slope_kind), a.slope))
+    return GL_ERR_ALIGN;
   const LinEpilogue e{a.bias, a.residual, a.y, a.slope, a.ldr, a.ldy, a.lds, a.dtype, a.act, a.slope_kind};
   const bool aligned = rows16(a.x, a.ldx, es) && rows16(a.w, a.ldw, es);
   cudaStream_t st = (cudaStream_t)stream;
@@ -557,8 +560,10 @@ extern "C" int gl_linear_bwd(const GlLinearBwdArgs* args, void* stream) {
   if (!a.dy || (a.slope_kind && !a.slope) || (a.dx && !a.w) ||
       (a.dw && !codes && !a.x) || (codes && !a.exps))
     return GL_ERR_NULL;
-  if (codes && ((uintptr_t)a.codes & 15)) return GL_ERR_ALIGN;
   const int es = a.dtype == GL_DTYPE_F32 ? 4 : 2;
+  if (off_type(es, a.dy, codes ? nullptr : a.x, a.w, a.dx) || off_type(a.accumulate ? 4 : es, a.dw, a.db) ||
+      off_type(slope_bytes(a.slope_kind), a.slope) || off_type(16, a.codes))
+    return GL_ERR_ALIGN;
   const bool aligned = (!a.dx || rows16(a.w, a.ldw, es)) && (!a.dw || codes || rows16(a.x, a.ldx, es));
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;

@@ -1357,6 +1357,9 @@ extern "C" int gl_norm_fwd(const GlNormArgs* args, void* stream) {
   if (a.px < a.C || a.sx < 0) return GL_ERR_SHAPE;
   if (a.S == 0 || a.P == 0) return GL_OK;
   if (!a.x || !a.y || !a.mean || !a.rstd) return GL_ERR_NULL;
+  if (off_type(a.dtype == GL_DTYPE_F32 ? 4 : 2, a.x, a.y) || off_type(a.pdtype == GL_DTYPE_F32 ? 4 : 2, a.w, a.b) ||
+      off_type(4, a.mean, a.rstd) || off_type(16, a.work))
+    return GL_ERR_ALIGN;
   int sms = 0, smem = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   if (int rc = device_smem_optin(&smem)) return rc;
@@ -1386,7 +1389,11 @@ extern "C" int gl_norm_bwd(const GlNormBwdArgs* args, void* stream) {
   cudaStream_t st = (cudaStream_t)stream;
   if (a.S == 0 || a.P == 0) return zero_params(a, st);
   if (!a.dy || !a.dx || !a.mean || !a.rstd || (!ckpt && !a.x) || (ckpt && !a.exps) || !a.work) return GL_ERR_NULL;
-  if (ckpt && ((uintptr_t)a.codes & 15)) return GL_ERR_ALIGN;
+  if (off_type(a.dtype == GL_DTYPE_F32 ? 4 : 2, ckpt ? nullptr : a.x, a.dy, a.dx) ||
+      off_type(a.pdtype == GL_DTYPE_F32 ? 4 : 2, a.w, a.b) ||
+      off_type(a.accumulate || a.pdtype == GL_DTYPE_F32 ? 4 : 2, a.dw, a.db) || off_type(4, a.mean, a.rstd) ||
+      off_type(16, a.work, a.codes))
+    return GL_ERR_ALIGN;
   int sms = 0, smem = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   if (int rc = device_smem_optin(&smem)) return rc;

@@ -496,7 +496,8 @@ int gl_k16_bwd_t5_f32(const GlK16Args* args, int32_t* status, void* stream);
  * Storage is fp32 or bf16 (`dtype`), all arithmetic and every sum fp32.  Rows have unit element stride and
  * the row strides given (elements).  Activations: GL_ACT_IDENTITY / RELU / GELU (erf form) / SILU.
  * `work` is caller-owned scratch of at least the *_work_bytes of the call's sizes (negative = GlStatus); it may be
- * NULL where that is 0.
+ * NULL where that is 0.  Pointers are multiples of their element's size (GL_ERR_ALIGN); `work` of 256 bytes for
+ * gl_linear_*, of 16 for gl_norm_*.
  * fp32 products run on the tensor cores as the six products of three-term bf16 splits (as gl_k16_fwd_tc_f32) and
  * agree with fp32 arithmetic to its rounding; an infinity in such an operand gives NaN.  Every wait in these
  * kernels has an iteration limit; a tile whose wait ran out is written as NaN. */
