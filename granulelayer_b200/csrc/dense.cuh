@@ -200,12 +200,15 @@ __device__ __forceinline__ float act8_scale(int byte) {
   return byte == 255 ? __int_as_float(0x7FC00000) : __int_as_float(byte << 23);
 }
 
-// act'(z) as one byte: rint(192 d) + 32, d in [-1/6, 1.161]; 0 and 1 are exact.
+// act'(z) as one byte: rint(192 d) + 32, d in [-1/6, 1.156]; 0 and 1 are exact.  Code 255, past every act' (the largest,
+// GELU's, is 1.129), is a NaN.
 __device__ __forceinline__ uint32_t slope_code(float d) {
-  return (uint32_t)(min(max(__float2int_rn(d * 192.f), -32), 223) + 32);
+  return d != d ? 255u : (uint32_t)(min(max(__float2int_rn(d * 192.f), -32), 222) + 32);
 }
 
-__device__ __forceinline__ float slope_value(uint32_t code) { return (float)((int)code - 32) * (1.f / 192.f); }
+__device__ __forceinline__ float slope_value(uint32_t code) {
+  return code == 255u ? __int_as_float(0x7FC00000) : (float)((int)code - 32) * (1.f / 192.f);
+}
 
 // act'(z) in 16 bits (bf16 layers): steps of 2^-14, exact at 0 and 1.  A NaN becomes the code that reads as -2, which
 // no act' has; it reads back as NaN.

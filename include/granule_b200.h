@@ -505,7 +505,7 @@ int gl_k16_bwd_t5_f32(const GlK16Args* args, int32_t* status, void* stream);
 /* Forward of a fused matrix product: y = act(z) + residual, z[m, n] = sum_k x[m, k] w[n, k] + bias[n].
  * `bias` [N] and `residual` [M, ldr] are optional.  For the backward pass the call also keeps act'(z) in `slope`
  * [M, lds] as `slope_kind` says: GL_SLOPE_F32 as it is, GL_SLOPE_I16 round(2^14 act'(z)), GL_SLOPE_U8
- * round(192 act'(z)) + 32 (both exact at 0 and 1). */
+ * round(192 act'(z)) + 32 (both exact at 0 and 1; a NaN is -2^15 or 255). */
 enum { GL_SLOPE_NONE = 0, GL_SLOPE_F32 = 1, GL_SLOPE_I16 = 2, GL_SLOPE_U8 = 3 };
 typedef struct GlLinearArgs {
   const void* x;            /* [M, ldx] */

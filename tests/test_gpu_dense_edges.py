@@ -47,3 +47,34 @@ def test_norm_non_finite_values_in_long_samples(dtype):
     hit[0, :, 0:4] = hit[1, :, 4:8] = hit[1, :, 12:16] = True
     hit = hit.expand(x.shape)
     assert torch.equal(y[~hit], clean[~hit]) and bool(torch.isnan(y[hit]).all())
+
+
+# ---- linear: non-finite values ----
+
+@pytest.mark.parametrize("ckpt", ["none", "int8"])
+@pytest.mark.parametrize("act", ["relu", "gelu", "silu"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("M", [3, 70])
+def test_linear_gradients_keep_a_nan(M, dtype, act, ckpt):
+    """A NaN in the bias makes act'(z) of its column NaN, one in a row of x that of its row: with a finite dy the
+    gradients that contain it are NaN, the others are what they were."""
+    x, w, b = data(M, 96, dtype=dtype, seed=1), data(40, 96, dtype=dtype, seed=2, scale=0.1), data(40, dtype=dtype, seed=3)
+    dy = data(M, 40, dtype=dtype, seed=4)
+
+    def grads(x, b):
+        leaves = [t.detach().clone().requires_grad_(True) for t in (x, w, b)]
+        return torch.autograd.grad(gl.linear_act(*leaves, activation=act, checkpoint=ckpt), leaves, dy)
+
+    dx0, dw0, db0 = grads(x, b)
+    bad = b.clone()
+    bad[7] = float("nan")
+    dx, dw, db = grads(x, bad)
+    keep = torch.arange(40, device="cuda") != 7
+    assert bool(torch.isnan(dx).all()) and bool(torch.isnan(dw[7]).all()) and bool(torch.isnan(db[7]))
+    assert torch.equal(dw[keep], dw0[keep]) and torch.equal(db[keep], db0[keep])
+    bad = x.clone()
+    bad[1, 5] = float("nan")
+    dx, dw, db = grads(bad, b)
+    keep = torch.arange(M, device="cuda") != 1
+    assert bool(torch.isnan(dx[1]).all()) and torch.equal(dx[keep], dx0[keep])
+    assert bool(torch.isnan(db).all()) and bool(torch.isnan(dw).all())
