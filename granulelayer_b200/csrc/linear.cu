@@ -4,7 +4,8 @@
 //
 // The products run on the tensor cores (mma.cu).  bf16 operands whose rows are 16-byte aligned are read where they
 // lie; others are first copied to aligned rows, and fp32 operands are split into three bf16 planes
-// (v = v1 + v2 + v3, 24 significand bits for 2^-110 <= |v| below bf16's largest value; an infinity gives NaN).
+// (v = v1 + v2 + v3, 24 significand bits for 2^-110 <= |v|; an infinity gives NaN, since it meets all of the other operand's
+// terms, of either sign or zero).
 // An 8-bit checkpoint of x is one plane even for fp32 layers: its values are bf16 numbers.  A few rows (serving
 // single tokens) run row kernels instead, which read w once and are bound by HBM.
 //
@@ -16,7 +17,13 @@ namespace gl {
 
 // ---- operands for the tensor cores ----
 
-// v as NP bf16 terms.  A NaN or an infinity stays in the first term (and its remainder is NaN).
+__device__ __forceinline__ float bf16_range(float v) {
+  constexpr float kMost = 3.38953138925153547590e38f;                 // 0x7F7F
+  return fabsf(v) < INFINITY ? fminf(fmaxf(v, -kMost), kMost) : v;    // a NaN or an infinity as it is
+}
+
+// v as NP bf16 terms.  A NaN or an infinity stays in the first term (and its remainder is NaN); of several terms the first
+// is at most bf16's largest value, so that finite values above it (to fp32's largest, 2^-9 more) stay finite.
 template <int NP>
 __device__ __forceinline__ void bf16_terms(const float (&v)[8], uint4 (&out)[NP]) {
   float r[8];
@@ -27,7 +34,7 @@ __device__ __forceinline__ void bf16_terms(const float (&v)[8], uint4 (&out)[NP]
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u[i] = pack_bf16(r[2 * i], r[2 * i + 1]);
+      u[i] = NP > 1 && j == 0 ? pack_bf16(bf16_range(r[2 * i]), bf16_range(r[2 * i + 1])) : pack_bf16(r[2 * i], r[2 * i + 1]);
       r[2 * i] -= __uint_as_float(u[i] << 16);
       r[2 * i + 1] -= __uint_as_float(u[i] & 0xFFFF0000u);
     }

@@ -78,3 +78,30 @@ def test_linear_gradients_keep_a_nan(M, dtype, act, ckpt):
     keep = torch.arange(M, device="cuda") != 1
     assert bool(torch.isnan(dx[1]).all()) and torch.equal(dx[keep], dx0[keep])
     assert bool(torch.isnan(db).all()) and bool(torch.isnan(dw).all())
+
+
+@pytest.mark.parametrize("M", [8, 9, 200])
+def test_linear_fp32_values_past_the_range_of_bf16(M):
+    """Finite fp32 values above bf16's largest, 3.39e38: their products with small weights and gradients are numbers,
+    by the row kernels (8 rows) and by the tensor cores alike.  Six products of split terms per 16 k in any order:
+    (16 + 6 K / 16) 2^-23 of the sum of magnitudes."""
+    K, N = 64, 48
+    x = data(M, K, seed=1)
+    x[0, 3], x[1, 40], x[M - 1, 0] = torch.finfo(F32).max, -3.4e38, 3.395e38
+    w = data(N, K, seed=2, scale=1e-3).requires_grad_(True)
+    x.requires_grad_(True)
+    dy = data(M, N, seed=3, scale=1e-3)
+    y = gl.linear_act(x, w)
+    dx, dw = torch.autograd.grad(y, (x, w), dy)
+    X, W, DY = x.detach().double(), w.detach().double(), dy.double()
+
+    def close(got, a, b, k):
+        err = (got.double() - a @ b).abs()
+        assert bool((err <= (16 + 6 * k / 16) * 2.0 ** -23 * (a.abs() @ b.abs())).all())
+
+    close(y, X, W.t(), K)
+    close(dw, DY.t(), X, M)
+    close(dx, DY, W, N)
+    big = torch.full((M, N), 3.4e38, device="cuda")                   # and as an output gradient
+    (dx,) = torch.autograd.grad(gl.linear_act(x, w), x, big * torch.eye(M, N, device="cuda"))
+    close(dx, (big * torch.eye(M, N, device="cuda")).double(), W, N)
