@@ -171,16 +171,19 @@ class LinearActFunction(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, act, checkpoint):
         N, K = weight.shape
+        need_x, need_w, need_b = ctx.needs_input_grad[:3]
         x2, w2 = _rows(x, K), _rows(weight, K)
         slope = codes = exps = None
-        if act != 0:
+        if act != 0 and (need_x or need_w or need_b):
             slope = x2.new_empty((x2.shape[0], N), dtype=torch.uint8 if checkpoint == "int8" else _SLOPE_DTYPES[x.dtype])
         y = _linear_forward(x2, w2, bias, None if residual is None else _rows(residual, N), act, slope)
-        if checkpoint == "int8":
+        if not need_w:                                   # only dW reads x
+            x2 = None
+        elif checkpoint == "int8":
             codes, exps = _encode(x2)
             x2 = None
-        ctx.save_for_backward(x2, codes, exps, weight, bias, slope)
-        ctx.xshape = x.shape
+        ctx.save_for_backward(x2, codes, exps, weight if need_x or need_w else None, bias if need_b else None, slope)
+        ctx.xshape, ctx.K = x.shape, K
         return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
 
     @staticmethod
@@ -188,7 +191,7 @@ class LinearActFunction(torch.autograd.Function):
         _no_double_backward("linear_act")
         x2, codes, exps, weight, bias, slope = ctx.saved_tensors
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
-        N, K = weight.shape
+        N, K = dy.shape[-1], ctx.K
         dx = w2 = None
         if need_x:
             dx, w2 = dy.new_empty(ctx.xshape), _rows(weight, K)

@@ -4,7 +4,7 @@ import pytest
 import torch
 
 import granulelayer_b200 as gl
-from granulelayer_b200 import dense
+from granulelayer_b200 import _native, dense
 
 pytestmark = pytest.mark.gpu
 F32, BF16 = torch.float32, torch.bfloat16
@@ -105,3 +105,67 @@ def test_linear_fp32_values_past_the_range_of_bf16(M):
     big = torch.full((M, N), 3.4e38, device="cuda")                   # and as an output gradient
     (dx,) = torch.autograd.grad(gl.linear_act(x, w), x, big * torch.eye(M, N, device="cuda"))
     close(dx, (big * torch.eye(M, N, device="cuda")).double(), W, N)
+
+
+# ---- what is kept between the passes ----
+
+def kept_by(call):
+    """(output, what autograd keeps for it as (shape, dtype)) of a call."""
+    kept = []
+
+    def pack(t):
+        kept.append((tuple(t.shape), t.dtype))
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(pack, lambda t: t):
+        out = call()
+    return out, kept
+
+
+@pytest.mark.parametrize("ckpt", ["none", "int8"])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("wants", ["x", "w", "b", "r", "xb", "wr"])
+def test_linear_keeps_what_its_gradients_need(wants, dtype, ckpt):
+    """x (or its codes, whose encoding is a launch) only for the weight's gradient, act'(z) only for those of x, weight
+    and bias; the gradients are those of a call that wants them all."""
+    M, K, N = 72, 160, 48
+    given = dict(x=data(M, K, dtype=dtype, seed=1), w=data(N, K, dtype=dtype, seed=2, scale=0.1),
+                 b=data(N, dtype=dtype, seed=3), r=data(M, N, dtype=dtype, seed=4))
+    dy = data(M, N, dtype=dtype, seed=5)
+
+    def run(names):
+        """The gradients that are asked for, of a call whose `names` can have one."""
+        leaves = {n: t.clone().requires_grad_(n in names) for n, t in given.items()}
+        n0 = _native.launch_count()
+        y, kept = kept_by(lambda: gl.linear_act(*leaves.values(), activation="gelu", checkpoint=ckpt))
+        launches = _native.launch_count() - n0
+        return dict(zip(wants, torch.autograd.grad(y, [leaves[n] for n in wants], dy))), kept, launches, y
+
+    every, _, most, y0 = run("xwbr")
+    got, kept, launches, y = run(wants)
+    assert torch.equal(y, y0)
+    for n in wants:
+        assert torch.equal(got[n], every[n]), n
+    shapes = [s for s, _ in kept]
+    assert ((M, K) in shapes) == ("w" in wants)                     # x, or its codes (K is whole blocks)
+    assert ((M, N) in shapes) == any(n in wants for n in "xwb")     # act'(z)
+    assert launches == most - (ckpt == "int8" and "w" not in wants)
+
+
+@pytest.mark.parametrize("ckpt,per_x,per_z", [("none", 2, 2), ("int8", 33 / 32, 1)])
+def test_checkpoints_lower_the_memory_between_the_passes(ckpt, per_x, per_z):
+    """Bytes held from a forward pass to its backward pass, beside output and parameters: x and act'(z) in two bytes
+    each (bf16), or in 33/32 and one.  The allocator rounds each of at most four tensors up to 512 bytes."""
+    M, K, N, G = 512, 1024, 768, 32
+    base = data(M, K, dtype=BF16, seed=1).requires_grad_(True)
+    w = data(N, K, dtype=BF16, seed=2, scale=0.03).requires_grad_(True)
+    gam = data(K, dtype=BF16, seed=3).requires_grad_(True)
+    for call, held in ((lambda x: gl.linear_act(x, w, activation="gelu", checkpoint=ckpt), M * K * per_x + M * N * per_z),
+                       (lambda x: gl.group_norm_act(x, G, gam, checkpoint=ckpt), M * K * per_x + 2 * M * G * 4)):
+        call(base * 1)                                              # anything that first calls allocate
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        y = call(base * 1)
+        now = torch.cuda.memory_allocated() - before - y.numel() * 2
+        assert held <= now <= held + 5 * 512, (now, held)
+        del y
