@@ -16,7 +16,7 @@ from pathlib import Path
 
 import torch
 
-ABI_VERSION = 18
+ABI_VERSION = 19
 LIB_PATH = Path(__file__).resolve().parent / "_lib" / "libgranule_b200.so"
 
 POOL_MEAN, POOL_SUM, POOL_MAX, POOL_LME, POOL_POWER, POOL_SOFTMAX, POOL_TOPK = 0, 1, 2, 3, 4, 5, 6
@@ -121,13 +121,14 @@ class GlK16Args(ctypes.Structure):
 
 
 class GlLinearArgs(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "w", "bias", "residual", "y", "slope", "work")] + \
+    _fields_ = [(n, ctypes.c_void_p) for n in ("x", "w", "bias", "residual", "y", "slope", "work", "status")] + \
                [(n, ctypes.c_int64) for n in ("M", "N", "K", "ldx", "ldw", "ldr", "ldy", "lds", "work_bytes")] + \
                [(n, ctypes.c_int32) for n in ("dtype", "act", "slope_kind", "reserved")]
 
 
 class GlLinearBwdArgs(ctypes.Structure):
-    _fields_ = [(n, ctypes.c_void_p) for n in ("dy", "slope", "x", "codes", "exps", "w", "dx", "dw", "db", "work")] + \
+    _fields_ = [(n, ctypes.c_void_p) for n in ("dy", "slope", "x", "codes", "exps", "w", "dx", "dw", "db", "work",
+                                                "status")] + \
                [(n, ctypes.c_int64) for n in ("M", "N", "K", "lddy", "lds", "ldx", "ldc", "ldw", "lddx",
                                               "work_bytes")] + \
                [(n, ctypes.c_int32) for n in ("dtype", "slope_kind", "accumulate", "reserved")]
@@ -750,6 +751,26 @@ def _launch(name: str, a, dev: torch.device):
         _check(lib, rc, name)
 
 
+_wait_word = None   # (pinned tensor, its int32, its address): set by a wait of a product that ran out, on any device
+
+
+def _wait_status() -> int:
+    """Where the products of the linear operator report a wait that ran out (0: nowhere yet, inside a graph capture).
+    Raises for one that has, at the first call after it (the launch itself succeeded, and what it left uncomputed is NaN).
+    Reading the word needs no synchronisation."""
+    global _wait_word
+    if _wait_word is None:
+        if torch.cuda.is_current_stream_capturing():
+            return 0
+        t = torch.zeros(1, dtype=torch.int32, pin_memory=True)
+        _wait_word = (t, ctypes.c_int32.from_address(t.data_ptr()), t.data_ptr())
+    word = _wait_word[1]
+    if word.value:
+        word.value = 0
+        raise NativeLibraryError("a wait inside an earlier linear_act product ran out of time; its results are NaN")
+    return _wait_word[2]
+
+
 def _unaligned(*rows) -> int:
     """GL_LINEAR_UNALIGNED where a matrix's base or row stride is no multiple of 16 bytes."""
     for t in rows:
@@ -771,8 +792,9 @@ def linear_fwd(x, w, bias, residual, y, slope, act: int):
     _launch("gl_linear_fwd", GlLinearArgs(
         x.data_ptr(), w.data_ptr(), 0 if bias is None else bias.data_ptr(),
         0 if residual is None else residual.data_ptr(), y.data_ptr(), 0 if slope is None else slope.data_ptr(),
-        work.data_ptr(), M, N, K, x.stride(0), w.stride(0), 0 if residual is None else residual.stride(0), N,
-        0 if slope is None else N, work.numel(), dt, act, 0 if slope is None else _SLOPE_KINDS[slope.dtype], 0), dev)
+        work.data_ptr(), _wait_status(), M, N, K, x.stride(0), w.stride(0),
+        0 if residual is None else residual.stride(0), N, 0 if slope is None else N, work.numel(), dt, act,
+        0 if slope is None else _SLOPE_KINDS[slope.dtype], 0), dev)
 
 
 def linear_bwd(dy, slope, x, codes, exps, w, dx, dw, db, K: int, accumulate: bool):
@@ -784,9 +806,9 @@ def linear_bwd(dy, slope, x, codes, exps, w, dx, dw, db, K: int, accumulate: boo
                  _unaligned(None if dx is None else w, None if dw is None else x))
     _launch("gl_linear_bwd", GlLinearBwdArgs(
         dy.data_ptr(), _ptr(slope), _ptr(x), _ptr(codes), _ptr(exps), _ptr(w), _ptr(dx), _ptr(dw), _ptr(db),
-        work.data_ptr(), M, N, K, dy.stride(0), 0 if slope is None else N, 0 if x is None else x.stride(0),
-        0 if codes is None else codes.stride(0), 0 if w is None else w.stride(0), K, work.numel(), dt,
-        0 if slope is None else _SLOPE_KINDS[slope.dtype], int(accumulate), 0), dev)
+        work.data_ptr(), _wait_status(), M, N, K, dy.stride(0), 0 if slope is None else N,
+        0 if x is None else x.stride(0), 0 if codes is None else codes.stride(0), 0 if w is None else w.stride(0), K,
+        work.numel(), dt, 0 if slope is None else _SLOPE_KINDS[slope.dtype], int(accumulate), 0), dev)
 
 
 def _pdtype(*params) -> int:

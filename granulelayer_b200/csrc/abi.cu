@@ -150,10 +150,10 @@ extern "C" const char* gl_status_string(int status) {
   F(D) F(G) F(NB16) F(Q) F(S) F(nbuckets) F(ldx) F(ldp) F(ldc) F(lddx) F(act) F(tokens)
 
 #define GL_LINEAR_FIELDS(F)                                                                                      \
-  F(x) F(w) F(bias) F(residual) F(y) F(slope) F(work) F(M) F(N) F(K) F(ldx) F(ldw) F(ldr) F(ldy) F(lds)          \
+  F(x) F(w) F(bias) F(residual) F(y) F(slope) F(work) F(status) F(M) F(N) F(K) F(ldx) F(ldw) F(ldr) F(ldy) F(lds)          \
   F(work_bytes) F(dtype) F(act) F(slope_kind) F(reserved)
 #define GL_LINEAR_BWD_FIELDS(F)                                                                                  \
-  F(dy) F(slope) F(x) F(codes) F(exps) F(w) F(dx) F(dw) F(db) F(work) F(M) F(N) F(K) F(lddy) F(lds) F(ldx)       \
+  F(dy) F(slope) F(x) F(codes) F(exps) F(w) F(dx) F(dw) F(db) F(work) F(status) F(M) F(N) F(K) F(lddy) F(lds) F(ldx)       \
   F(ldc) F(ldw) F(lddx) F(work_bytes) F(dtype) F(slope_kind) F(accumulate) F(reserved)
 #define GL_NORM_FIELDS(F)                                                                                        \
   F(x) F(w) F(b) F(y) F(mean) F(rstd) F(work) F(S) F(P) F(C) F(G) F(sx) F(px) F(work_bytes) F(dtype) F(pdtype)   \

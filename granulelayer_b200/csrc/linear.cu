@@ -417,7 +417,7 @@ static int run_linear_fwd(const GlLinearArgs& a, const LinEpilogue& e, const Lin
   const MmaOperand wt = pack.add(a.w, a.N, a.K, a.ldw, 0, work + w.w);
   if (int rc = pack.run(sms, st)) return rc;
   const MmaJob job{x, wt, a.M, a.N, a.K, e};
-  return mma_run(&job, 1, SumRows{}, work + w.split, st);
+  return mma_run(&job, 1, SumRows{}, work + w.split, a.status, st);
 }
 
 template <typename T, int KIND>
@@ -502,7 +502,7 @@ static int run_linear_bwd(const GlLinearBwdArgs& a, const LinWork& w, int sms, c
     dz.mn = 1;
     jobs[n++] = MmaJob{dz, x, a.N, a.K, a.M, e};
   }
-  return mma_run(jobs, n, db, work + w.split, st);
+  return mma_run(jobs, n, db, work + w.split, a.status, st);
 }
 
 }  // namespace gl
@@ -529,7 +529,8 @@ extern "C" int gl_linear_fwd(const GlLinearArgs* args, void* stream) {
   if (a.M == 0) return GL_OK;
   if (!a.x || !a.w || !a.y || (a.slope_kind && !a.slope)) return GL_ERR_NULL;
   const int es = a.dtype == GL_DTYPE_F32 ? 4 : 2;
-  if (off_type(es, a.x, a.w, a.bias, a.residual, a.y) || off_type(slope_bytes(a.slope_kind), a.slope))
+  if (off_type(es, a.x, a.w, a.bias, a.residual, a.y) || off_type(slope_bytes(a.slope_kind), a.slope) ||
+      off_type(4, a.status))
     return GL_ERR_ALIGN;
   const LinEpilogue e{a.bias, a.residual, a.y, a.slope, a.ldr, a.ldy, a.lds, a.dtype, a.act, a.slope_kind};
   const bool aligned = rows16(a.x, a.ldx, es) && rows16(a.w, a.ldw, es);
@@ -569,7 +570,7 @@ extern "C" int gl_linear_bwd(const GlLinearBwdArgs* args, void* stream) {
     return GL_ERR_NULL;
   const int es = a.dtype == GL_DTYPE_F32 ? 4 : 2;
   if (off_type(es, a.dy, codes ? nullptr : a.x, a.w, a.dx) || off_type(a.accumulate ? 4 : es, a.dw, a.db) ||
-      off_type(slope_bytes(a.slope_kind), a.slope) || off_type(16, a.codes))
+      off_type(slope_bytes(a.slope_kind), a.slope) || off_type(16, a.codes) || off_type(4, a.status))
     return GL_ERR_ALIGN;
   const bool aligned = (!a.dx || rows16(a.w, a.ldw, es)) && (!a.dw || codes || rows16(a.x, a.ldx, es));
   int sms = 0;

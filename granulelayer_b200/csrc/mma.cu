@@ -21,8 +21,8 @@
 //
 // K-major tiles are one TMA box (64 k wide, all rows of the tile); MN-major tiles are boxes of 64 rows by 64 k, which
 // the matrix descriptor walks with 2048 bytes per 16 k and 8192 bytes per 64 rows.  Edges in every dimension are
-// the tensor map's zero fill.  Every wait has an iteration limit; a CTA whose wait runs out writes NaN to what it
-// has not computed, waits (again bounded) for its own copies and leaves.
+// the tensor map's zero fill.  Every wait has a limit in time and in iterations; a CTA whose wait runs out sets the call's
+// status word, writes NaN to what it has not computed, waits (again bounded) for its own copies and leaves.
 #include <cuda.h>
 
 #include "mma.cuh"
@@ -31,7 +31,11 @@
 namespace gl {
 
 constexpr int kMmBM = 128, kMmBK = 64, kMmThreads = 320, kMmEpiWarps = 8, kMmMaxSlots = 20;
-constexpr uint32_t kMmWaitLimit = 1u << 20;
+// A wait gives up after 4 s by the GPU's clock and 2^17 polls, or after 2^28 polls.  The longest that a sound launch waits is
+// an epilogue for its tile's sum: at most 2^25 blocks of k in 32 splits, 0.4 s.
+constexpr uint64_t kMmWaitNs = 4000000000ull;
+constexpr uint32_t kMmWaitPolls = 1024, kMmWaitLeast = 128, kMmWaitMost = 1u << 18;
+constexpr uint32_t kMmWaitLimit = 1u << 20;                    // polls for copies that are on their way
 constexpr int kMmPitch = 36;                                   // floats per row of a warp's 32 x 32 epilogue tile
 constexpr uint32_t kMmEpiBytes = kMmEpiWarps * 32 * kMmPitch * 4;
 
@@ -49,6 +53,7 @@ struct MmaParams {
   int chunk, slots;
   uint32_t a_slot, b_bytes;    // bytes of a slot for A, for B
   SumRows side;
+  int32_t* status;             // optional: set to 1 by a wait that ran out
 };
 
 // A slot: a plane of A (128 rows, or as many as there are) and of B (this CTA's share of BN rows), 64 k each; the ring
@@ -60,6 +65,7 @@ struct MmaShared {
   uint64_t full[kMmMaxSlots], empty[kMmMaxSlots], done[4], free_[4];
   uint32_t tmem;
   int dead;
+  int32_t* status;
 };
 
 __device__ __forceinline__ void mm_expect(uint32_t bar, uint32_t bytes) {
@@ -97,16 +103,30 @@ __device__ __forceinline__ void mm_load(uint32_t dst, const CUtensorMap* map, in
   }
 }
 
+__device__ __forceinline__ uint64_t mm_now() {
+  uint64_t ns;
+  asm volatile("mov.u64 %0, %globaltimer;" : "=l"(ns));
+  return ns;
+}
+
 // Bounded wait; after the first one that ran out anywhere in the CTA all give up at once.
 __device__ __forceinline__ bool mm_wait(MmaShared& sh, uint64_t& bar, uint32_t parity) {
   const uint32_t a = t5_smem_u32(&bar);
   if (t5_mbar_wait(a, parity, 1)) return true;
   volatile int* dead = &sh.dead;
-  for (int i = 0; i < 64; ++i) {
+  uint64_t from = 0;
+  for (uint32_t i = 0; i < kMmWaitMost; ++i) {
     if (*dead) return false;
-    if (t5_mbar_wait(a, parity, kMmWaitLimit / 64)) return true;
+    if (t5_mbar_wait(a, parity, kMmWaitPolls)) return true;
+    const uint64_t now = mm_now();
+    if (i == 0) from = now;
+    if (i >= kMmWaitLeast && now - from > kMmWaitNs) break;
   }
   *dead = 1;
+  if (sh.status) {
+    *(volatile int32_t*)sh.status = 1;     // may lie in host memory
+    __threadfence_system();
+  }
   return false;
 }
 
@@ -312,6 +332,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
       t5_mbar_init(t5_smem_u32(&sh.free_[i]), kEpi * CTAS);
     }
     sh.dead = 0;
+    sh.status = p.status;
   }
   __syncwarp();
   t5_fence_before_sync();
@@ -743,7 +764,7 @@ static bool epilogue_vec(const LinEpilogue& e) {
          (ss == 1 ? e.slope == nullptr || (((uintptr_t)e.slope | e.lds) & 7) == 0 : aligned16(e.slope, e.lds, ss));
 }
 
-int mma_run(const MmaJob* jobs, int n, const SumRows& side, void* work, cudaStream_t st) {
+int mma_run(const MmaJob* jobs, int n, const SumRows& side, void* work, int32_t* status, cudaStream_t st) {
   int sms = 0;
   if (int rc = device_sm_count(&sms)) return rc;
   MmaSize z[2];
@@ -796,6 +817,7 @@ int mma_run(const MmaJob* jobs, int n, const SumRows& side, void* work, cudaStre
   p.slots = (int)(kMmRing / 1024 * 1024 / (p.a_slot + p.b_bytes));
   if (p.slots > kMmMaxSlots) p.slots = kMmMaxSlots;
   p.side = side;
+  p.status = status;
   const int rc = z[0].npa == 1 ? launch_jobs<1>(pl, map, p, n, full, sms, st) : launch_jobs<3>(pl, map, p, n, full, sms, st);
   if (rc) return rc;
   for (int j = 0; j < n; ++j) {

@@ -71,7 +71,8 @@ struct MmaSize {
 };
 
 int64_t mma_work_bytes(const MmaSize* sizes, int n, int sms);   // scratch for split sums
-int mma_run(const MmaJob* jobs, int n, const SumRows& side, void* work, cudaStream_t st);   // side.part NULL: none
+// side.part NULL: none; *status (NULL: not wanted) is set to 1 by a wait that ran out.
+int mma_run(const MmaJob* jobs, int n, const SumRows& side, void* work, int32_t* status, cudaStream_t st);
 
 // N elements of type T from p on: as 16-byte vectors where `vec`.
 template <typename T, int N>

@@ -44,7 +44,7 @@
 extern "C" {
 #endif
 
-#define GL_ABI_VERSION 18
+#define GL_ABI_VERSION 19
 
 typedef enum GlStatus {
   GL_OK = 0,
@@ -500,7 +500,8 @@ int gl_k16_bwd_t5_f32(const GlK16Args* args, int32_t* status, void* stream);
  * gl_linear_*, of 16 for gl_norm_*.
  * fp32 products run on the tensor cores as the six products of three-term bf16 splits (as gl_k16_fwd_tc_f32) and
  * agree with fp32 arithmetic to its rounding; an infinity in such an operand gives NaN.  Every wait in these
- * kernels has an iteration limit; a tile whose wait ran out is written as NaN. */
+ * kernels has a limit of a few seconds; what a wait that ran out leaves uncomputed is written as NaN, and `status` of
+ * gl_linear_* (optional: an int32 that the device can write, in its own or in pinned host memory) is set to 1. */
 
 /* Forward of a fused matrix product: y = act(z) + residual, z[m, n] = sum_k x[m, k] w[n, k] + bias[n].
  * `bias` [N] and `residual` [M, ldr] are optional.  For the backward pass the call also keeps act'(z) in `slope`
@@ -515,6 +516,7 @@ typedef struct GlLinearArgs {
   void* y;                  /* [M, ldy] */
   void* slope;
   void* work;
+  int32_t* status;
   int64_t M, N, K, ldx, ldw, ldr, ldy, lds, work_bytes;
   int32_t dtype, act, slope_kind, reserved;
 } GlLinearArgs;
@@ -536,6 +538,7 @@ typedef struct GlLinearBwdArgs {
   void* dw;
   void* db;
   void* work;
+  int32_t* status;
   int64_t M, N, K, lddy, lds, ldx, ldc, ldw, lddx, work_bytes;
   int32_t dtype, slope_kind, accumulate, reserved;
 } GlLinearBwdArgs;

@@ -116,3 +116,23 @@ def test_accumulated_gradients_are_fp32_pointers():
             a.accumulate = 1
             setattr(a, f, A + 2)
             assert fn(ctypes.byref(a), None) == -3
+
+
+# ---- products whose waits ran out ----
+
+def test_a_wait_that_ran_out_is_raised_by_the_next_call(monkeypatch):
+    """The kernels set a word in host memory; the next call reads it, resets it and raises."""
+    t = torch.zeros(1, dtype=torch.int32)
+    monkeypatch.setattr(_native, "_wait_word", (t, ctypes.c_int32.from_address(t.data_ptr()), t.data_ptr()))
+    assert _native._wait_status() == t.data_ptr()
+    t.fill_(1)
+    with pytest.raises(_native.NativeLibraryError, match="ran out"):
+        _native._wait_status()
+    assert _native._wait_status() == t.data_ptr() and int(t) == 0
+
+
+@pytest.mark.parametrize("entry,make", [("gl_linear_fwd", linear_args), ("gl_linear_bwd", linear_bwd_args)])
+def test_the_status_word_is_an_aligned_int32(entry, make):
+    a = make(1)
+    a.status = A + 2
+    assert getattr(_native.load(), entry)(ctypes.byref(a), None) == -3

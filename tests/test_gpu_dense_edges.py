@@ -169,3 +169,24 @@ def test_checkpoints_lower_the_memory_between_the_passes(ckpt, per_x, per_z):
         now = torch.cuda.memory_allocated() - before - y.numel() * 2
         assert held <= now <= held + 5 * 512, (now, held)
         del y
+
+
+# ---- products whose waits ran out ----
+
+def test_products_report_through_the_status_word():
+    """Products leave the word at 0; one that a product had set is raised by the next call, forward or backward, and
+    the call after that works."""
+    x, w = data(64, 128, dtype=BF16, seed=1).requires_grad_(True), data(64, 128, dtype=BF16, seed=2)
+    y = gl.linear_act(x, w)
+    (dx,) = torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+    torch.cuda.synchronize()
+    tensor, word, address = _native._wait_word
+    assert tensor.is_pinned() and address == tensor.data_ptr() and word.value == 0
+    word.value = 1
+    with pytest.raises(_native.NativeLibraryError, match="ran out"):
+        gl.linear_act(x, w)
+    assert torch.equal(gl.linear_act(x, w), y)
+    word.value = 1
+    with pytest.raises(_native.NativeLibraryError, match="ran out"):
+        torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
+    assert torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], dx)
