@@ -22,7 +22,9 @@
 // K-major tiles are one TMA box (64 k wide, all rows of the tile); MN-major tiles are boxes of 64 rows by 64 k, which
 // the matrix descriptor walks with 2048 bytes per 16 k and 8192 bytes per 64 rows.  Edges in every dimension are
 // the tensor map's zero fill.  Every wait has a limit in time and in iterations; a CTA whose wait runs out sets the call's
-// status word, writes NaN to what it has not computed, waits (again bounded) for its own copies and leaves.
+// status word, writes NaN to what it has not computed, waits (again bounded) for its own copies and products and leaves.
+// Otherwise it leaves when every slot has been given back: by then its copies have landed, the tensor core has read them,
+// and no arrival is on its way to a barrier of a CTA that is gone.
 #include <cuda.h>
 
 #include "mma.cuh"
@@ -35,7 +37,7 @@ constexpr int kMmBM = 128, kMmBK = 64, kMmThreads = 320, kMmEpiWarps = 8, kMmMax
 // an epilogue for its tile's sum: at most 2^25 blocks of k in 32 splits, 0.4 s.
 constexpr uint64_t kMmWaitNs = 4000000000ull;
 constexpr uint32_t kMmWaitPolls = 1024, kMmWaitLeast = 128, kMmWaitMost = 1u << 18;
-constexpr uint32_t kMmWaitLimit = 1u << 20;                    // polls for copies that are on their way
+constexpr uint32_t kMmDrainPolls = 1u << 16;                   // for what is on its way already
 constexpr int kMmPitch = 36;                                   // floats per row of a warp's 32 x 32 epilogue tile
 constexpr uint32_t kMmEpiBytes = kMmEpiWarps * 32 * kMmPitch * 4;
 
@@ -62,7 +64,7 @@ struct MmaParams {
 constexpr uint32_t kMmRing = 227 * 1024 - 2048 - kMmEpiBytes;
 
 struct MmaShared {
-  uint64_t full[kMmMaxSlots], empty[kMmMaxSlots], done[4], free_[4];
+  uint64_t full[kMmMaxSlots], empty[kMmMaxSlots], done[4], free_[4], last;
   uint32_t tmem;
   int dead;
   int32_t* status;
@@ -155,6 +157,7 @@ struct MmaRing {
       ++round;
     }
   }
+  __device__ __forceinline__ uint32_t uses(int slot) const { return round + (slot < s); }   // of a slot, so far
 };
 
 struct MmaTile {
@@ -331,6 +334,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
       t5_mbar_init(t5_smem_u32(&sh.done[i]), 1);
       t5_mbar_init(t5_smem_u32(&sh.free_[i]), kEpi * CTAS);
     }
+    t5_mbar_init(t5_smem_u32(&sh.last), 1);
     sh.dead = 0;
     sh.status = p.status;
   }
@@ -388,10 +392,15 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         }
       }
     }
-    if (!live && rank == 0) {   // the copies in flight must land before the shared memory goes away
-      const uint32_t n = (uint32_t)p.slots, it = r.round * n + r.s;
-      for (uint32_t j = it > n ? it - n : 0; j < it; ++j)
-        t5_mbar_wait(t5_smem_u32(&sh.full[j % n]), (j / n) & 1, kMmWaitLimit);
+    for (int i = 0; i < p.slots && live; ++i)      // every slot given back
+      if (r.uses(i)) live = mm_wait_warp(sh, sh.empty[i], (r.uses(i) - 1) & 1);
+    if (!live) {   // the copies in flight must land before the shared memory goes away
+      if (rank == 0) {
+        for (int i = 0; i < p.slots; ++i)
+          if (r.uses(i)) t5_mbar_wait(t5_smem_u32(&sh.full[i]), (r.uses(i) - 1) & 1, kMmDrainPolls);
+      } else {     // theirs count on the other CTA's barriers: time enough for any copy
+        for (int i = 0; i < 1000; ++i) __nanosleep(1000);
+      }
     }
   } else if (warp == 9) {
     if (rank == 0) {
@@ -465,6 +474,10 @@ __global__ void __launch_bounds__(kMmThreads, 1)
           }
           if (live) commit(sh.done[buf]);
         }
+      }
+      if (!live) {   // what has been issued must end before the tensor memory is freed
+        commit(sh.last);
+        t5_mbar_wait(t5_smem_u32(&sh.last), 0, kMmDrainPolls);
       }
     }
   } else if (warp < kEpi) {
