@@ -19,6 +19,13 @@
 // next one runs.  (One accumulator for all pairs needed chunks of 128 for 0.8e-6 in the 2-norm at K = 4096, where plain
 // fp32 products are 1.0e-6 off, and reading it that often cost a fifth of the time.)
 //
+// bf16 operands: a sum over k of terms of one sign that stays in one accumulator comes out small by up to k / 16 2^-23 of
+// itself (measured 2.2e-6 at k = 1024, 1.4e-5 at 4096, 1.8e-4 at 32768).  Where the result is kept in fp32 (added to an fp32 gradient, or a split's
+// partial tile) a sum over k is therefore cut into chunks of kMmLongChunk blocks too, and each chunk is added to memory, by
+// the thread that stored the one before, while the next one runs (dx and an fp32 dw of 8192 x 4096 x 4096: 404 -> 424 us;
+// 40000 rows, 4096 x 1024, one sign: 2.3e-4 -> below 1e-5 off).  A bf16 result takes one accumulator; splits see to it that
+// it sums at most kMmLongest blocks (7e-4 for one sign; half a bf16 step is 2^-9 to 2^-8).
+//
 // K-major tiles are one TMA box (64 k wide, all rows of the tile); MN-major tiles are boxes of 64 rows by 64 k, which
 // the matrix descriptor walks with 2048 bytes per 16 k and 8192 bytes per 64 rows.  Edges in every dimension are
 // the tensor map's zero fill.  Every wait has a limit in time and in iterations; a CTA whose wait runs out sets the call's
@@ -38,13 +45,14 @@ constexpr int kMmBM = 128, kMmBK = 64, kMmThreads = 320, kMmEpiWarps = 8, kMmMax
 constexpr uint64_t kMmWaitNs = 4000000000ull;
 constexpr uint32_t kMmWaitPolls = 1024, kMmWaitLeast = 128, kMmWaitMost = 1u << 18;
 constexpr uint32_t kMmDrainPolls = 1u << 16;                   // for what is on its way already
+constexpr int kMmLongChunk = 32, kMmLongest = 2048;            // in blocks of 64 k
 constexpr int kMmPitch = 36;                                   // floats per row of a warp's 32 x 32 epilogue tile
 constexpr uint32_t kMmEpiBytes = kMmEpiWarps * 32 * kMmPitch * 4;
 
 struct MmaOne {
   int64_t M, N;
   int tiles_m, tiles_n, kblocks, splits, split_blocks;
-  int a_mn, b_mn, vec, npb;
+  int a_mn, b_mn, vec, npb, chunk;   // chunk: blocks of k in one accumulator
   uint32_t a_bytes;            // of a plane of A as loaded
   float* part;
   LinEpilogue e;
@@ -52,7 +60,7 @@ struct MmaOne {
 struct MmaParams {
   MmaOne job[2];
   int64_t items0, items;       // work items of job 0, of all
-  int chunk, slots;
+  int slots;
   uint32_t a_slot, b_bytes;    // bytes of a slot for A, for B
   SumRows side;
   int32_t* status;             // optional: set to 1 by a wait that ran out
@@ -243,8 +251,11 @@ __device__ __forceinline__ void mm_finish8(const LinEpilogue& e, float (&z)[8], 
   }
 }
 
+// `more`: not the sum's first chunk (only where the sums are kept in fp32; of a gradient that is added to, the residual is
+// what the chunk before left).
 template <bool FULL, bool VEC>
-__device__ __forceinline__ void mm_store_rows(const MmaOne& p, const float* tile, int64_t m0, int64_t n0, int split) {
+__device__ __forceinline__ void mm_store_rows(const MmaOne& p, const float* tile, int64_t m0, int64_t n0, int split,
+                                              bool more) {
   const int lane = threadIdx.x & 31, rows = (int)min((int64_t)32, p.M - m0);
   const int c = VEC ? (lane & 3) * 8 : lane;
   const int64_t n = n0 + c;
@@ -265,11 +276,17 @@ __device__ __forceinline__ void mm_store_rows(const MmaOne& p, const float* tile
     if (p.part) {
       float* out = p.part + (split * p.M + m0 + r) * p.N + n;
       if constexpr (VEC) {
+        if (more) {
+          float t[8];
+          ld_span<float, 8>(out, true, t);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) z[i] += t[i];
+        }
         st_span<float, 8>(out, true, z);
       } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-          if (r + i < rows) out[i * p.N] = z[i];
+          if (r + i < rows) out[i * p.N] = more ? out[i * p.N] + z[i] : z[i];
       }
     } else if (p.e.dtype == GL_DTYPE_F32) {
       mm_finish8<float, FULL, VEC>(p.e, z, m0 + r, n, rows - r);
@@ -281,14 +298,14 @@ __device__ __forceinline__ void mm_store_rows(const MmaOne& p, const float* tile
 
 template <bool FULL>
 __device__ __forceinline__ void mm_store_block(const MmaOne& p, float* tile, const float* v, int64_t m0, int64_t n0,
-                                               int split) {
+                                               int split, bool more) {
   const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int j = 0; j < 32; j += 4)
     *reinterpret_cast<float4*>(tile + lane * kMmPitch + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
   __syncwarp();
-  if (p.vec && n0 + 32 <= p.N) mm_store_rows<FULL, true>(p, tile, m0, n0, split);
-  else mm_store_rows<FULL, false>(p, tile, m0, n0, split);
+  if (p.vec && n0 + 32 <= p.N) mm_store_rows<FULL, true>(p, tile, m0, n0, split, more);
+  else mm_store_rows<FULL, false>(p, tile, m0, n0, split, more);
   __syncwarp();
 }
 
@@ -421,10 +438,10 @@ __global__ void __launch_bounds__(kMmThreads, 1)
         const MmaTile t = mm_tile<JOBS>(p, item, BM, BN);
         const MmaOne& o = p.job[JOBS == 1 ? 0 : t.job];
         const uint32_t idesc = t5_idesc_bf16(BM, BN, 0, 0) | ((uint32_t)o.a_mn << 15) | ((uint32_t)o.b_mn << 16);
-        const int npb = o.npb;
+        const int npb = o.npb, chunk = o.chunk;
         const uint32_t ka = (o.a_mn ? 2048u : 32u) >> 4, kb_ = (o.b_mn ? 2048u : 32u) >> 4;   // 16-byte units per 16 k
-        for (int c0 = t.k0; c0 < t.k1 && live; c0 += p.chunk, ++ch) {
-          const int c1 = min(t.k1, c0 + p.chunk), buf = ch % NB;
+        for (int c0 = t.k0; c0 < t.k1 && live; c0 += chunk, ++ch) {
+          const int c1 = min(t.k1, c0 + chunk), buf = ch % NB;
           if (ch >= NB && !mm_wait_warp(sh, sh.free_[buf], (ch / NB - 1) & 1)) {
             live = false;
             break;
@@ -495,7 +512,7 @@ __global__ void __launch_bounds__(kMmThreads, 1)
       const int64_t m0 = t.m0 + kMmBM * rank + 32 * (warp & 3), n0 = t.n0 + half * HALF;
       float sum[MULTI ? HALF : 1];
       mm_prefetch(o, m0, n0, HALF);
-      for (int c0 = t.k0; c0 < t.k1; c0 += p.chunk, ++ch) {
+      for (int c0 = t.k0; c0 < t.k1; c0 += o.chunk, ++ch) {
         const int buf = ch % NB;
         const bool ok = mm_wait_warp(sh, sh.done[buf], (ch / NB) & 1);
         t5_fence_after_sync();
@@ -532,14 +549,14 @@ __global__ void __launch_bounds__(kMmThreads, 1)
               __syncwarp();
               if (lane == 0) mm_arrive<CTAS>(t5_smem_u32(&sh.free_[buf]));
             }
-            if (m0 < o.M && n0 + 32 * q < o.N) mm_store_block<FULL>(o, tile, v, m0, n0 + 32 * q, t.split);
+            if (m0 < o.M && n0 + 32 * q < o.N) mm_store_block<FULL>(o, tile, v, m0, n0 + 32 * q, t.split, c0 > t.k0);
           }
         }
       }
       if constexpr (MULTI) {
 #pragma unroll
         for (int q = 0; q < HALF / 32; ++q) {
-          if (m0 < o.M && n0 + 32 * q < o.N) mm_store_block<FULL>(o, tile, sum + 32 * q, m0, n0 + 32 * q, t.split);
+          if (m0 < o.M && n0 + 32 * q < o.N) mm_store_block<FULL>(o, tile, sum + 32 * q, m0, n0 + 32 * q, t.split, false);
         }
       }
     }
@@ -621,6 +638,10 @@ static MmaPlan mma_search(const MmaSize* z, int n, int sms) {
       for (int s1 : kSplits) {
         if (s1 > 1 && (n < 2 || s1 > kb[1])) break;
         const int s[2] = {s0, s1};
+        bool long_k = false;                                     // one accumulator over too much of it
+        for (int j = 0; j < n; ++j)
+          if (z[j].npa == 1 && (kb[j] + s[j] - 1) / s[j] > kMmLongest && s[j] < 32) long_k = true;
+        if (long_k) continue;
         double sum = 0, longest = 0, extra = 0, items = 0;
         for (int j = 0; j < n; ++j) {
           double t = (double)((kb[j] + s[j] - 1) / s[j]) * block[j];
@@ -820,12 +841,14 @@ int mma_run(const MmaJob* jobs, int n, const SumRows& side, void* work, int32_t*
     } else if (q.e.bias || q.e.act != GL_ACT_IDENTITY || q.e.slope_kind) {
       full = true;
     }
+    // bf16 operands: chunks only where each can be added to fp32 memory, else one (k block numbers stay below 2^25)
+    const bool added = o.part != nullptr || (q.e.dtype == GL_DTYPE_F32 && q.e.residual == q.e.out);
+    o.chunk = q.a.planes > 1 ? 8 : added ? kMmLongChunk : 1 << 30;
     p.items += (int64_t)o.tiles_m * o.tiles_n * o.splits;
     if (j == 0) p.items0 = p.items;
     if (o.a_bytes > p.a_slot) p.a_slot = o.a_bytes;
   }
   if (n == 1) map[2] = map[3] = map[0];
-  p.chunk = z[0].npa > 1 ? 8 : 1 << 30;   // one chunk; k block numbers stay below 2^25
   p.b_bytes = (uint32_t)(pl.BN / pl.ctas) * kMmBK * 2;
   p.slots = (int)(kMmRing / 1024 * 1024 / (p.a_slot + p.b_bytes));
   if (p.slots > kMmMaxSlots) p.slots = kMmMaxSlots;

@@ -87,3 +87,34 @@ def test_many_pair_launches_in_a_row():
         want = gl.linear_act(x, w)
         got = [gl.linear_act(x, w) for _ in range(200)]
     assert all(torch.equal(g, want) for g in got)
+
+
+@pytest.mark.parametrize("M,K,N", [(65536, 2048, 1800), (40000, 4096, 1024), (262144, 512, 512), (70001, 136, 200)])
+def test_long_sums_into_fp32_gradients(M, K, N):
+    """dW of many rows of one sign, added to an fp32 main_grad.  The tensor core truncates after each 16 k to 2^-23 of a
+    partial sum that grows evenly: over a chunk of 32 x 64 k by at most half of 128 2^-23 of the chunk's sum; chunks, splits
+    and the main_grad that is there are added in fp32, rounding to nearest: 2^-24 each."""
+    lay = gl.LinearAct(K, N, bias=False, dtype=BF16, device="cuda")
+    lay.enable_main_grad()
+    x, dy = data(M, K, dtype=BF16, seed=1).abs(), data(M, N, dtype=BF16, seed=2).abs()
+    want = torch.zeros(N, K, dtype=torch.float64, device="cuda")
+    for i in range(0, M, 8192):
+        want += dy[i:i + 8192].double().t() @ x[i:i + 8192].double()
+    for calls in (1, 2):
+        lay(x).backward(dy)
+        err = (lay.weight.main_grad.double() - calls * want).abs()
+        assert float((err / (calls * want)).max()) <= (128 / 2) * 2.0 ** -23 + (M / 2048 + 32 + calls) * 2.0 ** -24
+
+
+def test_bf16_gradients_of_very_many_rows():
+    """A bf16 dW sums at most 2048 blocks of 64 rows in one accumulator, that is 8192 truncations to 2^-23: what sums of one
+    sign lose on average.  (Rounding to bf16 averages out over columns of unlike size.)"""
+    M, K, N = 262144, 2048, 2304
+    x = data(M, K, dtype=BF16, seed=1).abs_()
+    dy = (data(M, N, seed=2).abs_() * torch.linspace(1, 2, N, device="cuda")).to(BF16)
+    w = data(N, K, dtype=BF16, seed=3).requires_grad_(True)
+    (dw,) = torch.autograd.grad(gl.linear_act(x, w), w, dy)
+    want = torch.zeros(N, K, dtype=torch.float64, device="cuda")
+    for i in range(0, M, 8192):
+        want += dy[i:i + 8192].double().t() @ x[i:i + 8192].double()
+    assert abs(float(((dw.double() - want) / want).mean())) <= 8192 * 2.0 ** -23
