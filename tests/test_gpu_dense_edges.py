@@ -190,3 +190,21 @@ def test_products_report_through_the_status_word():
     with pytest.raises(_native.NativeLibraryError, match="ran out"):
         torch.autograd.grad(y, x, torch.ones_like(y), retain_graph=True)
     assert torch.equal(torch.autograd.grad(y, x, torch.ones_like(y))[0], dx)
+
+
+# rows (token groups of a power of two and not, several samples), resident samples, long samples in chunks (aligned and
+# not), groups wider than a block
+@pytest.mark.parametrize("shape,G", [((9, 4096), 32), ((5, 96 * 8), 8), ((3, 130), 13), ((4, 37, 72), 9), ((2, 300, 64), 4),
+                                     ((1, 70000, 16), 4), ((40, 5000, 48), 6), ((2, 3000, 33), 3), ((2, 3, 65536), 1)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_norm_of_constant_groups(shape, G, dtype):
+    """Groups whose values are all alike, each a small whole number: every sum of up to 2^24 of its last bits is exact, the
+    mean is the value, the deviations are 0 and y is beta, however small eps is."""
+    S, C = shape[0], shape[-1]
+    c = torch.randint(1, 60, (S, G), generator=torch.Generator().manual_seed(3)).to("cuda")
+    x = c.repeat_interleave(C // G, 1).reshape(S, *[1] * (len(shape) - 2), C).expand(shape).to(dtype).contiguous()
+    gam, bet = 1 + data(C, dtype=dtype, seed=4, scale=0.1), data(C, dtype=dtype, seed=5)
+    y = gl.group_norm_act(x, G, gam, bet, eps=1e-9)
+    assert torch.equal(y, bet.expand(shape))
+    _, _, stats = dense._norm_forward(x, G, None, None, 0, 1e-9)
+    assert torch.equal(stats[0], c.float())
