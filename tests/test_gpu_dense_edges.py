@@ -208,3 +208,17 @@ def test_norm_of_constant_groups(shape, G, dtype):
     assert torch.equal(y, bet.expand(shape))
     _, _, stats = dense._norm_forward(x, G, None, None, 0, 1e-9)
     assert torch.equal(stats[0], c.float())
+
+
+# ---- activations ----
+
+@pytest.mark.parametrize("M", [1, 3, 2000])
+def test_bf16_gelu_in_its_tail(M):
+    """GELU of bf16 layers down to z = -12.5, where it is z times a tail probability of 1e-36: off by its rounding to bf16
+    (half a step, at most 2^-8) and the tail's 1.4e-4 < 2^-12, relative."""
+    z = torch.linspace(-12.5, -0.01, max(M, 60), device="cuda").to(BF16)
+    one = torch.ones(1, 1, device="cuda", dtype=BF16)
+    with torch.no_grad():
+        y = torch.cat([gl.linear_act(part.reshape(-1, 1), one, activation="gelu") for part in z.split(M)]).flatten()
+    want = z.double() * torch.special.erfc(-z.double() / 2 ** 0.5) / 2
+    assert bool(((y.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -12) * want.abs()).all())
