@@ -107,8 +107,9 @@ __device__ __forceinline__ void normal_cdf_pdf(float z, float& cdf, float& pdf) 
   if constexpr (FAST) {
     const float e = ex2_approx(z * z * (-0.5f * 1.4426950408889634f));       // e^(-z^2 / 2)
     const float s = rcp_approx(fmaf(fabsf(z), 0.3f, 1.f));
-    const float q = s * fmaf(s, fmaf(s, fmaf(s, fmaf(s, fmaf(s, -0.0817056596f, 0.229728952f), -0.0323179811f), 0.152237385f),
-                                     0.111820899f), 0.120235749f);
+    float q = fmaf(s, -0.0817056596f, 0.229728952f);
+    q = fmaf(s, fmaf(s, q, -0.0323179811f), 0.152237385f);
+    q = s * fmaf(s, fmaf(s, q, 0.111820899f), 0.120235749f);
     const float tail = q * e;
     cdf = z < 0.f ? tail : 1.f - tail;
     pdf = 0.3989422804014327f * e;

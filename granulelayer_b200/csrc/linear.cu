@@ -4,13 +4,15 @@
 //
 // The products run on the tensor cores (mma.cu).  bf16 operands whose rows are 16-byte aligned are read where they
 // lie; others are first copied to aligned rows, and fp32 operands are split into three bf16 planes
-// (v = v1 + v2 + v3, 24 significand bits for 2^-110 <= |v|; an infinity gives NaN, since it meets all of the other operand's
-// terms, of either sign or zero).
+// (v = v1 + v2 + v3, 24 significand bits for 2^-110 <= |v|; an infinity gives NaN, since it meets all of the other
+// operand's terms, of either sign or zero).
 // An 8-bit checkpoint of x is one plane even for fp32 layers: its values are bf16 numbers.  A few rows (serving
 // single tokens) run row kernels instead, which read w once and are bound by HBM.
 //
 // dz is written once, rounded to bf16 in bf16 layers and split in fp32 ones, with the column sums of its fp32
-// values; where dy itself is dz (identity, bf16, aligned) only the sums are taken.
+// values; where dy itself is dz (identity, bf16, aligned) only the sums are taken.  The rounding is what a bf16 operand of
+// the tensor cores costs: dx and dw of 1024 x 4096 x 4096 are 2.3e-3 off in the 2-norm, 1.7e-3 of which is their own
+// rounding; a second term of dz would double both products (355 of 654 us of kernels at 8192 x 4096 x 4096).
 #include "mma.cuh"
 
 namespace gl {
@@ -34,7 +36,11 @@ __device__ __forceinline__ void bf16_terms(const float (&v)[8], uint4 (&out)[NP]
     uint32_t u[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      u[i] = NP > 1 && j == 0 ? pack_bf16(bf16_range(r[2 * i]), bf16_range(r[2 * i + 1])) : pack_bf16(r[2 * i], r[2 * i + 1]);
+      if constexpr (NP > 1) {
+        u[i] = j == 0 ? pack_bf16(bf16_range(r[2 * i]), bf16_range(r[2 * i + 1])) : pack_bf16(r[2 * i], r[2 * i + 1]);
+      } else {
+        u[i] = pack_bf16(r[2 * i], r[2 * i + 1]);
+      }
       r[2 * i] -= __uint_as_float(u[i] << 16);
       r[2 * i + 1] -= __uint_as_float(u[i] & 0xFFFF0000u);
     }
@@ -217,7 +223,10 @@ __global__ void __launch_bounds__(128) lin_db_kernel(SumRows j) {
 // W warps per output column n: each streams its part of w's row n, four 16-byte loads in flight, against MT rows of x
 // (from L1), fp32 sums, shuffles and one shared-memory step between the W warps.  Bound by reading w; W grows with the
 // row, so that the machine has enough of it in flight (4096 -> 2048 fp32, one token: W = 1 10.2 us, W = 2 7.2 us,
-// 4.7 TB/s; 4096 -> 4096 bf16 W = 1 8.1 us, W = 2 8.8 us, eight loads 10.3 us).
+// 4.7 TB/s; 4096 -> 4096 bf16 W = 1 8.1 us, W = 2 8.8 us, eight loads 10.3 us).  What is left of a row after its last
+// 4 W 32 16-byte loads is read element by element, so that widths which are no multiple of that run below this rate (one
+// token to 4096 outputs, right after a write of 256 MB; K = 768, 1536, 4096, 5120, 11008, 14336: bf16 6.1, 7.0, 10.9,
+// 16.1, 29.0, 33.4 us, fp32 6.5, 8.7, 19.7, 23.3, 42.2, 50.0 us).
 template <typename T, int MT, int W, bool ALIGNED>
 __global__ void __launch_bounds__(128) lin_rows_kernel(const T* x, const T* w, int M, int64_t N, int64_t K,
                                                        int64_t ldx, int64_t ldw, LinEpilogue e) {
@@ -286,8 +295,9 @@ __global__ void __launch_bounds__(128) lin_rows_kernel(const T* x, const T* w, i
   if (n < N && lane < M) lin_finish<1>(e, lane, n, false, z);
 }
 
-// Rows up to which the row kernels run.  4096 -> 4096, bf16: 4 rows 12.5 us here, 13.7 us on the tensor cores (which the
-// rows' number hardly changes); fp32: 8 rows 27 us here, 16 rows 73 us through the split of w.
+// Rows up to which the row kernels run.  4096 -> 4096 right after a write of 256 MB: bf16 4 rows 15.6 us here; 5 rows 36.3 us
+// here and 16.5 us on the tensor cores, whose time the rows hardly change.  fp32 8 rows 37.5 us here; on the tensor cores 9
+// and 16 rows 79.6 us (29.6 in splitting w), where this kernel takes 41.3 and 54.8 us: fp32's limit is below where they meet.
 template <typename T>
 constexpr int kRows = sizeof(T) == 4 ? 8 : 4;
 

@@ -20,11 +20,12 @@
 // fp32 products are 1.0e-6 off, and reading it that often cost a fifth of the time.)
 //
 // bf16 operands: a sum over k of terms of one sign that stays in one accumulator comes out small by up to k / 16 2^-23 of
-// itself (measured 2.2e-6 at k = 1024, 1.4e-5 at 4096, 1.8e-4 at 32768).  Where the result is kept in fp32 (added to an fp32 gradient, or a split's
-// partial tile) a sum over k is therefore cut into chunks of kMmLongChunk blocks too, and each chunk is added to memory, by
-// the thread that stored the one before, while the next one runs (dx and an fp32 dw of 8192 x 4096 x 4096: 404 -> 424 us;
-// 40000 rows, 4096 x 1024, one sign: 2.3e-4 -> below 1e-5 off).  A bf16 result takes one accumulator; splits see to it that
-// it sums at most kMmLongest blocks (7e-4 for one sign; half a bf16 step is 2^-9 to 2^-8).
+// itself (measured 2.2e-6 at k = 1024, 1.4e-5 at 4096, 1.8e-4 at 32768).  Where the result is kept in fp32 (added to an
+// fp32 gradient, or a split's partial tile) a sum over k is therefore cut into chunks of kMmLongChunk blocks too, and each
+// chunk is added to memory, by the thread that stored the one before, while the next one runs (dx and an fp32 dw of
+// 8192 x 4096 x 4096: 404 -> 424 us; 40000 rows, 4096 x 1024, one sign: 2.3e-4 -> below 1e-5 off).  A bf16 result takes one
+// accumulator; splits see to it that it sums at most kMmLongest blocks (7e-4 for one sign; half a bf16 step is 2^-9 to
+// 2^-8).
 //
 // K-major tiles are one TMA box (64 k wide, all rows of the tile); MN-major tiles are boxes of 64 rows by 64 k, which
 // the matrix descriptor walks with 2048 bytes per 16 k and 8192 bytes per 64 rows.  Edges in every dimension are

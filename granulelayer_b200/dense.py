@@ -7,8 +7,10 @@
 
 ``checkpoint="int8"`` makes the first two keep what their backward pass reads in 8 bits: the input as int8 codes
 with one power-of-two scale per 32 channels (1.03 bytes per element), and ``linear_act`` the activation's
-derivative as one byte (multiples of 1/192, exact at 0 and 1).  The forward result does not change; the gradients
-are those of the read-back input.
+derivative as one byte (multiples of 1/192, exact at 0 and 1).  The forward result does not change.  The gradients are
+the usual formulas with the read-back input in the input's place, and with what the forward pass found: act'(z) of the
+original z (in steps of 1/192) for ``linear_act``, mean and 1 / deviation of the original input for ``group_norm_act``.
+They are close to those at the original input, and exactly those of no input.
 
 Storage is float32 or bfloat16; sums and statistics are float32.  The kernels run in the in-tree sm_100a library on
 the current CUDA stream; there is no CPU path (``NativeLibraryError``) and nothing falls back to PyTorch math.
@@ -221,7 +223,8 @@ def linear_act(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tenso
 
     ``activation``: "identity", "relu", "gelu" (erf form) or "silu".  ``checkpoint="int8"`` keeps the input and the
     activation's derivative in 8 bits for the backward pass.  All tensors share one dtype (float32 or bfloat16;
-    float32 products run as exact three-term bf16 splits on the tensor cores, or in fp32 for a few rows).
+    float32 products run as exact three-term bf16 splits on the tensor cores, where an infinity in x, weight or an output
+    gradient gives NaN, or in fp32 for up to 8 rows).  bfloat16 layers round the gradient of z to bfloat16 before its products.
     Parameters with a ``main_grad`` receive their gradients there."""
     act = _ACT_IDS.get(activation)
     xs, ws, dt, dev = x.shape, weight.shape, x.dtype, x.device
