@@ -771,8 +771,8 @@ __global__ void __launch_bounds__(NT, kBwdBlocks) norm_bwd_stats_kernel(NormPara
   const int64_t rf = norm_red(p.cs, N, NT);
   float* ra = sf;
   float* rb = sf + rf;
-  float* ga = rb + rf;
-  float* gb = ga + p.ng;
+  float* gq = rb + rf;                                  // [ng] sums of q h, of q
+  float* gs = gq + p.ng;
   const int cpg = a.cpg;
   if (a.live()) {
     for (int col = a.tx; col < a.nv; col += a.TX) {
@@ -822,11 +822,11 @@ __global__ void __launch_bounds__(NT, kBwdBlocks) norm_bwd_stats_kernel(NormPara
     rb[c] = vb * gam;
   }
   __syncthreads();
-  group_sums<NT>(ra, a.csl, 1, a.ngl, cpg, ga);
-  group_sums<NT>(rb, a.csl, 1, a.ngl, cpg, gb);
+  group_sums<NT>(ra, a.csl, 1, a.ngl, cpg, gq);
+  group_sums<NT>(rb, a.csl, 1, a.ngl, cpg, gs);
   __syncthreads();
   float2* out = reinterpret_cast<float2*>(p.gpart) + chunk * p.G * p.nsub + entry0(p, a.g0);
-  for (int g = threadIdx.x; g < a.ngl; g += NT) out[g] = make_float2(gb[g], ga[g]);
+  for (int g = threadIdx.x; g < a.ngl; g += NT) out[g] = make_float2(gs[g], gq[g]);
 }
 
 // dgamma / dbeta of 32 channels = the partial rows' sums in a fixed order: by `warps` row lanes.
